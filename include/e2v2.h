@@ -597,6 +597,35 @@ int e2v2_ln_silu_bwd2(const float* x, const float* g, const float* b, const floa
                       const float* qx, const float* qg, const float* qb, float* dgy, float* dx, float* part_g,
                       float* part_b, int n, int w, int n_part, hipStream_t s);
 
+/* ---- layer norm of rows, with its backward pass and that pass's derivative ----
+ * The nn.LayerNorm of any width up to 16384 on rows in fp32, bf16 or fp16 (the reference's LayerNorms:
+ * module_utils.py:2151-2178, 2230-2233); the rows' elements are consecutive, rows lie ld* elements apart (0: one row
+ * for all); y, gx, and the second order's dgy (in y) and dx (in gx) are written contiguous.  Parameters may be NULL (weight 1, bias
+ * 0) and have a type of their own.  Statistics and sums are fp32.
+ *   fwd:  y; stats [n][2] = (mean, rstd) unless NULL.
+ *   bwd:  gx from x, gy and stats; with gg / gb (either may be NULL) also the gradients of weight and bias.
+ *   bwd2: given the upstream gradients qx, qg, qb (each may be NULL: zero; qg and qb in the parameters' types) of
+ *         (gx, gg, gb): dgy, dx and, unless gg is NULL, the weight's gradient.
+ * The workspace holds one partial row of each parameter's sums per workgroup; needed where gg or gb is given. */
+#define E2V2_F32 0
+#define E2V2_BF16 1
+#define E2V2_F16 2
+typedef struct {
+  const void* x; const void* gy; const void* qx;
+  const void* g; const void* b; const void* qg; const void* qb;
+  void* y; void* gx;
+  float* stats;
+  int64_t n, ldx, ldgy, ldqx;
+  int32_t w, type, g_type, b_type;
+  float eps;
+} e2v2_layer_norm_args;
+int e2v2_layer_norm_fwd(const e2v2_layer_norm_args* args, hipStream_t s);
+int64_t e2v2_layer_norm_workspace(int64_t n, int w);
+int e2v2_layer_norm_bwd(const e2v2_layer_norm_args* args, void* gg, void* gb, float* workspace, int64_t workspace_bytes,
+                        hipStream_t s);
+int e2v2_layer_norm_bwd2(const e2v2_layer_norm_args* args, void* gg, float* workspace, int64_t workspace_bytes,
+                         hipStream_t s);
+
 /* ---- per-node dense layers: fp32 GEMMs on bf16 MFMA by the exact three-piece split ----
  * Replaces the GEMMs (forward and input gradient) of SO3_Linear_e2former (module_utils.py:2010-2052) and so of
  * FeedForwardNetwork_s3 (module_utils.py:2755-2797), the value projection and proj_first (e2former.py:215-219,

@@ -1,0 +1,79 @@
+"""What norms.layer_norm and its entry points refuse, before any kernel or HIP call.  No GPU needed."""
+import pytest
+import torch
+
+from ubio_molfm_amd import _lib, norms
+
+
+def test_host_rows_are_refused(monkeypatch):
+    monkeypatch.setattr(_lib, "call", lambda *a: pytest.fail("a kernel was called"))
+    with pytest.raises(RuntimeError, match="GPU only"):
+        norms.layer_norm(torch.rand(3, 8))
+    with pytest.raises(RuntimeError, match="GPU only"):
+        norms.layer_norm([1.0, 2.0])
+
+
+class _OnGpu(torch.Tensor):
+    """A host tensor that says it lies on the GPU: the checks behind the device's."""
+    is_cuda = True
+
+
+def _gpu(*shape, dtype=torch.float32):
+    return torch.zeros(shape, dtype=dtype).as_subclass(_OnGpu)
+
+
+@pytest.mark.parametrize("x,kw,match", [
+    (lambda: _gpu(3, 8, dtype=torch.float64), {}, "fp32, bf16 or fp16"),
+    (lambda: _gpu(3, 8, dtype=torch.int32), {}, "fp32, bf16 or fp16"),
+    (lambda: _gpu(), {}, "fp32, bf16 or fp16"),
+    (lambda: _gpu(3, 0), {}, "width 0"),
+    (lambda: _gpu(1, norms.MAX_WIDTH + 1), {}, "width 16385"),
+    (lambda: _gpu(3, 8), dict(weight=torch.ones(7)), "weight"),
+    (lambda: _gpu(3, 8), dict(bias=torch.ones(1, 8)), "bias"),
+    (lambda: _gpu(3, 8), dict(weight=torch.ones(8, dtype=torch.bfloat16)), "weight"),
+    (lambda: _gpu(3, 8, dtype=torch.bfloat16), dict(bias=torch.ones(8, dtype=torch.float16)), "bias"),
+    (lambda: _gpu(3, 8), dict(weight=torch.ones(8, device="meta")), "weight"),
+])
+def test_refusals(x, kw, match, monkeypatch):
+    monkeypatch.setattr(_lib, "call", lambda *a: pytest.fail("a kernel was called"))
+    with pytest.raises(ValueError, match=match):
+        norms.layer_norm(x(), **kw)
+
+
+@pytest.mark.parametrize("shape,stride,ld", [
+    ((4, 8), (8, 1), 8), ((4, 8), (24, 1), 24), ((4, 8), (0, 1), 0), ((2, 3, 8), (24, 8, 1), 8),
+    ((2, 3, 8), (48, 16, 1), 16), ((8,), (1,), 8), ((1, 1, 8), (5, 3, 1), 8), ((2, 1, 3, 8), (72, 7, 24, 1), 24),
+    ((4, 1), (3, 2), 3)])
+def test_rows_that_are_read_where_they_lie(shape, stride, ld):
+    t = torch.zeros(512).as_strided(shape, stride)
+    u, got = norms._rows(t)
+    assert u is t and got == ld
+
+
+@pytest.mark.parametrize("shape,stride", [((4, 8), (1, 4)), ((4, 8), (16, 2)), ((2, 3, 8), (100, 8, 1)),
+                                          ((2, 3, 8), (0, 8, 1))])
+def test_rows_that_are_copied(shape, stride):
+    t = torch.arange(512.0).as_strided(shape, stride)
+    u, ld = norms._rows(t)
+    assert u.is_contiguous() and ld == shape[-1] and torch.equal(u, t)
+
+
+def test_entry_point_checks():
+    lib = _lib.load()
+    a = _lib.LayerNormArgs()
+    a.n, a.w, a.x, a.y = 4, 16, 64, 64                  # never dereferenced: the checks fail first
+    for change, match in ((dict(w=0), b"width 0"), (dict(w=16385), b"width 16385"), (dict(n=-1), b"-1 rows"),
+                          (dict(type=3), b"types"), (dict(g_type=-1), b"types"), (dict(ldx=-8), b"stride"),
+                          (dict(x=66), b"misaligned"), (dict(stats=68), b"misaligned"), (dict(x=None), b"null")):
+        b = _lib.LayerNormArgs.from_buffer_copy(a)
+        for k, v in change.items():
+            setattr(b, k, v)
+        assert lib.e2v2_layer_norm_fwd(_lib.C.byref(b), None) != 0 and match in lib.e2v2_last_error(), change
+    assert lib.e2v2_layer_norm_bwd(_lib.C.byref(a), None, None, None, _lib.i64(0), None) != 0
+    assert b"null operand" in lib.e2v2_last_error()
+    a.gy = a.gx = a.stats = 64
+    need = lib.e2v2_layer_norm_workspace(4, 16)
+    assert need == 2 * 4 * 16 * 4 and lib.e2v2_layer_norm_workspace(0, 16) == 0
+    for fn, args in ((lib.e2v2_layer_norm_bwd, (_lib.vp(64), None, _lib.vp(64))),
+                     (lib.e2v2_layer_norm_bwd2, (_lib.vp(64), _lib.vp(64)))):
+        assert fn(_lib.C.byref(a), *args, _lib.i64(need - 4), None) != 0 and b"workspace" in lib.e2v2_last_error()

@@ -10,6 +10,7 @@ _lib.py        ctypes binding of libe2v2.so (fails loudly when it is missing)
 build.py       hipcc build of libe2v2.so (in-tree)
 ops.py         torch-facing operators and autograd Functions over the C-ABI
 sparse_ops.py  the reference's op-level sparse edge functions (first and second order)
+norms.py       layer norm of rows with its gradients to second order
 neighbors.py   periodic radius graph -> CSR (query rows, key columns); the reference's
                padded-batch construct_radius_neighbor
 modules.py     E2former module tree (reference names) on the HIP edge path

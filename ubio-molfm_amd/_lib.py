@@ -21,6 +21,7 @@ EXPORTS = [
     "e2v2_deg_bwd_workspace", "e2v2_deg_hidden_fwd", "e2v2_deg_hidden_bwd", "e2v2_deg_bias_grad",
     "e2v2_edge_to_pos", "e2v2_rmsnorm_fwd", "e2v2_add_rmsnorm_fwd", "e2v2_rmsnorm_bwd", "e2v2_rmsnorm_bwd_param", "e2v2_rmsnorm_bwd2", "e2v2_gate_fwd",
     "e2v2_gate_bwd", "e2v2_gate_bwd2", "e2v2_ln_silu_fwd", "e2v2_ln_silu_bwd", "e2v2_ln_silu_bwd_param", "e2v2_ln_silu_bwd2",
+    "e2v2_layer_norm_fwd", "e2v2_layer_norm_workspace", "e2v2_layer_norm_bwd", "e2v2_layer_norm_bwd2",
     "e2v2_pairdot_fwd", "e2v2_pairdot_bwd", "e2v2_qk_proj_fwd", "e2v2_qk_proj_bwd",
     "e2v2_qk_proj_fwd_bf16", "e2v2_qk_proj_bwd_bf16",
     "e2v2_segment_metadata", "e2v2_pair_count", "e2v2_pair_emit", "e2v2_seg_dot", "e2v2_seg_reduce",
@@ -104,6 +105,12 @@ class GemmArgs(C.Structure):
                 ("a_bf16", i32), ("c_bf16", i32)]
 
 
+class LayerNormArgs(C.Structure):
+    _fields_ = [("x", vp), ("gy", vp), ("qx", vp), ("g", vp), ("b", vp), ("qg", vp), ("qb", vp), ("y", vp), ("gx", vp),
+                ("stats", vp), ("n", i64), ("ldx", i64), ("ldgy", i64), ("ldqx", i64), ("w", i32), ("type", i32),
+                ("g_type", i32), ("b_type", i32), ("eps", f32)]
+
+
 class AttnLayer(C.Structure):
     _fields_ = [("pieces", i32), ("zero_order", i32), ("hid", i32), ("c", i32), ("heads", i32), ("n_out", i32),
                 ("qk_fwd", vp), ("qk_bwd", vp), ("qk_bias", vp), ("v_fwd", vp), ("v_bias", vp),
@@ -152,6 +159,8 @@ def load():
     lib.e2v2_deg_bwd_workspace.argtypes = [C.c_int64]
     lib.e2v2_qkdot_gate_bwd_workspace.restype = C.c_size_t
     lib.e2v2_qkdot_gate_bwd_workspace.argtypes = [C.c_int64]
+    lib.e2v2_layer_norm_workspace.restype = C.c_int64
+    lib.e2v2_layer_norm_workspace.argtypes = [C.c_int64, C.c_int32]
     lib.e2v2_gemm_packed_bytes.restype = C.c_int64
     lib.e2v2_gemm_packed_bytes.argtypes = [C.c_int32, C.c_int32, C.c_int32, C.c_int32]
     _lib = lib

@@ -1,0 +1,495 @@
+// Layer norm of rows [n][w] in fp32, bf16 or fp16, its backward pass with the weight's and the bias's gradients, and
+// the derivative of that backward pass (force training differentiates the forces once more).  With <.> the mean over
+// a row, xh = (x - <x>) r and r = (<(x - <x>)^2> + eps)^(-1/2):
+//   forward        y = xh g + b
+//   backward       u = gy g,  gx = r (u - <u> - xh <u xh>),  dg = sum_rows gy xh,  db = sum_rows gy
+//   second order   (upstream qx, qg, qb of gx, dg, db)
+//                  A = r (qx - <qx> - xh <qx xh>),  c = <u xh>,  m = <qx xh>,
+//                  dgy = g A + qg xh + qb,  X = -r (c qx + m u) + qg gy,
+//                  dx = r (X - <X> - xh <X xh>) - r <qx gx> xh,  d(g) = sum_rows gy A
+// (<qx gx> is r (<qx u> - <qx> <u> - c m); d(b) is zero.)  Rows are rounded to their type once, at the store;
+// statistics, row sums and the parameters' sums are fp32, the variance taken about the mean in a second pass over the
+// registers.
+//
+// One pass over memory: a row stays in the registers of kL lanes (16, 32 or 64 of a wavefront, or a workgroup of 256
+// or 1024), at most 16 elements a lane, read as 16-byte vectors where width, strides and addresses allow and element
+// by element where not.  A workgroup strides over the rows and keeps its columns' parameter sums in registers; each
+// leaves one partial row, added in order by a second launch, so results repeat bitwise.  Bound: HBM.
+#include <algorithm>
+
+#include "common.h"
+#include "../../include/e2v2.h"
+
+namespace e2v2 {
+namespace {
+
+constexpr int kLnElems = 16;           // elements of a row in a lane's registers
+constexpr int kLnMaxWidth = 1024 * kLnElems;
+constexpr int kLnMaxParts = 1024;      // workgroups of a pass that leaves parameter sums: four per CU
+
+template <typename T, int V>
+struct RowVec {
+  typedef T type __attribute__((ext_vector_type(V)));
+  typedef float ftype __attribute__((ext_vector_type(V)));
+};
+
+template <typename T, int V>
+__device__ __forceinline__ void load_row(const T* p, float* out) {
+  if constexpr (V == 1) {
+    out[0] = (float)p[0];
+  } else {
+    const auto f = __builtin_convertvector(*reinterpret_cast<const typename RowVec<T, V>::type*>(p),
+                                           typename RowVec<T, V>::ftype);
+#pragma unroll
+    for (int k = 0; k < V; ++k) out[k] = f[k];
+  }
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void store_row(const float* v, T* p) {
+  if constexpr (V == 1) {
+    p[0] = (T)v[0];
+  } else {
+    typename RowVec<T, V>::ftype f;
+#pragma unroll
+    for (int k = 0; k < V; ++k) f[k] = v[k];
+    *reinterpret_cast<typename RowVec<T, V>::type*>(p) = __builtin_convertvector(f, typename RowVec<T, V>::type);
+  }
+}
+
+// Element c of a parameter vector (NULL: the value of an absent one).
+__device__ __forceinline__ float load_param(const void* p, int type, int c, float absent) {
+  if (!p) return absent;
+  if (type == E2V2_F32) return static_cast<const float*>(p)[c];
+  return type == E2V2_BF16 ? (float)static_cast<const __bf16*>(p)[c] : (float)static_cast<const _Float16*>(p)[c];
+}
+
+// Sums of K values over the kL lanes that hold a row, in every lane.  red: two buffers of [K][waves], used in turn, so
+// that one barrier a sum is enough (a buffer is written again two sums later, behind the barrier between).
+template <int kL, int K>
+__device__ __forceinline__ void group_sum(float (&v)[K], float (*red)[4][16], int& turn) {
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    v[k] = dpp_row_sum16(v[k]);
+    if constexpr (kL >= 32) v[k] += __shfl_xor(v[k], 16, 64);
+    if constexpr (kL >= 64) v[k] += __shfl_xor(v[k], 32, 64);
+  }
+  if constexpr (kL > 64) {
+    constexpr int kWaves = kL / 64;
+    const int wv = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) red[turn][k][wv] = v[k];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      v[k] = 0.f;
+#pragma unroll
+      for (int i = 0; i < kWaves; ++i) v[k] += red[turn][k][i];
+    }
+    turn ^= 1;
+  }
+}
+
+struct LnArgs {
+  const void* x; const void* gy; const void* qx;
+  const void* g; const void* b; const void* qg; const void* qb;
+  void* y; void* gx;                 // forward: y; backward: gx; second order: y is dgy, gx is dx
+  float* stats;                      // [n][2] mean, rstd
+  float* part;                       // [2 or 1][gridDim.x][w], or NULL
+  int64_t n, ldx, ldgy, ldq;
+  int w, g_type, b_type;
+  float eps;
+};
+
+// The lane's columns: vector k starts at column (l + k kL) V.
+template <int V, int kL, int NV, typename F>
+__device__ __forceinline__ void each_vec(int l, int w, F&& f) {
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int c = (l + k * kL) * V;
+    f(k, c, c < w);
+  }
+}
+
+template <int V, int kL, int NV>
+__device__ __forceinline__ void load_params(const void* p, int type, int l, int w, float absent, float (&out)[NV * V]) {
+  each_vec<V, kL, NV>(l, w, [&](int k, int c, bool in) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) out[k * V + e] = in ? load_param(p, type, c + e, absent) : 0.f;
+  });
+}
+
+// Adds the workgroup's row groups' parameter sums and writes them as partial row blockIdx.x.
+template <int V, int kL, int NV>
+__device__ __forceinline__ void write_part(const float (&acc)[NV * V], int l, int rg, int w, float* out) {
+  if constexpr (kL > 64) {
+    each_vec<V, kL, NV>(l, w, [&](int k, int c, bool in) {
+      if (in) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) out[c + e] = acc[k * V + e];
+      }
+    });
+  } else {
+    constexpr int kR = 256 / kL, kC = kL * NV * V;
+    __shared__ float red[kR][kC];
+    __syncthreads();
+    each_vec<V, kL, NV>(l, w, [&](int k, int c, bool in) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) red[rg][c + e] = acc[k * V + e];
+    });
+    __syncthreads();
+    for (int c = threadIdx.x; c < w; c += 256) {
+      float s = 0.f;
+#pragma unroll
+      for (int r = 0; r < kR; ++r) s += red[r][c];
+      out[c] = s;
+    }
+  }
+}
+
+template <typename T, int V, int kL, int NV>
+__global__ __launch_bounds__(kL > 64 ? kL : 256) void k_layer_norm_fwd(LnArgs P) {
+  constexpr int kR = kL > 64 ? 1 : 256 / kL, E = NV * V;
+  __shared__ float red[2][4][16];
+  const int l = threadIdx.x % kL, rg = threadIdx.x / kL, w = P.w;
+  const float inv = 1.0f / (float)w;
+  float g[E], b[E];
+  load_params<V, kL, NV>(P.g, P.g_type, l, w, 1.f, g);
+  load_params<V, kL, NV>(P.b, P.b_type, l, w, 0.f, b);
+  int turn = 0;
+  for (int64_t row = (int64_t)blockIdx.x * kR + rg; row < P.n; row += (int64_t)gridDim.x * kR) {
+    const T* xr = static_cast<const T*>(P.x) + row * P.ldx;
+    float x[E], s[1] = {0.f}, q[1] = {0.f};
+    each_vec<V, kL, NV>(l, w, [&](int k, int c, bool in) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) x[k * V + e] = 0.f;
+      if (in) load_row<T, V>(xr + c, x + k * V);
+#pragma unroll
+      for (int e = 0; e < V; ++e) s[0] += x[k * V + e];
+    });
+    group_sum<kL, 1>(s, red, turn);
+    const float mean = s[0] / (float)w;       // a true quotient: exact for a row of one short value
+    each_vec<V, kL, NV>(l, w, [&](int k, int c, bool in) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        x[k * V + e] = in ? x[k * V + e] - mean : 0.f;
+        q[0] = fmaf(x[k * V + e], x[k * V + e], q[0]);
+      }
+    });
+    group_sum<kL, 1>(q, red, turn);
+    const float rstd = 1.0f / sqrtf(q[0] * inv + P.eps);
+    T* yr = static_cast<T*>(P.y) + row * w;
+    each_vec<V, kL, NV>(l, w, [&](int k, int c, bool in) {
+      float o[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) o[e] = fmaf(x[k * V + e] * rstd, g[k * V + e], b[k * V + e]);
+      if (in) store_row<T, V>(o, yr + c);
+    });
+    if (P.stats && l == 0) *reinterpret_cast<float2*>(P.stats + 2 * row) = make_float2(mean, rstd);
+  }
+}
+
+template <typename T, int V, int kL, int NV>
+__global__ __launch_bounds__(kL > 64 ? kL : 256) void k_layer_norm_bwd(LnArgs P) {
+  constexpr int kR = kL > 64 ? 1 : 256 / kL, E = NV * V;
+  __shared__ float red[2][4][16];
+  const int l = threadIdx.x % kL, rg = threadIdx.x / kL, w = P.w;
+  const float inv = 1.0f / (float)w;
+  float g[E], ag[E], ab[E];
+  load_params<V, kL, NV>(P.g, P.g_type, l, w, 1.f, g);
+#pragma unroll
+  for (int e = 0; e < E; ++e) ag[e] = ab[e] = 0.f;
+  int turn = 0;
+  for (int64_t row = (int64_t)blockIdx.x * kR + rg; row < P.n; row += (int64_t)gridDim.x * kR) {
+    const T* xr = static_cast<const T*>(P.x) + row * P.ldx;
+    const T* gr = static_cast<const T*>(P.gy) + row * P.ldgy;
+    const float2 st = *reinterpret_cast<const float2*>(P.stats + 2 * row);
+    float xh[E], gy[E], s[2] = {0.f, 0.f};
+    each_vec<V, kL, NV>(l, w, [&](int k, int c, bool in) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) xh[k * V + e] = gy[k * V + e] = 0.f;
+      if (in) {
+        load_row<T, V>(xr + c, xh + k * V);
+        load_row<T, V>(gr + c, gy + k * V);
+      }
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        float& h = xh[k * V + e];
+        h = in ? (h - st.x) * st.y : 0.f;
+        const float u = gy[k * V + e] * g[k * V + e];
+        ag[k * V + e] = fmaf(gy[k * V + e], h, ag[k * V + e]);
+        ab[k * V + e] += gy[k * V + e];
+        s[0] += u;
+        s[1] = fmaf(u, h, s[1]);
+      }
+    });
+    group_sum<kL, 2>(s, red, turn);
+    const float m1 = s[0] * inv, m2 = s[1] * inv;
+    T* o = static_cast<T*>(P.gx) + row * w;
+    each_vec<V, kL, NV>(l, w, [&](int k, int c, bool in) {
+      float v[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[e] = st.y * (gy[k * V + e] * g[k * V + e] - m1 - xh[k * V + e] * m2);
+      if (in) store_row<T, V>(v, o + c);
+    });
+  }
+  if (P.part) {
+    write_part<V, kL, NV>(ag, l, rg, w, P.part + (int64_t)blockIdx.x * w);
+    write_part<V, kL, NV>(ab, l, rg, w, P.part + ((int64_t)gridDim.x + blockIdx.x) * w);
+  }
+}
+
+template <typename T, int V, int kL, int NV>
+__global__ __launch_bounds__(kL > 64 ? kL : 256) void k_layer_norm_bwd2(LnArgs P) {
+  constexpr int kR = kL > 64 ? 1 : 256 / kL, E = NV * V;
+  __shared__ float red[2][4][16];
+  const int l = threadIdx.x % kL, rg = threadIdx.x / kL, w = P.w;
+  const float inv = 1.0f / (float)w;
+  float g[E], qg[E], qb[E], ag[E];
+  load_params<V, kL, NV>(P.g, P.g_type, l, w, 1.f, g);
+  load_params<V, kL, NV>(P.qg, P.g_type, l, w, 0.f, qg);
+  load_params<V, kL, NV>(P.qb, P.b_type, l, w, 0.f, qb);
+#pragma unroll
+  for (int e = 0; e < E; ++e) ag[e] = 0.f;
+  int turn = 0;
+  for (int64_t row = (int64_t)blockIdx.x * kR + rg; row < P.n; row += (int64_t)gridDim.x * kR) {
+    const T* xr = static_cast<const T*>(P.x) + row * P.ldx;
+    const T* gr = static_cast<const T*>(P.gy) + row * P.ldgy;
+    const T* qr = static_cast<const T*>(P.qx) + row * P.ldq;
+    const float2 st = *reinterpret_cast<const float2*>(P.stats + 2 * row);
+    const float r = st.y;
+    float xh[E], gy[E], q[E];
+    float s[4] = {0.f, 0.f, 0.f, 0.f}, squ[1] = {0.f};
+    each_vec<V, kL, NV>(l, w, [&](int k, int c, bool in) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) xh[k * V + e] = gy[k * V + e] = q[k * V + e] = 0.f;
+      if (in) {
+        load_row<T, V>(xr + c, xh + k * V);
+        load_row<T, V>(gr + c, gy + k * V);
+        if (P.qx) load_row<T, V>(qr + c, q + k * V);
+      }
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        float& h = xh[k * V + e];
+        h = in ? (h - st.x) * r : 0.f;
+        const float u = gy[k * V + e] * g[k * V + e], v = q[k * V + e];
+        s[0] += u;
+        s[1] = fmaf(u, h, s[1]);
+        s[2] += v;
+        s[3] = fmaf(v, h, s[3]);
+        squ[0] = fmaf(v, u, squ[0]);
+      }
+    });
+    group_sum<kL, 4>(s, red, turn);
+    group_sum<kL, 1>(squ, red, turn);
+    const float ub = s[0] * inv, c_ = s[1] * inv, qm = s[2] * inv, m = s[3] * inv;
+    const float rr = r * r * (squ[0] * inv - qm * ub - c_ * m);      // r <qx gx>
+    float t[2] = {0.f, 0.f};
+    T* o1 = static_cast<T*>(P.y) + row * w;
+    each_vec<V, kL, NV>(l, w, [&](int k, int c, bool in) {
+      float v[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const int i = k * V + e;
+        const float a = in ? r * (q[i] - qm - xh[i] * m) : 0.f;
+        v[e] = g[i] * a + qg[i] * xh[i] + qb[i];
+        ag[i] = fmaf(gy[i], a, ag[i]);
+        const float x = qg[i] * gy[i] - r * (c_ * q[i] + m * gy[i] * g[i]);
+        q[i] = x;
+        t[0] += x;
+        t[1] = fmaf(x, xh[i], t[1]);
+      }
+      if (in) store_row<T, V>(v, o1 + c);
+    });
+    group_sum<kL, 2>(t, red, turn);
+    const float mx = t[0] * inv, mxx = t[1] * inv;
+    T* o2 = static_cast<T*>(P.gx) + row * w;
+    each_vec<V, kL, NV>(l, w, [&](int k, int c, bool in) {
+      float v[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[e] = r * (q[k * V + e] - mx - xh[k * V + e] * mxx) - rr * xh[k * V + e];
+      if (in) store_row<T, V>(v, o2 + c);
+    });
+  }
+  if (P.part) write_part<V, kL, NV>(ag, l, rg, w, P.part + (int64_t)blockIdx.x * w);
+}
+
+// out_a[c] = the sum over the n_part rows of part [a][n_part][w], a = blockIdx.y: 32 lanes take every 32nd row, then
+// a tree; rounded once to the parameter's type.
+__global__ __launch_bounds__(1024) void k_layer_norm_params(const float* __restrict__ part, int n_part, int w,
+                                                            void* out0, int type0, void* out1, int type1) {
+  __shared__ float red[32][33];
+  const int c = blockIdx.x * 32 + (threadIdx.x & 31), r = threadIdx.x >> 5;
+  const float* p = part + (int64_t)blockIdx.y * n_part * w;
+  float s = 0.f;
+  if (c < w) {
+#pragma unroll 8
+    for (int i = r; i < n_part; i += 32) s += p[(int64_t)i * w + c];
+  }
+  red[r][threadIdx.x & 31] = s;
+  __syncthreads();
+  if (r == 0 && c < w) {
+    s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) s += red[i][threadIdx.x];
+    void* out = blockIdx.y ? out1 : out0;
+    const int type = blockIdx.y ? type1 : type0;
+    if (!out) return;
+    if (type == E2V2_F32) static_cast<float*>(out)[c] = s;
+    else if (type == E2V2_BF16) static_cast<__bf16*>(out)[c] = (__bf16)s;
+    else static_cast<_Float16*>(out)[c] = (_Float16)s;
+  }
+}
+
+enum class LnPass { kFwd, kBwd, kBwd2 };
+
+template <LnPass kPass, typename T, int V, int kL, int NV>
+void ln_launch(const LnArgs& P, unsigned grid, hipStream_t s) {
+  const dim3 block(kL > 64 ? kL : 256);
+  if constexpr (kPass == LnPass::kFwd)
+    hipLaunchKernelGGL((k_layer_norm_fwd<T, V, kL, NV>), dim3(grid), block, 0, s, P);
+  else if constexpr (kPass == LnPass::kBwd)
+    hipLaunchKernelGGL((k_layer_norm_bwd<T, V, kL, NV>), dim3(grid), block, 0, s, P);
+  else
+    hipLaunchKernelGGL((k_layer_norm_bwd2<T, V, kL, NV>), dim3(grid), block, 0, s, P);
+}
+
+// Rows in flight in a workgroup for a width in vectors of v elements.
+int ln_rows_per_wg(int w, int v) {
+  const int nv = (w + v - 1) / v, most = kLnElems / v;
+  return nv <= 16 ? 16 : nv <= 32 ? 8 : nv <= 64 * most ? 4 : 1;
+}
+
+template <LnPass kPass, typename T, int V>
+void ln_dispatch(const LnArgs& P, unsigned grid, hipStream_t s) {
+  constexpr int M = kLnElems / V;                 // vectors a lane can hold
+  const int nv = (P.w + V - 1) / V;
+  if (nv <= 16) return ln_launch<kPass, T, V, 16, 1>(P, grid, s);
+  if (nv <= 32) return ln_launch<kPass, T, V, 32, 1>(P, grid, s);
+  if (nv <= 64) return ln_launch<kPass, T, V, 64, 1>(P, grid, s);
+  if (nv <= 128) return ln_launch<kPass, T, V, 64, 2>(P, grid, s);
+  if constexpr (M >= 4) {
+    if (nv <= 256) return ln_launch<kPass, T, V, 64, 4>(P, grid, s);
+  }
+  if constexpr (M >= 16) {
+    if (nv <= 512) return ln_launch<kPass, T, V, 64, 8>(P, grid, s);
+    if (nv <= 1024) return ln_launch<kPass, T, V, 64, 16>(P, grid, s);
+    if (nv <= 2048) return ln_launch<kPass, T, V, 256, 8>(P, grid, s);
+  }
+  if (nv <= 256 * M) return ln_launch<kPass, T, V, 256, M>(P, grid, s);
+  if constexpr (M >= 16) {
+    if (nv <= 1024 * 8) return ln_launch<kPass, T, V, 1024, 8>(P, grid, s);
+  }
+  return ln_launch<kPass, T, V, 1024, M>(P, grid, s);
+}
+
+int type_size(int t) { return t == E2V2_F32 ? 4 : 2; }
+bool type_ok(int t) { return t == E2V2_F32 || t == E2V2_BF16 || t == E2V2_F16; }
+
+// Elements of a 16-byte vector if every row of every operand lies on 16-byte boundaries, else 1.
+int ln_vec(const LnArgs& P, int type) {
+  const int v = 16 / type_size(type);
+  const uintptr_t a = (uintptr_t)P.x | (uintptr_t)P.gy | (uintptr_t)P.qx | (uintptr_t)P.y | (uintptr_t)P.gx;
+  return a % 16 == 0 && P.w % v == 0 && P.ldx % v == 0 && P.ldgy % v == 0 && P.ldq % v == 0 ? v : 1;
+}
+
+template <LnPass kPass>
+void ln_run(const LnArgs& P, int type, unsigned grid, hipStream_t s) {
+  const int v = ln_vec(P, type);
+  if (type == E2V2_F32)
+    v > 1 ? ln_dispatch<kPass, float, 4>(P, grid, s) : ln_dispatch<kPass, float, 1>(P, grid, s);
+  else if (type == E2V2_BF16)
+    v > 1 ? ln_dispatch<kPass, __bf16, 8>(P, grid, s) : ln_dispatch<kPass, __bf16, 1>(P, grid, s);
+  else
+    v > 1 ? ln_dispatch<kPass, _Float16, 8>(P, grid, s) : ln_dispatch<kPass, _Float16, 1>(P, grid, s);
+}
+
+unsigned ln_grid(const LnArgs& P, int type, int64_t most) {
+  const int r = ln_rows_per_wg(P.w, ln_vec(P, type));
+  return (unsigned)std::min<int64_t>((P.n + r - 1) / r, most);
+}
+
+int ln_check(const char* what, const e2v2_layer_norm_args* a, bool bwd, bool bwd2) {
+  E2V2_REQUIRE(a, "%s: null arguments", what);
+  E2V2_REQUIRE(a->n >= 0 && a->w > 0 && a->w <= kLnMaxWidth, "%s: %lld rows of width %d (1 to %d)", what,
+               (long long)a->n, a->w, kLnMaxWidth);
+  E2V2_REQUIRE(type_ok(a->type) && type_ok(a->g_type) && type_ok(a->b_type), "%s: types %d, %d, %d", what, a->type,
+               a->g_type, a->b_type);
+  E2V2_REQUIRE(a->ldx >= 0 && a->ldgy >= 0 && a->ldqx >= 0, "%s: negative row stride", what);
+  const uintptr_t mask = type_size(a->type) - 1;
+  E2V2_REQUIRE((((uintptr_t)a->x | (uintptr_t)a->gy | (uintptr_t)a->qx | (uintptr_t)a->y | (uintptr_t)a->gx) & mask) == 0 &&
+                   ((uintptr_t)a->stats & 7) == 0,
+               "%s: misaligned operand", what);
+  if (a->n == 0) return 0;
+  E2V2_REQUIRE(a->x && (bwd || a->y) && (!bwd || (a->gy && a->stats && a->gx)) && (!bwd2 || a->y),
+               "%s: null operand", what);
+  return 0;
+}
+
+LnArgs ln_args(const e2v2_layer_norm_args* a) {
+  return LnArgs{a->x, a->gy, a->qx, a->g, a->b, a->qg, a->qb, a->y, a->gx, a->stats, nullptr, a->n, a->ldx, a->ldgy,
+                a->ldqx, a->w, a->g_type, a->b_type, a->eps};
+}
+
+int ln_params(const float* part, int n_part, int w, int arrays, void* o0, int t0, void* o1, int t1, hipStream_t s) {
+  hipLaunchKernelGGL(k_layer_norm_params, dim3((w + 31) / 32, arrays), dim3(1024), 0, s, part, n_part, w, o0, t0, o1,
+                     t1);
+  E2V2_LAUNCHED("k_layer_norm_params");
+  return 0;
+}
+
+}  // namespace
+}  // namespace e2v2
+
+using namespace e2v2;
+
+E2V2_API int e2v2_layer_norm_fwd(const e2v2_layer_norm_args* a, hipStream_t s) {
+  if (const int rc = ln_check("layer_norm_fwd", a, false, false)) return rc;
+  if (a->n == 0) return 0;
+  LnArgs P = ln_args(a);
+  P.gy = P.qx = P.gx = nullptr;
+  P.ldgy = P.ldq = 0;
+  ln_run<LnPass::kFwd>(P, a->type, ln_grid(P, a->type, 1 << 20), s);
+  E2V2_LAUNCHED("k_layer_norm_fwd");
+  return 0;
+}
+
+E2V2_API int64_t e2v2_layer_norm_workspace(int64_t n, int w) {
+  if (n <= 0 || w <= 0) return 0;
+  return 2 * std::min<int64_t>(n, kLnMaxParts) * w * 4;
+}
+
+E2V2_API int e2v2_layer_norm_bwd(const e2v2_layer_norm_args* a, void* gg, void* gb, float* ws, int64_t ws_bytes,
+                                 hipStream_t s) {
+  if (const int rc = ln_check("layer_norm_bwd", a, true, false)) return rc;
+  const bool params = gg || gb;
+  E2V2_REQUIRE(!params || (ws_bytes >= e2v2_layer_norm_workspace(a->n, a->w) && (ws || a->n == 0)),
+               "layer_norm_bwd: workspace of %lld bytes", (long long)ws_bytes);
+  LnArgs P = ln_args(a);
+  P.qx = P.y = nullptr;
+  P.ldq = 0;
+  P.part = params ? ws : nullptr;
+  const unsigned grid = ln_grid(P, a->type, params ? kLnMaxParts : 1 << 20);
+  if (grid) {
+    ln_run<LnPass::kBwd>(P, a->type, grid, s);
+    E2V2_LAUNCHED("k_layer_norm_bwd");
+  }
+  return params ? ln_params(ws, (int)grid, a->w, 2, gg, a->g_type, gb, a->b_type, s) : 0;
+}
+
+E2V2_API int e2v2_layer_norm_bwd2(const e2v2_layer_norm_args* a, void* gg, float* ws, int64_t ws_bytes,
+                                  hipStream_t s) {
+  if (const int rc = ln_check("layer_norm_bwd2", a, true, true)) return rc;
+  E2V2_REQUIRE(!gg || (ws_bytes >= e2v2_layer_norm_workspace(a->n, a->w) && (ws || a->n == 0)),
+               "layer_norm_bwd2: workspace of %lld bytes", (long long)ws_bytes);
+  LnArgs P = ln_args(a);
+  P.part = gg ? ws : nullptr;
+  const unsigned grid = ln_grid(P, a->type, gg ? kLnMaxParts : 1 << 20);
+  if (grid) {
+    ln_run<LnPass::kBwd2>(P, a->type, grid, s);
+    E2V2_LAUNCHED("k_layer_norm_bwd2");
+  }
+  return gg ? ln_params(ws, (int)grid, a->w, 1, gg, a->g_type, nullptr, 0, s) : 0;
+}

@@ -1,0 +1,158 @@
+"""Layer norm of rows (the reference's nn.LayerNorm, module_utils.py:2151-2178, 2230-2233) as HIP kernels of
+libe2v2.so: any width up to 16384, fp32, bf16 or fp16 rows, weight and bias in the rows' type or fp32 or absent,
+with the gradients of rows, weight and bias and the derivative of that backward pass (force training differentiates
+the forces once more).  Statistics, row sums and the parameters' sums are fp32; each result is rounded once.
+
+The equivariant RMS norm is in ``modules`` / ``second_order``, the fused LayerNorm + SiLU of the radial profiles in
+``second_order.ln_silu``.  There is no CPU path."""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+
+MAX_WIDTH = 16384
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _ptr(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+def _rows(t: torch.Tensor):
+    """(t as the kernels read it, its row stride): consecutive elements in a row, rows one stride apart, on the
+    boundaries of the element type; a copy where t does not lie so."""
+    if t.stride(-1) == 1 or t.shape[-1] == 1:
+        ld = None
+        for size, stride in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+            if size == 1:
+                continue
+            if ld is None:
+                ld, span = stride, size * stride
+            elif stride == span:
+                span = size * stride
+            else:
+                break
+        else:
+            return t, t.shape[-1] if ld is None else ld
+    return t.contiguous(), t.shape[-1]
+
+
+def _will_run(node) -> bool:
+    """Whether the running backward needs the gradient flowing into node (False
+    only when the engine reports that it will not execute it: autograd.grad of
+    other inputs, as the forces' first differentiation)."""
+    if node is None:
+        return False
+    try:
+        return bool(torch._C._will_engine_execute_node(node))
+    except (AttributeError, RuntimeError):
+        return True
+
+
+def _args(x, g, b, stats, eps, gy=None, qx=None, qg=None, qb=None, y=None, gx=None):
+    """The kernels' arguments, and the copies that have to live until the call is enqueued."""
+    w = x.shape[-1]
+    keep, ld = [], []
+    for t in (x, gy, qx):
+        u, s = (None, 0) if t is None else _rows(t)
+        keep.append(u)
+        ld.append(s)
+    p = [None if t is None else t.contiguous() for t in (g, b, qg, qb)]
+    gt, bt = (_TYPES[torch.float32 if t is None else t.dtype] for t in (g, b))
+    a = _lib.LayerNormArgs(*map(_ptr, keep), *map(_ptr, p), _ptr(y), _ptr(gx), _ptr(stats), x.numel() // w, *ld, w,
+                           _TYPES[x.dtype], gt, bt, eps)
+    return a, keep + p
+
+
+def _workspace(x):
+    n = int(_lib.load().e2v2_layer_norm_workspace(x.numel() // x.shape[-1], x.shape[-1]))
+    return torch.empty(n // 4, dtype=torch.float32, device=x.device), n
+
+
+def _call(name, dev, *args):
+    with torch.cuda.device(dev):
+        _lib.call(name, *args, _lib.stream(dev))
+
+
+class _LayerNormFn(torch.autograd.Function):
+
+    @staticmethod
+    def forward(ctx, x, g, b, eps: float):
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        stats = None
+        if any(ctx.needs_input_grad):
+            stats = torch.empty(x.numel() // x.shape[-1], 2, dtype=torch.float32, device=x.device)
+        a, keep = _args(x, g, b, stats, eps, y=y)
+        _call("e2v2_layer_norm_fwd", x.device, _lib.C.byref(a))
+        ctx.save_for_backward(x, g, b, stats)
+        ctx.eps = eps
+        return y
+
+    @staticmethod
+    def backward(ctx, gy):
+        x, g, b, stats = ctx.saved_tensors
+        # next_functions has an entry for each tensor among the inputs
+        nodes = iter(ctx.next_functions[1:])
+        nodes = [None if t is None else next(nodes)[0] for t in (g, b)]
+        need = [ctx.needs_input_grad[k + 1] and _will_run(nodes[k]) for k in range(2)]
+        gx, gg, gb = _LayerNormGradFn.apply(gy, x, g, b, stats, ctx.eps, *need)
+        return gx if ctx.needs_input_grad[0] else None, gg, gb, None
+
+
+class _LayerNormGradFn(torch.autograd.Function):
+    """(gx, dg, db) of _LayerNormFn given gy; mean and rstd enter as constants, the second-order pass
+    differentiates through them by its formulas."""
+
+    @staticmethod
+    def forward(ctx, gy, x, g, b, stats, eps, need_g, need_b):
+        gx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        gg = torch.empty_like(g, memory_format=torch.contiguous_format) if need_g else None
+        gb = torch.empty_like(b, memory_format=torch.contiguous_format) if need_b else None
+        ws, n = _workspace(x) if need_g or need_b else (None, 0)
+        a, keep = _args(x, g, b, stats, eps, gy=gy, gx=gx)
+        _call("e2v2_layer_norm_bwd", x.device, _lib.C.byref(a), _lib.vp(_ptr(gg)), _lib.vp(_ptr(gb)),
+              _lib.vp(_ptr(ws)), _lib.i64(n))
+        ctx.save_for_backward(gy, x, g, b, stats)
+        ctx.eps = eps
+        ctx.set_materialize_grads(False)
+        return gx, gg, gb
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, qx, qg, qb):
+        gy, x, g, b, stats = ctx.saved_tensors
+        if qx is None and qg is None and qb is None:
+            return (None,) * 8
+        dgy, dx = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for _ in range(2))
+        dg = torch.empty_like(g, memory_format=torch.contiguous_format) if ctx.needs_input_grad[2] else None
+        ws, n = _workspace(x) if dg is not None else (None, 0)
+        a, keep = _args(x, g, b, stats, ctx.eps, gy=gy, qx=qx, qg=qg, qb=qb, y=dgy, gx=dx)
+        _call("e2v2_layer_norm_bwd2", x.device, _lib.C.byref(a), _lib.vp(_ptr(dg)), _lib.vp(_ptr(ws)), _lib.i64(n))
+        return dgy, dx, dg, None, None, None, None, None
+
+
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+               eps: float = 1e-5) -> torch.Tensor:
+    """(x - mean) / sqrt(var + eps) * weight + bias over the last dimension of x, as
+    torch.nn.functional.layer_norm(x, (w,), weight, bias, eps).
+
+    x: fp32, bf16 or fp16 on the GPU, of any shape with a last dimension of 1 to 16384; read where it lies if its rows
+    are consecutive and evenly spaced.  weight, bias: [w], fp32 or x's type, or None.  The result has x's type
+    and is contiguous.  Differentiable twice (a third derivative raises)."""
+    if not isinstance(x, torch.Tensor) or not x.is_cuda:
+        raise RuntimeError("layer_norm runs on the GPU only (HIP library, no CPU path): got "
+                           f"{x.device if isinstance(x, torch.Tensor) else type(x).__name__}")
+    if x.dtype not in _TYPES or x.dim() == 0:
+        raise ValueError(f"layer_norm: rows in fp32, bf16 or fp16, got {tuple(x.shape)} {x.dtype}")
+    w = x.shape[-1]
+    if not 1 <= w <= MAX_WIDTH:
+        raise ValueError(f"layer_norm: width {w} (1 to {MAX_WIDTH})")
+    for name, p in (("weight", weight), ("bias", bias)):
+        if p is not None and (p.shape != (w,) or p.dtype not in (torch.float32, x.dtype) or p.device != x.device):
+            raise ValueError(f"layer_norm: {name} [{w}] in fp32 or {x.dtype} on {x.device}, got {tuple(p.shape)} "
+                             f"{p.dtype} on {p.device}")
+    return _LayerNormFn.apply(x, weight, bias, float(eps))

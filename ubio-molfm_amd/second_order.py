@@ -38,6 +38,7 @@ import torch.nn.functional as F
 from . import _lib
 from . import so3
 from . import sparse_ops
+from .norms import MAX_WIDTH as _LN_MAX_WIDTH, _will_run, layer_norm
 from .ops import ENV_A, ENV_B, ENV_C
 
 _EXPAND = {}
@@ -147,18 +148,6 @@ class _LNSiLUGradFn(torch.autograd.Function):
 _EDGE_ROWS = 16384   # rows from which a Linear takes the split-K weight gradient
 
 
-def _will_run(node) -> bool:
-    """Whether the running backward needs the gradient flowing into node (False
-    only when the engine reports that it will not execute it: autograd.grad of
-    other inputs, as the forces' first differentiation)."""
-    if node is None:
-        return False
-    try:
-        return bool(torch._C._will_engine_execute_node(node))
-    except (AttributeError, RuntimeError):
-        return True
-
-
 def _splitk_tn(a: torch.Tensor, b: torch.Tensor) -> torch.Tensor:
     """a^T b for a [E, m], b [E, n] with E >> m, n: s batched partial products
     over row blocks, summed (one GEMM with K = E leaves most of the chip idle)."""
@@ -237,10 +226,17 @@ def ln_silu(ln: nn.LayerNorm, x: torch.Tensor) -> torch.Tensor:
     return y.view(x.shape)
 
 
+def _layer_norm_takes(ln: nn.LayerNorm, x: torch.Tensor) -> bool:
+    """Whether norms.layer_norm computes ln(x): fp32 rows on the GPU, normalised over their last dimension."""
+    w = x.shape[-1]
+    return (x.is_cuda and x.dtype == torch.float32 and tuple(ln.normalized_shape) == (w,) and w <= _LN_MAX_WIDTH
+            and all(p is None or (p.is_cuda and p.dtype == torch.float32) for p in (ln.weight, ln.bias)))
+
+
 def run_seq(mods, h: torch.Tensor) -> torch.Tensor:
     """nn.Sequential over mods with each nn.LayerNorm + nn.SiLU pair as ln_silu (where
-    ln_silu_fusable; other widths run the two modules) and each nn.Linear on at
-    least _EDGE_ROWS rows as edge_linear."""
+    ln_silu_fusable), every other nn.LayerNorm on GPU rows as norms.layer_norm and
+    each nn.Linear on at least _EDGE_ROWS rows as edge_linear."""
     mods = list(mods) if isinstance(mods, (nn.Sequential, list, tuple)) else [mods]
     i = 0
     while i < len(mods):
@@ -248,6 +244,9 @@ def run_seq(mods, h: torch.Tensor) -> torch.Tensor:
                 and ln_silu_fusable(mods[i], h)):
             h = ln_silu(mods[i], h)
             i += 2
+        elif isinstance(mods[i], nn.LayerNorm) and _layer_norm_takes(mods[i], h):
+            h = layer_norm(h, mods[i].weight, mods[i].bias, mods[i].eps)
+            i += 1
         elif isinstance(mods[i], nn.Linear) and h.dim() == 2 and h.shape[0] >= _EDGE_ROWS:
             h = edge_linear(mods[i], h)
             i += 1
