@@ -349,7 +349,7 @@ def train_line(args, dev):
     one Adam step; positions fixed, the neighbour list rebuilt inside every forward as in training."""
     import numpy as np
     import torch
-    from ubio_molfm_amd import model, neighbors, systems
+    from ubio_molfm_amd import model, neighbors, optim, systems
     torch.manual_seed(0)
     margs = model.default_args()
     margs.backbone_config.update(tp_type=args.tp_type, with_cluster=args.with_cluster)
@@ -361,7 +361,7 @@ def train_line(args, dev):
     nl = neighbors.build_neighbors(torch.as_tensor(sysd["pos"], device=dev), sysd["graph_ptr"], sysd["cell"],
                                    sysd["pbc"], 6.0)
     E = nl.n_edges
-    opt = torch.optim.Adam(m.parameters(), lr=1e-5)
+    opt = optim.AdamW(m.parameters(), lr=1e-5, weight_decay=0.0)
 
     def step():
         b = dict(bd)

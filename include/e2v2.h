@@ -626,6 +626,54 @@ int e2v2_layer_norm_bwd(const e2v2_layer_norm_args* args, void* gg, void* gb, fl
 int e2v2_layer_norm_bwd2(const e2v2_layer_norm_args* args, void* gg, float* workspace, int64_t workspace_bytes,
                          hipStream_t s);
 
+/* ---- the parameter update of training, over many tensors at once ----
+ * No counterpart in the reference's own code: its trainer calls torch's clipping and optimizer
+ * (src/molfm/pipeline/trainer.py:114-662).  Tensors are contiguous fp32, bf16 or fp16; `grads` and `numel` are host arrays,
+ * a NULL gradient leaves its tensor out.
+ *   grad_norm        partial sums of the squares in fp64; *n_parts (host) partial sums are there before the call and
+ *                    grow by what it adds, so that several lists join; grad_norm_parts: the most that one list adds.
+ *   grad_norm_value  norm = the root of the partial sums' sum.
+ *   grad_scale       every gradient times min(1, max_norm / (norm + 1e-6)); norm written unless NULL.
+ *   adamw            one step (decoupled weight decay) of the tensors whose chunks the table lists, the gradients scaled
+ *                    as by grad_scale where n_parts > 0 (max_norm infinite: not scaled).  skip_nonfinite: a norm that
+ *                    is not finite leaves everything as it was and adds 1 to *skipped.  steps[chunk] counts the
+ *                    steps taken.  Moments: fp32, or codes of 8 bits (bits = 8) with a scale byte for each run of 32 elements
+ *                    in ms and vs (csrc/optim.hip); an element's place `off + i` in them counts from the chunk's off,
+ *                    a multiple of 64, and the run that a tensor ends in is padded with zeros.
+ *   moments          the values of n codes (a multiple of 32) in fp32, bf16 or fp16. */
+#define E2V2_OPT_CHUNK 4096
+typedef struct {
+  void* p;              /* the parameter */
+  int64_t at;           /* the chunk's first element in it, a multiple of E2V2_OPT_CHUNK */
+  int64_t off;          /* that element's place in the moments */
+  int32_t n;            /* elements, at most E2V2_OPT_CHUNK */
+  int32_t tensor;
+} e2v2_opt_chunk;
+typedef struct {
+  const e2v2_opt_chunk* chunks;   /* device */
+  int32_t* steps;                 /* device, [n_chunks] */
+  void* const* grads;             /* host, [n_tensors]: gradients of tensors first_tensor .. */
+  void* m; void* v;
+  uint8_t* ms; uint8_t* vs;
+  const float* lr_dev;            /* device learning rate, or NULL: lr */
+  const double* parts;
+  float* norm;                    /* device, written unless NULL where n_parts > 0 */
+  int32_t* skipped;               /* device */
+  double lr, beta1, beta2, eps, weight_decay;
+  float max_norm;
+  int32_t n_chunks, n_tensors, first_tensor, type, bits, n_parts, skip_nonfinite;
+  uint32_t seed;
+} e2v2_adamw_args;
+int e2v2_grad_norm_parts(const int64_t* numel, int n);
+int e2v2_grad_norm(void* const* grads, const int64_t* numel, int n, int type, double* parts, int capacity,
+                   int* n_parts, hipStream_t s);
+int e2v2_grad_norm_value(const double* parts, int n_parts, float* norm, hipStream_t s);
+int e2v2_grad_scale(void* const* grads, const int64_t* numel, int n, int type, const double* parts, int n_parts,
+                    float max_norm, float* norm, hipStream_t s);
+int e2v2_adamw(const e2v2_adamw_args* args, hipStream_t s);
+int e2v2_moments(const uint8_t* mc, const uint8_t* ms, const uint8_t* vc, const uint8_t* vs, void* m, void* v, int type,
+                 int64_t n, hipStream_t s);
+
 /* ---- per-node dense layers: fp32 GEMMs on bf16 MFMA by the exact three-piece split ----
  * Replaces the GEMMs (forward and input gradient) of SO3_Linear_e2former (module_utils.py:2010-2052) and so of
  * FeedForwardNetwork_s3 (module_utils.py:2755-2797), the value projection and proj_first (e2former.py:215-219,

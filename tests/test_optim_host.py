@@ -1,0 +1,89 @@
+"""What optim refuses and checks without a GPU, and the entry points' checks of their arguments."""
+import pytest
+import torch
+
+from ubio_molfm_amd import _lib, optim
+
+
+@pytest.fixture(autouse=True)
+def _no_kernels(monkeypatch):
+    monkeypatch.setattr(_lib, "call", lambda *a: pytest.fail("a kernel was called"))
+
+
+def _p(*shape):
+    p = torch.zeros(shape, requires_grad=True)
+    p.grad = torch.ones(shape)
+    return p
+
+
+@pytest.mark.parametrize("kw,match", [
+    (dict(lr=-1.0), "lr"), (dict(lr=float("nan")), "lr"), (dict(lr=torch.zeros(2)), "lr"), (dict(betas=(1.0, 0.9)), "betas"),
+    (dict(betas=(0.9, -0.1)), "betas"), (dict(eps=-1e-8), "eps"), (dict(weight_decay=-0.1), "weight_decay"),
+    (dict(state_bits=16), "16 bits"), (dict(max_norm=0.0), "max_norm"), (dict(max_norm=float("nan")), "max_norm")])
+def test_constructor_refuses(kw, match):
+    with pytest.raises(ValueError, match=match):
+        optim.AdamW([_p(3)], **kw)
+
+
+def test_group_values_are_checked():
+    opt = optim.AdamW([_p(3)])
+    with pytest.raises(ValueError, match="lr"):
+        opt.add_param_group(dict(params=[_p(4)], lr=-2.0))
+    assert len(opt.param_groups) == 1
+
+
+def test_host_tensors_are_refused():
+    for call in (lambda: optim.AdamW([_p(3)]).step(), lambda: optim.AdamW([_p(3)]).moments(),
+                 lambda: optim.clip_grad_norm_([_p(3)], 1.0), lambda: optim.grad_norm([torch.ones(3)]),
+                 lambda: optim.grad_norm(torch.ones(3))):
+        with pytest.raises(RuntimeError, match="GPU only"):
+            call()
+    with pytest.raises(ValueError, match="max_norm"):
+        optim.clip_grad_norm_([_p(3)], -1.0)
+
+
+def test_entry_point_checks():
+    lib, C = _lib.load(), _lib.C
+    ptrs, numel = (_lib.vp * 2)(64, 128), (_lib.i64 * 2)(5, 1 << 33)
+    assert lib.e2v2_grad_norm_parts(numel, 2) == 512 and lib.e2v2_grad_norm_parts(numel, 0) == 0
+    many = (_lib.i64 * 600)(*([7] * 600))
+    assert lib.e2v2_grad_norm_parts(many, 600) == 3 * 512
+    count = C.c_int(0)
+
+    def norm(n=2, type=0, parts=64, cap=0):
+        return lib.e2v2_grad_norm(ptrs, numel, n, type, _lib.vp(parts), cap, C.byref(count), None)
+
+    assert norm(n=-1) != 0 and b"-1 tensors" in lib.e2v2_last_error()
+    assert norm(type=5) != 0 and b"type 5" in lib.e2v2_last_error()
+    assert norm(parts=None) != 0 and b"null operand" in lib.e2v2_last_error()
+    assert norm() != 0 and b"room for 0" in lib.e2v2_last_error() and count.value == 0
+    ptrs[1] = 66
+    assert norm() != 0 and b"tensor 1" in lib.e2v2_last_error()
+    ptrs[1], numel[0] = 128, -1
+    assert norm() != 0 and b"tensor 0 of -1" in lib.e2v2_last_error()
+    assert lib.e2v2_grad_scale(ptrs, numel, 2, 0, None, 0, _lib.f32(1), None, None) != 0
+    assert lib.e2v2_grad_norm_value(None, 1, _lib.vp(64), None) != 0
+    a = _lib.AdamWArgs()
+    a.n_chunks, a.n_tensors, a.bits = 1, 1, 32
+    a.chunks = a.steps = a.grads = a.m = a.v = C.addressof(ptrs)
+    a.m = a.v = 64
+    a.beta1 = a.beta2 = 0.9
+    ptrs[0] = 64
+    for change, match in ((dict(n_tensors=385), b"385"), (dict(n_chunks=-1), b"-1 chunks"), (dict(bits=4), b"4 bits"),
+                          (dict(type=3), b"type 3"), (dict(bits=8), b"null operand"), (dict(m=None), b"null operand"),
+                          (dict(m=72), b"16-byte"), (dict(n_parts=2), b"null operand"),
+                          (dict(skip_nonfinite=1), b"null operand"), (dict(beta2=1.0), b"betas")):
+        b = _lib.AdamWArgs.from_buffer_copy(a)
+        for k, v in change.items():
+            setattr(b, k, v)
+        assert lib.e2v2_adamw(C.byref(b), None) != 0 and match in lib.e2v2_last_error(), change
+    ptrs[0] = 66
+    assert lib.e2v2_adamw(C.byref(a), None) != 0 and b"misaligned gradient 0" in lib.e2v2_last_error()
+    v = _lib.vp(64)
+    assert lib.e2v2_moments(v, v, v, v, v, v, 0, _lib.i64(33), None) != 0
+    assert lib.e2v2_moments(v, v, _lib.vp(68), v, v, v, 0, _lib.i64(32), None) != 0
+    assert lib.e2v2_moments(v, None, v, v, v, v, 0, _lib.i64(32), None) != 0
+
+
+def test_chunk_layout():
+    assert _lib.C.sizeof(_lib.OptChunk) == 32 and _lib.OptChunk.n.offset == 24

@@ -22,6 +22,7 @@ EXPORTS = [
     "e2v2_edge_to_pos", "e2v2_rmsnorm_fwd", "e2v2_add_rmsnorm_fwd", "e2v2_rmsnorm_bwd", "e2v2_rmsnorm_bwd_param", "e2v2_rmsnorm_bwd2", "e2v2_gate_fwd",
     "e2v2_gate_bwd", "e2v2_gate_bwd2", "e2v2_ln_silu_fwd", "e2v2_ln_silu_bwd", "e2v2_ln_silu_bwd_param", "e2v2_ln_silu_bwd2",
     "e2v2_layer_norm_fwd", "e2v2_layer_norm_workspace", "e2v2_layer_norm_bwd", "e2v2_layer_norm_bwd2",
+    "e2v2_grad_norm_parts", "e2v2_grad_norm", "e2v2_grad_norm_value", "e2v2_grad_scale", "e2v2_adamw", "e2v2_moments",
     "e2v2_pairdot_fwd", "e2v2_pairdot_bwd", "e2v2_qk_proj_fwd", "e2v2_qk_proj_bwd",
     "e2v2_qk_proj_fwd_bf16", "e2v2_qk_proj_bwd_bf16",
     "e2v2_segment_metadata", "e2v2_pair_count", "e2v2_pair_emit", "e2v2_seg_dot", "e2v2_seg_reduce",
@@ -109,6 +110,18 @@ class LayerNormArgs(C.Structure):
     _fields_ = [("x", vp), ("gy", vp), ("qx", vp), ("g", vp), ("b", vp), ("qg", vp), ("qb", vp), ("y", vp), ("gx", vp),
                 ("stats", vp), ("n", i64), ("ldx", i64), ("ldgy", i64), ("ldqx", i64), ("w", i32), ("type", i32),
                 ("g_type", i32), ("b_type", i32), ("eps", f32)]
+
+
+class OptChunk(C.Structure):
+    _fields_ = [("p", vp), ("at", i64), ("off", i64), ("n", i32), ("tensor", i32)]
+
+
+class AdamWArgs(C.Structure):
+    _fields_ = [("chunks", vp), ("steps", vp), ("grads", vp), ("m", vp), ("v", vp), ("ms", vp), ("vs", vp),
+                ("lr_dev", vp), ("parts", vp), ("norm", vp), ("skipped", vp), ("lr", C.c_double), ("beta1", C.c_double),
+                ("beta2", C.c_double), ("eps", C.c_double), ("weight_decay", C.c_double), ("max_norm", f32),
+                ("n_chunks", i32), ("n_tensors", i32), ("first_tensor", i32), ("type", i32), ("bits", i32),
+                ("n_parts", i32), ("skip_nonfinite", i32), ("seed", C.c_uint32)]
 
 
 class AttnLayer(C.Structure):

@@ -1,0 +1,411 @@
+"""The parameter update of training over many tensors at once (HIP kernels of libe2v2.so, csrc/optim.hip):
+``AdamW`` with moments in 32 or in 8 bits, ``clip_grad_norm_`` and ``grad_norm``.
+
+One launch updates all tensors of a parameter group (two with clipping: the norm's sums, then the update, which applies
+the clipping factor to each gradient as it reads it), whatever their number and sizes; nothing is read back to
+the host.  The reference's trainer calls torch's counterparts (src/molfm/pipeline/trainer.py:114-662).  There is no
+CPU path."""
+from __future__ import annotations
+
+import ctypes as C
+import math
+from itertools import chain
+from typing import Iterable, Optional, Tuple, Union
+
+import torch
+
+from . import _lib
+
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_CHUNK = 4096           # E2V2_OPT_CHUNK
+_LIST = 384             # tensors of one step launch
+_ALIGN = 64             # a tensor's moments start at a multiple of this many elements
+_RUN = 32               # elements that share a scale byte
+
+
+def _tensors(params) -> list:
+    """The gradients of parameters that have one."""
+    params = [params] if isinstance(params, torch.Tensor) else list(params)
+    return [p.grad for p in params if p.grad is not None]
+
+
+def _check(grads, what: str):
+    """One device, known types, dense; by type."""
+    by_type = {}
+    for g in grads:
+        if not g.is_cuda:
+            raise RuntimeError(f"{what} runs on the GPU only (HIP library, no CPU path): got a tensor on {g.device}")
+        if g.layout != torch.strided or g.dtype not in _TYPES:
+            raise ValueError(f"{what}: dense fp32, bf16 or fp16 tensors, got {g.dtype} {g.layout}")
+        if g.device != grads[0].device:
+            raise ValueError(f"{what}: tensors on {grads[0].device} and {g.device}")
+        by_type.setdefault(g.dtype, []).append(g)
+    return by_type
+
+
+class _Lists:
+    """The tensors of one type as the library takes them."""
+
+    def __init__(self, dtype, ptrs, numels):
+        self.n = len(ptrs)
+        self.type = _lib.i32(_TYPES[dtype])
+        self.ptrs = (_lib.vp * self.n)(*ptrs)
+        self.numel = (_lib.i64 * self.n)(*numels)
+
+    def parts(self) -> int:
+        return int(_lib.load().e2v2_grad_norm_parts(self.numel, _lib.i32(self.n)))
+
+    def norm(self, parts, count, st):
+        _lib.call("e2v2_grad_norm", self.ptrs, self.numel, _lib.i32(self.n), self.type, _lib.vp(parts.data_ptr()),
+                  _lib.i32(parts.numel()), C.byref(count), st)
+
+
+def _norm_parts(by_type, st):
+    lists = [_Lists(d, [g.data_ptr() for g in gs], [g.numel() for g in gs]) for d, gs in by_type.items()]
+    dev = next(iter(by_type.values()))[0].device
+    parts = torch.empty(max(1, sum(l.parts() for l in lists)), dtype=torch.float64, device=dev)
+    count = C.c_int(0)
+    for l in lists:
+        l.norm(parts, count, st)
+    return lists, parts, count
+
+
+def grad_norm(tensors: Iterable[torch.Tensor]) -> torch.Tensor:
+    """The 2-norm of all elements of the tensors (dense, fp32, bf16 or fp16, one device), as an fp32 tensor of one element on
+    that device; the squares are summed in fp64.  An empty list has norm 0 (on the current device)."""
+    ts = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+    if not ts:
+        return torch.zeros((), device="cuda")
+    by_type = {d: [t.contiguous() for t in v] for d, v in _check(ts, "grad_norm").items()}
+    dev = ts[0].device
+    out = torch.empty((), dtype=torch.float32, device=dev)
+    with torch.cuda.device(dev):
+        st = _lib.stream(dev)
+        _, parts, count = _norm_parts(by_type, st)
+        _lib.call("e2v2_grad_norm_value", _lib.vp(parts.data_ptr()), _lib.i32(count.value), _lib.vp(out.data_ptr()), st)
+    return out
+
+
+def clip_grad_norm_(parameters, max_norm: float) -> torch.Tensor:
+    """Scales the parameters' gradients in place by min(1, max_norm / (norm + 1e-6)), norm their global 2-norm, which is
+    returned (an fp32 tensor of one element), as torch.nn.utils.clip_grad_norm_.  A norm that is not finite scales by what
+    the quotient gives (0, or NaN); nothing is read back to the host."""
+    max_norm = float(max_norm)
+    if not max_norm >= 0:
+        raise ValueError(f"clip_grad_norm_: max_norm {max_norm}")
+    grads = _tensors(parameters)
+    if not grads:
+        return torch.zeros((), device="cuda" if torch.cuda.is_available() else None)
+    _check(grads, "clip_grad_norm_")
+    dense = [g.contiguous() for g in grads]
+    by_type = _check(dense, "clip_grad_norm_")
+    dev = grads[0].device
+    out = torch.zeros((), dtype=torch.float32, device=dev)
+    with torch.cuda.device(dev):
+        st = _lib.stream(dev)
+        lists, parts, count = _norm_parts(by_type, st)
+        for l in lists:
+            _lib.call("e2v2_grad_scale", l.ptrs, l.numel, _lib.i32(l.n), l.type, _lib.vp(parts.data_ptr()), count,
+                      _lib.f32(max_norm), _lib.vp(out.data_ptr()), st)
+    for g, d in zip(grads, dense):
+        if d is not g:
+            g.copy_(d)
+    torch.autograd.graph.increment_version(grads)
+    return out
+
+
+def _usable(p) -> bool:
+    return p.is_cuda and p.layout == torch.strided and p.dtype in _TYPES and p.is_contiguous()
+
+
+def _refuse(params):
+    """Parameters that a step cannot take: an error if one has a gradient."""
+    for p in params:
+        if p.grad is None:
+            continue
+        if not p.is_cuda:
+            raise RuntimeError(f"AdamW runs on the GPU only (HIP library, no CPU path): got a parameter on {p.device}")
+        raise ValueError("AdamW: contiguous parameters in fp32, bf16 or fp16, got "
+                         f"{tuple(p.shape)} {p.dtype} with strides {p.stride()}")
+
+
+class _Launch:
+    """One step launch: up to _LIST parameters of one group and type, and their chunks of the table."""
+
+    def __init__(self, group, dtype, params, first_tensor, chunk0, n_chunks):
+        self.group, self.dtype, self.params = group, dtype, params
+        self.first_tensor, self.chunk0, self.n_chunks = first_tensor, chunk0, n_chunks
+        self.grads = _Lists(dtype, [None] * len(params), [p.numel() for p in params])
+        self.args = _lib.AdamWArgs()
+
+
+class _Plan:
+    """What stays from step to step: moments and step counts of all parameters, the chunks' table, the launches."""
+
+    def __init__(self, opt: "AdamW"):
+        groups = opt.param_groups
+        every = [p for g in groups for p in g["params"]]
+        # the others may stand in the groups as long as they have no gradient (a model's constants)
+        params = [p for p in every if _usable(p)]
+        self.outside = [p for p in every if not _usable(p)]
+        _refuse(self.outside)
+        for p in params:
+            if p.device != params[0].device:
+                raise ValueError(f"AdamW: parameters on {params[0].device} and {p.device}")
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamW: the first step, and the one after a change of parameters or state, cannot be captured: "
+                               "take it before the capture")
+        self.device = dev = params[0].device if params else torch.device("cuda", torch.cuda.current_device())
+        self.ptrs = [p.data_ptr() for p in params]
+        self.params = params
+        bits = opt.state_bits
+        off, self.offs = 0, []
+        for p in params:
+            self.offs.append(off)
+            off += -(-p.numel() // _ALIGN) * _ALIGN
+        self.total = off
+        place = dict(zip(params, self.offs))
+        dt = torch.float32 if bits == 32 else torch.uint8
+        self.m, self.v = (torch.zeros(off, dtype=dt, device=dev) for _ in range(2))
+        self.ms, self.vs = ((torch.zeros(off // _RUN, dtype=torch.uint8, device=dev) for _ in range(2)) if bits == 8
+                            else (None, None))
+        table, first, self.launches, tensors = [], {}, [], 0
+        for group in groups:
+            by_type = {}
+            for p in group["params"]:
+                if p in place:
+                    by_type.setdefault(p.dtype, []).append(p)
+            for dtype, ps in by_type.items():
+                for k in range(0, len(ps), _LIST):
+                    part, chunk0 = ps[k:k + _LIST], len(table)
+                    for j, p in enumerate(part):
+                        first[p] = len(table)
+                        table += [(p.data_ptr(), at, place[p] + at, min(_CHUNK, p.numel() - at), tensors + j)
+                                  for at in range(0, p.numel(), _CHUNK)]
+                    self.launches.append(_Launch(group, dtype, part, tensors, chunk0, len(table) - chunk0))
+                    tensors += len(part)
+        n = len(table)
+        host = (_lib.OptChunk * max(n, 1))(*table)
+        self.chunks = torch.frombuffer(bytearray(host), dtype=torch.uint8).to(dev)
+        self.steps = torch.zeros(max(n, 1), dtype=torch.int32, device=dev)
+        self.parts = torch.empty(max(1, sum(l.grads.parts() for l in self.launches)), dtype=torch.float64, device=dev)
+        self.norm = torch.zeros((), dtype=torch.float32, device=dev)
+        for l in self.launches:
+            a = l.args
+            a.chunks = self.chunks.data_ptr() + l.chunk0 * C.sizeof(_lib.OptChunk)
+            a.steps = self.steps.data_ptr() + l.chunk0 * 4
+            a.grads = C.addressof(l.grads.ptrs)
+            a.m, a.v = self.m.data_ptr(), self.v.data_ptr()
+            if bits == 8:
+                a.ms, a.vs = self.ms.data_ptr(), self.vs.data_ptr()
+            a.n_chunks, a.n_tensors, a.first_tensor = l.n_chunks, len(l.params), l.first_tensor
+            a.type, a.bits, a.seed = _TYPES[l.dtype], bits, opt.seed & 0xFFFFFFFF
+        olds = [(p, opt.state.get(p)) for p in params]
+        taken = torch.stack([torch.as_tensor(old["step"]).to(dev, torch.int32).view(()) for _, old in olds if old]
+                            or [torch.zeros((), dtype=torch.int32)])
+        taken = iter(taken.unbind(0))
+        for p, old in olds:
+            opt.state[p] = st = self._views(p, place[p], first.get(p, 0))
+            if old:
+                step = next(taken)
+                st["step"].copy_(step)
+                self.steps[first[p]:first[p] + -(-p.numel() // _CHUNK)] = step
+                for k in st:
+                    if k != "step":
+                        st[k].copy_(old[k])
+
+    def _views(self, p, o, chunk):
+        """The parameter's state: views of the plan's buffers."""
+        n = p.numel()
+        st = {"step": self.steps[chunk] if n else torch.zeros((), dtype=torch.int32, device=p.device)}
+        for k, t, s in (("exp_avg", self.m, self.ms), ("exp_avg_sq", self.v, self.vs)):
+            st[k] = t[o:o + n].view(p.shape)
+            if s is not None:
+                st[k + "_scale"] = s[o // _RUN:o // _RUN + -(-n // _RUN)]
+        return st
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW (decoupled weight decay; Adam for weight_decay=0) over all parameters at once.
+
+        m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2
+        p = p (1 - lr weight_decay) - lr / (1 - b1^t) m / (sqrt(v / (1 - b2^t)) + eps)
+
+    params: contiguous fp32, bf16 or fp16 parameters on one GPU (others only without a gradient), or groups of them with their own lr, betas, eps and
+    weight_decay (lr may be a tensor of one fp32 element on that GPU, read by the step itself).  Parameters without a gradient are left
+    out of a step, as in torch.  Arithmetic and 32-bit moments are fp32 whatever the parameters' type, which are
+    rounded to nearest once a step.
+
+    state_bits=8 keeps both moments in 8 bits (runs of 32 elements share a power-of-two scale; 3 mantissa
+    bits, rounded stochastically by a hash of ``seed``, step and element, so that runs repeat): 2.1 bytes a parameter
+    instead of 8.  ``state[p]`` then holds codes ("exp_avg", "exp_avg_sq") and scale bytes ("..._scale"); ``moments`` gives
+    values.
+
+    max_norm scales the gradients by min(1, max_norm / (norm + 1e-6)), norm their global 2-norm over all groups, as
+    they are read (they stay as they were); skip_nonfinite leaves parameters, moments and step counts as they were where that norm
+    is not finite and counts such steps in ``skipped``.  ``grad_norm`` is the last step's norm (None without either).
+
+    A step after the first can be captured into a graph and replayed: step counts are on the device.  ``state`` entries are
+    views of flat buffers: write into them in place, or through load_state_dict."""
+
+    _plan: Optional[_Plan] = None
+    _OPTIONS = ("state_bits", "max_norm", "skip_nonfinite", "seed")
+
+    def __init__(self, params, lr: Union[float, torch.Tensor] = 1e-3, betas: Tuple[float, float] = (0.9, 0.999),
+                 eps: float = 1e-8, weight_decay: float = 1e-2, *, state_bits: int = 32,
+                 max_norm: Optional[float] = None, skip_nonfinite: bool = False, seed: int = 0):
+        if state_bits not in (8, 32):
+            raise ValueError(f"AdamW: moments of {state_bits} bits (8 or 32)")
+        if max_norm is not None and not float(max_norm) > 0:
+            raise ValueError(f"AdamW: max_norm {max_norm}")
+        self.state_bits, self.seed = int(state_bits), int(seed)
+        self.max_norm = None if max_norm is None else float(max_norm)
+        self.skip_nonfinite = bool(skip_nonfinite)
+        self._skipped = None
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
+
+    @staticmethod
+    def _check_group(g):
+        lr, (b1, b2) = g["lr"], g["betas"]
+        if not isinstance(lr, torch.Tensor) and not 0.0 <= lr < math.inf:
+            raise ValueError(f"AdamW: lr {lr}")
+        if isinstance(lr, torch.Tensor) and lr.numel() != 1:
+            raise ValueError(f"AdamW: lr of {lr.numel()} elements")
+        if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0):
+            raise ValueError(f"AdamW: betas {g['betas']}")
+        if not g["eps"] >= 0.0 or not g["weight_decay"] >= 0.0:
+            raise ValueError(f"AdamW: eps {g['eps']}, weight_decay {g['weight_decay']}")
+
+    def add_param_group(self, group):
+        super().add_param_group(group)
+        try:
+            self._check_group(self.param_groups[-1])
+        except ValueError:
+            self.param_groups.pop()
+            raise
+        self._plan = None
+
+    def __getstate__(self):
+        return {**super().__getstate__(), **{k: getattr(self, k) for k in self._OPTIONS}, "_skipped": self._skipped}
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self._plan = None
+
+    @property
+    def grad_norm(self) -> Optional[torch.Tensor]:
+        """The global norm of the last step's gradients (before scaling); None where no step computes it."""
+        if self._plan is None or (self.max_norm is None and not self.skip_nonfinite):
+            return None
+        return self._plan.norm
+
+    @property
+    def skipped(self) -> Optional[torch.Tensor]:
+        """Steps left out because the norm was not finite (an int32 tensor of one element); None without skip_nonfinite."""
+        return self._skipped if self.skip_nonfinite else None
+
+    def load_state_dict(self, state_dict):
+        """As torch's, with moments kept in their own types: fp32, or codes and scale bytes."""
+        saved, groups = state_dict["state"], state_dict["param_groups"]
+        names = ["step", "exp_avg", "exp_avg_sq"] + (["exp_avg_scale", "exp_avg_sq_scale"] if self.state_bits == 8 else [])
+        new = {}
+        for i, p in zip(chain.from_iterable(g["params"] for g in groups),
+                        chain.from_iterable(g["params"] for g in self.param_groups)):
+            e = saved.get(i)
+            if not e:
+                continue
+            if not _usable(p):
+                raise ValueError(f"AdamW: state for parameter {i}, which is not contiguous in fp32, bf16 or fp16 on the GPU")
+            for k in names:
+                if k not in e:
+                    raise ValueError(f"AdamW: the state of parameter {i} has no {k} (moments of {self.state_bits} bits)")
+            for k in names[1:]:
+                size = (-(-p.numel() // _RUN),) if k.endswith("scale") else tuple(p.shape)
+                right = e[k].is_floating_point() if self.state_bits == 32 else e[k].dtype == torch.uint8
+                if tuple(e[k].shape) != size or not right:
+                    raise ValueError(f"AdamW: {k} of parameter {i} is {tuple(e[k].shape)} {e[k].dtype}, not {size} "
+                                     f"{'in a floating type' if self.state_bits == 32 else torch.uint8}")
+            new[p] = {k: e[k] for k in names}
+        super().load_state_dict({**state_dict, "state": {}})      # refuses groups of other sizes
+        self.state.update(new)
+        self._plan = _Plan(self)
+
+    def moments(self, dtype: Optional[torch.dtype] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+        """(m, v) of all parameters in the order of the groups, flat, each parameter's from a multiple of 64 elements on
+        (the gaps are zero).  32 bits without a dtype: the state itself; else values in dtype (fp32, bf16, fp16;
+        8-bit moments are exact in each as long as they are normal there)."""
+        if dtype not in (None, *_TYPES):
+            raise ValueError(f"AdamW.moments: {dtype}")
+        plan = self._current()
+        if self.state_bits == 32:
+            return (plan.m, plan.v) if dtype is None else (plan.m.to(dtype), plan.v.to(dtype))
+        dtype = dtype or torch.float32
+        m, v = (torch.empty(plan.total, dtype=dtype, device=plan.device) for _ in range(2))
+        with torch.cuda.device(plan.device):
+            _lib.call("e2v2_moments", *(_lib.vp(t.data_ptr()) for t in (plan.m, plan.ms, plan.v, plan.vs, m, v)),
+                      _lib.i32(_TYPES[dtype]), _lib.i64(plan.total), _lib.stream(plan.device))
+        return m, v
+
+    def _current(self) -> _Plan:
+        """The plan, made anew where parameters moved."""
+        plan = self._plan
+        if plan is None or [p.data_ptr() for p in plan.params] != plan.ptrs:
+            self._plan = plan = _Plan(self)
+        return plan
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        plan = self._current()
+        if torch.cuda.current_device() == plan.device.index:
+            self._launch(plan)
+        else:
+            with torch.cuda.device(plan.device):
+                self._launch(plan)
+        return loss
+
+    def _launch(self, plan: _Plan):
+        st = _lib.stream(plan.device)
+        normed = self.max_norm is not None or self.skip_nonfinite
+        if self.skip_nonfinite and self._skipped is None:
+            self._skipped = torch.zeros((), dtype=torch.int32, device=plan.device)
+        _refuse(plan.outside)
+        count = C.c_int(0)
+        keep = []
+        for l in plan.launches:
+            grads = [p.grad for p in l.params]
+            for i, g in enumerate(grads):
+                if g is None:
+                    continue
+                if g.dtype != l.dtype or g.layout != torch.strided:
+                    raise ValueError(f"AdamW: a gradient of type {g.dtype} {g.layout} for a parameter in {l.dtype}")
+                if not g.is_contiguous():
+                    grads[i] = g.contiguous()
+            keep.append(grads)
+            l.grads.ptrs[:] = [None if g is None else g.data_ptr() for g in grads]
+            if normed:
+                l.grads.norm(plan.parts, count, st)
+        if normed and not count.value:
+            plan.norm.zero_()                  # no gradient at all
+        norm = plan.norm.data_ptr()
+        for l in plan.launches:
+            a, g = l.args, l.group
+            lr = g["lr"]
+            if isinstance(lr, torch.Tensor) and lr.device == plan.device and lr.dtype == torch.float32:
+                a.lr_dev, a.lr = lr.data_ptr(), 0.0
+            else:
+                a.lr_dev, a.lr = None, float(lr)
+            a.beta1, a.beta2 = g["betas"]
+            a.eps, a.weight_decay = g["eps"], g["weight_decay"]
+            a.parts, a.n_parts = plan.parts.data_ptr(), count.value
+            a.max_norm = math.inf if self.max_norm is None else self.max_norm
+            a.norm, norm = norm, None
+            a.skip_nonfinite = int(self.skip_nonfinite)
+            a.skipped = self._skipped.data_ptr() if self.skip_nonfinite else None
+            _lib.call("e2v2_adamw", C.byref(a), st)
+        # what is kept per weight version (packed weights, radial tables) is made anew
+        torch.autograd.graph.increment_version([p for l, grads in zip(plan.launches, keep)
+                                                for p, g in zip(l.params, grads) if g is not None])
