@@ -72,6 +72,10 @@ def test_entry_point_checks():
     assert lib.e2v2_layer_norm_bwd(_lib.C.byref(a), None, None, None, _lib.i64(0), None) != 0
     assert b"null operand" in lib.e2v2_last_error()
     a.gy = a.gx = a.stats = 64
+    for rows, w in ((1, 7), (999, 64), (1025, 3), (10 ** 6, 16384)):
+        x = torch.empty(rows, w, device="meta")
+        ws, n = norms._workspace(x)
+        assert n == lib.e2v2_layer_norm_workspace(rows, w) == 4 * ws.numel()
     need = lib.e2v2_layer_norm_workspace(4, 16)
     assert need == 2 * 4 * 16 * 4 and lib.e2v2_layer_norm_workspace(0, 16) == 0
     for fn, args in ((lib.e2v2_layer_norm_bwd, (_lib.vp(64), None, _lib.vp(64))),

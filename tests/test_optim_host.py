@@ -45,9 +45,9 @@ def test_host_tensors_are_refused():
 def test_entry_point_checks():
     lib, C = _lib.load(), _lib.C
     ptrs, numel = (_lib.vp * 2)(64, 128), (_lib.i64 * 2)(5, 1 << 33)
-    assert lib.e2v2_grad_norm_parts(numel, 2) == 512 and lib.e2v2_grad_norm_parts(numel, 0) == 0
+    assert lib.e2v2_grad_norm_parts(numel, 2) == 1024 and lib.e2v2_grad_norm_parts(numel, 0) == 0
     many = (_lib.i64 * 600)(*([7] * 600))
-    assert lib.e2v2_grad_norm_parts(many, 600) == 3 * 512
+    assert lib.e2v2_grad_norm_parts(many, 600) == 3 * 1024
     count = C.c_int(0)
 
     def norm(n=2, type=0, parts=64, cap=0):

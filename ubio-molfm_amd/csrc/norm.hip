@@ -12,8 +12,8 @@
 // registers.
 //
 // One pass over memory: a row stays in the registers of kL lanes (16, 32 or 64 of a wavefront, or a workgroup of 256
-// or 1024), at most 16 elements a lane, read as 16-byte vectors where width, strides and addresses allow and element
-// by element where not.  A workgroup strides over the rows and keeps its columns' parameter sums in registers; each
+// or 1024), read as 16-byte vectors on whatever element boundary the row starts (the hardware takes them unaligned), the
+// rest of a row element by element.  A workgroup strides over the rows and keeps its columns' parameter sums in registers; each
 // leaves one partial row, added in order by a second launch, so results repeat bitwise.  Bound: HBM.
 #include <algorithm>
 
@@ -23,45 +23,67 @@
 namespace e2v2 {
 namespace {
 
-constexpr int kLnElems = 16;           // elements of a row in a lane's registers
-constexpr int kLnMaxWidth = 1024 * kLnElems;
-constexpr int kLnMaxParts = 1024;      // workgroups of a pass that leaves parameter sums: four per CU
+constexpr int kLnMaxWidth = 16384;     // 1024 lanes of 16 elements
+constexpr int kLnMaxParts = 1024;      // workgroups of a pass that leaves parameter sums, at most (ln_grid)
 
-template <typename T, int V>
+template <typename T>
 struct RowVec {
-  typedef T type __attribute__((ext_vector_type(V)));
-  typedef float ftype __attribute__((ext_vector_type(V)));
+  static constexpr int n = 16 / sizeof(T);
+  typedef T type __attribute__((ext_vector_type(16 / sizeof(T))));
+  typedef T any __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));   // on any element boundary
+  typedef float ftype __attribute__((ext_vector_type(16 / sizeof(T))));
 };
 
+// Elements c .. c + V of a row of w; those past its end are zero.
 template <typename T, int V>
-__device__ __forceinline__ void load_row(const T* p, float* out) {
-  if constexpr (V == 1) {
-    out[0] = (float)p[0];
-  } else {
-    const auto f = __builtin_convertvector(*reinterpret_cast<const typename RowVec<T, V>::type*>(p),
-                                           typename RowVec<T, V>::ftype);
+__device__ __forceinline__ void load_row(const T* row, int c, int w, float* out) {
+  if (c + V <= w) {
+    const typename RowVec<T>::type v = *reinterpret_cast<const typename RowVec<T>::any*>(row + c);
+    const auto f = __builtin_convertvector(v, typename RowVec<T>::ftype);
 #pragma unroll
     for (int k = 0; k < V; ++k) out[k] = f[k];
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; ++k) out[k] = c + k < w ? (float)row[c + k] : 0.f;
   }
 }
 
 template <typename T, int V>
-__device__ __forceinline__ void store_row(const float* v, T* p) {
-  if constexpr (V == 1) {
-    p[0] = (T)v[0];
-  } else {
-    typename RowVec<T, V>::ftype f;
+__device__ __forceinline__ void store_row(const float* v, T* row, int c, int w) {
+  if (c + V <= w) {
+    typename RowVec<T>::ftype f;
 #pragma unroll
     for (int k = 0; k < V; ++k) f[k] = v[k];
-    *reinterpret_cast<typename RowVec<T, V>::type*>(p) = __builtin_convertvector(f, typename RowVec<T, V>::type);
+    const typename RowVec<T>::type o = __builtin_convertvector(f, typename RowVec<T>::type);
+    *reinterpret_cast<typename RowVec<T>::any*>(row + c) = o;
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; ++k)
+      if (c + k < w) row[c + k] = (T)v[k];
   }
 }
 
-// Element c of a parameter vector (NULL: the value of an absent one).
-__device__ __forceinline__ float load_param(const void* p, int type, int c, float absent) {
-  if (!p) return absent;
-  if (type == E2V2_F32) return static_cast<const float*>(p)[c];
-  return type == E2V2_BF16 ? (float)static_cast<const __bf16*>(p)[c] : (float)static_cast<const _Float16*>(p)[c];
+// v + its partner's, kLanes lanes away, by an exchange of rows of 16 lanes or of halves in registers (no trip through
+// LDS).  The results are taken as integers first: a bit cast of a vector's element casts element 0 here.
+template <int kLanes>
+__device__ __forceinline__ float swap_sum(float v) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, v);
+  uint32_t lo, hi;
+  if constexpr (kLanes == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    lo = r[0], hi = r[1];
+  } else {
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    lo = r[0], hi = r[1];
+  }
+  return __builtin_bit_cast(float, lo) + __builtin_bit_cast(float, hi);
+}
+
+// a b, rounded by itself: fused with the subtraction of its own row mean it would leave the rounding where the
+// difference is zero.
+__device__ __forceinline__ float rounded_product(float a, float b) {
+#pragma clang fp contract(off)
+  return a * b;
 }
 
 // Sums of K values over the kL lanes that hold a row, in every lane.  red: two buffers of [K][waves], used in turn, so
@@ -71,8 +93,8 @@ __device__ __forceinline__ void group_sum(float (&v)[K], float (*red)[4][16], in
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     v[k] = dpp_row_sum16(v[k]);
-    if constexpr (kL >= 32) v[k] += __shfl_xor(v[k], 16, 64);
-    if constexpr (kL >= 64) v[k] += __shfl_xor(v[k], 32, 64);
+    if constexpr (kL >= 32) v[k] = swap_sum<16>(v[k]);
+    if constexpr (kL >= 64) v[k] = swap_sum<32>(v[k]);
   }
   if constexpr (kL > 64) {
     constexpr int kWaves = kL / 64;
@@ -105,37 +127,55 @@ struct LnArgs {
 
 // The lane's columns: vector k starts at column (l + k kL) V.
 template <int V, int kL, int NV, typename F>
-__device__ __forceinline__ void each_vec(int l, int w, F&& f) {
+__device__ __forceinline__ void each_vec(int l, F&& f) {
 #pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    const int c = (l + k * kL) * V;
-    f(k, c, c < w);
-  }
+  for (int k = 0; k < NV; ++k) f(k, (l + k * kL) * V);
 }
 
+template <typename W, int V, int kL, int NV>
+__device__ __forceinline__ void load_params_as(const W* p, int l, int w, float (&out)[NV * V]) {
+  typedef W any __attribute__((ext_vector_type(V), aligned(sizeof(W))));
+  each_vec<V, kL, NV>(l, [&](int k, int c) {
+    if (c + V <= w) {
+      const any v = *reinterpret_cast<const any*>(p + c);
+#pragma unroll
+      for (int e = 0; e < V; ++e) out[k * V + e] = (float)v[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e) out[k * V + e] = c + e < w ? (float)p[c + e] : 0.f;
+    }
+  });
+}
+
+// The lane's elements of a parameter vector (NULL: the value of an absent one).
 template <int V, int kL, int NV>
 __device__ __forceinline__ void load_params(const void* p, int type, int l, int w, float absent, float (&out)[NV * V]) {
-  each_vec<V, kL, NV>(l, w, [&](int k, int c, bool in) {
+  if (!p) {
 #pragma unroll
-    for (int e = 0; e < V; ++e) out[k * V + e] = in ? load_param(p, type, c + e, absent) : 0.f;
-  });
+    for (int e = 0; e < NV * V; ++e) out[e] = absent;
+  } else if (type == E2V2_F32) {
+    load_params_as<float, V, kL, NV>(static_cast<const float*>(p), l, w, out);
+  } else if (type == E2V2_BF16) {
+    load_params_as<__bf16, V, kL, NV>(static_cast<const __bf16*>(p), l, w, out);
+  } else {
+    load_params_as<_Float16, V, kL, NV>(static_cast<const _Float16*>(p), l, w, out);
+  }
 }
 
 // Adds the workgroup's row groups' parameter sums and writes them as partial row blockIdx.x.
 template <int V, int kL, int NV>
 __device__ __forceinline__ void write_part(const float (&acc)[NV * V], int l, int rg, int w, float* out) {
   if constexpr (kL > 64) {
-    each_vec<V, kL, NV>(l, w, [&](int k, int c, bool in) {
-      if (in) {
+    each_vec<V, kL, NV>(l, [&](int k, int c) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) out[c + e] = acc[k * V + e];
-      }
+      for (int e = 0; e < V; ++e)
+        if (c + e < w) out[c + e] = acc[k * V + e];
     });
   } else {
     constexpr int kR = 256 / kL, kC = kL * NV * V;
     __shared__ float red[kR][kC];
     __syncthreads();
-    each_vec<V, kL, NV>(l, w, [&](int k, int c, bool in) {
+    each_vec<V, kL, NV>(l, [&](int k, int c) {
 #pragma unroll
       for (int e = 0; e < V; ++e) red[rg][c + e] = acc[k * V + e];
     });
@@ -162,30 +202,28 @@ __global__ __launch_bounds__(kL > 64 ? kL : 256) void k_layer_norm_fwd(LnArgs P)
   for (int64_t row = (int64_t)blockIdx.x * kR + rg; row < P.n; row += (int64_t)gridDim.x * kR) {
     const T* xr = static_cast<const T*>(P.x) + row * P.ldx;
     float x[E], s[1] = {0.f}, q[1] = {0.f};
-    each_vec<V, kL, NV>(l, w, [&](int k, int c, bool in) {
-#pragma unroll
-      for (int e = 0; e < V; ++e) x[k * V + e] = 0.f;
-      if (in) load_row<T, V>(xr + c, x + k * V);
+    each_vec<V, kL, NV>(l, [&](int k, int c) {
+      load_row<T, V>(xr, c, w, x + k * V);
 #pragma unroll
       for (int e = 0; e < V; ++e) s[0] += x[k * V + e];
     });
     group_sum<kL, 1>(s, red, turn);
     const float mean = s[0] / (float)w;       // a true quotient: exact for a row of one short value
-    each_vec<V, kL, NV>(l, w, [&](int k, int c, bool in) {
+    each_vec<V, kL, NV>(l, [&](int k, int c) {
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        x[k * V + e] = in ? x[k * V + e] - mean : 0.f;
+        x[k * V + e] = c + e < w ? x[k * V + e] - mean : 0.f;
         q[0] = fmaf(x[k * V + e], x[k * V + e], q[0]);
       }
     });
     group_sum<kL, 1>(q, red, turn);
     const float rstd = 1.0f / sqrtf(q[0] * inv + P.eps);
     T* yr = static_cast<T*>(P.y) + row * w;
-    each_vec<V, kL, NV>(l, w, [&](int k, int c, bool in) {
+    each_vec<V, kL, NV>(l, [&](int k, int c) {
       float o[V];
 #pragma unroll
       for (int e = 0; e < V; ++e) o[e] = fmaf(x[k * V + e] * rstd, g[k * V + e], b[k * V + e]);
-      if (in) store_row<T, V>(o, yr + c);
+      store_row<T, V>(o, yr, c, w);
     });
     if (P.stats && l == 0) *reinterpret_cast<float2*>(P.stats + 2 * row) = make_float2(mean, rstd);
   }
@@ -207,20 +245,17 @@ __global__ __launch_bounds__(kL > 64 ? kL : 256) void k_layer_norm_bwd(LnArgs P)
     const T* gr = static_cast<const T*>(P.gy) + row * P.ldgy;
     const float2 st = *reinterpret_cast<const float2*>(P.stats + 2 * row);
     float xh[E], gy[E], s[2] = {0.f, 0.f};
-    each_vec<V, kL, NV>(l, w, [&](int k, int c, bool in) {
-#pragma unroll
-      for (int e = 0; e < V; ++e) xh[k * V + e] = gy[k * V + e] = 0.f;
-      if (in) {
-        load_row<T, V>(xr + c, xh + k * V);
-        load_row<T, V>(gr + c, gy + k * V);
-      }
+    each_vec<V, kL, NV>(l, [&](int k, int c) {
+      load_row<T, V>(xr, c, w, xh + k * V);
+      load_row<T, V>(gr, c, w, gy + k * V);
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         float& h = xh[k * V + e];
-        h = in ? (h - st.x) * st.y : 0.f;
-        const float u = gy[k * V + e] * g[k * V + e];
-        ag[k * V + e] = fmaf(gy[k * V + e], h, ag[k * V + e]);
-        ab[k * V + e] += gy[k * V + e];
+        h = c + e < w ? (h - st.x) * st.y : 0.f;
+        float& u = gy[k * V + e];
+        ag[k * V + e] = fmaf(u, h, ag[k * V + e]);
+        ab[k * V + e] += u;
+        u = rounded_product(u, g[k * V + e]);
         s[0] += u;
         s[1] = fmaf(u, h, s[1]);
       }
@@ -228,11 +263,11 @@ __global__ __launch_bounds__(kL > 64 ? kL : 256) void k_layer_norm_bwd(LnArgs P)
     group_sum<kL, 2>(s, red, turn);
     const float m1 = s[0] * inv, m2 = s[1] * inv;
     T* o = static_cast<T*>(P.gx) + row * w;
-    each_vec<V, kL, NV>(l, w, [&](int k, int c, bool in) {
+    each_vec<V, kL, NV>(l, [&](int k, int c) {
       float v[V];
 #pragma unroll
-      for (int e = 0; e < V; ++e) v[e] = st.y * (gy[k * V + e] * g[k * V + e] - m1 - xh[k * V + e] * m2);
-      if (in) store_row<T, V>(v, o + c);
+      for (int e = 0; e < V; ++e) v[e] = st.y * (gy[k * V + e] - m1 - xh[k * V + e] * m2);
+      store_row<T, V>(v, o, c, w);
     });
   }
   if (P.part) {
@@ -262,18 +297,16 @@ __global__ __launch_bounds__(kL > 64 ? kL : 256) void k_layer_norm_bwd2(LnArgs P
     const float r = st.y;
     float xh[E], gy[E], q[E];
     float s[4] = {0.f, 0.f, 0.f, 0.f}, squ[1] = {0.f};
-    each_vec<V, kL, NV>(l, w, [&](int k, int c, bool in) {
+    each_vec<V, kL, NV>(l, [&](int k, int c) {
 #pragma unroll
-      for (int e = 0; e < V; ++e) xh[k * V + e] = gy[k * V + e] = q[k * V + e] = 0.f;
-      if (in) {
-        load_row<T, V>(xr + c, xh + k * V);
-        load_row<T, V>(gr + c, gy + k * V);
-        if (P.qx) load_row<T, V>(qr + c, q + k * V);
-      }
+      for (int e = 0; e < V; ++e) q[k * V + e] = 0.f;
+      load_row<T, V>(xr, c, w, xh + k * V);
+      load_row<T, V>(gr, c, w, gy + k * V);
+      if (P.qx) load_row<T, V>(qr, c, w, q + k * V);
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         float& h = xh[k * V + e];
-        h = in ? (h - st.x) * r : 0.f;
+        h = c + e < w ? (h - st.x) * r : 0.f;
         const float u = gy[k * V + e] * g[k * V + e], v = q[k * V + e];
         s[0] += u;
         s[1] = fmaf(u, h, s[1]);
@@ -288,12 +321,12 @@ __global__ __launch_bounds__(kL > 64 ? kL : 256) void k_layer_norm_bwd2(LnArgs P
     const float rr = r * r * (squ[0] * inv - qm * ub - c_ * m);      // r <qx gx>
     float t[2] = {0.f, 0.f};
     T* o1 = static_cast<T*>(P.y) + row * w;
-    each_vec<V, kL, NV>(l, w, [&](int k, int c, bool in) {
+    each_vec<V, kL, NV>(l, [&](int k, int c) {
       float v[V];
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         const int i = k * V + e;
-        const float a = in ? r * (q[i] - qm - xh[i] * m) : 0.f;
+        const float a = c + e < w ? r * (q[i] - qm - xh[i] * m) : 0.f;
         v[e] = g[i] * a + qg[i] * xh[i] + qb[i];
         ag[i] = fmaf(gy[i], a, ag[i]);
         const float x = qg[i] * gy[i] - r * (c_ * q[i] + m * gy[i] * g[i]);
@@ -301,16 +334,16 @@ __global__ __launch_bounds__(kL > 64 ? kL : 256) void k_layer_norm_bwd2(LnArgs P
         t[0] += x;
         t[1] = fmaf(x, xh[i], t[1]);
       }
-      if (in) store_row<T, V>(v, o1 + c);
+      store_row<T, V>(v, o1, c, w);
     });
     group_sum<kL, 2>(t, red, turn);
     const float mx = t[0] * inv, mxx = t[1] * inv;
     T* o2 = static_cast<T*>(P.gx) + row * w;
-    each_vec<V, kL, NV>(l, w, [&](int k, int c, bool in) {
+    each_vec<V, kL, NV>(l, [&](int k, int c) {
       float v[V];
 #pragma unroll
       for (int e = 0; e < V; ++e) v[e] = r * (q[k * V + e] - mx - xh[k * V + e] * mxx) - rr * xh[k * V + e];
-      if (in) store_row<T, V>(v, o2 + c);
+      store_row<T, V>(v, o2, c, w);
     });
   }
   if (P.part) write_part<V, kL, NV>(ag, l, rg, w, P.part + (int64_t)blockIdx.x * w);
@@ -356,58 +389,91 @@ void ln_launch(const LnArgs& P, unsigned grid, hipStream_t s) {
     hipLaunchKernelGGL((k_layer_norm_bwd2<T, V, kL, NV>), dim3(grid), block, 0, s, P);
 }
 
-// Rows in flight in a workgroup for a width in vectors of v elements.
-int ln_rows_per_wg(int w, int v) {
-  const int nv = (w + v - 1) / v, most = kLnElems / v;
-  return nv <= 16 ? 16 : nv <= 32 ? 8 : nv <= 64 * most ? 4 : 1;
+// Lanes that hold a row, and 16-byte vectors a lane holds of it.  Up to 1024 elements a part of a wavefront, so that no
+// barrier stands in the way: of the shapes that hold the row the one with the fewest idle places (129 fp32 elements, 33 vectors:
+// 16 lanes of 3 instead of 64 of 1).  Wider rows take a workgroup, up to 32 elements a lane forward
+// (5001 bf16 elements: 38 us with 256 lanes, 42 with 1024) and 16 backward, where more would not leave registers
+// for two wavefronts a SIMD (5001 fp32, second order: 195 us with 256 lanes, 147 with 1024).
+struct LnShape {
+  int lanes, vecs;
+};
+
+LnShape ln_shape(int w, int v, bool fwd) {
+  const int nv = (w + v - 1) / v;
+  if (nv <= 16) return {16, 1};
+  if (nv <= 32) return {32, 1};
+  if (nv <= 48) return {16, 3};
+  if (nv <= 64) return {64, 1};
+  if (nv <= 96) return {32, 3};
+  if (nv <= 128) return {64, 2};
+  if (w <= 1024) return {64, nv <= 192 ? 3 : 4};
+  if (w <= (fwd ? 8192 : 4096)) {
+    for (int k = 1;; k *= 2)
+      if (nv <= 256 * k) return {256, k};
+  }
+  return {1024, w <= 8192 ? 8 / v : 16 / v};
 }
 
-template <LnPass kPass, typename T, int V>
+template <LnPass kPass, typename T>
 void ln_dispatch(const LnArgs& P, unsigned grid, hipStream_t s) {
-  constexpr int M = kLnElems / V;                 // vectors a lane can hold
-  const int nv = (P.w + V - 1) / V;
-  if (nv <= 16) return ln_launch<kPass, T, V, 16, 1>(P, grid, s);
-  if (nv <= 32) return ln_launch<kPass, T, V, 32, 1>(P, grid, s);
-  if (nv <= 64) return ln_launch<kPass, T, V, 64, 1>(P, grid, s);
-  if (nv <= 128) return ln_launch<kPass, T, V, 64, 2>(P, grid, s);
-  if constexpr (M >= 4) {
-    if (nv <= 256) return ln_launch<kPass, T, V, 64, 4>(P, grid, s);
+  constexpr int V = RowVec<T>::n;
+  constexpr bool kFwd = kPass == LnPass::kFwd;
+  const LnShape f = ln_shape(P.w, V, kFwd);
+  switch (f.lanes * 16 + f.vecs) {
+    case 16 * 16 + 1: return ln_launch<kPass, T, V, 16, 1>(P, grid, s);
+    case 32 * 16 + 1: return ln_launch<kPass, T, V, 32, 1>(P, grid, s);
+    case 16 * 16 + 3: return ln_launch<kPass, T, V, 16, 3>(P, grid, s);
+    case 64 * 16 + 1: return ln_launch<kPass, T, V, 64, 1>(P, grid, s);
+    case 32 * 16 + 3: return ln_launch<kPass, T, V, 32, 3>(P, grid, s);
+    case 64 * 16 + 2: return ln_launch<kPass, T, V, 64, 2>(P, grid, s);
   }
-  if constexpr (M >= 16) {
-    if (nv <= 512) return ln_launch<kPass, T, V, 64, 8>(P, grid, s);
-    if (nv <= 1024) return ln_launch<kPass, T, V, 64, 16>(P, grid, s);
-    if (nv <= 2048) return ln_launch<kPass, T, V, 256, 8>(P, grid, s);
+  if constexpr (V == 4) {
+    switch (f.lanes * 16 + f.vecs) {
+      case 64 * 16 + 3: return ln_launch<kPass, T, V, 64, 3>(P, grid, s);
+      case 64 * 16 + 4: return ln_launch<kPass, T, V, 64, 4>(P, grid, s);
+      case 256 * 16 + 8:
+        if constexpr (kFwd) return ln_launch<kPass, T, V, 256, 8>(P, grid, s);
+    }
   }
-  if (nv <= 256 * M) return ln_launch<kPass, T, V, 256, M>(P, grid, s);
-  if constexpr (M >= 16) {
-    if (nv <= 1024 * 8) return ln_launch<kPass, T, V, 1024, 8>(P, grid, s);
+  switch (f.lanes * 16 + f.vecs) {
+    case 256 * 16 + 1:
+      if constexpr (V == 8) return ln_launch<kPass, T, V, 256, 1>(P, grid, s);
+      break;
+    case 256 * 16 + 2: return ln_launch<kPass, T, V, 256, 2>(P, grid, s);
+    case 256 * 16 + 4:
+      if constexpr (kFwd || V == 4) return ln_launch<kPass, T, V, 256, 4>(P, grid, s);
+      break;
+    case 1024 * 16 + 8 / V:
+      if constexpr (!kFwd) return ln_launch<kPass, T, V, 1024, 8 / V>(P, grid, s);
+      break;
+    default: return ln_launch<kPass, T, V, 1024, 16 / V>(P, grid, s);
   }
-  return ln_launch<kPass, T, V, 1024, M>(P, grid, s);
 }
 
 int type_size(int t) { return t == E2V2_F32 ? 4 : 2; }
 bool type_ok(int t) { return t == E2V2_F32 || t == E2V2_BF16 || t == E2V2_F16; }
 
-// Elements of a 16-byte vector if every row of every operand lies on 16-byte boundaries, else 1.
-int ln_vec(const LnArgs& P, int type) {
-  const int v = 16 / type_size(type);
-  const uintptr_t a = (uintptr_t)P.x | (uintptr_t)P.gy | (uintptr_t)P.qx | (uintptr_t)P.y | (uintptr_t)P.gx;
-  return a % 16 == 0 && P.w % v == 0 && P.ldx % v == 0 && P.ldgy % v == 0 && P.ldq % v == 0 ? v : 1;
-}
-
 template <LnPass kPass>
 void ln_run(const LnArgs& P, int type, unsigned grid, hipStream_t s) {
-  const int v = ln_vec(P, type);
-  if (type == E2V2_F32)
-    v > 1 ? ln_dispatch<kPass, float, 4>(P, grid, s) : ln_dispatch<kPass, float, 1>(P, grid, s);
-  else if (type == E2V2_BF16)
-    v > 1 ? ln_dispatch<kPass, __bf16, 8>(P, grid, s) : ln_dispatch<kPass, __bf16, 1>(P, grid, s);
-  else
-    v > 1 ? ln_dispatch<kPass, _Float16, 8>(P, grid, s) : ln_dispatch<kPass, _Float16, 1>(P, grid, s);
+  if (type == E2V2_F32) ln_dispatch<kPass, float>(P, grid, s);
+  else if (type == E2V2_BF16) ln_dispatch<kPass, __bf16>(P, grid, s);
+  else ln_dispatch<kPass, _Float16>(P, grid, s);
 }
 
-unsigned ln_grid(const LnArgs& P, int type, int64_t most) {
-  const int r = ln_rows_per_wg(P.w, ln_vec(P, type));
+// Workgroups of a pass.  They stride over the rows, with the parameters loaded once: a workgroup for every few rows loads them again
+// each time (forward, 127,113 x 128 fp32: 26 us with 1,024 workgroups, 38 with one for 8 rows; 32,768 x 2048 bf16: 51 with
+// 2,048, 232 with one a row).  Where sums of the parameters are left, fewer partial rows are fewer bytes, but one vector a lane needs four
+// workgroups a CU to have enough loads in flight (200,000 x 256 bf16: 60 us with 1,024, 83 with 512; 60,000 x 512 fp32, two
+// vectors: 76 and 72; 6,007 x 5001 fp32, 1024 lanes: 99 and, with 256, 81).  Without sums and with narrow
+// rows the backward pass only reloads the weight, which the caches hold: one row a lane group (853,991 x 128 fp32: 215
+// us, 244 with 1,024).
+unsigned ln_grid(const LnArgs& P, int type, LnPass pass, bool sums) {
+  const int v = 16 / type_size(type);
+  const LnShape f = ln_shape(P.w, v, pass == LnPass::kFwd);
+  const int r = f.lanes > 64 ? 1 : 256 / f.lanes;
+  int64_t most = f.lanes == 1024 ? 512 : f.lanes == 256 ? 2048 : 1024;
+  if (sums) most = f.lanes == 1024 ? 256 : f.vecs == 1 ? 1024 : 512;
+  else if (pass != LnPass::kFwd && f.lanes <= 32) most = 1 << 30;
   return (unsigned)std::min<int64_t>((P.n + r - 1) / r, most);
 }
 
@@ -451,7 +517,7 @@ E2V2_API int e2v2_layer_norm_fwd(const e2v2_layer_norm_args* a, hipStream_t s) {
   LnArgs P = ln_args(a);
   P.gy = P.qx = P.gx = nullptr;
   P.ldgy = P.ldq = 0;
-  ln_run<LnPass::kFwd>(P, a->type, ln_grid(P, a->type, 1 << 20), s);
+  ln_run<LnPass::kFwd>(P, a->type, ln_grid(P, a->type, LnPass::kFwd, false), s);
   E2V2_LAUNCHED("k_layer_norm_fwd");
   return 0;
 }
@@ -471,7 +537,7 @@ E2V2_API int e2v2_layer_norm_bwd(const e2v2_layer_norm_args* a, void* gg, void* 
   P.qx = P.y = nullptr;
   P.ldq = 0;
   P.part = params ? ws : nullptr;
-  const unsigned grid = ln_grid(P, a->type, params ? kLnMaxParts : 1 << 20);
+  const unsigned grid = ln_grid(P, a->type, LnPass::kBwd, params);
   if (grid) {
     ln_run<LnPass::kBwd>(P, a->type, grid, s);
     E2V2_LAUNCHED("k_layer_norm_bwd");
@@ -486,7 +552,7 @@ E2V2_API int e2v2_layer_norm_bwd2(const e2v2_layer_norm_args* a, void* gg, float
                "layer_norm_bwd2: workspace of %lld bytes", (long long)ws_bytes);
   LnArgs P = ln_args(a);
   P.part = gg ? ws : nullptr;
-  const unsigned grid = ln_grid(P, a->type, gg ? kLnMaxParts : 1 << 20);
+  const unsigned grid = ln_grid(P, a->type, LnPass::kBwd2, gg != nullptr);
   if (grid) {
     ln_run<LnPass::kBwd2>(P, a->type, grid, s);
     E2V2_LAUNCHED("k_layer_norm_bwd2");

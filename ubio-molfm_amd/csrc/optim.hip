@@ -31,7 +31,7 @@ constexpr int kOptThreads = 256;
 constexpr int kOptChunk = E2V2_OPT_CHUNK;
 constexpr int kNormList = 256;         // gradients of a norm launch (a thread each finds the chunks' tensors)
 constexpr int kNormChunk = 8192;
-constexpr int kNormParts = 512;        // workgroups of a norm launch at most
+constexpr int kNormParts = 1024;       // workgroups of a norm launch at most
 constexpr int kStepList = 384;         // gradients of a step launch (3 KB of the 4 KB of kernel arguments)
 
 template <typename T>
@@ -312,7 +312,7 @@ __global__ __launch_bounds__(kOptThreads) void k_adamw(StepArgs P) {
       const float x = gv[e] * c;
       m[e] = fmaf(P.one_b1, x, P.b1 * m[e]);
       v[e] = fmaf(P.one_b2 * x, x, P.b2 * v[e]);
-      pv[e] -= fmaf(decay, pv[e], size * (m[e] / fmaf(sqrtf(v[e]), root, P.eps)));
+      pv[e] -= fmaf(decay, pv[e], size * (m[e] * frcp(fmaf(__builtin_amdgcn_sqrtf(v[e]), root, P.eps))));
     }
     store_some<T, N>(pv, p, i, ch.n, vec);
     if constexpr (kBits == 32) {

@@ -15,6 +15,7 @@ from torch.autograd.function import once_differentiable
 from . import _lib
 
 MAX_WIDTH = 16384
+_MAX_PARTS = 1024       # kLnMaxParts of csrc/norm.hip
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
@@ -25,6 +26,8 @@ def _ptr(t: Optional[torch.Tensor]):
 def _rows(t: torch.Tensor):
     """(t as the kernels read it, its row stride): consecutive elements in a row, rows one stride apart, on the
     boundaries of the element type; a copy where t does not lie so."""
+    if t.is_contiguous():
+        return t, t.shape[-1]
     if t.stride(-1) == 1 or t.shape[-1] == 1:
         ld = None
         for size, stride in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
@@ -69,11 +72,15 @@ def _args(x, g, b, stats, eps, gy=None, qx=None, qg=None, qb=None, y=None, gx=No
 
 
 def _workspace(x):
-    n = int(_lib.load().e2v2_layer_norm_workspace(x.numel() // x.shape[-1], x.shape[-1]))
-    return torch.empty(n // 4, dtype=torch.float32, device=x.device), n
+    """Room for the parameters' partial sums, as e2v2_layer_norm_workspace says, and its bytes."""
+    w = x.shape[-1]
+    n = 2 * min(x.numel() // w, _MAX_PARTS) * w
+    return torch.empty(n, dtype=torch.float32, device=x.device), 4 * n
 
 
 def _call(name, dev, *args):
+    if torch.cuda.current_device() == dev.index:
+        return _lib.call(name, *args, _lib.stream(dev))
     with torch.cuda.device(dev):
         _lib.call(name, *args, _lib.stream(dev))
 
@@ -95,12 +102,26 @@ class _LayerNormFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, gy):
         x, g, b, stats = ctx.saved_tensors
-        # next_functions has an entry for each tensor among the inputs
+        # next_functions has an entry for each tensor among the inputs; the sums of weight and bias come together
         nodes = iter(ctx.next_functions[1:])
+        need = [ctx.needs_input_grad[1 + k] and t is not None for k, t in enumerate((g, b))]
         nodes = [None if t is None else next(nodes)[0] for t in (g, b)]
-        need = [ctx.needs_input_grad[k + 1] and _will_run(nodes[k]) for k in range(2)]
-        gx, gg, gb = _LayerNormGradFn.apply(gy, x, g, b, stats, ctx.eps, *need)
+        if True in need and not any(n and _will_run(node) for n, node in zip(need, nodes)):
+            need = [False, False]
+        gx, gg, gb = (_LayerNormGradFn.apply if torch.is_grad_enabled() else _layer_norm_grad)(
+            gy, x, g, b, stats, ctx.eps, *need)
         return gx if ctx.needs_input_grad[0] else None, gg, gb, None
+
+
+def _layer_norm_grad(gy, x, g, b, stats, eps, need_g, need_b):
+    gx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    gg = torch.empty(g.shape, dtype=g.dtype, device=x.device) if need_g else None
+    gb = torch.empty(b.shape, dtype=b.dtype, device=x.device) if need_b else None
+    ws, n = _workspace(x) if need_g or need_b else (None, 0)
+    a, keep = _args(x, g, b, stats, eps, gy=gy, gx=gx)
+    _call("e2v2_layer_norm_bwd", x.device, _lib.C.byref(a), _lib.vp(_ptr(gg)), _lib.vp(_ptr(gb)), _lib.vp(_ptr(ws)),
+          _lib.i64(n))
+    return gx, gg, gb
 
 
 class _LayerNormGradFn(torch.autograd.Function):
@@ -109,17 +130,11 @@ class _LayerNormGradFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, gy, x, g, b, stats, eps, need_g, need_b):
-        gx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        gg = torch.empty_like(g, memory_format=torch.contiguous_format) if need_g else None
-        gb = torch.empty_like(b, memory_format=torch.contiguous_format) if need_b else None
-        ws, n = _workspace(x) if need_g or need_b else (None, 0)
-        a, keep = _args(x, g, b, stats, eps, gy=gy, gx=gx)
-        _call("e2v2_layer_norm_bwd", x.device, _lib.C.byref(a), _lib.vp(_ptr(gg)), _lib.vp(_ptr(gb)),
-              _lib.vp(_ptr(ws)), _lib.i64(n))
+        out = _layer_norm_grad(gy, x, g, b, stats, eps, need_g, need_b)
         ctx.save_for_backward(gy, x, g, b, stats)
         ctx.eps = eps
         ctx.set_materialize_grads(False)
-        return gx, gg, gb
+        return out
 
     @staticmethod
     @once_differentiable

@@ -9,6 +9,8 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+from array import array
+from contextlib import nullcontext
 from itertools import chain
 from typing import Iterable, Optional, Tuple, Union
 
@@ -23,51 +25,65 @@ _ALIGN = 64             # a tensor's moments start at a multiple of this many el
 _RUN = 32               # elements that share a scale byte
 
 
-def _tensors(params) -> list:
-    """The gradients of parameters that have one."""
-    params = [params] if isinstance(params, torch.Tensor) else list(params)
-    return [p.grad for p in params if p.grad is not None]
-
-
-def _check(grads, what: str):
-    """One device, known types, dense; by type."""
-    by_type = {}
-    for g in grads:
-        if not g.is_cuda:
-            raise RuntimeError(f"{what} runs on the GPU only (HIP library, no CPU path): got a tensor on {g.device}")
-        if g.layout != torch.strided or g.dtype not in _TYPES:
-            raise ValueError(f"{what}: dense fp32, bf16 or fp16 tensors, got {g.dtype} {g.layout}")
-        if g.device != grads[0].device:
-            raise ValueError(f"{what}: tensors on {grads[0].device} and {g.device}")
-        by_type.setdefault(g.dtype, []).append(g)
-    return by_type
-
-
 class _Lists:
-    """The tensors of one type as the library takes them."""
+    """Dense tensors of one type as the library takes them: their addresses (0: left out) and sizes."""
 
     def __init__(self, dtype, ptrs, numels):
-        self.n = len(ptrs)
-        self.type = _lib.i32(_TYPES[dtype])
-        self.ptrs = (_lib.vp * self.n)(*ptrs)
-        self.numel = (_lib.i64 * self.n)(*numels)
+        self.n, self.type = _lib.i32(len(ptrs)), _lib.i32(_TYPES[dtype])
+        self.numel = array("q", numels)
+        self.set(ptrs)
+
+    def set(self, ptrs):
+        self.ptrs = array("Q", ptrs)
+
+    def address(self) -> int:
+        return self.ptrs.buffer_info()[0]
 
     def parts(self) -> int:
-        return int(_lib.load().e2v2_grad_norm_parts(self.numel, _lib.i32(self.n)))
+        return int(_lib.load().e2v2_grad_norm_parts(_lib.vp(self.numel.buffer_info()[0]), self.n))
 
     def norm(self, parts, count, st):
-        _lib.call("e2v2_grad_norm", self.ptrs, self.numel, _lib.i32(self.n), self.type, _lib.vp(parts.data_ptr()),
-                  _lib.i32(parts.numel()), C.byref(count), st)
+        _lib.call("e2v2_grad_norm", _lib.vp(self.address()), _lib.vp(self.numel.buffer_info()[0]), self.n, self.type,
+                  _lib.vp(parts.data_ptr()), _lib.i32(parts.numel()), C.byref(count), st)
+
+    def scale(self, parts, count, max_norm, norm, st):
+        _lib.call("e2v2_grad_scale", _lib.vp(self.address()), _lib.vp(self.numel.buffer_info()[0]), self.n, self.type,
+                  _lib.vp(parts.data_ptr()), count, _lib.f32(max_norm), _lib.vp(norm.data_ptr()), st)
 
 
-def _norm_parts(by_type, st):
-    lists = [_Lists(d, [g.data_ptr() for g in gs], [g.numel() for g in gs]) for d, gs in by_type.items()]
-    dev = next(iter(by_type.values()))[0].device
-    parts = torch.empty(max(1, sum(l.parts() for l in lists)), dtype=torch.float64, device=dev)
+def _check(ts, what: str):
+    """One GPU, known types, dense: the device and the tensors made contiguous.  A few hundred tensors pass here every
+    step, so that each property is one comprehension."""
+    devices, types = {t.device for t in ts}, {t.dtype for t in ts}
+    for d in devices:
+        if d.type != "cuda":
+            raise RuntimeError(f"{what} runs on the GPU only (HIP library, no CPU path): got a tensor on {d}")
+    if len(devices) > 1:
+        raise ValueError(f"{what}: tensors on {' and '.join(sorted(map(str, devices)))}")
+    layouts = {t.layout for t in ts} - {torch.strided}
+    if layouts or not types <= _TYPES.keys():
+        raise ValueError(f"{what}: dense fp32, bf16 or fp16 tensors, got {', '.join(map(str, [*layouts, *types]))}")
+    if not all([t.is_contiguous() for t in ts]):
+        ts = [t.contiguous() for t in ts]
+    return devices.pop(), types, ts
+
+
+def _norm_parts(ts, types, dev, st):
+    """The lists by type, and their norm's partial sums."""
+    lists = []
+    for d in types:
+        of = ts if len(types) == 1 else [t for t in ts if t.dtype == d]
+        lists.append(_Lists(d, [t.data_ptr() for t in of], [t.numel() for t in of]))
+    parts = torch.empty(max(1, sum([l.parts() for l in lists])), dtype=torch.float64, device=dev)
     count = C.c_int(0)
     for l in lists:
         l.norm(parts, count, st)
     return lists, parts, count
+
+
+def _on(dev):
+    """A context with dev as the current device."""
+    return nullcontext() if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
 
 
 def grad_norm(tensors: Iterable[torch.Tensor]) -> torch.Tensor:
@@ -76,13 +92,12 @@ def grad_norm(tensors: Iterable[torch.Tensor]) -> torch.Tensor:
     ts = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
     if not ts:
         return torch.zeros((), device="cuda")
-    by_type = {d: [t.contiguous() for t in v] for d, v in _check(ts, "grad_norm").items()}
-    dev = ts[0].device
+    dev, types, ts = _check(ts, "grad_norm")
     out = torch.empty((), dtype=torch.float32, device=dev)
-    with torch.cuda.device(dev):
+    with _on(dev):
         st = _lib.stream(dev)
-        _, parts, count = _norm_parts(by_type, st)
-        _lib.call("e2v2_grad_norm_value", _lib.vp(parts.data_ptr()), _lib.i32(count.value), _lib.vp(out.data_ptr()), st)
+        _, parts, count = _norm_parts(ts, types, dev, st)
+        _lib.call("e2v2_grad_norm_value", _lib.vp(parts.data_ptr()), count, _lib.vp(out.data_ptr()), st)
     return out
 
 
@@ -93,23 +108,21 @@ def clip_grad_norm_(parameters, max_norm: float) -> torch.Tensor:
     max_norm = float(max_norm)
     if not max_norm >= 0:
         raise ValueError(f"clip_grad_norm_: max_norm {max_norm}")
-    grads = _tensors(parameters)
+    parameters = [parameters] if isinstance(parameters, torch.Tensor) else parameters
+    grads = [g for g in [p.grad for p in parameters] if g is not None]
     if not grads:
         return torch.zeros((), device="cuda" if torch.cuda.is_available() else None)
-    _check(grads, "clip_grad_norm_")
-    dense = [g.contiguous() for g in grads]
-    by_type = _check(dense, "clip_grad_norm_")
-    dev = grads[0].device
+    dev, types, dense = _check(grads, "clip_grad_norm_")
     out = torch.zeros((), dtype=torch.float32, device=dev)
-    with torch.cuda.device(dev):
+    with _on(dev):
         st = _lib.stream(dev)
-        lists, parts, count = _norm_parts(by_type, st)
+        lists, parts, count = _norm_parts(dense, types, dev, st)
         for l in lists:
-            _lib.call("e2v2_grad_scale", l.ptrs, l.numel, _lib.i32(l.n), l.type, _lib.vp(parts.data_ptr()), count,
-                      _lib.f32(max_norm), _lib.vp(out.data_ptr()), st)
-    for g, d in zip(grads, dense):
-        if d is not g:
-            g.copy_(d)
+            l.scale(parts, count, max_norm, out, st)
+    if dense is not grads:
+        for g, d in zip(grads, dense):
+            if d is not g:
+                g.copy_(d)
     torch.autograd.graph.increment_version(grads)
     return out
 
@@ -135,7 +148,7 @@ class _Launch:
     def __init__(self, group, dtype, params, first_tensor, chunk0, n_chunks):
         self.group, self.dtype, self.params = group, dtype, params
         self.first_tensor, self.chunk0, self.n_chunks = first_tensor, chunk0, n_chunks
-        self.grads = _Lists(dtype, [None] * len(params), [p.numel() for p in params])
+        self.grads = _Lists(dtype, [0] * len(params), [p.numel() for p in params])
         self.args = _lib.AdamWArgs()
 
 
@@ -194,7 +207,6 @@ class _Plan:
             a = l.args
             a.chunks = self.chunks.data_ptr() + l.chunk0 * C.sizeof(_lib.OptChunk)
             a.steps = self.steps.data_ptr() + l.chunk0 * 4
-            a.grads = C.addressof(l.grads.ptrs)
             a.m, a.v = self.m.data_ptr(), self.v.data_ptr()
             if bits == 8:
                 a.ms, a.vs = self.ms.data_ptr(), self.vs.data_ptr()
@@ -341,7 +353,7 @@ class AdamW(torch.optim.Optimizer):
             return (plan.m, plan.v) if dtype is None else (plan.m.to(dtype), plan.v.to(dtype))
         dtype = dtype or torch.float32
         m, v = (torch.empty(plan.total, dtype=dtype, device=plan.device) for _ in range(2))
-        with torch.cuda.device(plan.device):
+        with _on(plan.device):
             _lib.call("e2v2_moments", *(_lib.vp(t.data_ptr()) for t in (plan.m, plan.ms, plan.v, plan.vs, m, v)),
                       _lib.i32(_TYPES[dtype]), _lib.i64(plan.total), _lib.stream(plan.device))
         return m, v
@@ -360,11 +372,8 @@ class AdamW(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         plan = self._current()
-        if torch.cuda.current_device() == plan.device.index:
+        with _on(plan.device):
             self._launch(plan)
-        else:
-            with torch.cuda.device(plan.device):
-                self._launch(plan)
         return loss
 
     def _launch(self, plan: _Plan):
@@ -374,18 +383,21 @@ class AdamW(torch.optim.Optimizer):
             self._skipped = torch.zeros((), dtype=torch.int32, device=plan.device)
         _refuse(plan.outside)
         count = C.c_int(0)
-        keep = []
+        keep, updated = [], []
         for l in plan.launches:
             grads = [p.grad for p in l.params]
-            for i, g in enumerate(grads):
-                if g is None:
-                    continue
-                if g.dtype != l.dtype or g.layout != torch.strided:
-                    raise ValueError(f"AdamW: a gradient of type {g.dtype} {g.layout} for a parameter in {l.dtype}")
-                if not g.is_contiguous():
-                    grads[i] = g.contiguous()
-            keep.append(grads)
-            l.grads.ptrs[:] = [None if g is None else g.data_ptr() for g in grads]
+            some = [g for g in grads if g is not None]
+            if some:
+                dev, types, dense = _check(some, "AdamW")
+                if dev != plan.device or types != {l.dtype}:
+                    raise ValueError(f"AdamW: gradients of type {types} on {dev} for parameters in {l.dtype} on {plan.device}")
+                updated += [p for p in l.params if p.grad is not None] if len(some) < len(grads) else l.params
+                it = iter(dense)
+                l.grads.set([next(it).data_ptr() if g is not None else 0 for g in grads] if len(some) < len(grads)
+                            else [g.data_ptr() for g in dense])
+                keep.append(dense)
+            else:
+                l.grads.set([0] * len(grads))
             if normed:
                 l.grads.norm(plan.parts, count, st)
         if normed and not count.value:
@@ -393,6 +405,7 @@ class AdamW(torch.optim.Optimizer):
         norm = plan.norm.data_ptr()
         for l in plan.launches:
             a, g = l.args, l.group
+            a.grads = l.grads.address()
             lr = g["lr"]
             if isinstance(lr, torch.Tensor) and lr.device == plan.device and lr.dtype == torch.float32:
                 a.lr_dev, a.lr = lr.data_ptr(), 0.0
@@ -407,5 +420,4 @@ class AdamW(torch.optim.Optimizer):
             a.skipped = self._skipped.data_ptr() if self.skip_nonfinite else None
             _lib.call("e2v2_adamw", C.byref(a), st)
         # what is kept per weight version (packed weights, radial tables) is made anew
-        torch.autograd.graph.increment_version([p for l, grads in zip(plan.launches, keep)
-                                                for p, g in zip(l.params, grads) if g is not None])
+        torch.autograd.graph.increment_version(updated)
