@@ -58,6 +58,21 @@ def test_rows_that_are_copied(shape, stride):
     assert u.is_contiguous() and ld == shape[-1] and torch.equal(u, t)
 
 
+def test_arguments_as_bytes():
+    """What _args packs is e2v2_layer_norm_args field by field."""
+    x, g, b, st = torch.zeros(3, 8), torch.zeros(8), torch.zeros(8, dtype=torch.bfloat16), torch.zeros(3, 2)
+    gy, qx, y, gx = (torch.zeros(3, 8) for _ in range(4))
+    gy = torch.zeros(3, 16)[:, :8]
+    raw, keep = norms._args(x, g, b, st, 0.5, gy=gy, qx=qx, qg=g, qb=b, y=y, gx=gx)
+    assert len(raw) == _lib.C.sizeof(_lib.LayerNormArgs)
+    a = _lib.LayerNormArgs.from_buffer_copy(raw)
+    want = dict(x=x, gy=gy, qx=qx, g=g, b=b, qg=g, qb=b, y=y, gx=gx, stats=st)
+    assert all(getattr(a, k) == t.data_ptr() for k, t in want.items())
+    assert (a.n, a.ldx, a.ldgy, a.ldqx, a.w, a.type, a.g_type, a.b_type, a.eps) == (3, 8, 16, 8, 8, 0, 0, 1, 0.5)
+    a = _lib.LayerNormArgs.from_buffer_copy(norms._args(x, None, None, None, 0.5)[0])
+    assert a.g is None and a.gy is None and a.stats is None and a.ldgy == 0
+
+
 def test_entry_point_checks():
     lib = _lib.load()
     a = _lib.LayerNormArgs()

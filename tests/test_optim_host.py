@@ -85,5 +85,14 @@ def test_entry_point_checks():
     assert lib.e2v2_moments(v, None, v, v, v, v, 0, _lib.i64(32), None) != 0
 
 
-def test_chunk_layout():
-    assert _lib.C.sizeof(_lib.OptChunk) == 32 and _lib.OptChunk.n.offset == 24
+def test_chunk_table():
+    """Every element of every tensor in one chunk, in order, in the layout of e2v2_opt_chunk."""
+    sizes, ptrs = [5, 0, 4096, 4097, 20000], [1 << 40, 64, 128, 256, 512]
+    offs = [0, 64, 64, 4160, 8320]
+    t, first = optim._chunk_table(ptrs, offs, sizes)
+    assert first == [0, 1, 1, 2, 4] and len(t) == 9 and t.dtype.itemsize == _lib.C.sizeof(_lib.OptChunk) == 32
+    rows = (_lib.OptChunk * len(t)).from_buffer_copy(t.tobytes())
+    got = [(r.p, r.at, r.off, r.n, r.tensor) for r in rows]
+    assert got == [(ptrs[k], at, offs[k] + at, min(4096, n - at), k) for k, n in enumerate(sizes)
+                   for at in range(0, n, 4096)]
+    assert [len(x) for x in optim._chunk_table([], [], [])] == [0, 0]

@@ -7,6 +7,7 @@ The equivariant RMS norm is in ``modules`` / ``second_order``, the fused LayerNo
 ``second_order.ln_silu``.  There is no CPU path."""
 from __future__ import annotations
 
+import struct
 from typing import Optional
 
 import torch
@@ -20,7 +21,7 @@ _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
 def _ptr(t: Optional[torch.Tensor]):
-    return None if t is None else t.data_ptr()
+    return None if t is None else _lib.vp(t.data_ptr())
 
 
 def _rows(t: torch.Tensor):
@@ -56,19 +57,26 @@ def _will_run(node) -> bool:
         return True
 
 
+# e2v2_layer_norm_args as bytes: packing them is a few times faster than filling a ctypes structure
+_ARGS = struct.Struct("10Q4q4if4x")
+
+
 def _args(x, g, b, stats, eps, gy=None, qx=None, qg=None, qb=None, y=None, gx=None):
     """The kernels' arguments, and the copies that have to live until the call is enqueued."""
     w = x.shape[-1]
-    keep, ld = [], []
-    for t in (x, gy, qx):
-        u, s = (None, 0) if t is None else _rows(t)
-        keep.append(u)
-        ld.append(s)
-    p = [None if t is None else t.contiguous() for t in (g, b, qg, qb)]
-    gt, bt = (_TYPES[torch.float32 if t is None else t.dtype] for t in (g, b))
-    a = _lib.LayerNormArgs(*map(_ptr, keep), *map(_ptr, p), _ptr(y), _ptr(gx), _ptr(stats), x.numel() // w, *ld, w,
-                           _TYPES[x.dtype], gt, bt, eps)
-    return a, keep + p
+    rows, ld = [x, gy, qx], [0, 0, 0]
+    for k in range(3):
+        if rows[k] is not None:
+            rows[k], ld[k] = _rows(rows[k])
+    params = [t if t is None or t.is_contiguous() else t.contiguous() for t in (g, b, qg, qb)]
+    a = _ARGS.pack(*[0 if t is None else t.data_ptr() for t in (*rows, *params, y, gx, stats)], x.numel() // w, *ld, w,
+                   _TYPES[x.dtype], 0 if g is None else _TYPES[g.dtype], 0 if b is None else _TYPES[b.dtype], eps)
+    return a, (rows, params)
+
+
+def _empty_rows(x):
+    """A contiguous tensor of x's shape and type."""
+    return torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
 
 
 def _workspace(x):
@@ -85,16 +93,29 @@ def _call(name, dev, *args):
         _lib.call(name, *args, _lib.stream(dev))
 
 
+def _forward(x, g, b, eps, stats):
+    y = _empty_rows(x)
+    a, keep = _args(x, g, b, stats, eps, y=y)
+    _call("e2v2_layer_norm_fwd", x.device, a)
+    return y
+
+
+def _backward(gy, x, g, b, stats, eps, need_g, need_b):
+    gx = _empty_rows(x)
+    gg = torch.empty(g.shape, dtype=g.dtype, device=x.device) if need_g else None
+    gb = torch.empty(b.shape, dtype=b.dtype, device=x.device) if need_b else None
+    ws, n = _workspace(x) if need_g or need_b else (None, 0)
+    a, keep = _args(x, g, b, stats, eps, gy=gy, gx=gx)
+    _call("e2v2_layer_norm_bwd", x.device, a, _ptr(gg), _ptr(gb), _ptr(ws), _lib.i64(n))
+    return gx, gg, gb
+
+
 class _LayerNormFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, g, b, eps: float):
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        stats = None
-        if any(ctx.needs_input_grad):
-            stats = torch.empty(x.numel() // x.shape[-1], 2, dtype=torch.float32, device=x.device)
-        a, keep = _args(x, g, b, stats, eps, y=y)
-        _call("e2v2_layer_norm_fwd", x.device, _lib.C.byref(a))
+        stats = torch.empty(x.numel() // x.shape[-1], 2, dtype=torch.float32, device=x.device)
+        y = _forward(x, g, b, eps, stats)
         ctx.save_for_backward(x, g, b, stats)
         ctx.eps = eps
         return y
@@ -102,26 +123,18 @@ class _LayerNormFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, gy):
         x, g, b, stats = ctx.saved_tensors
-        # next_functions has an entry for each tensor among the inputs; the sums of weight and bias come together
-        nodes = iter(ctx.next_functions[1:])
-        need = [ctx.needs_input_grad[1 + k] and t is not None for k, t in enumerate((g, b))]
-        nodes = [None if t is None else next(nodes)[0] for t in (g, b)]
-        if True in need and not any(n and _will_run(node) for n, node in zip(need, nodes)):
-            need = [False, False]
-        gx, gg, gb = (_LayerNormGradFn.apply if torch.is_grad_enabled() else _layer_norm_grad)(
-            gy, x, g, b, stats, ctx.eps, *need)
+        need_g, need_b = ctx.needs_input_grad[1:3]
+        if not torch.is_grad_enabled():
+            gx, gg, gb = _backward(gy, x, g, b, stats, ctx.eps, need_g, need_b)
+        else:
+            # the forces' first differentiation asks for neither weight nor bias; their sums come together.
+            # next_functions has an entry for each tensor among the inputs
+            nodes = iter(ctx.next_functions[1:])
+            nodes = [next(nodes)[0] for t in (g, b) if t is not None]
+            if not any([_will_run(n) for n in nodes]):
+                need_g = need_b = False
+            gx, gg, gb = _LayerNormGradFn.apply(gy, x, g, b, stats, ctx.eps, need_g, need_b)
         return gx if ctx.needs_input_grad[0] else None, gg, gb, None
-
-
-def _layer_norm_grad(gy, x, g, b, stats, eps, need_g, need_b):
-    gx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    gg = torch.empty(g.shape, dtype=g.dtype, device=x.device) if need_g else None
-    gb = torch.empty(b.shape, dtype=b.dtype, device=x.device) if need_b else None
-    ws, n = _workspace(x) if need_g or need_b else (None, 0)
-    a, keep = _args(x, g, b, stats, eps, gy=gy, gx=gx)
-    _call("e2v2_layer_norm_bwd", x.device, _lib.C.byref(a), _lib.vp(_ptr(gg)), _lib.vp(_ptr(gb)), _lib.vp(_ptr(ws)),
-          _lib.i64(n))
-    return gx, gg, gb
 
 
 class _LayerNormGradFn(torch.autograd.Function):
@@ -130,7 +143,7 @@ class _LayerNormGradFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, gy, x, g, b, stats, eps, need_g, need_b):
-        out = _layer_norm_grad(gy, x, g, b, stats, eps, need_g, need_b)
+        out = _backward(gy, x, g, b, stats, eps, need_g, need_b)
         ctx.save_for_backward(gy, x, g, b, stats)
         ctx.eps = eps
         ctx.set_materialize_grads(False)
@@ -142,11 +155,11 @@ class _LayerNormGradFn(torch.autograd.Function):
         gy, x, g, b, stats = ctx.saved_tensors
         if qx is None and qg is None and qb is None:
             return (None,) * 8
-        dgy, dx = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for _ in range(2))
-        dg = torch.empty_like(g, memory_format=torch.contiguous_format) if ctx.needs_input_grad[2] else None
+        dgy, dx = _empty_rows(x), _empty_rows(x)
+        dg = torch.empty(g.shape, dtype=g.dtype, device=x.device) if ctx.needs_input_grad[2] else None
         ws, n = _workspace(x) if dg is not None else (None, 0)
         a, keep = _args(x, g, b, stats, ctx.eps, gy=gy, qx=qx, qg=qg, qb=qb, y=dgy, gx=dx)
-        _call("e2v2_layer_norm_bwd2", x.device, _lib.C.byref(a), _lib.vp(_ptr(dg)), _lib.vp(_ptr(ws)), _lib.i64(n))
+        _call("e2v2_layer_norm_bwd2", x.device, a, _ptr(dg), _ptr(ws), _lib.i64(n))
         return dgy, dx, dg, None, None, None, None, None
 
 
@@ -170,4 +183,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
         if p is not None and (p.shape != (w,) or p.dtype not in (torch.float32, x.dtype) or p.device != x.device):
             raise ValueError(f"layer_norm: {name} [{w}] in fp32 or {x.dtype} on {x.device}, got {tuple(p.shape)} "
                              f"{p.dtype} on {p.device}")
-    return _LayerNormFn.apply(x, weight, bias, float(eps))
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
+                                    or (bias is not None and bias.requires_grad)):
+        return _LayerNormFn.apply(x, weight, bias, float(eps))
+    return _forward(x, weight, bias, float(eps), None)

@@ -14,6 +14,7 @@ from contextlib import nullcontext
 from itertools import chain
 from typing import Iterable, Optional, Tuple, Union
 
+import numpy as np
 import torch
 
 from . import _lib
@@ -51,21 +52,31 @@ class _Lists:
                   _lib.vp(parts.data_ptr()), count, _lib.f32(max_norm), _lib.vp(norm.data_ptr()), st)
 
 
-def _check(ts, what: str):
-    """One GPU, known types, dense: the device and the tensors made contiguous.  A few hundred tensors pass here every
-    step, so that each property is one comprehension."""
-    devices, types = {t.device for t in ts}, {t.dtype for t in ts}
-    for d in devices:
-        if d.type != "cuda":
-            raise RuntimeError(f"{what} runs on the GPU only (HIP library, no CPU path): got a tensor on {d}")
-    if len(devices) > 1:
-        raise ValueError(f"{what}: tensors on {' and '.join(sorted(map(str, devices)))}")
-    layouts = {t.layout for t in ts} - {torch.strided}
-    if layouts or not types <= _TYPES.keys():
-        raise ValueError(f"{what}: dense fp32, bf16 or fp16 tensors, got {', '.join(map(str, [*layouts, *types]))}")
-    if not all([t.is_contiguous() for t in ts]):
+def _dense(ts, what: str):
+    """The tensors in known types and contiguous (copies where they are not), and their types.  A few hundred pass here every
+    step: each property is read in one sweep."""
+    types = {t.dtype for t in ts}
+    try:
+        contiguous = all(map(torch.Tensor.is_contiguous, ts))
+    except RuntimeError:                       # sparse tensors do not answer
+        contiguous = False
+    if not contiguous or not types <= _TYPES.keys():
+        layouts = {t.layout for t in ts} - {torch.strided}
+        if layouts or not types <= _TYPES.keys():
+            raise ValueError(f"{what}: dense fp32, bf16 or fp16 tensors, got {', '.join(map(str, [*layouts, *types]))}")
         ts = [t.contiguous() for t in ts]
-    return devices.pop(), types, ts
+    return types, ts
+
+
+def _check(ts, what: str):
+    """As _dense, for tensors that have to lie on one GPU, which comes first."""
+    devices = set(map(torch.Tensor.get_device, ts))
+    if -1 in devices:
+        raise RuntimeError(f"{what} runs on the GPU only (HIP library, no CPU path): got a tensor on "
+                           f"{next(t.device for t in ts if not t.is_cuda)}")
+    if len(devices) > 1:
+        raise ValueError(f"{what}: tensors on the GPUs {sorted(devices)}")
+    return ts[0].device, *_dense(ts, what)
 
 
 def _norm_parts(ts, types, dev, st):
@@ -152,6 +163,21 @@ class _Launch:
         self.args = _lib.AdamWArgs()
 
 
+def _chunk_table(ptrs, offs, sizes):
+    """The e2v2_opt_chunk table of tensors at ptrs whose moments start at offs, and each tensor's first chunk."""
+    counts = np.array([-(-n // _CHUNK) for n in sizes], np.int64)
+    first = np.cumsum(counts) - counts
+    which = np.repeat(np.arange(len(sizes)), counts)
+    t = np.zeros(len(which), np.dtype([("p", np.uint64), ("at", np.int64), ("off", np.int64), ("n", np.int32),
+                                       ("tensor", np.int32)]))
+    t["p"] = np.array(ptrs, np.uint64)[which]
+    t["at"] = (np.arange(len(which)) - first[which]) * _CHUNK
+    t["off"] = np.array(offs, np.int64)[which] + t["at"]
+    t["n"] = np.minimum(np.array(sizes, np.int64)[which] - t["at"], _CHUNK)
+    t["tensor"] = which
+    return t, first.tolist()
+
+
 class _Plan:
     """What stays from step to step: moments and step counts of all parameters, the chunks' table, the launches."""
 
@@ -172,17 +198,15 @@ class _Plan:
         self.ptrs = [p.data_ptr() for p in params]
         self.params = params
         bits = opt.state_bits
-        off, self.offs = 0, []
-        for p in params:
-            self.offs.append(off)
-            off += -(-p.numel() // _ALIGN) * _ALIGN
-        self.total = off
-        place = dict(zip(params, self.offs))
+        sizes = [p.numel() for p in params]
+        ends = np.cumsum([0] + [-(-n // _ALIGN) * _ALIGN for n in sizes]).tolist()
+        self.total = ends[-1]
+        place = dict(zip(params, ends))
         dt = torch.float32 if bits == 32 else torch.uint8
-        self.m, self.v = (torch.zeros(off, dtype=dt, device=dev) for _ in range(2))
-        self.ms, self.vs = ((torch.zeros(off // _RUN, dtype=torch.uint8, device=dev) for _ in range(2)) if bits == 8
-                            else (None, None))
-        table, first, self.launches, tensors = [], {}, [], 0
+        self.m, self.v = (torch.zeros(self.total, dtype=dt, device=dev) for _ in range(2))
+        self.ms, self.vs = ((torch.zeros(self.total // _RUN, dtype=torch.uint8, device=dev) for _ in range(2))
+                            if bits == 8 else (None, None))
+        self.launches, order, chunks = [], [], 0
         for group in groups:
             by_type = {}
             for p in group["params"]:
@@ -190,17 +214,15 @@ class _Plan:
                     by_type.setdefault(p.dtype, []).append(p)
             for dtype, ps in by_type.items():
                 for k in range(0, len(ps), _LIST):
-                    part, chunk0 = ps[k:k + _LIST], len(table)
-                    for j, p in enumerate(part):
-                        first[p] = len(table)
-                        table += [(p.data_ptr(), at, place[p] + at, min(_CHUNK, p.numel() - at), tensors + j)
-                                  for at in range(0, p.numel(), _CHUNK)]
-                    self.launches.append(_Launch(group, dtype, part, tensors, chunk0, len(table) - chunk0))
-                    tensors += len(part)
-        n = len(table)
-        host = (_lib.OptChunk * max(n, 1))(*table)
-        self.chunks = torch.frombuffer(bytearray(host), dtype=torch.uint8).to(dev)
-        self.steps = torch.zeros(max(n, 1), dtype=torch.int32, device=dev)
+                    part = ps[k:k + _LIST]
+                    n = sum([-(-p.numel() // _CHUNK) for p in part])
+                    self.launches.append(_Launch(group, dtype, part, len(order), chunks, n))
+                    order += part
+                    chunks += n
+        table, first = _chunk_table([p.data_ptr() for p in order], [place[p] for p in order], [p.numel() for p in order])
+        self.chunks = torch.from_numpy(table.view(np.uint8)).to(dev)
+        self.steps = torch.zeros(max(len(table), 1), dtype=torch.int32, device=dev)
+        first = dict(zip(order, first))
         self.parts = torch.empty(max(1, sum(l.grads.parts() for l in self.launches)), dtype=torch.float64, device=dev)
         self.norm = torch.zeros((), dtype=torch.float32, device=dev)
         for l in self.launches:
@@ -213,18 +235,20 @@ class _Plan:
             a.n_chunks, a.n_tensors, a.first_tensor = l.n_chunks, len(l.params), l.first_tensor
             a.type, a.bits, a.seed = _TYPES[l.dtype], bits, opt.seed & 0xFFFFFFFF
         olds = [(p, opt.state.get(p)) for p in params]
-        taken = torch.stack([torch.as_tensor(old["step"]).to(dev, torch.int32).view(()) for _, old in olds if old]
-                            or [torch.zeros((), dtype=torch.int32)])
-        taken = iter(taken.unbind(0))
-        for p, old in olds:
-            opt.state[p] = st = self._views(p, place[p], first.get(p, 0))
-            if old:
-                step = next(taken)
-                st["step"].copy_(step)
-                self.steps[first[p]:first[p] + -(-p.numel() // _CHUNK)] = step
-                for k in st:
-                    if k != "step":
-                        st[k].copy_(old[k])
+        for p, _ in olds:
+            opt.state[p] = self._views(p, place[p], first[p])
+        olds = [(p, old) for p, old in olds if old]
+        if olds:
+            steps = torch.stack([torch.as_tensor(old["step"]).to(dev, torch.int32).view(()) for _, old in olds])
+            where = [torch.arange(first[p], first[p] - (-p.numel() // _CHUNK)) for p, _ in olds]
+            self.steps[torch.cat(where).to(dev)] = steps.repeat_interleave(
+                torch.tensor([len(w) for w in where], device=dev))
+            for (p, old), step in zip(olds, steps):
+                if not p.numel():
+                    opt.state[p]["step"].copy_(step)
+            keys = [k for k in opt.state[olds[0][0]] if k != "step"]
+            pairs = [(opt.state[p][k], old[k]) for p, old in olds for k in keys]
+            torch._foreach_copy_([d for d, _ in pairs], [o for _, o in pairs])
 
     def _views(self, p, o, chunk):
         """The parameter's state: views of the plan's buffers."""
@@ -258,7 +282,7 @@ class AdamW(torch.optim.Optimizer):
     is not finite and counts such steps in ``skipped``.  ``grad_norm`` is the last step's norm (None without either).
 
     A step after the first can be captured into a graph and replayed: step counts are on the device.  ``state`` entries are
-    views of flat buffers: write into them in place, or through load_state_dict."""
+    views of flat buffers: moments can be written in place, step counts through load_state_dict."""
 
     _plan: Optional[_Plan] = None
     _OPTIONS = ("state_bits", "max_norm", "skip_nonfinite", "seed")
@@ -361,7 +385,7 @@ class AdamW(torch.optim.Optimizer):
     def _current(self) -> _Plan:
         """The plan, made anew where parameters moved."""
         plan = self._plan
-        if plan is None or [p.data_ptr() for p in plan.params] != plan.ptrs:
+        if plan is None or list(map(torch.Tensor.data_ptr, plan.params)) != plan.ptrs:
             self._plan = plan = _Plan(self)
         return plan
 
@@ -388,13 +412,14 @@ class AdamW(torch.optim.Optimizer):
             grads = [p.grad for p in l.params]
             some = [g for g in grads if g is not None]
             if some:
-                dev, types, dense = _check(some, "AdamW")
-                if dev != plan.device or types != {l.dtype}:
-                    raise ValueError(f"AdamW: gradients of type {types} on {dev} for parameters in {l.dtype} on {plan.device}")
+                # a gradient lies on its parameter's device (torch sees to it where it is set)
+                types, dense = _dense(some, "AdamW")
+                if types != {l.dtype}:
+                    raise ValueError(f"AdamW: gradients of type {types} for parameters in {l.dtype}")
                 updated += [p for p in l.params if p.grad is not None] if len(some) < len(grads) else l.params
                 it = iter(dense)
-                l.grads.set([next(it).data_ptr() if g is not None else 0 for g in grads] if len(some) < len(grads)
-                            else [g.data_ptr() for g in dense])
+                l.grads.set([0 if g is None else next(it).data_ptr() for g in grads] if len(some) < len(grads)
+                            else map(torch.Tensor.data_ptr, dense))
                 keep.append(dense)
             else:
                 l.grads.set([0] * len(grads))
