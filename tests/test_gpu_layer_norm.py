@@ -59,7 +59,7 @@ def _check_first(x, gy, w, b, y, gx, gg, gb):
         assert (got.double() - ref).abs().le(tol).all(), "parameters"
 
 
-WIDTHS = [1, 2, 3, 16, 17, 32, 64, 65, 100, 128, 129, 255, 256, 257, 512, 520, 1000, 1024, 1025, 1032, 2048, 2049, 4096,
+WIDTHS = [1, 2, 3, 5, 8, 9, 16, 17, 31, 32, 33, 64, 65, 100, 128, 129, 255, 256, 257, 512, 520, 1000, 1024, 1025, 1032, 2048, 2049, 4096,
           4097, 4104, 5001, 8192, 8193, 16383, 16384]
 
 
@@ -80,7 +80,7 @@ def test_values_and_first_order(pkg, cuda, w, dtype, wdtype):
         _check_first(x, gy, wt, b, y, gx, gg, gb)
 
 
-@pytest.mark.parametrize("w", [1, 24, 128, 129, 1000])
+@pytest.mark.parametrize("w", [1, 7, 15, 24, 60, 128, 129, 300, 1000])
 def test_many_rows(pkg, cuda, w):
     """More rows than a pass of all workgroups holds: each strides over several."""
     from ubio_molfm_amd import norms

@@ -11,7 +11,7 @@
 // statistics, row sums and the parameters' sums are fp32, the variance taken about the mean in a second pass over the
 // registers.
 //
-// One pass over memory: a row stays in the registers of kL lanes (16, 32 or 64 of a wavefront, or a workgroup of 256
+// One pass over memory: a row stays in the registers of kL lanes (2 to 64 of a wavefront, or a workgroup of 256
 // or 1024), read as 16-byte vectors on whatever element boundary the row starts (the hardware takes them unaligned), the
 // rest of a row element by element.  A workgroup strides over the rows and keeps its columns' parameter sums in registers; each
 // leaves one partial row, added in order by a second launch, so results repeat bitwise.  Bound: HBM.
@@ -92,7 +92,10 @@ template <int kL, int K>
 __device__ __forceinline__ void group_sum(float (&v)[K], float (*red)[4][16], int& turn) {
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    v[k] = dpp_row_sum16(v[k]);
+    if constexpr (kL >= 2) v[k] += dpp_mov<0xB1>(v[k]);    // lane ^ 1
+    if constexpr (kL >= 4) v[k] += dpp_mov<0x4E>(v[k]);    // lane ^ 2
+    if constexpr (kL >= 8) v[k] += dpp_mov<0x141>(v[k]);   // the other half of 8
+    if constexpr (kL >= 16) v[k] += dpp_mov<0x140>(v[k]);  // the other half of 16
     if constexpr (kL >= 32) v[k] = swap_sum<16>(v[k]);
     if constexpr (kL >= 64) v[k] = swap_sum<32>(v[k]);
   }
@@ -162,9 +165,10 @@ __device__ __forceinline__ void load_params(const void* p, int type, int l, int 
   }
 }
 
-// Adds the workgroup's row groups' parameter sums and writes them as partial row blockIdx.x.
+// Adds the workgroup's row groups' parameter sums (those of a wavefront in registers, then the four wavefronts') and
+// writes them as partial row blockIdx.x.
 template <int V, int kL, int NV>
-__device__ __forceinline__ void write_part(const float (&acc)[NV * V], int l, int rg, int w, float* out) {
+__device__ __forceinline__ void write_part(const float (&acc)[NV * V], int l, int w, float* out) {
   if constexpr (kL > 64) {
     each_vec<V, kL, NV>(l, [&](int k, int c) {
 #pragma unroll
@@ -172,20 +176,25 @@ __device__ __forceinline__ void write_part(const float (&acc)[NV * V], int l, in
         if (c + e < w) out[c + e] = acc[k * V + e];
     });
   } else {
-    constexpr int kR = 256 / kL, kC = kL * NV * V;
-    __shared__ float red[kR][kC];
+    constexpr int kC = kL * NV * V;
+    __shared__ float red[4][kC];
+    const int wv = threadIdx.x >> 6;
+    const bool mine = (threadIdx.x & 63) < kL;
     __syncthreads();
     each_vec<V, kL, NV>(l, [&](int k, int c) {
 #pragma unroll
-      for (int e = 0; e < V; ++e) red[rg][c + e] = acc[k * V + e];
+      for (int e = 0; e < V; ++e) {
+        float v = acc[k * V + e];
+        if constexpr (kL <= 2) v += dpp_mov<0x4E>(v);      // lane ^ 2
+        if constexpr (kL <= 4) v += dpp_mov<0x124>(v);     // four lanes round a row of 16
+        if constexpr (kL <= 8) v += dpp_mov<0x128>(v);     // eight lanes round
+        if constexpr (kL <= 16) v = swap_sum<16>(v);
+        if constexpr (kL <= 32) v = swap_sum<32>(v);
+        if (mine) red[wv][c + e] = v;
+      }
     });
     __syncthreads();
-    for (int c = threadIdx.x; c < w; c += 256) {
-      float s = 0.f;
-#pragma unroll
-      for (int r = 0; r < kR; ++r) s += red[r][c];
-      out[c] = s;
-    }
+    for (int c = threadIdx.x; c < w; c += 256) out[c] = (red[0][c] + red[1][c]) + (red[2][c] + red[3][c]);
   }
 }
 
@@ -271,8 +280,8 @@ __global__ __launch_bounds__(kL > 64 ? kL : 256) void k_layer_norm_bwd(LnArgs P)
     });
   }
   if (P.part) {
-    write_part<V, kL, NV>(ag, l, rg, w, P.part + (int64_t)blockIdx.x * w);
-    write_part<V, kL, NV>(ab, l, rg, w, P.part + ((int64_t)gridDim.x + blockIdx.x) * w);
+    write_part<V, kL, NV>(ag, l, w, P.part + (int64_t)blockIdx.x * w);
+    write_part<V, kL, NV>(ab, l, w, P.part + ((int64_t)gridDim.x + blockIdx.x) * w);
   }
 }
 
@@ -346,7 +355,7 @@ __global__ __launch_bounds__(kL > 64 ? kL : 256) void k_layer_norm_bwd2(LnArgs P
       store_row<T, V>(v, o2, c, w);
     });
   }
-  if (P.part) write_part<V, kL, NV>(ag, l, rg, w, P.part + (int64_t)blockIdx.x * w);
+  if (P.part) write_part<V, kL, NV>(ag, l, w, P.part + (int64_t)blockIdx.x * w);
 }
 
 // out_a[c] = the sum over the n_part rows of part [a][n_part][w], a = blockIdx.y: 32 lanes take every 32nd row, then
@@ -400,7 +409,7 @@ struct LnShape {
 
 LnShape ln_shape(int w, int v, bool fwd) {
   const int nv = (w + v - 1) / v;
-  if (nv <= 16) return {16, 1};
+  if (nv <= 16) return {nv <= 2 ? 2 : nv <= 4 ? 4 : nv <= 8 ? 8 : 16, 1};
   if (nv <= 32) return {32, 1};
   if (nv <= 48) return {16, 3};
   if (nv <= 64) return {64, 1};
@@ -420,6 +429,9 @@ void ln_dispatch(const LnArgs& P, unsigned grid, hipStream_t s) {
   constexpr bool kFwd = kPass == LnPass::kFwd;
   const LnShape f = ln_shape(P.w, V, kFwd);
   switch (f.lanes * 16 + f.vecs) {
+    case 2 * 16 + 1: return ln_launch<kPass, T, V, 2, 1>(P, grid, s);
+    case 4 * 16 + 1: return ln_launch<kPass, T, V, 4, 1>(P, grid, s);
+    case 8 * 16 + 1: return ln_launch<kPass, T, V, 8, 1>(P, grid, s);
     case 16 * 16 + 1: return ln_launch<kPass, T, V, 16, 1>(P, grid, s);
     case 32 * 16 + 1: return ln_launch<kPass, T, V, 32, 1>(P, grid, s);
     case 16 * 16 + 3: return ln_launch<kPass, T, V, 16, 3>(P, grid, s);

@@ -30,7 +30,7 @@ namespace {
 constexpr int kOptThreads = 256;
 constexpr int kOptChunk = E2V2_OPT_CHUNK;
 constexpr int kNormList = 256;         // gradients of a norm launch (a thread each finds the chunks' tensors)
-constexpr int kNormChunk = 8192;
+constexpr int kNormChunk = 4096;
 constexpr int kNormParts = 1024;       // workgroups of a norm launch at most
 constexpr int kStepList = 384;         // gradients of a step launch (3 KB of the 4 KB of kernel arguments)
 
