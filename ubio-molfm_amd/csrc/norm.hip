@@ -34,33 +34,71 @@ struct RowVec {
   typedef float ftype __attribute__((ext_vector_type(16 / sizeof(T))));
 };
 
-// Elements c .. c + V of a row of w; those past its end are zero.
-template <typename T, int V>
-__device__ __forceinline__ void load_row(const T* row, int c, int w, float* out) {
-  if (c + V <= w) {
-    const typename RowVec<T>::type v = *reinterpret_cast<const typename RowVec<T>::any*>(row + c);
-    const auto f = __builtin_convertvector(v, typename RowVec<T>::ftype);
+// The lane's columns: vector k starts at column (l + k kL) V.
+template <int V, int kL, int NV, typename F>
+__device__ __forceinline__ void each_vec(int l, F&& f) {
 #pragma unroll
-    for (int k = 0; k < V; ++k) out[k] = f[k];
-  } else {
-#pragma unroll
-    for (int k = 0; k < V; ++k) out[k] = c + k < w ? (float)row[c + k] : 0.f;
-  }
+  for (int k = 0; k < NV; ++k) f(k, (l + k * kL) * V);
 }
+
+// A lane's vectors of a row of w >= V elements (any w for V = 1).  All loads are unconditional, so that those of a row's operands
+// are in flight together: a vector that would pass the end starts V before it instead (a branch would wait for its load in
+// place: 100,000 x 129 fp32 backward 57 us).  get() then moves what belongs to the row down and clears the rest.
+template <typename T, int V, int kL, int NV>
+struct RowLoad {
+  typename RowVec<T>::type raw[V > 1 ? NV : 1];
+  T one[V > 1 ? 1 : NV];
+
+  __device__ __forceinline__ void load(const T* row, int l, int w) {
+    each_vec<V, kL, NV>(l, [&](int k, int c) {
+      if constexpr (V > 1) raw[k] = *reinterpret_cast<const typename RowVec<T>::any*>(row + min(c, w - V));
+      else one[k] = row[min(c, w - 1)];
+    });
+  }
+
+  __device__ __forceinline__ void get(int l, int w, float (&out)[NV * V]) const {
+    each_vec<V, kL, NV>(l, [&](int k, int c) {
+      if constexpr (V > 1) {
+        const auto f = __builtin_convertvector(raw[k], typename RowVec<T>::ftype);
+#pragma unroll
+        for (int e = 0; e < V; ++e) out[k * V + e] = f[e];
+      } else {
+        out[k] = (float)one[k];
+      }
+    });
+    if (w == kL * NV * V) return;
+    const int past = w % V ? V - w % V : 0;        // elements by which the row's last vector starts early
+    each_vec<V, kL, NV>(l, [&](int k, int c) {
+      float* v = out + k * V;
+      const bool moved = c < w && c + V > w;
+#pragma unroll
+      for (int d = V / 2; d > 0; d /= 2) {
+        if (past & d) {
+#pragma unroll
+          for (int e = 0; e < V; ++e) v[e] = moved ? (e + d < V ? v[e + d] : 0.f) : v[e];
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[e] = c < w ? v[e] : 0.f;
+    });
+  }
+};
 
 template <typename T, int V>
 __device__ __forceinline__ void store_row(const float* v, T* row, int c, int w) {
-  if (c + V <= w) {
-    typename RowVec<T>::ftype f;
+  if constexpr (V > 1) {
+    if (c + V <= w) {
+      typename RowVec<T>::ftype f;
 #pragma unroll
-    for (int k = 0; k < V; ++k) f[k] = v[k];
-    const typename RowVec<T>::type o = __builtin_convertvector(f, typename RowVec<T>::type);
-    *reinterpret_cast<typename RowVec<T>::any*>(row + c) = o;
-  } else {
-#pragma unroll
-    for (int k = 0; k < V; ++k)
-      if (c + k < w) row[c + k] = (T)v[k];
+      for (int k = 0; k < V; ++k) f[k] = v[k];
+      const typename RowVec<T>::type o = __builtin_convertvector(f, typename RowVec<T>::type);
+      *reinterpret_cast<typename RowVec<T>::any*>(row + c) = o;
+      return;
+    }
   }
+#pragma unroll
+  for (int k = 0; k < V; ++k)
+    if (c + k < w) row[c + k] = (T)v[k];
 }
 
 // v + its partner's, kLanes lanes away, by an exchange of rows of 16 lanes or of halves in registers (no trip through
@@ -127,13 +165,6 @@ struct LnArgs {
   int w, g_type, b_type;
   float eps;
 };
-
-// The lane's columns: vector k starts at column (l + k kL) V.
-template <int V, int kL, int NV, typename F>
-__device__ __forceinline__ void each_vec(int l, F&& f) {
-#pragma unroll
-  for (int k = 0; k < NV; ++k) f(k, (l + k * kL) * V);
-}
 
 template <typename W, int V, int kL, int NV>
 __device__ __forceinline__ void load_params_as(const W* p, int l, int w, float (&out)[NV * V]) {
@@ -211,11 +242,11 @@ __global__ __launch_bounds__(kL > 64 ? kL : 256) void k_layer_norm_fwd(LnArgs P)
   for (int64_t row = (int64_t)blockIdx.x * kR + rg; row < P.n; row += (int64_t)gridDim.x * kR) {
     const T* xr = static_cast<const T*>(P.x) + row * P.ldx;
     float x[E], s[1] = {0.f}, q[1] = {0.f};
-    each_vec<V, kL, NV>(l, [&](int k, int c) {
-      load_row<T, V>(xr, c, w, x + k * V);
+    RowLoad<T, V, kL, NV> rx;
+    rx.load(xr, l, w);
+    rx.get(l, w, x);
 #pragma unroll
-      for (int e = 0; e < V; ++e) s[0] += x[k * V + e];
-    });
+    for (int e = 0; e < E; ++e) s[0] += x[e];
     group_sum<kL, 1>(s, red, turn);
     const float mean = s[0] / (float)w;       // a true quotient: exact for a row of one short value
     each_vec<V, kL, NV>(l, [&](int k, int c) {
@@ -254,9 +285,12 @@ __global__ __launch_bounds__(kL > 64 ? kL : 256) void k_layer_norm_bwd(LnArgs P)
     const T* gr = static_cast<const T*>(P.gy) + row * P.ldgy;
     const float2 st = *reinterpret_cast<const float2*>(P.stats + 2 * row);
     float xh[E], gy[E], s[2] = {0.f, 0.f};
+    RowLoad<T, V, kL, NV> rx, ry;
+    rx.load(xr, l, w);
+    ry.load(gr, l, w);
+    rx.get(l, w, xh);
+    ry.get(l, w, gy);
     each_vec<V, kL, NV>(l, [&](int k, int c) {
-      load_row<T, V>(xr, c, w, xh + k * V);
-      load_row<T, V>(gr, c, w, gy + k * V);
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         float& h = xh[k * V + e];
@@ -306,12 +340,16 @@ __global__ __launch_bounds__(kL > 64 ? kL : 256) void k_layer_norm_bwd2(LnArgs P
     const float r = st.y;
     float xh[E], gy[E], q[E];
     float s[4] = {0.f, 0.f, 0.f, 0.f}, squ[1] = {0.f};
-    each_vec<V, kL, NV>(l, [&](int k, int c) {
+    RowLoad<T, V, kL, NV> rx, ry, rq;
+    rx.load(xr, l, w);
+    ry.load(gr, l, w);
+    if (P.qx) rq.load(qr, l, w);
+    rx.get(l, w, xh);
+    ry.get(l, w, gy);
 #pragma unroll
-      for (int e = 0; e < V; ++e) q[k * V + e] = 0.f;
-      load_row<T, V>(xr, c, w, xh + k * V);
-      load_row<T, V>(gr, c, w, gy + k * V);
-      if (P.qx) load_row<T, V>(qr, c, w, q + k * V);
+    for (int e = 0; e < E; ++e) q[e] = 0.f;
+    if (P.qx) rq.get(l, w, q);
+    each_vec<V, kL, NV>(l, [&](int k, int c) {
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         float& h = xh[k * V + e];
@@ -404,10 +442,11 @@ void ln_launch(const LnArgs& P, unsigned grid, hipStream_t s) {
 // (5001 bf16 elements: 38 us with 256 lanes, 42 with 1024) and 16 backward, where more would not leave registers
 // for two wavefronts a SIMD (5001 fp32, second order: 195 us with 256 lanes, 147 with 1024).
 struct LnShape {
-  int lanes, vecs;
+  int lanes, vecs;       // vecs 0: rows shorter than a vector, one element a lane
 };
 
 LnShape ln_shape(int w, int v, bool fwd) {
+  if (w < v) return {w <= 2 ? 2 : w <= 4 ? 4 : 8, 0};
   const int nv = (w + v - 1) / v;
   if (nv <= 16) return {nv <= 2 ? 2 : nv <= 4 ? 4 : nv <= 8 ? 8 : 16, 1};
   if (nv <= 32) return {32, 1};
@@ -429,6 +468,9 @@ void ln_dispatch(const LnArgs& P, unsigned grid, hipStream_t s) {
   constexpr bool kFwd = kPass == LnPass::kFwd;
   const LnShape f = ln_shape(P.w, V, kFwd);
   switch (f.lanes * 16 + f.vecs) {
+    case 2 * 16: return ln_launch<kPass, T, 1, 2, 1>(P, grid, s);
+    case 4 * 16: return ln_launch<kPass, T, 1, 4, 1>(P, grid, s);
+    case 8 * 16: return ln_launch<kPass, T, 1, 8, 1>(P, grid, s);
     case 2 * 16 + 1: return ln_launch<kPass, T, V, 2, 1>(P, grid, s);
     case 4 * 16 + 1: return ln_launch<kPass, T, V, 4, 1>(P, grid, s);
     case 8 * 16 + 1: return ln_launch<kPass, T, V, 8, 1>(P, grid, s);
@@ -484,7 +526,7 @@ unsigned ln_grid(const LnArgs& P, int type, LnPass pass, bool sums) {
   const LnShape f = ln_shape(P.w, v, pass == LnPass::kFwd);
   const int r = f.lanes > 64 ? 1 : 256 / f.lanes;
   int64_t most = f.lanes == 1024 ? 512 : f.lanes == 256 ? 2048 : 1024;
-  if (sums) most = f.lanes == 1024 ? 256 : f.vecs == 1 ? 1024 : 512;
+  if (sums) most = f.lanes == 1024 ? 256 : f.vecs <= 1 ? 1024 : 512;
   else if (pass != LnPass::kFwd && f.lanes <= 32) most = 1 << 30;
   return (unsigned)std::min<int64_t>((P.n + r - 1) / r, most);
 }
