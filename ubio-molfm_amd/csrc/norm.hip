@@ -16,6 +16,7 @@
 // rest of a row element by element.  A workgroup strides over the rows and keeps its columns' parameter sums in registers; each
 // leaves one partial row, added in order by a second launch, so results repeat bitwise.  Bound: HBM.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.h"
 #include "../../include/e2v2.h"
@@ -41,9 +42,21 @@ __device__ __forceinline__ void each_vec(int l, F&& f) {
   for (int k = 0; k < NV; ++k) f(k, (l + k * kL) * V);
 }
 
+// The same with whole = true_type for a vector that every lane has in full, false_type where elements from w on have to
+// be left out: masks on every element made 6,007 x 5001 bf16 rows bound by the VALU.
+template <int V, int kL, int NV, typename F>
+__device__ __forceinline__ void each_vec(int l, int w, F&& f) {
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int c = (l + k * kL) * V;
+    if ((k + 1) * kL * V <= w) f(k, c, std::true_type{});
+    else f(k, c, std::false_type{});
+  }
+}
+
 // A lane's vectors of a row of w >= V elements (any w for V = 1).  All loads are unconditional, so that those of a row's operands
 // are in flight together: a vector that would pass the end starts V before it instead (a branch would wait for its load in
-// place: 100,000 x 129 fp32 backward 57 us).  get() then moves what belongs to the row down and clears the rest.
+// place: 100,000 x 129 fp32 backward 57 us).  get() then moves what belongs to the row down and, with kClear, clears the rest.
 template <typename T, int V, int kL, int NV>
 struct RowLoad {
   typename RowVec<T>::type raw[V > 1 ? NV : 1];
@@ -56,6 +69,7 @@ struct RowLoad {
     });
   }
 
+  template <bool kClear = true>
   __device__ __forceinline__ void get(int l, int w, float (&out)[NV * V]) const {
     each_vec<V, kL, NV>(l, [&](int k, int c) {
       if constexpr (V > 1) {
@@ -66,9 +80,9 @@ struct RowLoad {
         out[k] = (float)one[k];
       }
     });
-    if (w == kL * NV * V) return;
     const int past = w % V ? V - w % V : 0;        // elements by which the row's last vector starts early
-    each_vec<V, kL, NV>(l, [&](int k, int c) {
+    each_vec<V, kL, NV>(l, w, [&](int k, int c, auto whole) {
+      if constexpr (decltype(whole)::value) return;
       float* v = out + k * V;
       const bool moved = c < w && c + V > w;
 #pragma unroll
@@ -78,27 +92,51 @@ struct RowLoad {
           for (int e = 0; e < V; ++e) v[e] = moved ? (e + d < V ? v[e + d] : 0.f) : v[e];
         }
       }
+      if constexpr (kClear) {
 #pragma unroll
-      for (int e = 0; e < V; ++e) v[e] = c < w ? v[e] : 0.f;
+        for (int e = 0; e < V; ++e) v[e] = c < w ? v[e] : 0.f;
+      }
     });
   }
 };
 
+// The lane's V elements from column c on, or those of them that the row has: pieces of a half, a quarter, ... of a vector as
+// the bits of w % V say.
 template <typename T, int V>
-__device__ __forceinline__ void store_row(const float* v, T* row, int c, int w) {
-  if constexpr (V > 1) {
-    if (c + V <= w) {
-      typename RowVec<T>::ftype f;
+__device__ __forceinline__ void store_row(const float* v, T* row, int c, int w, bool whole) {
+  if constexpr (V == 1) {
+    if (c < w) row[c] = (T)v[0];
+  } else {
+    T o[V];
 #pragma unroll
-      for (int k = 0; k < V; ++k) f[k] = v[k];
-      const typename RowVec<T>::type o = __builtin_convertvector(f, typename RowVec<T>::type);
-      *reinterpret_cast<typename RowVec<T>::any*>(row + c) = o;
-      return;
+    for (int k = 0; k < V; ++k) o[k] = (T)v[k];
+    if (whole || c + V <= w) {
+      typename RowVec<T>::type f;
+#pragma unroll
+      for (int k = 0; k < V; ++k) f[k] = o[k];
+      *reinterpret_cast<typename RowVec<T>::any*>(row + c) = f;
+    } else if (c < w) {
+      T* at = row + c;
+      auto piece = [&](auto size) {
+        constexpr int D = decltype(size)::value;
+        if constexpr (D < V) {
+          if (w & D) {
+            typedef T part __attribute__((ext_vector_type(D), aligned(sizeof(T))));
+            part f;
+#pragma unroll
+            for (int k = 0; k < D; ++k) f[k] = o[k];
+            *reinterpret_cast<part*>(at) = f;
+            at += D;
+#pragma unroll
+            for (int k = 0; k + D < V; ++k) o[k] = o[k + D];
+          }
+        }
+      };
+      piece(std::integral_constant<int, 4>{});
+      piece(std::integral_constant<int, 2>{});
+      piece(std::integral_constant<int, 1>{});
     }
   }
-#pragma unroll
-  for (int k = 0; k < V; ++k)
-    if (c + k < w) row[c + k] = (T)v[k];
 }
 
 // v + its partner's, kLanes lanes away, by an exchange of rows of 16 lanes or of halves in registers (no trip through
@@ -249,21 +287,21 @@ __global__ __launch_bounds__(kL > 64 ? kL : 256) void k_layer_norm_fwd(LnArgs P)
     for (int e = 0; e < E; ++e) s[0] += x[e];
     group_sum<kL, 1>(s, red, turn);
     const float mean = s[0] / (float)w;       // a true quotient: exact for a row of one short value
-    each_vec<V, kL, NV>(l, [&](int k, int c) {
+    each_vec<V, kL, NV>(l, w, [&](int k, int c, auto whole) {
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        x[k * V + e] = c + e < w ? x[k * V + e] - mean : 0.f;
+        x[k * V + e] = whole || c + e < w ? x[k * V + e] - mean : 0.f;
         q[0] = fmaf(x[k * V + e], x[k * V + e], q[0]);
       }
     });
     group_sum<kL, 1>(q, red, turn);
     const float rstd = 1.0f / sqrtf(q[0] * inv + P.eps);
     T* yr = static_cast<T*>(P.y) + row * w;
-    each_vec<V, kL, NV>(l, [&](int k, int c) {
+    each_vec<V, kL, NV>(l, w, [&](int k, int c, auto whole) {
       float o[V];
 #pragma unroll
       for (int e = 0; e < V; ++e) o[e] = fmaf(x[k * V + e] * rstd, g[k * V + e], b[k * V + e]);
-      store_row<T, V>(o, yr, c, w);
+      store_row<T, V>(o, yr, c, w, whole);
     });
     if (P.stats && l == 0) *reinterpret_cast<float2*>(P.stats + 2 * row) = make_float2(mean, rstd);
   }
@@ -288,29 +326,26 @@ __global__ __launch_bounds__(kL > 64 ? kL : 256) void k_layer_norm_bwd(LnArgs P)
     RowLoad<T, V, kL, NV> rx, ry;
     rx.load(xr, l, w);
     ry.load(gr, l, w);
-    rx.get(l, w, xh);
+    rx.template get<false>(l, w, xh);              // past the row's end gy is zero, and so is all that x enters
     ry.get(l, w, gy);
-    each_vec<V, kL, NV>(l, [&](int k, int c) {
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        float& h = xh[k * V + e];
-        h = c + e < w ? (h - st.x) * st.y : 0.f;
-        float& u = gy[k * V + e];
-        ag[k * V + e] = fmaf(u, h, ag[k * V + e]);
-        ab[k * V + e] += u;
-        u = rounded_product(u, g[k * V + e]);
-        s[0] += u;
-        s[1] = fmaf(u, h, s[1]);
-      }
-    });
+    for (int e = 0; e < E; ++e) {
+      const float h = xh[e] = (xh[e] - st.x) * st.y;
+      float& u = gy[e];
+      ag[e] = fmaf(u, h, ag[e]);
+      ab[e] += u;
+      u = rounded_product(u, g[e]);
+      s[0] += u;
+      s[1] = fmaf(u, h, s[1]);
+    }
     group_sum<kL, 2>(s, red, turn);
     const float m1 = s[0] * inv, m2 = s[1] * inv;
     T* o = static_cast<T*>(P.gx) + row * w;
-    each_vec<V, kL, NV>(l, [&](int k, int c) {
+    each_vec<V, kL, NV>(l, w, [&](int k, int c, auto whole) {
       float v[V];
 #pragma unroll
       for (int e = 0; e < V; ++e) v[e] = st.y * (gy[k * V + e] - m1 - xh[k * V + e] * m2);
-      store_row<T, V>(v, o, c, w);
+      store_row<T, V>(v, o, c, w, whole);
     });
   }
   if (P.part) {
@@ -344,36 +379,33 @@ __global__ __launch_bounds__(kL > 64 ? kL : 256) void k_layer_norm_bwd2(LnArgs P
     rx.load(xr, l, w);
     ry.load(gr, l, w);
     if (P.qx) rq.load(qr, l, w);
-    rx.get(l, w, xh);
+    rx.template get<false>(l, w, xh);              // past the row's end gy, qx, qg and qb are zero
     ry.get(l, w, gy);
 #pragma unroll
     for (int e = 0; e < E; ++e) q[e] = 0.f;
     if (P.qx) rq.get(l, w, q);
-    each_vec<V, kL, NV>(l, [&](int k, int c) {
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        float& h = xh[k * V + e];
-        h = c + e < w ? (h - st.x) * r : 0.f;
-        const float u = gy[k * V + e] * g[k * V + e], v = q[k * V + e];
-        s[0] += u;
-        s[1] = fmaf(u, h, s[1]);
-        s[2] += v;
-        s[3] = fmaf(v, h, s[3]);
-        squ[0] = fmaf(v, u, squ[0]);
-      }
-    });
+    for (int e = 0; e < E; ++e) {
+      const float h = xh[e] = (xh[e] - st.x) * r;
+      const float u = gy[e] * g[e], v = q[e];
+      s[0] += u;
+      s[1] = fmaf(u, h, s[1]);
+      s[2] += v;
+      s[3] = fmaf(v, h, s[3]);
+      squ[0] = fmaf(v, u, squ[0]);
+    }
     group_sum<kL, 4>(s, red, turn);
     group_sum<kL, 1>(squ, red, turn);
     const float ub = s[0] * inv, c_ = s[1] * inv, qm = s[2] * inv, m = s[3] * inv;
     const float rr = r * r * (squ[0] * inv - qm * ub - c_ * m);      // r <qx gx>
     float t[2] = {0.f, 0.f};
     T* o1 = static_cast<T*>(P.y) + row * w;
-    each_vec<V, kL, NV>(l, [&](int k, int c) {
+    each_vec<V, kL, NV>(l, w, [&](int k, int c, auto whole) {
       float v[V];
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         const int i = k * V + e;
-        const float a = c + e < w ? r * (q[i] - qm - xh[i] * m) : 0.f;
+        const float a = r * (q[i] - qm - xh[i] * m);
         v[e] = g[i] * a + qg[i] * xh[i] + qb[i];
         ag[i] = fmaf(gy[i], a, ag[i]);
         const float x = qg[i] * gy[i] - r * (c_ * q[i] + m * gy[i] * g[i]);
@@ -381,16 +413,16 @@ __global__ __launch_bounds__(kL > 64 ? kL : 256) void k_layer_norm_bwd2(LnArgs P
         t[0] += x;
         t[1] = fmaf(x, xh[i], t[1]);
       }
-      store_row<T, V>(v, o1, c, w);
+      store_row<T, V>(v, o1, c, w, whole);
     });
     group_sum<kL, 2>(t, red, turn);
     const float mx = t[0] * inv, mxx = t[1] * inv;
     T* o2 = static_cast<T*>(P.gx) + row * w;
-    each_vec<V, kL, NV>(l, [&](int k, int c) {
+    each_vec<V, kL, NV>(l, w, [&](int k, int c, auto whole) {
       float v[V];
 #pragma unroll
       for (int e = 0; e < V; ++e) v[e] = r * (q[k * V + e] - mx - xh[k * V + e] * mxx) - rr * xh[k * V + e];
-      store_row<T, V>(v, o2, c, w);
+      store_row<T, V>(v, o2, c, w, whole);
     });
   }
   if (P.part) write_part<V, kL, NV>(ag, l, w, P.part + (int64_t)blockIdx.x * w);
@@ -445,18 +477,21 @@ struct LnShape {
   int lanes, vecs;       // vecs 0: rows shorter than a vector, one element a lane
 };
 
-LnShape ln_shape(int w, int v, bool fwd) {
+LnShape ln_shape(int w, int v, LnPass pass) {
   if (w < v) return {w <= 2 ? 2 : w <= 4 ? 4 : 8, 0};
   const int nv = (w + v - 1) / v;
-  if (nv <= 16) return {nv <= 2 ? 2 : nv <= 4 ? 4 : nv <= 8 ? 8 : 16, 1};
+  if (nv <= 8) return {nv <= 2 ? 2 : nv <= 4 ? 4 : 8, 1};
+  if (nv <= 12) return {4, 3};
+  if (nv <= 16) return {16, 1};
+  if (nv <= 24) return {8, 3};
   if (nv <= 32) return {32, 1};
   if (nv <= 48) return {16, 3};
   if (nv <= 64) return {64, 1};
   if (nv <= 96) return {32, 3};
   if (nv <= 128) return {64, 2};
   if (w <= 1024) return {64, nv <= 192 ? 3 : 4};
-  if (w <= (fwd ? 8192 : 4096)) {
-    for (int k = 1;; k *= 2)
+  if (w <= (pass == LnPass::kFwd ? 8192 : pass == LnPass::kBwd && v == 8 ? 6144 : 4096)) {
+    for (int k = 1;; k = k < 4 ? k + 1 : 8)
       if (nv <= 256 * k) return {256, k};
   }
   return {1024, w <= 8192 ? 8 / v : 16 / v};
@@ -466,7 +501,7 @@ template <LnPass kPass, typename T>
 void ln_dispatch(const LnArgs& P, unsigned grid, hipStream_t s) {
   constexpr int V = RowVec<T>::n;
   constexpr bool kFwd = kPass == LnPass::kFwd;
-  const LnShape f = ln_shape(P.w, V, kFwd);
+  const LnShape f = ln_shape(P.w, V, kPass);
   switch (f.lanes * 16 + f.vecs) {
     case 2 * 16: return ln_launch<kPass, T, 1, 2, 1>(P, grid, s);
     case 4 * 16: return ln_launch<kPass, T, 1, 4, 1>(P, grid, s);
@@ -476,6 +511,8 @@ void ln_dispatch(const LnArgs& P, unsigned grid, hipStream_t s) {
     case 8 * 16 + 1: return ln_launch<kPass, T, V, 8, 1>(P, grid, s);
     case 16 * 16 + 1: return ln_launch<kPass, T, V, 16, 1>(P, grid, s);
     case 32 * 16 + 1: return ln_launch<kPass, T, V, 32, 1>(P, grid, s);
+    case 4 * 16 + 3: return ln_launch<kPass, T, V, 4, 3>(P, grid, s);
+    case 8 * 16 + 3: return ln_launch<kPass, T, V, 8, 3>(P, grid, s);
     case 16 * 16 + 3: return ln_launch<kPass, T, V, 16, 3>(P, grid, s);
     case 64 * 16 + 1: return ln_launch<kPass, T, V, 64, 1>(P, grid, s);
     case 32 * 16 + 3: return ln_launch<kPass, T, V, 32, 3>(P, grid, s);
@@ -494,6 +531,9 @@ void ln_dispatch(const LnArgs& P, unsigned grid, hipStream_t s) {
       if constexpr (V == 8) return ln_launch<kPass, T, V, 256, 1>(P, grid, s);
       break;
     case 256 * 16 + 2: return ln_launch<kPass, T, V, 256, 2>(P, grid, s);
+    case 256 * 16 + 3:
+      if constexpr (kPass != LnPass::kBwd2 || V == 4) return ln_launch<kPass, T, V, 256, 3>(P, grid, s);
+      break;
     case 256 * 16 + 4:
       if constexpr (kFwd || V == 4) return ln_launch<kPass, T, V, 256, 4>(P, grid, s);
       break;
@@ -523,11 +563,11 @@ void ln_run(const LnArgs& P, int type, unsigned grid, hipStream_t s) {
 // us, 244 with 1,024).
 unsigned ln_grid(const LnArgs& P, int type, LnPass pass, bool sums) {
   const int v = 16 / type_size(type);
-  const LnShape f = ln_shape(P.w, v, pass == LnPass::kFwd);
+  const LnShape f = ln_shape(P.w, v, pass);
   const int r = f.lanes > 64 ? 1 : 256 / f.lanes;
   int64_t most = f.lanes == 1024 ? 512 : f.lanes == 256 ? 2048 : 1024;
   if (sums) most = f.lanes == 1024 ? 256 : f.vecs <= 1 ? 1024 : 512;
-  else if (pass != LnPass::kFwd && f.lanes <= 32) most = 1 << 30;
+  else if (pass != LnPass::kFwd && f.lanes <= 32 && f.vecs <= 1) most = 1 << 30;
   return (unsigned)std::min<int64_t>((P.n + r - 1) / r, most);
 }
 
