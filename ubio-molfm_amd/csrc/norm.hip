@@ -469,10 +469,11 @@ void ln_launch(const LnArgs& P, unsigned grid, hipStream_t s) {
 }
 
 // Lanes that hold a row, and 16-byte vectors a lane holds of it.  Up to 1024 elements a part of a wavefront, so that no
-// barrier stands in the way: of the shapes that hold the row the one with the fewest idle places (129 fp32 elements, 33 vectors:
-// 16 lanes of 3 instead of 64 of 1).  Wider rows take a workgroup, up to 32 elements a lane forward
-// (5001 bf16 elements: 38 us with 256 lanes, 42 with 1024) and 16 backward, where more would not leave registers
-// for two wavefronts a SIMD (5001 fp32, second order: 195 us with 256 lanes, 147 with 1024).
+// barrier stands in the way: of the shapes that hold the row one with few idle places (400,000 x 129 bf16 forward: 52 us
+// on 8 lanes of 3 vectors, 82 on 32 of one; 100,000 x 129 fp32: 24 on 16 of 3, 41 on 64 of one).  Wider rows take a workgroup of
+// 256, up to 32 elements a lane (6,007 x 5001 bf16 forward: 35 us, on 1024 lanes 45; second order, 4,000 x 8192 fp32: 147
+// and 188), in the backward pass with its two sums a column 16 (fp32: 6,007 x 5001 85 us with 24, 79 on 1024 lanes) or 24
+// (bf16: 4,000 x 8192 64 us with 32, 56 on 1024 lanes).
 struct LnShape {
   int lanes, vecs;       // vecs 0: rows shorter than a vector, one element a lane
 };
@@ -490,7 +491,7 @@ LnShape ln_shape(int w, int v, LnPass pass) {
   if (nv <= 96) return {32, 3};
   if (nv <= 128) return {64, 2};
   if (w <= 1024) return {64, nv <= 192 ? 3 : 4};
-  if (w <= (pass == LnPass::kFwd ? 8192 : pass == LnPass::kBwd && v == 8 ? 6144 : 4096)) {
+  if (w <= (pass != LnPass::kBwd ? 8192 : v == 8 ? 6144 : 4096)) {
     for (int k = 1;; k = k < 4 ? k + 1 : 8)
       if (nv <= 256 * k) return {256, k};
   }
@@ -500,7 +501,7 @@ LnShape ln_shape(int w, int v, LnPass pass) {
 template <LnPass kPass, typename T>
 void ln_dispatch(const LnArgs& P, unsigned grid, hipStream_t s) {
   constexpr int V = RowVec<T>::n;
-  constexpr bool kFwd = kPass == LnPass::kFwd;
+  constexpr bool kBwd = kPass == LnPass::kBwd;
   const LnShape f = ln_shape(P.w, V, kPass);
   switch (f.lanes * 16 + f.vecs) {
     case 2 * 16: return ln_launch<kPass, T, 1, 2, 1>(P, grid, s);
@@ -523,7 +524,7 @@ void ln_dispatch(const LnArgs& P, unsigned grid, hipStream_t s) {
       case 64 * 16 + 3: return ln_launch<kPass, T, V, 64, 3>(P, grid, s);
       case 64 * 16 + 4: return ln_launch<kPass, T, V, 64, 4>(P, grid, s);
       case 256 * 16 + 8:
-        if constexpr (kFwd) return ln_launch<kPass, T, V, 256, 8>(P, grid, s);
+        if constexpr (!kBwd) return ln_launch<kPass, T, V, 256, 8>(P, grid, s);
     }
   }
   switch (f.lanes * 16 + f.vecs) {
@@ -531,14 +532,12 @@ void ln_dispatch(const LnArgs& P, unsigned grid, hipStream_t s) {
       if constexpr (V == 8) return ln_launch<kPass, T, V, 256, 1>(P, grid, s);
       break;
     case 256 * 16 + 2: return ln_launch<kPass, T, V, 256, 2>(P, grid, s);
-    case 256 * 16 + 3:
-      if constexpr (kPass != LnPass::kBwd2 || V == 4) return ln_launch<kPass, T, V, 256, 3>(P, grid, s);
-      break;
+    case 256 * 16 + 3: return ln_launch<kPass, T, V, 256, 3>(P, grid, s);
     case 256 * 16 + 4:
-      if constexpr (kFwd || V == 4) return ln_launch<kPass, T, V, 256, 4>(P, grid, s);
+      if constexpr (!kBwd || V == 4) return ln_launch<kPass, T, V, 256, 4>(P, grid, s);
       break;
     case 1024 * 16 + 8 / V:
-      if constexpr (!kFwd) return ln_launch<kPass, T, V, 1024, 8 / V>(P, grid, s);
+      if constexpr (kBwd) return ln_launch<kPass, T, V, 1024, 8 / V>(P, grid, s);
       break;
     default: return ln_launch<kPass, T, V, 1024, 16 / V>(P, grid, s);
   }
