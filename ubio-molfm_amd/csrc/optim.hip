@@ -3,7 +3,8 @@
 // t:
 //   m = b1 m + (1 - b1) c g,   v = b2 v + (1 - b2) (c g)^2
 //   p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v / (1 - b2^t)) + eps)
-// All arithmetic is fp32 (the norm's sum fp64: it neither loses small tensors beside large ones nor overflows);
+// Arithmetic is fp32 (the norm's sum fp64: it neither loses small tensors beside large ones nor overflows; 8-bit moments
+// fp64 up to their code);
 // bf16 and fp16 parameters are rounded to nearest once.  Every element is read and written once by one thread,
 // the sums run in a fixed order: no atomics, results repeat bitwise.  Bound: HBM.
 //
@@ -20,6 +21,7 @@
 // zero would let the next step divide by eps.  The random bits are a hash of seed, step and element.  A value
 // that is not finite becomes the NaN of its own element.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.h"
 #include "../../include/e2v2.h"
@@ -38,16 +40,18 @@ template <typename T>
 struct Vec16 {
   static constexpr int n = 16 / sizeof(T);
   typedef T type __attribute__((ext_vector_type(16 / sizeof(T))));
+  typedef T any __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));   // on any element boundary
   typedef float ftype __attribute__((ext_vector_type(16 / sizeof(T))));
 };
 
+// N elements at p, on any element boundary (the hardware takes 16 bytes unaligned).
 template <typename T, int N>
 __device__ __forceinline__ void load_n(const T* p, float (&out)[N]) {
   constexpr int V = Vec16<T>::n;
 #pragma unroll
   for (int k = 0; k < N; k += V) {
-    const auto f = __builtin_convertvector(*reinterpret_cast<const typename Vec16<T>::type*>(p + k),
-                                           typename Vec16<T>::ftype);
+    const typename Vec16<T>::type v = *reinterpret_cast<const typename Vec16<T>::any*>(p + k);
+    const auto f = __builtin_convertvector(v, typename Vec16<T>::ftype);
 #pragma unroll
     for (int e = 0; e < V; ++e) out[k + e] = f[e];
   }
@@ -61,14 +65,15 @@ __device__ __forceinline__ void store_n(const float (&v)[N], T* p) {
     typename Vec16<T>::ftype f;
 #pragma unroll
     for (int e = 0; e < V; ++e) f[e] = v[k + e];
-    *reinterpret_cast<typename Vec16<T>::type*>(p + k) = __builtin_convertvector(f, typename Vec16<T>::type);
+    const typename Vec16<T>::type o = __builtin_convertvector(f, typename Vec16<T>::type);
+    *reinterpret_cast<typename Vec16<T>::any*>(p + k) = o;
   }
 }
 
-// Elements i .. i + N of p, those past n zero.
-template <typename T, int N>
-__device__ __forceinline__ void load_some(const T* p, int i, int n, bool vec, float (&out)[N]) {
-  if (vec && i + N <= n) {
+// Elements i .. i + N of n at p, those past n zero; kWhole: all are there.
+template <bool kWhole, typename T, int N>
+__device__ __forceinline__ void load_some(const T* p, int i, int n, float (&out)[N]) {
+  if (kWhole || i + N <= n) {
     load_n<T, N>(p + i, out);
   } else {
 #pragma unroll
@@ -76,9 +81,9 @@ __device__ __forceinline__ void load_some(const T* p, int i, int n, bool vec, fl
   }
 }
 
-template <typename T, int N>
-__device__ __forceinline__ void store_some(const float (&v)[N], T* p, int i, int n, bool vec) {
-  if (vec && i + N <= n) {
+template <bool kWhole, typename T, int N>
+__device__ __forceinline__ void store_some(const float (&v)[N], T* p, int i, int n) {
+  if (kWhole || i + N <= n) {
     store_n<T, N>(v, p + i);
   } else {
 #pragma unroll
@@ -106,9 +111,9 @@ __device__ __forceinline__ double norm_of_parts(const double* parts, int n) {
 }
 
 // The factor that brings a norm to max_norm (none: infinity), and a NaN for a NaN.
-__device__ __forceinline__ float clip_factor(double norm, float max_norm) {
+__device__ __forceinline__ double clip_factor(double norm, float max_norm) {
   const double c = (double)max_norm / (norm + 1e-6);
-  return c < 1.0 || c != c ? (float)c : 1.f;
+  return c < 1.0 || c != c ? c : 1.0;
 }
 
 // ---- norm and scaling of a list of tensors
@@ -157,15 +162,18 @@ __global__ __launch_bounds__(kOptThreads) void k_grad_norm(NormArgs P) {
   double s = 0;
   each_chunk(P, [&](int t, uint32_t at, int n) {
     const T* g = static_cast<const T*>(P.p[t]) + at;
-    const bool vec = (uintptr_t)g % 16 == 0;
-#pragma unroll 4
-    for (int i = threadIdx.x * N; i < kNormChunk; i += kOptThreads * N) {
-      if (i >= n) continue;
-      float v[N];
-      load_some<T, N>(g, i, n, vec, v);
+    auto add = [&](auto whole) {
 #pragma unroll
-      for (int e = 0; e < N; ++e) s = fma((double)v[e], (double)v[e], s);
-    }
+      for (int k = 0; k < kNormChunk / (kOptThreads * N); ++k) {
+        const int i = (k * kOptThreads + threadIdx.x) * N;
+        float v[N];
+        load_some<decltype(whole)::value>(g, i, n, v);
+#pragma unroll
+        for (int e = 0; e < N; ++e) s = fma((double)v[e], (double)v[e], s);
+      }
+    };
+    if (n == kNormChunk) add(std::true_type{});
+    else add(std::false_type{});
   });
   s = block_sum(s);
   if (threadIdx.x == 0) P.parts[blockIdx.x] = s;
@@ -175,20 +183,24 @@ template <typename T>
 __global__ __launch_bounds__(kOptThreads) void k_grad_scale(NormArgs P) {
   constexpr int N = 8;
   const double norm = norm_of_parts(P.parts, P.n_parts);
-  const float c = clip_factor(norm, P.max_norm);
+  const float c = (float)clip_factor(norm, P.max_norm);
   if (blockIdx.x == 0 && threadIdx.x == 0 && P.norm) *P.norm = (float)norm;
   each_chunk(P, [&](int t, uint32_t at, int n) {
     T* g = static_cast<T*>(P.p[t]) + at;
-    const bool vec = (uintptr_t)g % 16 == 0;
-#pragma unroll 2
-    for (int i = threadIdx.x * N; i < kNormChunk; i += kOptThreads * N) {
-      if (i >= n) continue;
-      float v[N];
-      load_some<T, N>(g, i, n, vec, v);
+    auto scale = [&](auto whole) {
+      constexpr int K = kNormChunk / (kOptThreads * N);
+      float v[K][N];
 #pragma unroll
-      for (int e = 0; e < N; ++e) v[e] *= c;
-      store_some<T, N>(v, g, i, n, vec);
-    }
+      for (int k = 0; k < K; ++k) load_some<decltype(whole)::value>(g, (k * kOptThreads + threadIdx.x) * N, n, v[k]);
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[k][e] *= c;
+        store_some<decltype(whole)::value>(v[k], g, (k * kOptThreads + threadIdx.x) * N, n);
+      }
+    };
+    if (n == kNormChunk) scale(std::true_type{});
+    else scale(std::false_type{});
   });
 }
 
@@ -255,17 +267,106 @@ struct StepArgs {
   int n_parts, first_tensor, skip_nonfinite;
   uint32_t seed;
   float lr, b1, b2, one_b1, one_b2, ln_b1, ln_b2, eps, wd, max_norm;
+  double b1d, b2d, one_b1d, one_b2d;
 };
+
+// a towards zero in fp32.
+__device__ __forceinline__ float truncated(double a) {
+  return (float)__builtin_bit_cast(double, __builtin_bit_cast(uint64_t, a) & ~0x1FFFFFFFull);
+}
+
+struct StepFactors {
+  double c;                            // of the gradients
+  float size, root, decay;             // lr / (1 - b1^t), (1 - b2^t)^(-1/2), lr wd
+  uint32_t key;
+};
+
+// One chunk.  kWhole: all of its elements are there; then the loads of both halves are in flight before the first is used.
+template <bool kWhole, typename T, int kBits>
+__device__ __forceinline__ void adamw_chunk(const StepArgs& P, const StepFactors& F, const T* g, T* p, int n,
+                                            int64_t off) {
+  constexpr int N = 8, K = kOptChunk / (kOptThreads * N);
+  float pv[K][N], gv[K][N], m[K][N], v[K][N];
+  uint2 mc[K], vc[K];
+  int ms[K], vs[K];
+  // whole runs of 32, padded with zeros, take part: a run's lanes share its scale
+  const int padded = kWhole ? kOptChunk : (n + 31) / 32 * 32;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int i = (k * kOptThreads + threadIdx.x) * N;
+    if (!kWhole && i >= padded) break;
+    load_some<kWhole>(p, i, n, pv[k]);
+    load_some<kWhole>(g, i, n, gv[k]);
+    if constexpr (kBits == 32) {
+      load_n(static_cast<const float*>(P.m) + off + i, m[k]);
+      load_n(static_cast<const float*>(P.v) + off + i, v[k]);
+    } else {
+      mc[k] = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(P.m) + off + i);
+      vc[k] = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(P.v) + off + i);
+      ms[k] = P.ms[(off + i) / 32];
+      vs[k] = P.vs[(off + i) / 32];
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int i = (k * kOptThreads + threadIdx.x) * N;
+    if (!kWhole && i >= padded) break;
+    const int64_t at = off + i;
+    if constexpr (kBits == 8) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        m[k][e] = decode8<true>((e < 4 ? mc[k].x : mc[k].y) >> (8 * (e % 4)) & 255u, ms[k]);
+        v[k][e] = decode8<false>((e < 4 ? vc[k].x : vc[k].y) >> (8 * (e % 4)) & 255u, vs[k]);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      float &a = m[k][e], &b = v[k][e];
+      if constexpr (kBits == 32) {
+        const float x = gv[k][e] * (float)F.c;
+        a = fmaf(P.one_b1, x, P.b1 * a);
+        b = fmaf(P.one_b2 * x, x, P.b2 * b);
+      } else {
+        // fp64 up to the code: truncated to fp32 a value keeps every bit that its code hangs on, so that the codes are those
+        // of the exact moments (a value next to a border would take the other code by its fp32 rounding)
+        const double x = (double)gv[k][e] * F.c;
+        a = truncated(fma(P.one_b1d, x, P.b1d * (double)a));
+        b = truncated(fma(P.one_b2d * x, x, P.b2d * (double)b));
+      }
+      pv[k][e] -= fmaf(F.decay, pv[k][e], F.size * (a * frcp(fmaf(__builtin_amdgcn_sqrtf(b), F.root, P.eps))));
+    }
+    store_some<kWhole>(pv[k], p, i, n);
+    if constexpr (kBits == 32) {
+      store_n(m[k], static_cast<float*>(P.m) + at);
+      store_n(v[k], static_cast<float*>(P.v) + at);
+    } else {
+      const int s = scale8<true>(m[k]), r = scale8<false>(v[k]);
+      uint32_t mo[2] = {0, 0}, vo[2] = {0, 0};
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const uint32_t u = mix32((uint32_t)(at + e) ^ F.key);
+        mo[e / 4] |= encode8<true>(m[k][e], s, u & 0xFFFFu) << (8 * (e % 4));
+        vo[e / 4] |= encode8<false>(v[k][e], r, u >> 16) << (8 * (e % 4));
+      }
+      *reinterpret_cast<uint2*>(static_cast<uint8_t*>(P.m) + at) = make_uint2(mo[0], mo[1]);
+      *reinterpret_cast<uint2*>(static_cast<uint8_t*>(P.v) + at) = make_uint2(vo[0], vo[1]);
+      if (i % 32 == 0) {
+        P.ms[at / 32] = (uint8_t)s;
+        P.vs[at / 32] = (uint8_t)r;
+      }
+    }
+  }
+}
 
 template <typename T, int kBits>
 __global__ __launch_bounds__(kOptThreads) void k_adamw(StepArgs P) {
-  constexpr int N = 8;
   const e2v2_opt_chunk ch = P.chunks[blockIdx.x];
-  float c = 1.f;
+  StepFactors F;
+  F.c = 1.0;
   bool skip = false;
   if (P.parts) {
     const double norm = norm_of_parts(P.parts, P.n_parts);
-    c = clip_factor(norm, P.max_norm);
+    F.c = clip_factor(norm, P.max_norm);
     skip = P.skip_nonfinite && !(norm < (double)__builtin_inff());
     if (blockIdx.x == 0 && threadIdx.x == 0 && P.norm) {
       *P.norm = (float)norm;
@@ -274,67 +375,18 @@ __global__ __launch_bounds__(kOptThreads) void k_adamw(StepArgs P) {
   }
   const T* g = static_cast<const T*>(P.grad[ch.tensor - P.first_tensor]);
   if (skip || !g) return;
-  g += ch.at;
-  T* p = static_cast<T*>(ch.p) + ch.at;
-  const bool vec = ((uintptr_t)p | (uintptr_t)g) % 16 == 0;
   const int t = P.steps[blockIdx.x] + 1;
   __syncthreads();
   if (threadIdx.x == 0) P.steps[blockIdx.x] = t;
   const float lr = P.lr_dev ? *P.lr_dev : P.lr;
   const float bc1 = -expm1f((float)t * P.ln_b1), bc2 = -expm1f((float)t * P.ln_b2);
-  const float size = lr / bc1, root = 1.0f / sqrtf(bc2), decay = lr * P.wd;
-  uint32_t key = 0;
-  if constexpr (kBits == 8)
-    key = mix32(mix32(P.seed) + (uint32_t)t * kGolden + (uint32_t)((uint64_t)ch.off >> 32) * kRoot2);
-  for (int i = threadIdx.x * N; i < kOptChunk; i += kOptThreads * N) {
-    // whole runs of 32, padded with zeros, take part: a run's lanes share its scale
-    if (i >= (ch.n + 31) / 32 * 32) continue;
-    float pv[N], gv[N], m[N], v[N];
-    load_some<T, N>(p, i, ch.n, vec, pv);
-    load_some<T, N>(g, i, ch.n, vec, gv);
-    const int64_t at = ch.off + i;
-    uint32_t mc[2], vc[2];
-    if constexpr (kBits == 32) {
-      load_n<float, N>(static_cast<const float*>(P.m) + at, m);
-      load_n<float, N>(static_cast<const float*>(P.v) + at, v);
-    } else {
-      *reinterpret_cast<uint2*>(mc) = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(P.m) + at);
-      *reinterpret_cast<uint2*>(vc) = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(P.v) + at);
-      const int ms = P.ms[at / 32], vs = P.vs[at / 32];
-#pragma unroll
-      for (int e = 0; e < N; ++e) {
-        m[e] = decode8<true>(mc[e / 4] >> (8 * (e % 4)) & 255u, ms);
-        v[e] = decode8<false>(vc[e / 4] >> (8 * (e % 4)) & 255u, vs);
-      }
-    }
-#pragma unroll
-    for (int e = 0; e < N; ++e) {
-      const float x = gv[e] * c;
-      m[e] = fmaf(P.one_b1, x, P.b1 * m[e]);
-      v[e] = fmaf(P.one_b2 * x, x, P.b2 * v[e]);
-      pv[e] -= fmaf(decay, pv[e], size * (m[e] * frcp(fmaf(__builtin_amdgcn_sqrtf(v[e]), root, P.eps))));
-    }
-    store_some<T, N>(pv, p, i, ch.n, vec);
-    if constexpr (kBits == 32) {
-      store_n<float, N>(m, static_cast<float*>(P.m) + at);
-      store_n<float, N>(v, static_cast<float*>(P.v) + at);
-    } else {
-      const int ms = scale8<true>(m), vs = scale8<false>(v);
-      mc[0] = mc[1] = vc[0] = vc[1] = 0;
-#pragma unroll
-      for (int e = 0; e < N; ++e) {
-        const uint32_t u = mix32((uint32_t)(at + e) ^ key);
-        mc[e / 4] |= encode8<true>(m[e], ms, u & 0xFFFFu) << (8 * (e % 4));
-        vc[e / 4] |= encode8<false>(v[e], vs, u >> 16) << (8 * (e % 4));
-      }
-      *reinterpret_cast<uint2*>(static_cast<uint8_t*>(P.m) + at) = *reinterpret_cast<uint2*>(mc);
-      *reinterpret_cast<uint2*>(static_cast<uint8_t*>(P.v) + at) = *reinterpret_cast<uint2*>(vc);
-      if (i % 32 == 0) {
-        P.ms[at / 32] = (uint8_t)ms;
-        P.vs[at / 32] = (uint8_t)vs;
-      }
-    }
-  }
+  F.size = lr / bc1;
+  F.root = 1.0f / sqrtf(bc2);
+  F.decay = lr * P.wd;
+  F.key = kBits == 8 ? mix32(mix32(P.seed) + (uint32_t)t * kGolden + (uint32_t)((uint64_t)ch.off >> 32) * kRoot2) : 0;
+  T* p = static_cast<T*>(ch.p) + ch.at;
+  if (ch.n == kOptChunk) adamw_chunk<true, T, kBits>(P, F, g + ch.at, p, ch.n, ch.off);
+  else adamw_chunk<false, T, kBits>(P, F, g + ch.at, p, ch.n, ch.off);
 }
 
 // The values that codes stand for, eight a thread; exact in each of the three types as long as they are normal there.
@@ -481,6 +533,8 @@ E2V2_API int e2v2_adamw(const e2v2_adamw_args* a, hipStream_t s) {
   P.b1 = (float)a->beta1; P.b2 = (float)a->beta2;
   P.one_b1 = (float)(1 - a->beta1); P.one_b2 = (float)(1 - a->beta2);
   P.ln_b1 = (float)log(a->beta1); P.ln_b2 = (float)log(a->beta2);
+  P.b1d = a->beta1; P.b2d = a->beta2;
+  P.one_b1d = 1 - a->beta1; P.one_b2d = 1 - a->beta2;
   P.eps = (float)a->eps;
   P.wd = (float)a->weight_decay;
   P.max_norm = a->max_norm;

@@ -75,7 +75,7 @@ def _args(x, g, b, stats, eps, gy=None, qx=None, qg=None, qb=None, y=None, gx=No
 
 
 def _empty_rows(x):
-    """A contiguous tensor of x's shape and type."""
+    """A contiguous tensor of x's shape, type and device."""
     return torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
 
 
@@ -83,7 +83,7 @@ def _workspace(x):
     """Room for the parameters' partial sums, as e2v2_layer_norm_workspace says, and its bytes."""
     w = x.shape[-1]
     n = 2 * min(x.numel() // w, _MAX_PARTS) * w
-    return torch.empty(n, dtype=torch.float32, device=x.device), 4 * n
+    return x.new_empty(n, dtype=torch.float32), 4 * n
 
 
 def _call(name, dev, *args):
@@ -102,8 +102,8 @@ def _forward(x, g, b, eps, stats):
 
 def _backward(gy, x, g, b, stats, eps, need_g, need_b):
     gx = _empty_rows(x)
-    gg = torch.empty(g.shape, dtype=g.dtype, device=x.device) if need_g else None
-    gb = torch.empty(b.shape, dtype=b.dtype, device=x.device) if need_b else None
+    gg = _empty_rows(g) if need_g else None
+    gb = _empty_rows(b) if need_b else None
     ws, n = _workspace(x) if need_g or need_b else (None, 0)
     a, keep = _args(x, g, b, stats, eps, gy=gy, gx=gx)
     _call("e2v2_layer_norm_bwd", x.device, a, _ptr(gg), _ptr(gb), _ptr(ws), _lib.i64(n))
@@ -114,7 +114,7 @@ class _LayerNormFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, g, b, eps: float):
-        stats = torch.empty(x.numel() // x.shape[-1], 2, dtype=torch.float32, device=x.device)
+        stats = x.new_empty(2 * (x.numel() // x.shape[-1]), dtype=torch.float32)
         y = _forward(x, g, b, eps, stats)
         ctx.save_for_backward(x, g, b, stats)
         ctx.eps = eps
@@ -156,7 +156,7 @@ class _LayerNormGradFn(torch.autograd.Function):
         if qx is None and qg is None and qb is None:
             return (None,) * 8
         dgy, dx = _empty_rows(x), _empty_rows(x)
-        dg = torch.empty(g.shape, dtype=g.dtype, device=x.device) if ctx.needs_input_grad[2] else None
+        dg = _empty_rows(g) if ctx.needs_input_grad[2] else None
         ws, n = _workspace(x) if dg is not None else (None, 0)
         a, keep = _args(x, g, b, stats, ctx.eps, gy=gy, qx=qx, qg=qg, qb=qb, y=dgy, gx=dx)
         _call("e2v2_layer_norm_bwd2", x.device, a, _ptr(dg), _ptr(ws), _lib.i64(n))
@@ -174,14 +174,16 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     if not isinstance(x, torch.Tensor) or not x.is_cuda:
         raise RuntimeError("layer_norm runs on the GPU only (HIP library, no CPU path): got "
                            f"{x.device if isinstance(x, torch.Tensor) else type(x).__name__}")
-    if x.dtype not in _TYPES or x.dim() == 0:
-        raise ValueError(f"layer_norm: rows in fp32, bf16 or fp16, got {tuple(x.shape)} {x.dtype}")
+    dtype = x.dtype
+    if dtype not in _TYPES or x.dim() == 0:
+        raise ValueError(f"layer_norm: rows in fp32, bf16 or fp16, got {tuple(x.shape)} {dtype}")
     w = x.shape[-1]
     if not 1 <= w <= MAX_WIDTH:
         raise ValueError(f"layer_norm: width {w} (1 to {MAX_WIDTH})")
     for name, p in (("weight", weight), ("bias", bias)):
-        if p is not None and (p.shape != (w,) or p.dtype not in (torch.float32, x.dtype) or p.device != x.device):
-            raise ValueError(f"layer_norm: {name} [{w}] in fp32 or {x.dtype} on {x.device}, got {tuple(p.shape)} "
+        if p is not None and (p.dim() != 1 or p.shape[0] != w or (p.dtype != dtype and p.dtype != torch.float32)
+                              or not p.is_cuda or p.get_device() != x.get_device()):
+            raise ValueError(f"layer_norm: {name} [{w}] in fp32 or {dtype} on {x.device}, got {tuple(p.shape)} "
                              f"{p.dtype} on {p.device}")
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
                                     or (bias is not None and bias.requires_grad)):
