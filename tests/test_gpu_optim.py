@@ -521,3 +521,97 @@ def test_parameters_without_gradients_of_any_kind(pkg, cuda):
     empty = optim.AdamW(odd[:1])
     empty.step()
     assert empty.moments()[0].numel() == 0
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_graph_goes_on_after_load_state_dict(pkg, cuda, bits):
+    """A loaded state goes into the buffers that are there: a step captured before takes up the new state."""
+    from ubio_molfm_amd import optim
+    ps, qs = (_params(SHAPES, torch.float32, cuda, 51) for _ in range(2))
+    a, b = (optim.AdamW(x, lr=1e-3, state_bits=bits, seed=2) for x in (ps, qs))
+    a.step(), b.step()
+    saved = copy.deepcopy(a.state_dict())
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        a.step()
+    graph.replay()
+    torch.cuda.synchronize()
+    ptr = a.state[ps[3]]["exp_avg"].data_ptr()
+    a.load_state_dict(saved)
+    assert a.state[ps[3]]["exp_avg"].data_ptr() == ptr and int(a.state[ps[3]]["step"]) == 1
+    for p, q in zip(ps, qs):
+        p.data.copy_(q.data)
+    for _ in range(2):
+        graph.replay()
+        torch.cuda.synchronize()
+        b.step()
+        assert all(torch.equal(p, q) for p, q in zip(ps, qs))
+    a.param_groups[0]["lr"] = 0.0                                    # the groups are the loaded ones
+    before = ps[3].detach().clone()
+    a.step()
+    assert torch.equal(ps[3], before) and int(a.state[ps[3]]["step"]) == 4
+
+
+def test_states_that_are_taken_out_start_anew(pkg, cuda):
+    from ubio_molfm_amd import optim
+    ps = _params([(100,), (5000,)], torch.float32, cuda, 52)
+    opt = optim.AdamW(ps, lr=1e-3)
+    for _ in range(3):
+        opt.step()
+    kept = opt.state[ps[1]]["exp_avg"].clone()
+    del opt.state[ps[0]]
+    opt.step()
+    assert int(opt.state[ps[0]]["step"]) == 1 and int(opt.state[ps[1]]["step"]) == 4
+    assert not torch.equal(opt.state[ps[1]]["exp_avg"], kept)
+    opt.state.clear()
+    opt.step()
+    assert {int(opt.state[p]["step"]) for p in ps} == {1}
+
+
+def test_what_cannot_be_updated_is_refused(pkg, cuda):
+    """Memory that two parameters or two gradients share would be written by two workgroups at once; a checkpoint of another
+    method would go on as this one."""
+    from ubio_molfm_amd import optim
+    flat = torch.zeros(100, device=cuda)
+    a, b = flat[:60].requires_grad_(True), flat[50:].requires_grad_(True)
+    a.grad, b.grad = torch.ones_like(a), torch.ones_like(b)
+    with pytest.raises(ValueError, match="share memory"):
+        optim.AdamW([a, b]).step()
+    optim.AdamW([flat[:50].requires_grad_(True), flat[50:].requires_grad_(True)]).step()
+    with pytest.raises(ValueError, match="twice"):
+        optim.clip_grad_norm_([a, a], 1.0)
+    p = torch.zeros(3, device=cuda, requires_grad=True)
+    p.grad = torch.ones_like(p)
+    for other, match in ((torch.optim.AdamW([p], amsgrad=True), "amsgrad"), (torch.optim.AdamW([p], maximize=True), "maximize"),
+                         (torch.optim.Adam([p], weight_decay=0.1), "decay")):
+        other.step()
+        opt = optim.AdamW([p], lr=0.25)
+        with pytest.raises(ValueError, match=match):
+            opt.load_state_dict(other.state_dict())
+        assert opt.param_groups[0]["lr"] == 0.25
+    good = torch.optim.Adam([p], lr=2e-3)
+    good.step()
+    opt = optim.AdamW([p])
+    opt.load_state_dict(good.state_dict())
+    assert opt.param_groups[0]["lr"] == 2e-3 and int(opt.state[p]["step"]) == 1
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_loading_its_own_state_changes_nothing(pkg, cuda, bits):
+    """state_dict refers to the state itself; loading it back keeps it, and parameters that a checkpoint leaves out start anew."""
+    from ubio_molfm_amd import optim
+    ps = _params(SHAPES, torch.float32, cuda, 53)
+    opt = optim.AdamW(ps, lr=1e-3, state_bits=bits)
+    opt.step(), opt.step()
+    before = [x.clone() for x in opt.moments()]
+    sd = opt.state_dict()
+    opt.load_state_dict(sd)
+    assert all(torch.equal(x, y) for x, y in zip(before, opt.moments())) and int(opt.state[ps[5]]["step"]) == 2
+    sd = copy.deepcopy(sd)
+    del sd["state"][5]
+    opt.load_state_dict(sd)
+    assert int(opt.state[ps[5]]["step"]) == 0 and not opt.state[ps[5]]["exp_avg"].any()
+    assert int(opt.state[ps[8]]["step"]) == 2
+    opt.step()
+    assert int(opt.state[ps[5]]["step"]) == 1 and int(opt.state[ps[8]]["step"]) == 3

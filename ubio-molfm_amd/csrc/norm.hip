@@ -566,7 +566,7 @@ unsigned ln_grid(const LnArgs& P, int type, LnPass pass, bool sums) {
   const int r = f.lanes > 64 ? 1 : 256 / f.lanes;
   int64_t most = f.lanes == 1024 ? 512 : f.lanes == 256 ? 2048 : 1024;
   if (sums) most = f.lanes == 1024 ? 256 : f.vecs <= 1 ? 1024 : 512;
-  else if (pass != LnPass::kFwd && f.lanes <= 32 && f.vecs <= 1) most = 1 << 30;
+  else if (pass != LnPass::kFwd && f.lanes <= 32 && f.vecs <= 1) most = 1 << 23;
   return (unsigned)std::min<int64_t>((P.n + r - 1) / r, most);
 }
 

@@ -500,7 +500,7 @@ E2V2_API int e2v2_grad_scale(void* const* grads, const int64_t* numel, int n, in
 
 E2V2_API int e2v2_adamw(const e2v2_adamw_args* a, hipStream_t s) {
   E2V2_REQUIRE(a, "adamw: null arguments");
-  E2V2_REQUIRE(a->n_chunks >= 0 && a->n_tensors >= 0 && a->n_tensors <= kStepList,
+  E2V2_REQUIRE(a->n_chunks >= 0 && a->n_chunks < 1 << 24 && a->n_tensors >= 0 && a->n_tensors <= kStepList,
                "adamw: %d chunks of %d tensors (at most %d)", a->n_chunks, a->n_tensors, kStepList);
   E2V2_REQUIRE(opt_type_ok(a->type) && (a->bits == 32 || a->bits == 8), "adamw: type %d, moments of %d bits", a->type,
                a->bits);
@@ -553,7 +553,7 @@ E2V2_API int e2v2_adamw(const e2v2_adamw_args* a, hipStream_t s) {
 
 E2V2_API int e2v2_moments(const uint8_t* mc, const uint8_t* ms, const uint8_t* vc, const uint8_t* vs, void* m, void* v,
                           int type, int64_t n, hipStream_t s) {
-  E2V2_REQUIRE(n >= 0 && n % 32 == 0 && n < (1LL << 41) && opt_type_ok(type), "moments: %lld elements, type %d",
+  E2V2_REQUIRE(n >= 0 && n % 32 == 0 && n < (1LL << 34) && opt_type_ok(type), "moments: %lld elements, type %d",
                (long long)n, type);
   if (n == 0) return 0;
   E2V2_REQUIRE(mc && ms && vc && vs && m && v, "moments: null operand");

@@ -124,6 +124,9 @@ def clip_grad_norm_(parameters, max_norm: float) -> torch.Tensor:
     if not grads:
         return torch.zeros((), device="cuda" if torch.cuda.is_available() else None)
     dev, types, dense = _check(grads, "clip_grad_norm_")
+    ptrs = [p for p in map(torch.Tensor.data_ptr, dense) if p]
+    if len(set(ptrs)) < len(ptrs):
+        raise ValueError("clip_grad_norm_: the same gradient twice")
     out = torch.zeros((), dtype=torch.float32, device=dev)
     with _on(dev):
         st = _lib.stream(dev)
@@ -191,6 +194,9 @@ class _Plan:
         for p in params:
             if p.device != params[0].device:
                 raise ValueError(f"AdamW: parameters on {params[0].device} and {p.device}")
+        spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()) for p in params if p.numel())
+        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+            raise ValueError("AdamW: parameters that share memory")
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("AdamW: the first step, and the one after a change of parameters or state, cannot be captured: "
                                "take it before the capture")
@@ -207,7 +213,7 @@ class _Plan:
         self.ms, self.vs = ((torch.zeros(self.total // _RUN, dtype=torch.uint8, device=dev) for _ in range(2))
                             if bits == 8 else (None, None))
         self.launches, order, chunks = [], [], 0
-        for group in groups:
+        for k_group, group in enumerate(groups):
             by_type = {}
             for p in group["params"]:
                 if p in place:
@@ -216,7 +222,7 @@ class _Plan:
                 for k in range(0, len(ps), _LIST):
                     part = ps[k:k + _LIST]
                     n = sum([-(-p.numel() // _CHUNK) for p in part])
-                    self.launches.append(_Launch(group, dtype, part, len(order), chunks, n))
+                    self.launches.append(_Launch(k_group, dtype, part, len(order), chunks, n))
                     order += part
                     chunks += n
         table, first = _chunk_table([p.data_ptr() for p in order], [place[p] for p in order], [p.numel() for p in order])
@@ -234,21 +240,33 @@ class _Plan:
                 a.ms, a.vs = self.ms.data_ptr(), self.vs.data_ptr()
             a.n_chunks, a.n_tensors, a.first_tensor = l.n_chunks, len(l.params), l.first_tensor
             a.type, a.bits, a.seed = _TYPES[l.dtype], bits, opt.seed & 0xFFFFFFFF
-        olds = [(p, opt.state.get(p)) for p in params]
-        for p, _ in olds:
-            opt.state[p] = self._views(p, place[p], first[p])
-        olds = [(p, old) for p, old in olds if old]
-        if olds:
-            steps = torch.stack([torch.as_tensor(old["step"]).to(dev, torch.int32).view(()) for _, old in olds])
-            where = [torch.arange(first[p], first[p] - (-p.numel() // _CHUNK)) for p, _ in olds]
-            self.steps[torch.cat(where).to(dev)] = steps.repeat_interleave(
-                torch.tensor([len(w) for w in where], device=dev))
-            for (p, old), step in zip(olds, steps):
-                if not p.numel():
-                    opt.state[p]["step"].copy_(step)
-            keys = [k for k in opt.state[olds[0][0]] if k != "step"]
-            pairs = [(opt.state[p][k], old[k]) for p, old in olds for k in keys]
-            torch._foreach_copy_([d for d, _ in pairs], [o for _, o in pairs])
+        self.first = first
+        self.state = {p: self._views(p, place[p], first[p]) for p in params}
+        if opt._skipped is None or opt._skipped.device != dev:
+            opt._skipped = torch.zeros((), dtype=torch.int32, device=dev)
+        self.fill({p: opt.state[p] for p in params if opt.state.get(p)})
+        opt.state.update(self.state)
+
+    def fill(self, entries):
+        """Takes over the states in entries (of the plan's parameters)."""
+        if not entries:
+            return
+        dev = self.device
+        steps = torch.stack([torch.as_tensor(e["step"]).to(dev, torch.int32).view(()) for e in entries.values()])
+        where = [torch.arange(self.first[p], self.first[p] - (-p.numel() // _CHUNK)) for p in entries]
+        self.steps[torch.cat(where).to(dev)] = steps.repeat_interleave(torch.tensor([len(w) for w in where], device=dev))
+        for p, step in zip(entries, steps):
+            if not p.numel():
+                self.state[p]["step"].copy_(step)
+        pairs = [(t, e[k]) for p, e in entries.items() for k, t in self.state[p].items() if k != "step"]
+        torch._foreach_copy_([d for d, _ in pairs], [o for _, o in pairs])
+
+    def clear(self, params):
+        """Zero states for some of the plan's parameters."""
+        for p in params:
+            self.steps[self.first[p]:self.first[p] - (-p.numel() // _CHUNK)].zero_()
+            for t in self.state[p].values():
+                t.zero_()
 
     def _views(self, p, o, chunk):
         """The parameter's state: views of the plan's buffers."""
@@ -281,8 +299,9 @@ class AdamW(torch.optim.Optimizer):
     they are read (they stay as they were); skip_nonfinite leaves parameters, moments and step counts as they were where that norm
     is not finite and counts such steps in ``skipped``.  ``grad_norm`` is the last step's norm (None without either).
 
-    A step after the first can be captured into a graph and replayed: step counts are on the device.  ``state`` entries are
-    views of flat buffers: moments can be written in place, step counts through load_state_dict."""
+    A step after the first can be captured into a graph and replayed: step counts are on the device.  Such a graph goes on after
+    load_state_dict; parameters that move and groups that are added void it.  ``state`` entries are views of flat buffers: moments
+    can be written in place, step counts through load_state_dict; an entry that is taken out starts anew."""
 
     _plan: Optional[_Plan] = None
     _OPTIONS = ("state_bits", "max_norm", "skip_nonfinite", "seed")
@@ -303,6 +322,11 @@ class AdamW(torch.optim.Optimizer):
     @staticmethod
     def _check_group(g):
         lr, (b1, b2) = g["lr"], g["betas"]
+        for k in ("amsgrad", "maximize", "differentiable"):
+            if g.get(k):
+                raise ValueError(f"AdamW: {k} is not supported")
+        if not g.get("decoupled_weight_decay", True) and g["weight_decay"]:
+            raise ValueError("AdamW: weight decay as a part of the gradient is not supported")
         if not isinstance(lr, torch.Tensor) and not 0.0 <= lr < math.inf:
             raise ValueError(f"AdamW: lr {lr}")
         if isinstance(lr, torch.Tensor) and lr.numel() != 1:
@@ -362,9 +386,18 @@ class AdamW(torch.optim.Optimizer):
                     raise ValueError(f"AdamW: {k} of parameter {i} is {tuple(e[k].shape)} {e[k].dtype}, not {size} "
                                      f"{'in a floating type' if self.state_bits == 32 else torch.uint8}")
             new[p] = {k: e[k] for k in names}
+        for g in groups:
+            self._check_group(g)
+        plan = self._plan if self._valid() else None
         super().load_state_dict({**state_dict, "state": {}})      # refuses groups of other sizes
-        self.state.update(new)
-        self._plan = _Plan(self)
+        if plan is None:
+            self.state.update(new)
+            self._plan = _Plan(self)
+        else:                                                     # in place: captured steps go on with the new state
+            plan.fill(new)                                        # new may be the plan's own state
+            plan.clear([p for p in plan.params if p not in new])
+            self.state.update(plan.state)
+            self._plan = plan
 
     def moments(self, dtype: Optional[torch.dtype] = None) -> Tuple[torch.Tensor, torch.Tensor]:
         """(m, v) of all parameters in the order of the groups, flat, each parameter's from a multiple of 64 elements on
@@ -382,12 +415,16 @@ class AdamW(torch.optim.Optimizer):
                       _lib.i32(_TYPES[dtype]), _lib.i64(plan.total), _lib.stream(plan.device))
         return m, v
 
-    def _current(self) -> _Plan:
-        """The plan, made anew where parameters moved."""
+    def _valid(self) -> bool:
+        """Whether the plan holds: no parameter moved, no state was taken out."""
         plan = self._plan
-        if plan is None or list(map(torch.Tensor.data_ptr, plan.params)) != plan.ptrs:
-            self._plan = plan = _Plan(self)
-        return plan
+        return (plan is not None and len(self.state) >= len(plan.params)
+                and list(map(torch.Tensor.data_ptr, plan.params)) == plan.ptrs)
+
+    def _current(self) -> _Plan:
+        if not self._valid():
+            self._plan = _Plan(self)
+        return self._plan
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -403,8 +440,6 @@ class AdamW(torch.optim.Optimizer):
     def _launch(self, plan: _Plan):
         st = _lib.stream(plan.device)
         normed = self.max_norm is not None or self.skip_nonfinite
-        if self.skip_nonfinite and self._skipped is None:
-            self._skipped = torch.zeros((), dtype=torch.int32, device=plan.device)
         _refuse(plan.outside)
         count = C.c_int(0)
         keep, updated = [], []
@@ -429,7 +464,7 @@ class AdamW(torch.optim.Optimizer):
             plan.norm.zero_()                  # no gradient at all
         norm = plan.norm.data_ptr()
         for l in plan.launches:
-            a, g = l.args, l.group
+            a, g = l.args, self.param_groups[l.group]
             a.grads = l.grads.address()
             lr = g["lr"]
             if isinstance(lr, torch.Tensor) and lr.device == plan.device and lr.dtype == torch.float32:
@@ -442,7 +477,7 @@ class AdamW(torch.optim.Optimizer):
             a.max_norm = math.inf if self.max_norm is None else self.max_norm
             a.norm, norm = norm, None
             a.skip_nonfinite = int(self.skip_nonfinite)
-            a.skipped = self._skipped.data_ptr() if self.skip_nonfinite else None
+            a.skipped = self._skipped.data_ptr()
             _lib.call("e2v2_adamw", C.byref(a), st)
         # what is kept per weight version (packed weights, radial tables) is made anew
         torch.autograd.graph.increment_version(updated)
