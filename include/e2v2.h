@@ -600,8 +600,8 @@ int e2v2_ln_silu_bwd2(const float* x, const float* g, const float* b, const floa
 /* ---- layer norm of rows, with its backward pass and that pass's derivative ----
  * The nn.LayerNorm of any width up to 16384 on rows in fp32, bf16 or fp16 (the reference's LayerNorms:
  * module_utils.py:2151-2178, 2230-2233); the rows' elements are consecutive, rows lie ld* elements apart (0: one row
- * for all); y, gx, and the second order's dgy (in y) and dx (in gx) are written contiguous.  Parameters may be NULL (weight 1, bias
- * 0) and have a type of their own.  Statistics and sums are fp32.
+ * for all); y, gx, and the second order's dgy (in y) and dx (in gx) are written contiguous.  Parameters may be NULL
+ * (weight 1, bias 0) and have a type of their own.  Statistics and sums are fp32.
  *   fwd:  y; stats [n][2] = (mean, rstd) unless NULL.
  *   bwd:  gx from x, gy and stats; with gg / gb (either may be NULL) also the gradients of weight and bias.
  *   bwd2: given the upstream gradients qx, qg, qb (each may be NULL: zero; qg and qb in the parameters' types) of
@@ -628,18 +628,18 @@ int e2v2_layer_norm_bwd2(const e2v2_layer_norm_args* args, void* gg, float* work
 
 /* ---- the parameter update of training, over many tensors at once ----
  * No counterpart in the reference's own code: its trainer calls torch's clipping and optimizer
- * (src/molfm/pipeline/trainer.py:114-662).  Tensors are contiguous fp32, bf16 or fp16; `grads` and `numel` are host arrays,
- * a NULL gradient leaves its tensor out.
+ * (src/molfm/pipeline/trainer.py:114-662).  Tensors are contiguous fp32, bf16 or fp16; `grads` and `numel` are host
+ * arrays, a NULL gradient leaves its tensor out.
  *   grad_norm        partial sums of the squares in fp64; *n_parts (host) partial sums are there before the call and
  *                    grow by what it adds, so that several lists join; grad_norm_parts: the most that one list adds.
  *   grad_norm_value  norm = the root of the partial sums' sum.
  *   grad_scale       every gradient times min(1, max_norm / (norm + 1e-6)); norm written unless NULL.
- *   adamw            one step (decoupled weight decay) of the tensors whose chunks the table lists, the gradients scaled
- *                    as by grad_scale where n_parts > 0 (max_norm infinite: not scaled).  skip_nonfinite: a norm that
- *                    is not finite leaves everything as it was and adds 1 to *skipped.  steps[chunk] counts the
- *                    steps taken.  Moments: fp32, or codes of 8 bits (bits = 8) with a scale byte for each run of 32 elements
- *                    in ms and vs (csrc/optim.hip); an element's place `off + i` in them counts from the chunk's off,
- *                    a multiple of 64, and the run that a tensor ends in is padded with zeros.
+ *   adamw            one step (decoupled weight decay) of the tensors whose chunks the table lists, the gradients
+ *                    scaled as by grad_scale where n_parts > 0 (max_norm infinite: not scaled).  skip_nonfinite: a
+ *                    norm that is not finite leaves everything as it was and adds 1 to *skipped.  steps[chunk] counts
+ *                    the steps taken.  Moments: fp32, or codes of 8 bits (bits = 8) with a scale byte for each run of
+ *                    32 elements in ms and vs (csrc/optim.hip); an element's place `off + i` in them counts from the
+ *                    chunk's off, a multiple of 64, and the run that a tensor ends in is padded with zeros.
  *   moments          the values of n codes (a multiple of 32) in fp32, bf16 or fp16. */
 #define E2V2_OPT_CHUNK 4096
 typedef struct {

@@ -59,7 +59,8 @@ def _check_first(x, gy, w, b, y, gx, gg, gb):
         assert (got.double() - ref).abs().le(tol).all(), "parameters"
 
 
-WIDTHS = [1, 2, 3, 5, 8, 9, 16, 17, 31, 32, 33, 64, 65, 100, 128, 129, 255, 256, 257, 512, 520, 1000, 1024, 1025, 1032, 2048, 2049, 4096,
+WIDTHS = [1, 2, 3, 5, 8, 9, 16, 17, 31, 32, 33, 64, 65, 100, 128, 129, 255, 256, 257, 512, 520, 1000, 1024, 1025, 1032,
+          2048, 2049, 4096,
           4097, 4104, 5001, 8192, 8193, 16383, 16384]
 
 
@@ -96,8 +97,8 @@ def test_many_rows(pkg, cuda, w):
 
 def test_second_order(pkg, cuda):
     """L = <gx, R0> + <dg, R1> + <db, R2>, differentiated in x, the weight, the bias and gy.  Five dependent row sums,
-    each within 64 u of magnitudes that are at most four times the result's in the 2-norm: 2e-5 relative, plus the type's half
-    step for each of two roundings (of gx or its factor, and of the result)."""
+    each within 64 u of magnitudes that are at most four times the result's in the 2-norm: 2e-5 relative, plus the
+    type's half step for each of two roundings (of gx or its factor, and of the result)."""
     from ubio_molfm_amd import norms
     for w, n, dtype in [(1, 5, torch.float32), (16, 300, torch.float32), (100, 40, torch.float32),
                         (128, 20000, torch.float32), (129, 777, torch.float32), (256, 1, torch.float32),
@@ -167,7 +168,8 @@ def test_absent_parameters(pkg, cuda, affine):
     ref_leaves = [t.detach().double().requires_grad_(True) for t in leaves]
     it = iter(ref_leaves)
     X = next(it)
-    ref_y = _ref(X, next(it) if W is not None else one.detach().double(), next(it) if B is not None else zero.detach().double())
+    ref_y = _ref(X, next(it) if W is not None else one.detach().double(),
+                 next(it) if B is not None else zero.detach().double())
     ref = torch.autograd.grad(ref_y, ref_leaves, gy.double(), create_graph=True)
     for a, r in zip((y, *got), (ref_y, *ref)):
         assert float((a.double() - r).norm() / r.norm()) < 64 * U
@@ -178,9 +180,9 @@ def test_absent_parameters(pkg, cuda, affine):
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_layouts(pkg, cuda, dtype):
-    """Rows of a wider matrix, rows off 16-byte boundaries, every second row, a transposed operand, one row broadcast, and upstream
-    gradients that lie in those ways: bitwise the results of contiguous copies, in which the same sums run (where the
-    layout takes the elementwise variant, within its bounds)."""
+    """Rows of a wider matrix, rows off 16-byte boundaries, every second row, a transposed operand, one row broadcast,
+    and upstream gradients that lie in those ways: bitwise the results of contiguous copies, in which the same sums run
+    (where the layout takes the elementwise variant, within its bounds)."""
     from ubio_molfm_amd import norms
     n, w = 45, 128
     g = torch.Generator().manual_seed(2)
@@ -189,7 +191,8 @@ def test_layouts(pkg, cuda, dtype):
     wt = torch.randn(w, generator=g).to(cuda)
     b = torch.randn(w, generator=g).to(cuda)
     layouts = {"columns": big[:n, w:2 * w], "shifted": big[:n, 3:3 + w], "every second": big[:2 * n:2, :w],
-               "transposed": base.t(), "broadcast": big[:1, :w].expand(n, w), "blocks": big[:2 * 20].view(2, 20, -1)[..., :w]}
+               "transposed": base.t(), "broadcast": big[:1, :w].expand(n, w),
+               "blocks": big[:2 * 20].view(2, 20, -1)[..., :w]}
     for name, x in layouts.items():
         for gy_name in (name, "plain"):
             X = x.detach().clone().requires_grad_(True)
@@ -261,7 +264,8 @@ def test_streams_and_graph(pkg, cuda):
         with torch.cuda.stream(s):
             outs.append(step(*args))
     torch.cuda.synchronize()
-    assert all(torch.equal(a, r) for a, r in zip(outs[0], want)) and all(torch.equal(a, r) for a, r in zip(outs[1], want2))
+    for out, ref in zip(outs, (want, want2)):
+        assert all(torch.equal(a, r) for a, r in zip(out, ref))
     del outs
     sx, sg = x.clone(), gy.clone()
     side = torch.cuda.Stream()
@@ -304,7 +308,7 @@ def test_run_seq_uses_it(pkg, cuda, w, silu, monkeypatch):
     from ubio_molfm_amd import _lib
     from ubio_molfm_amd import second_order as so
     torch.manual_seed(w)
-    mods = [torch.nn.Linear(24, w), torch.nn.LayerNorm(w)] + ([torch.nn.SiLU()] if silu else []) + [torch.nn.Linear(w, 5)]
+    mods = [torch.nn.Linear(24, w), torch.nn.LayerNorm(w), *([torch.nn.SiLU()] if silu else []), torch.nn.Linear(w, 5)]
     net = torch.nn.Sequential(*mods).to(cuda)
     with torch.no_grad():
         net[1].weight.normal_(1, 0.3)
@@ -324,4 +328,5 @@ def test_run_seq_uses_it(pkg, cuda, w, silu, monkeypatch):
     assert {"e2v2_layer_norm_fwd", "e2v2_layer_norm_bwd", "e2v2_layer_norm_bwd2"} <= set(called)
     ref = run(lambda m, h: m(h), copy.deepcopy(net).double(), p.double())
     for a, r in zip(got, ref):
-        assert float((a.double() - r).norm() / r.norm()) < 1e-4       # the linears' fp32 products included, as ln_silu's test
+        # the linears' fp32 products are in it too: the bound of ln_silu's own test
+        assert float((a.double() - r).norm() / r.norm()) < 1e-4

@@ -1,10 +1,10 @@
 """optim.AdamW, clip_grad_norm_ and grad_norm (csrc/optim.hip) against their formulas in float64, one step at a time
 from the kernel's own state, so that errors do not compound.
 
-Tolerances (u = 2^-24, half a step of fp32): a moment is two products and a sum of numbers that carry a scaled gradient's two
-roundings: 6 u of the two terms' magnitudes.  The update's factor has an expm1 of a rounded argument (4 u), two quotients, two
-roots and three products: 24 u of its magnitude, besides the moments' errors (the root halves v's).  A parameter adds
-one subtraction and its type's rounding uT."""
+Tolerances (u = 2^-24, half a step of fp32): a moment is two products and a sum of numbers that carry a scaled
+gradient's two roundings: 6 u of the two terms' magnitudes.  The update's factor has an expm1 of a rounded argument (4
+u), two quotients, two roots and three products: 24 u of its magnitude, besides the moments' errors (the root halves
+v's).  A parameter adds one subtraction and its type's rounding uT."""
 import copy
 import math
 
@@ -15,7 +15,8 @@ pytestmark = pytest.mark.gpu
 
 U = 2.0 ** -24
 UT = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
-SHAPES = [(1,), (3,), (63,), (64,), (65,), (37, 129), (0,), (4096,), (4097,), (2, 5, 8191), (31,), (32,), (33,), (20001,)]
+SHAPES = [(1,), (3,), (63,), (64,), (65,), (37, 129), (0,), (4096,), (4097,), (2, 5, 8191), (31,), (32,), (33,),
+          (20001,)]
 
 
 def _params(shapes, dtype, cuda, seed, shift=0):
@@ -55,8 +56,8 @@ def _check_step(p, p0, g, m0, v0, m, v, t, hyper, bits=32):
 
 
 @pytest.mark.parametrize("bits", [32, 8])
-@pytest.mark.parametrize("dtype,shift", [(torch.float32, 0), (torch.float32, 1), (torch.bfloat16, 0), (torch.bfloat16, 3),
-                                         (torch.float16, 0), (torch.float16, 1)])
+@pytest.mark.parametrize("dtype,shift", [(torch.float32, 0), (torch.float32, 1), (torch.bfloat16, 0),
+                                         (torch.bfloat16, 3), (torch.float16, 0), (torch.float16, 1)])
 def test_steps(pkg, cuda, dtype, shift, bits):
     """Several steps with new gradients, two groups with their own values, clipped."""
     from ubio_molfm_amd import optim
@@ -107,8 +108,8 @@ def _grid(x, bits):
 
 def test_eight_bit_codes(pkg, cuda):
     """The stored moments: each is the float64 result rounded down or up to a code as the hash of seed, step and
-    element says, but where fp32 rounding (2^-18 of a step at most: 6 u of a value of at most 16 steps, and the move into place) takes
-    the sum of fraction and random part across one."""
+    element says, but where fp32 rounding (2^-18 of a step at most: 6 u of a value of at most 16 steps, and the move
+    into place) takes the sum of fraction and random part across one."""
     from ubio_molfm_amd import optim
     ps = _params([(5000,), (96,), (33,)], torch.float32, cuda, 4)
     opt = optim.AdamW(ps, lr=1e-3, state_bits=8, seed=77)
@@ -138,9 +139,10 @@ def test_eight_bit_codes(pkg, cuda):
 
 
 def test_eight_bit_moments_follow_the_mean(pkg, cuda):
-    """Constant gradients, 500 steps.  A step moves v by 0.1% of its distance: the nearest code, 6% to 12% apart, would never
-    be left.  Stochastically rounded, v's mean is that of the recursion; a step's rounding has variance at most (0.001 + 0.001) v^2 / 8
-    with memory 1/0.002, 0.35 v over one element and 0.0055 v over 4,096: five of those, and likewise m (0.1 / 8 and 1/0.19)."""
+    """Constant gradients, 500 steps.  A step moves v by 0.1% of its distance: the nearest code, 6% to 12% apart, would
+    never be left.  Stochastically rounded, v's mean is that of the recursion; a step's rounding has variance at most
+    (0.001 + 0.001) v^2 / 8 with memory 1/0.002, 0.35 v over one element and 0.0055 v over 4,096: five of those, and
+    likewise m (0.1 / 8 and 1/0.19)."""
     from ubio_molfm_amd import optim
     p = torch.zeros(4096, device=cuda, requires_grad=True)
     p.grad = torch.full_like(p, 0.7)
@@ -228,7 +230,7 @@ def test_norms_at_the_edges(pkg, cuda):
     small = torch.full((4,), 1e-30, device=cuda)
     assert abs(float(optim.grad_norm([small])) / 2e-30 - 1) < 4 * U
     assert float(optim.grad_norm([])) == 0 and float(optim.grad_norm([torch.empty(0, device=cuda)])) == 0
-    mixed = [torch.ones(3, device=cuda), torch.ones(6, device=cuda, dtype=torch.bfloat16), torch.ones(7, device=cuda).half()]
+    mixed = [torch.ones(3, device=cuda), torch.ones(6, device=cuda).bfloat16(), torch.ones(7, device=cuda).half()]
     assert float(optim.grad_norm(mixed)) == 4.0
     p = torch.zeros(4, device=cuda, requires_grad=True)
     p.grad = torch.tensor([1.0, float("inf"), 2.0, -3.0], device=cuda)
@@ -257,9 +259,11 @@ def test_skipped_steps(pkg, cuda, bits):
     assert int(opt.skipped) == 2 and int(opt.state[ps[0]]["step"]) == 2 and not torch.equal(ps[0].detach(), keep[0])
 
 
-@pytest.mark.parametrize("bits,dtype", [(32, torch.float32), (32, torch.bfloat16), (8, torch.float32), (8, torch.bfloat16)])
+@pytest.mark.parametrize("bits,dtype", [(32, torch.float32), (32, torch.bfloat16), (8, torch.float32),
+                                        (8, torch.bfloat16)])
 def test_state_goes_on(pkg, cuda, bits, dtype):
-    """A saved and loaded state, a copied optimizer, parameters that moved, and one more group: each goes on bitwise as the first."""
+    """A saved and loaded state, a copied optimizer, parameters that moved, and one more group: each goes on bitwise as
+    the first."""
     from ubio_molfm_amd import optim
 
     def fresh(src):
@@ -329,8 +333,8 @@ def test_takes_a_torch_checkpoint(pkg, cuda):
 
 @pytest.mark.parametrize("bits", [32, 8])
 def test_graph_and_streams(pkg, cuda, bits):
-    """A captured step with a learning rate on the device, replayed on new gradients with eager work between, against eager
-    steps; and a step on a stream of its own."""
+    """A captured step with a learning rate on the device, replayed on new gradients with eager work between, against
+    eager steps; and a step on a stream of its own."""
     from ubio_molfm_amd import optim
     ps, qs = (_params(SHAPES, torch.float32, cuda, 21) for _ in range(2))
     lr_a, lr_b = (torch.tensor(1e-3, device=cuda) for _ in range(2))
@@ -445,10 +449,10 @@ def test_scheduler_and_closure(pkg, cuda):
 
 
 def test_training_run(pkg, cuda):
-    """The operators as they are used: a net with layer norms whose loss holds a gradient (forces), clipped AdamW steps;
-    against torch's modules, clipping and AdamW in float64.  Each of five steps moves a parameter by at most about lr = 1e-3; the
-    gradients agree to 1e-5, the steps' directions where sqrt(v) is not small against that: 1e-3 of the distance travelled, in
-    the 2-norm."""
+    """The operators as they are used: a net with layer norms whose loss holds a gradient (forces), clipped AdamW
+    steps; against torch's modules, clipping and AdamW in float64.  Each of five steps moves a parameter by at most
+    about lr = 1e-3; the gradients agree to 1e-5, the steps' directions where sqrt(v) is not small against that: 1e-3
+    of the distance travelled, in the 2-norm."""
     from ubio_molfm_amd import optim
     from ubio_molfm_amd import second_order as so
     torch.manual_seed(3)
@@ -480,8 +484,8 @@ def test_training_run(pkg, cuda):
 
 
 def test_model_sees_the_new_weights(pkg, cuda):
-    """What the model keeps per weight version (packed weights, distance tables) is made anew after a step: its energies are
-    bitwise those of a new model with the same weights."""
+    """What the model keeps per weight version (packed weights, distance tables) is made anew after a step: its
+    energies are bitwise those of a new model with the same weights."""
     from ubio_molfm_amd import model, optim, systems
     torch.manual_seed(0)
     m = model.MolfmAtomic(model.default_args()).to(cuda)
@@ -570,8 +574,8 @@ def test_states_that_are_taken_out_start_anew(pkg, cuda):
 
 
 def test_what_cannot_be_updated_is_refused(pkg, cuda):
-    """Memory that two parameters or two gradients share would be written by two workgroups at once; a checkpoint of another
-    method would go on as this one."""
+    """Memory that two parameters or two gradients share would be written by two workgroups at once; a checkpoint of
+    another method would go on as this one."""
     from ubio_molfm_amd import optim
     flat = torch.zeros(100, device=cuda)
     a, b = flat[:60].requires_grad_(True), flat[50:].requires_grad_(True)
@@ -583,7 +587,8 @@ def test_what_cannot_be_updated_is_refused(pkg, cuda):
         optim.clip_grad_norm_([a, a], 1.0)
     p = torch.zeros(3, device=cuda, requires_grad=True)
     p.grad = torch.ones_like(p)
-    for other, match in ((torch.optim.AdamW([p], amsgrad=True), "amsgrad"), (torch.optim.AdamW([p], maximize=True), "maximize"),
+    for other, match in ((torch.optim.AdamW([p], amsgrad=True), "amsgrad"),
+                         (torch.optim.AdamW([p], maximize=True), "maximize"),
                          (torch.optim.Adam([p], weight_decay=0.1), "decay")):
         other.step()
         opt = optim.AdamW([p], lr=0.25)
@@ -599,7 +604,8 @@ def test_what_cannot_be_updated_is_refused(pkg, cuda):
 
 @pytest.mark.parametrize("bits", [32, 8])
 def test_loading_its_own_state_changes_nothing(pkg, cuda, bits):
-    """state_dict refers to the state itself; loading it back keeps it, and parameters that a checkpoint leaves out start anew."""
+    """state_dict refers to the state itself; loading it back keeps it, and parameters that a checkpoint leaves out
+    start anew."""
     from ubio_molfm_amd import optim
     ps = _params(SHAPES, torch.float32, cuda, 53)
     opt = optim.AdamW(ps, lr=1e-3, state_bits=bits)

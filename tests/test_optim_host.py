@@ -17,7 +17,8 @@ def _p(*shape):
 
 
 @pytest.mark.parametrize("kw,match", [
-    (dict(lr=-1.0), "lr"), (dict(lr=float("nan")), "lr"), (dict(lr=torch.zeros(2)), "lr"), (dict(betas=(1.0, 0.9)), "betas"),
+    (dict(lr=-1.0), "lr"), (dict(lr=float("nan")), "lr"), (dict(lr=torch.zeros(2)), "lr"),
+    (dict(betas=(1.0, 0.9)), "betas"),
     (dict(betas=(0.9, -0.1)), "betas"), (dict(eps=-1e-8), "eps"), (dict(weight_decay=-0.1), "weight_decay"),
     (dict(state_bits=16), "16 bits"), (dict(max_norm=0.0), "max_norm"), (dict(max_norm=float("nan")), "max_norm")])
 def test_constructor_refuses(kw, match):

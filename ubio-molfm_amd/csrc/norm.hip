@@ -11,10 +11,12 @@
 // statistics, row sums and the parameters' sums are fp32, the variance taken about the mean in a second pass over the
 // registers.
 //
-// One pass over memory: a row stays in the registers of kL lanes (2 to 64 of a wavefront, or a workgroup of 256
-// or 1024), read as 16-byte vectors on whatever element boundary the row starts (the hardware takes them unaligned), the
-// rest of a row element by element.  A workgroup strides over the rows and keeps its columns' parameter sums in registers; each
-// leaves one partial row, added in order by a second launch, so results repeat bitwise.  Bound: HBM.
+// One pass over memory: a row stays in the registers of kL lanes (2 to 64 of a wavefront, or a workgroup of 256 or
+// 1024), read as 16-byte vectors on whatever element boundary the row starts (the hardware takes them unaligned); a
+// row's last vector may start early, its end is stored in pieces.  A workgroup strides over the rows and keeps its
+// columns' parameter sums in registers; each leaves one partial row, added in order by a second launch, so results
+// repeat bitwise.  Bound: HBM (127,113 x 128 fp32: forward 25 us, 5.2 TB/s; backward with the parameters 42, 4.7;
+// second order 67, 4.8; 32,768 x 2048 bf16: 52, 88 and 140 us).
 #include <algorithm>
 #include <type_traits>
 
@@ -54,9 +56,10 @@ __device__ __forceinline__ void each_vec(int l, int w, F&& f) {
   }
 }
 
-// A lane's vectors of a row of w >= V elements (any w for V = 1).  All loads are unconditional, so that those of a row's operands
-// are in flight together: a vector that would pass the end starts V before it instead (a branch would wait for its load in
-// place: 100,000 x 129 fp32 backward 57 us).  get() then moves what belongs to the row down and, with kClear, clears the rest.
+// A lane's vectors of a row of w >= V elements (any w for V = 1).  All loads are unconditional, so that those of a
+// row's operands are in flight together: a vector that would pass the end starts V before it instead (a branch would
+// wait for its load in place: 100,000 x 129 fp32 backward 57 us).  get() then moves what belongs to the row down and,
+// with kClear, clears the rest.
 template <typename T, int V, int kL, int NV>
 struct RowLoad {
   typename RowVec<T>::type raw[V > 1 ? NV : 1];
@@ -100,8 +103,8 @@ struct RowLoad {
   }
 };
 
-// The lane's V elements from column c on, or those of them that the row has: pieces of a half, a quarter, ... of a vector as
-// the bits of w % V say.
+// The lane's V elements from column c on, or those of them that the row has: pieces of a half, a quarter, ... of a
+// vector as the bits of w % V say.
 template <typename T, int V>
 __device__ __forceinline__ void store_row(const float* v, T* row, int c, int w, bool whole) {
   if constexpr (V == 1) {
@@ -468,12 +471,12 @@ void ln_launch(const LnArgs& P, unsigned grid, hipStream_t s) {
     hipLaunchKernelGGL((k_layer_norm_bwd2<T, V, kL, NV>), dim3(grid), block, 0, s, P);
 }
 
-// Lanes that hold a row, and 16-byte vectors a lane holds of it.  Up to 1024 elements a part of a wavefront, so that no
-// barrier stands in the way: of the shapes that hold the row one with few idle places (400,000 x 129 bf16 forward: 52 us
-// on 8 lanes of 3 vectors, 82 on 32 of one; 100,000 x 129 fp32: 24 on 16 of 3, 41 on 64 of one).  Wider rows take a workgroup of
-// 256, up to 32 elements a lane (6,007 x 5001 bf16 forward: 35 us, on 1024 lanes 45; second order, 4,000 x 8192 fp32: 147
-// and 188), in the backward pass with its two sums a column 16 (fp32: 6,007 x 5001 85 us with 24, 79 on 1024 lanes) or 24
-// (bf16: 4,000 x 8192 64 us with 32, 56 on 1024 lanes).
+// Lanes that hold a row, and 16-byte vectors a lane holds of it.  Up to 1024 elements a part of a wavefront, so that
+// no barrier stands in the way: of the shapes that hold the row one with few idle places (400,000 x 129 bf16 forward:
+// 52 us on 8 lanes of 3 vectors, 82 on 32 of one; 100,000 x 129 fp32: 24 on 16 of 3, 41 on 64 of one).  Wider rows
+// take a workgroup of 256, up to 32 elements a lane (6,007 x 5001 bf16 forward: 35 us, on 1024 lanes 45; second order,
+// 4,000 x 8192 fp32: 147 and 188), in the backward pass with its two sums a column 16 (fp32: 6,007 x 5001 85 us with
+// 24, 79 on 1024 lanes) or 24 (bf16: 4,000 x 8192 64 us with 32, 56 on 1024 lanes).
 struct LnShape {
   int lanes, vecs;       // vecs 0: rows shorter than a vector, one element a lane
 };
@@ -553,13 +556,13 @@ void ln_run(const LnArgs& P, int type, unsigned grid, hipStream_t s) {
   else ln_dispatch<kPass, _Float16>(P, grid, s);
 }
 
-// Workgroups of a pass.  They stride over the rows, with the parameters loaded once: a workgroup for every few rows loads them again
-// each time (forward, 127,113 x 128 fp32: 26 us with 1,024 workgroups, 38 with one for 8 rows; 32,768 x 2048 bf16: 51 with
-// 2,048, 232 with one a row).  Where sums of the parameters are left, fewer partial rows are fewer bytes, but one vector a lane needs four
-// workgroups a CU to have enough loads in flight (200,000 x 256 bf16: 60 us with 1,024, 83 with 512; 60,000 x 512 fp32, two
-// vectors: 76 and 72; 6,007 x 5001 fp32, 1024 lanes: 99 and, with 256, 81).  Without sums and with narrow
-// rows the backward pass only reloads the weight, which the caches hold: one row a lane group (853,991 x 128 fp32: 215
-// us, 244 with 1,024).
+// Workgroups of a pass.  They stride over the rows, with the parameters loaded once: a workgroup for every few rows
+// loads them again each time (forward, 127,113 x 128 fp32: 26 us with 1,024 workgroups, 38 with one for 8 rows; 32,768
+// x 2048 bf16: 51 with 2,048, 232 with one a row).  Where sums of the parameters are left, fewer partial rows are
+// fewer bytes, but one vector a lane needs four workgroups a CU to have enough loads in flight (200,000 x 256 bf16: 60
+// us with 1,024, 83 with 512; 60,000 x 512 fp32, two vectors: 76 and 72; 6,007 x 5001 fp32, 1024 lanes: 99 and, with
+// 256, 81).  Without sums and with narrow rows the backward pass only reloads the weight, which the caches hold: one
+// row a lane group (853,991 x 128 fp32: 215 us, 244 with 1,024).
 unsigned ln_grid(const LnArgs& P, int type, LnPass pass, bool sums) {
   const int v = 16 / type_size(type);
   const LnShape f = ln_shape(P.w, v, pass);
@@ -577,10 +580,8 @@ int ln_check(const char* what, const e2v2_layer_norm_args* a, bool bwd, bool bwd
   E2V2_REQUIRE(type_ok(a->type) && type_ok(a->g_type) && type_ok(a->b_type), "%s: types %d, %d, %d", what, a->type,
                a->g_type, a->b_type);
   E2V2_REQUIRE(a->ldx >= 0 && a->ldgy >= 0 && a->ldqx >= 0, "%s: negative row stride", what);
-  const uintptr_t mask = type_size(a->type) - 1;
-  E2V2_REQUIRE((((uintptr_t)a->x | (uintptr_t)a->gy | (uintptr_t)a->qx | (uintptr_t)a->y | (uintptr_t)a->gx) & mask) == 0 &&
-                   ((uintptr_t)a->stats & 7) == 0,
-               "%s: misaligned operand", what);
+  const uintptr_t all = (uintptr_t)a->x | (uintptr_t)a->gy | (uintptr_t)a->qx | (uintptr_t)a->y | (uintptr_t)a->gx;
+  E2V2_REQUIRE(all % type_size(a->type) == 0 && (uintptr_t)a->stats % 8 == 0, "%s: misaligned operand", what);
   if (a->n == 0) return 0;
   E2V2_REQUIRE(a->x && (bwd || a->y) && (!bwd || (a->gy && a->stats && a->gx)) && (!bwd2 || a->y),
                "%s: null operand", what);

@@ -3,22 +3,24 @@
 // t:
 //   m = b1 m + (1 - b1) c g,   v = b2 v + (1 - b2) (c g)^2
 //   p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v / (1 - b2^t)) + eps)
-// Arithmetic is fp32 (the norm's sum fp64: it neither loses small tensors beside large ones nor overflows; 8-bit moments
-// fp64 up to their code);
-// bf16 and fp16 parameters are rounded to nearest once.  Every element is read and written once by one thread,
-// the sums run in a fixed order: no atomics, results repeat bitwise.  Bound: HBM.
+// Arithmetic is fp32 (the norm's sum fp64: it neither loses small tensors beside large ones nor overflows; 8-bit
+// moments fp64 up to their code); bf16 and fp16 parameters are rounded to nearest once.  Every element is read and
+// written once by one thread, the sums run in a fixed order: no atomics, results repeat bitwise.  Bound: HBM (241 M
+// bf16 parameters with 32-bit moments 1.02 ms, 5.2 TB/s; 241 M fp32 parameters with 8-bit moments 0.74 ms, 5.2 TB/s;
+// 24.5 M fp32 in 240 tensors 133 us, a norm before it 20 us cold).
 //
-// The tensors are cut into chunks, one workgroup each.  What does not change from step to step (addresses and places of the
-// parameters) is a table in device memory; the gradients' addresses, which may, come with the launch.  The step count is kept per
-// chunk, so that each workgroup advances its own without waiting for another and a captured step counts its replays.
+// The tensors are cut into chunks, one workgroup each.  What does not change from step to step (addresses and places
+// of the parameters) is a table in device memory; the gradients' addresses, which may, come with the launch.  The step
+// count is kept per chunk, so that each workgroup advances its own without waiting for another and a captured step
+// counts its replays.
 //
 // Moments in 8 bits: runs of 32 consecutive elements share a scale byte s, 2^(s - 127) being the binade of the run's
 // largest value; m has a sign, 4 exponent and 3 mantissa bits (code 0x80: NaN), v no sign, 5 exponent and 3 mantissa
 // bits (code 255: NaN).  Moved by 2^(15 - s) or 2^(31 - s) a value's fp32 exponent field is the code's exponent field,
-// subnormals included, so that encoding is one ldexp, an addition and a shift, and decoding the reverse.  The
-// addition rounds stochastically: with b2 = 0.999 a step changes v by 0.1%, and rounding to the nearest of codes 6 to 12%
-// apart would leave it where it is for ever; here the stored value's mean is the value.  A v above zero keeps a code above zero:
-// zero would let the next step divide by eps.  The random bits are a hash of seed, step and element.  A value
+// subnormals included, so that encoding is one ldexp, an addition and a shift, and decoding the reverse.  The addition
+// rounds stochastically: with b2 = 0.999 a step changes v by 0.1%, and rounding to the nearest of codes 6 to 12% apart
+// would leave it where it is for ever; here the stored value's mean is the value.  A v above zero keeps a code above
+// zero: zero would let the next step divide by eps.  The random bits are a hash of seed, step and element.  A value
 // that is not finite becomes the NaN of its own element.
 #include <algorithm>
 #include <type_traits>
@@ -281,7 +283,8 @@ struct StepFactors {
   uint32_t key;
 };
 
-// One chunk.  kWhole: all of its elements are there; then the loads of both halves are in flight before the first is used.
+// One chunk.  kWhole: all of its elements are there; then the loads of both halves are in flight before the first is
+// used.
 template <bool kWhole, typename T, int kBits>
 __device__ __forceinline__ void adamw_chunk(const StepArgs& P, const StepFactors& F, const T* g, T* p, int n,
                                             int64_t off) {
@@ -327,8 +330,8 @@ __device__ __forceinline__ void adamw_chunk(const StepArgs& P, const StepFactors
         a = fmaf(P.one_b1, x, P.b1 * a);
         b = fmaf(P.one_b2 * x, x, P.b2 * b);
       } else {
-        // fp64 up to the code: truncated to fp32 a value keeps every bit that its code hangs on, so that the codes are those
-        // of the exact moments (a value next to a border would take the other code by its fp32 rounding)
+        // fp64 up to the code: truncated to fp32 a value keeps every bit that its code hangs on, so that the codes are
+        // those of the exact moments (a value next to a border would take the other code by its fp32 rounding)
         const double x = (double)gv[k][e] * F.c;
         a = truncated(fma(P.one_b1d, x, P.b1d * (double)a));
         b = truncated(fma(P.one_b2d * x, x, P.b2d * (double)b));

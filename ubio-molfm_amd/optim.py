@@ -30,8 +30,9 @@ class _Lists:
     """Dense tensors of one type as the library takes them: their addresses (0: left out) and sizes."""
 
     def __init__(self, dtype, ptrs, numels):
-        self.n, self.type = _lib.i32(len(ptrs)), _lib.i32(_TYPES[dtype])
+        self.type = _lib.i32(_TYPES[dtype])
         self.numel = array("q", numels)
+        self.n = _lib.i32(len(self.numel))
         self.set(ptrs)
 
     def set(self, ptrs):
@@ -53,8 +54,8 @@ class _Lists:
 
 
 def _dense(ts, what: str):
-    """The tensors in known types and contiguous (copies where they are not), and their types.  A few hundred pass here every
-    step: each property is read in one sweep."""
+    """The tensors in known types and contiguous (copies where they are not), and their types.  A few hundred pass here
+    every step: each property is read in one sweep."""
     types = {t.dtype for t in ts}
     try:
         contiguous = all(map(torch.Tensor.is_contiguous, ts))
@@ -79,17 +80,22 @@ def _check(ts, what: str):
     return ts[0].device, *_dense(ts, what)
 
 
-def _norm_parts(ts, types, dev, st):
-    """The lists by type, and their norm's partial sums."""
+def _by_type(ts, types):
+    """The tensors' lists."""
     lists = []
-    for d in types:
+    for d in sorted(types, key=_TYPES.get):
         of = ts if len(types) == 1 else [t for t in ts if t.dtype == d]
-        lists.append(_Lists(d, [t.data_ptr() for t in of], [t.numel() for t in of]))
+        lists.append(_Lists(d, map(torch.Tensor.data_ptr, of), map(torch.Tensor.numel, of)))
+    return lists
+
+
+def _norm_parts(lists, dev, st):
+    """The partial sums of the norm of all lists, and how many there are."""
     parts = torch.empty(max(1, sum([l.parts() for l in lists])), dtype=torch.float64, device=dev)
     count = C.c_int(0)
     for l in lists:
         l.norm(parts, count, st)
-    return lists, parts, count
+    return parts, count
 
 
 def _on(dev):
@@ -98,8 +104,8 @@ def _on(dev):
 
 
 def grad_norm(tensors: Iterable[torch.Tensor]) -> torch.Tensor:
-    """The 2-norm of all elements of the tensors (dense, fp32, bf16 or fp16, one device), as an fp32 tensor of one element on
-    that device; the squares are summed in fp64.  An empty list has norm 0 (on the current device)."""
+    """The 2-norm of all elements of the tensors (dense, fp32, bf16 or fp16, one device), as an fp32 tensor of one
+    element on that device; the squares are summed in fp64.  An empty list has norm 0 (on the current device)."""
     ts = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
     if not ts:
         return torch.zeros((), device="cuda")
@@ -107,15 +113,16 @@ def grad_norm(tensors: Iterable[torch.Tensor]) -> torch.Tensor:
     out = torch.empty((), dtype=torch.float32, device=dev)
     with _on(dev):
         st = _lib.stream(dev)
-        _, parts, count = _norm_parts(ts, types, dev, st)
+        lists = _by_type(ts, types)
+        parts, count = _norm_parts(lists, dev, st)
         _lib.call("e2v2_grad_norm_value", _lib.vp(parts.data_ptr()), count, _lib.vp(out.data_ptr()), st)
     return out
 
 
 def clip_grad_norm_(parameters, max_norm: float) -> torch.Tensor:
-    """Scales the parameters' gradients in place by min(1, max_norm / (norm + 1e-6)), norm their global 2-norm, which is
-    returned (an fp32 tensor of one element), as torch.nn.utils.clip_grad_norm_.  A norm that is not finite scales by what
-    the quotient gives (0, or NaN); nothing is read back to the host."""
+    """Scales the parameters' gradients in place by min(1, max_norm / (norm + 1e-6)), norm their global 2-norm, which
+    is returned (an fp32 tensor of one element), as torch.nn.utils.clip_grad_norm_.  A norm that is not finite scales
+    by what the quotient gives (0, or NaN); nothing is read back to the host."""
     max_norm = float(max_norm)
     if not max_norm >= 0:
         raise ValueError(f"clip_grad_norm_: max_norm {max_norm}")
@@ -124,13 +131,14 @@ def clip_grad_norm_(parameters, max_norm: float) -> torch.Tensor:
     if not grads:
         return torch.zeros((), device="cuda" if torch.cuda.is_available() else None)
     dev, types, dense = _check(grads, "clip_grad_norm_")
-    ptrs = [p for p in map(torch.Tensor.data_ptr, dense) if p]
+    lists = _by_type(dense, types)
+    ptrs = [p for l in lists for p in l.ptrs if p]
     if len(set(ptrs)) < len(ptrs):
         raise ValueError("clip_grad_norm_: the same gradient twice")
     out = torch.zeros((), dtype=torch.float32, device=dev)
     with _on(dev):
         st = _lib.stream(dev)
-        lists, parts, count = _norm_parts(dense, types, dev, st)
+        parts, count = _norm_parts(lists, dev, st)
         for l in lists:
             l.scale(parts, count, max_norm, out, st)
     if dense is not grads:
@@ -198,8 +206,8 @@ class _Plan:
         if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
             raise ValueError("AdamW: parameters that share memory")
         if torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("AdamW: the first step, and the one after a change of parameters or state, cannot be captured: "
-                               "take it before the capture")
+            raise RuntimeError("AdamW: the first step, and the one after a change of parameters or groups, cannot be "
+                               "captured: take it before the capture")
         self.device = dev = params[0].device if params else torch.device("cuda", torch.cuda.current_device())
         self.ptrs = [p.data_ptr() for p in params]
         self.params = params
@@ -225,7 +233,8 @@ class _Plan:
                     self.launches.append(_Launch(k_group, dtype, part, len(order), chunks, n))
                     order += part
                     chunks += n
-        table, first = _chunk_table([p.data_ptr() for p in order], [place[p] for p in order], [p.numel() for p in order])
+        table, first = _chunk_table([p.data_ptr() for p in order], [place[p] for p in order],
+                                    [p.numel() for p in order])
         self.chunks = torch.from_numpy(table.view(np.uint8)).to(dev)
         self.steps = torch.zeros(max(len(table), 1), dtype=torch.int32, device=dev)
         first = dict(zip(order, first))
@@ -254,7 +263,8 @@ class _Plan:
         dev = self.device
         steps = torch.stack([torch.as_tensor(e["step"]).to(dev, torch.int32).view(()) for e in entries.values()])
         where = [torch.arange(self.first[p], self.first[p] - (-p.numel() // _CHUNK)) for p in entries]
-        self.steps[torch.cat(where).to(dev)] = steps.repeat_interleave(torch.tensor([len(w) for w in where], device=dev))
+        counts = torch.tensor([len(w) for w in where], device=dev)
+        self.steps[torch.cat(where).to(dev)] = steps.repeat_interleave(counts)
         for p, step in zip(entries, steps):
             if not p.numel():
                 self.state[p]["step"].copy_(step)
@@ -285,23 +295,26 @@ class AdamW(torch.optim.Optimizer):
         m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2
         p = p (1 - lr weight_decay) - lr / (1 - b1^t) m / (sqrt(v / (1 - b2^t)) + eps)
 
-    params: contiguous fp32, bf16 or fp16 parameters on one GPU (others only without a gradient), or groups of them with their own lr, betas, eps and
-    weight_decay (lr may be a tensor of one fp32 element on that GPU, read by the step itself).  Parameters without a gradient are left
-    out of a step, as in torch.  Arithmetic and 32-bit moments are fp32 whatever the parameters' type, which are
-    rounded to nearest once a step.
+    params: contiguous fp32, bf16 or fp16 parameters on one GPU (others only without a gradient), or groups of them
+    with their own lr, betas, eps and weight_decay (lr may be a tensor of one fp32 element on that GPU, read by the
+    step itself).  Parameters without a gradient are left out of a step, as in torch.  Arithmetic and 32-bit moments
+    are fp32 whatever the parameters' type, which are rounded to nearest once a step.
 
-    state_bits=8 keeps both moments in 8 bits (runs of 32 elements share a power-of-two scale; 3 mantissa
-    bits, rounded stochastically by a hash of ``seed``, step and element, so that runs repeat): 2.1 bytes a parameter
-    instead of 8.  ``state[p]`` then holds codes ("exp_avg", "exp_avg_sq") and scale bytes ("..._scale"); ``moments`` gives
-    values.
+    state_bits=8 keeps both moments in 8 bits (runs of 32 elements share a power-of-two scale; 3 mantissa bits, rounded
+    stochastically by a hash of ``seed``, step and element, so that runs repeat): 2.1 bytes a parameter instead of 8.
+    ``state[p]`` then holds codes ("exp_avg", "exp_avg_sq") and scale bytes ("..._scale"); ``moments`` gives values.
 
     max_norm scales the gradients by min(1, max_norm / (norm + 1e-6)), norm their global 2-norm over all groups, as
-    they are read (they stay as they were); skip_nonfinite leaves parameters, moments and step counts as they were where that norm
-    is not finite and counts such steps in ``skipped``.  ``grad_norm`` is the last step's norm (None without either).
+    they are read (they stay as they were); skip_nonfinite leaves parameters, moments and step counts as they were
+    where that norm is not finite and counts such steps in ``skipped``.  ``grad_norm`` is the last step's norm (None
+    without either).
 
-    A step after the first can be captured into a graph and replayed: step counts are on the device.  Such a graph goes on after
-    load_state_dict; parameters that move and groups that are added void it.  ``state`` entries are views of flat buffers: moments
-    can be written in place, step counts through load_state_dict; an entry that is taken out starts anew."""
+    A step after the first can be captured into a graph and replayed: step counts are on the device.  Such a graph goes
+    on after load_state_dict; parameters that move and groups that are added void it.  As with any graph torch does not
+    see that a replay changed the parameters: torch.autograd.graph.increment_version(parameters) says so to what is
+    kept per weight version (the evaluation path's packed weights and tables).  ``state`` entries are views of flat
+    buffers: moments can be written in place, step counts through load_state_dict; an entry that is taken out starts
+    anew."""
 
     _plan: Optional[_Plan] = None
     _OPTIONS = ("state_bits", "max_norm", "skip_nonfinite", "seed")
@@ -361,13 +374,16 @@ class AdamW(torch.optim.Optimizer):
 
     @property
     def skipped(self) -> Optional[torch.Tensor]:
-        """Steps left out because the norm was not finite (an int32 tensor of one element); None without skip_nonfinite."""
+        """Steps left out because the norm was not finite (an int32 tensor of one element); None without
+        skip_nonfinite."""
         return self._skipped if self.skip_nonfinite else None
 
     def load_state_dict(self, state_dict):
         """As torch's, with moments kept in their own types: fp32, or codes and scale bytes."""
         saved, groups = state_dict["state"], state_dict["param_groups"]
-        names = ["step", "exp_avg", "exp_avg_sq"] + (["exp_avg_scale", "exp_avg_sq_scale"] if self.state_bits == 8 else [])
+        names = ["step", "exp_avg", "exp_avg_sq"]
+        if self.state_bits == 8:
+            names += ["exp_avg_scale", "exp_avg_sq_scale"]
         new = {}
         for i, p in zip(chain.from_iterable(g["params"] for g in groups),
                         chain.from_iterable(g["params"] for g in self.param_groups)):
@@ -375,10 +391,12 @@ class AdamW(torch.optim.Optimizer):
             if not e:
                 continue
             if not _usable(p):
-                raise ValueError(f"AdamW: state for parameter {i}, which is not contiguous in fp32, bf16 or fp16 on the GPU")
+                raise ValueError(f"AdamW: state for parameter {i}, which is not contiguous in fp32, bf16 or fp16 on "
+                                 "the GPU")
             for k in names:
                 if k not in e:
-                    raise ValueError(f"AdamW: the state of parameter {i} has no {k} (moments of {self.state_bits} bits)")
+                    raise ValueError(f"AdamW: the state of parameter {i} has no {k} (moments of {self.state_bits} "
+                                     "bits)")
             for k in names[1:]:
                 size = (-(-p.numel() // _RUN),) if k.endswith("scale") else tuple(p.shape)
                 right = e[k].is_floating_point() if self.state_bits == 32 else e[k].dtype == torch.uint8
