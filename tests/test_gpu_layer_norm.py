@@ -330,3 +330,18 @@ def test_run_seq_uses_it(pkg, cuda, w, silu, monkeypatch):
     for a, r in zip(got, ref):
         # the linears' fp32 products are in it too: the bound of ln_silu's own test
         assert float((a.double() - r).norm() / r.norm()) < 1e-4
+
+
+def test_run_seq_calls_modules_that_do_more(pkg, cuda):
+    """Hooks on a LayerNorm and subclasses of it run as they do in nn.Sequential."""
+    from ubio_molfm_amd import second_order as so
+
+    class Scaled(torch.nn.LayerNorm):
+        def forward(self, x):
+            return 3 * super().forward(x)
+
+    x = torch.randn(7, 24, device=cuda)
+    hooked = torch.nn.LayerNorm(24).to(cuda)
+    hooked.register_forward_hook(lambda m, i, o: o + 1)
+    for net in (torch.nn.Sequential(hooked), torch.nn.Sequential(Scaled(24).to(cuda))):
+        assert torch.equal(so.run_seq(net, x), net(x))

@@ -227,9 +227,12 @@ def ln_silu(ln: nn.LayerNorm, x: torch.Tensor) -> torch.Tensor:
 
 
 def _layer_norm_takes(ln: nn.LayerNorm, x: torch.Tensor) -> bool:
-    """Whether norms.layer_norm computes ln(x): fp32 rows on the GPU, normalised over their last dimension."""
+    """Whether norms.layer_norm computes ln(x): fp32 rows on the GPU, normalised over their last dimension, by a module
+    that does no more (a subclass or a hook may)."""
     w = x.shape[-1]
-    return (x.is_cuda and x.dtype == torch.float32 and tuple(ln.normalized_shape) == (w,) and w <= _LN_MAX_WIDTH
+    return (type(ln) is nn.LayerNorm and not (ln._forward_hooks or ln._forward_pre_hooks or ln._backward_hooks
+                                              or ln._backward_pre_hooks)
+            and x.is_cuda and x.dtype == torch.float32 and tuple(ln.normalized_shape) == (w,) and w <= _LN_MAX_WIDTH
             and all(p is None or (p.is_cuda and p.dtype == torch.float32) for p in (ln.weight, ln.bias)))
 
 
