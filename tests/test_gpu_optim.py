@@ -621,3 +621,86 @@ def test_loading_its_own_state_changes_nothing(pkg, cuda, bits):
     assert int(opt.state[ps[8]]["step"]) == 2
     opt.step()
     assert int(opt.state[ps[5]]["step"]) == 1 and int(opt.state[ps[8]]["step"]) == 3
+
+
+def test_tiny_gradients_without_eps(pkg, cuda):
+    """Second moments below the smallest normal number (g^2 (1 - b2) from 1e-43 on) still scale the update: against the
+    formula in float64 from the moments that the kernel stored, with the update's factor as above."""
+    from ubio_molfm_amd import optim
+    p = torch.zeros(4100, device=cuda).requires_grad_(True)
+    p.grad = torch.logspace(-20, -12, 4100, device=cuda) * (1 - 2 * (torch.arange(4100, device=cuda) % 2))
+    opt = optim.AdamW([p], lr=1e-3, eps=0.0, weight_decay=0.0)
+    opt.step()
+    m, v = (opt.state[p][k].double() for k in ("exp_avg", "exp_avg_sq"))
+    assert (v > 0).all() and v.min() < 1e-42
+    want = -1e-3 / (1 - 0.9) * m / (v / (1 - 0.999)).sqrt()
+    assert (p.detach().double() - want).abs().le((24 + 3) * U * want.abs()).all()
+    q = torch.ones(5, device=cuda).requires_grad_(True)
+    q.grad = torch.zeros(5, device=cuda)
+    optim.AdamW([q], eps=1e-42, weight_decay=0.0).step()
+    assert torch.equal(q.detach(), torch.ones(5, device=cuda))
+
+
+def test_groups_that_are_changed_by_hand(pkg, cuda):
+    """A group or a parameter taken out stays as it is, one put in its place or added is updated, the others go on."""
+    from ubio_molfm_amd import optim
+    ps = _params([(70,), (64,), (4100,), (9,)], torch.float32, cuda, 4)
+    ref = [torch.nn.Parameter(p.detach().clone()) for p in ps]
+    for p, r in zip(ps, ref):
+        r.grad = p.grad.clone()
+    kw = dict(lr=1e-2, weight_decay=0.1)
+    opts = [cls([dict(params=q[:2]), dict(params=[q[2]], lr=2e-2)], **kw)
+            for cls, q in ((optim.AdamW, ps), (torch.optim.AdamW, ref))]
+
+    def check():
+        for o in opts:
+            o.step()
+        for p, r in zip(ps, ref):
+            # each of up to 4 steps: 27 u of an update below 2 lr, and the sums' roundings, on both sides
+            assert (p - r).abs().max() <= 4 * 2 * (27 * U * 4e-2 + 3 * U * float(r.detach().abs().max()))
+
+    check()
+    for o in opts:
+        o.param_groups.pop()
+    check()
+    for o, q in zip(opts, (ps, ref)):
+        o.param_groups[0]["params"][1] = q[3]
+    check()
+    for o, q in zip(opts, (ps, ref)):
+        o.param_groups[0]["params"].append(q[2])
+    check()
+
+
+def test_parameters_whose_memory_is_cut_turned_or_brought(pkg, cuda):
+    """.data that starts where it did with fewer elements or other strides, gradients of another size, a parameter that
+    comes to the GPU after a step: each is seen before the launch."""
+    from ubio_molfm_amd import optim
+    p = torch.ones(5000, device=cuda).requires_grad_(True)
+    whole = p.detach()
+    host = torch.ones(6).requires_grad_(True)
+    opt = optim.AdamW([p, host], lr=1e-2, weight_decay=0.0)
+    p.grad = torch.ones(5000, device=cuda)
+    opt.step()
+    p.grad = None
+    p.data = whole[:100]
+    p.grad = torch.ones(100, device=cuda)
+    del opt.state[p]
+    after = whole.clone()
+    opt.step()
+    assert (whole[:100] < after[:100]).all() and torch.equal(whole[100:], after[100:])
+    host.data = host.data.to(cuda)
+    host.grad = torch.ones(6, device=cuda)
+    opt.step()
+    assert (host.detach() < 1).all()
+    p.data = whole[:200]                       # the gradient is still that of 100 elements
+    del opt.state[p]
+    with pytest.raises(ValueError, match="other sizes"):
+        opt.step()
+
+    q = torch.ones(8, 8, device=cuda).requires_grad_(True)
+    opt = optim.AdamW([q])
+    q.grad = torch.ones(8, 8, device=cuda)
+    opt.step()
+    q.data = q.data.t()
+    with pytest.raises(ValueError, match="contiguous"):
+        opt.step()

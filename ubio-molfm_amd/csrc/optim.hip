@@ -23,6 +23,7 @@
 // zero: zero would let the next step divide by eps.  The random bits are a hash of seed, step and element.  A value
 // that is not finite becomes the NaN of its own element.
 #include <algorithm>
+#include <cfloat>
 #include <type_traits>
 
 #include "common.h"
@@ -277,6 +278,14 @@ __device__ __forceinline__ float truncated(double a) {
   return (float)__builtin_bit_cast(double, __builtin_bit_cast(uint64_t, a) & ~0x1FFFFFFFull);
 }
 
+// The root of a >= 0.  The instruction takes numbers below the smallest normal one for zero, and with eps = 0 the update
+// would be infinite: they are moved up before.  (1 ulp, as the instruction.)
+__device__ __forceinline__ float root_of(float a) {
+  const bool low = a < 0x1p-100f;
+  const float r = __builtin_amdgcn_sqrtf(low ? a * 0x1p64f : a);
+  return low ? r * 0x1p-32f : r;
+}
+
 struct StepFactors {
   double c;                            // of the gradients
   float size, root, decay;             // lr / (1 - b1^t), (1 - b2^t)^(-1/2), lr wd
@@ -336,7 +345,7 @@ __device__ __forceinline__ void adamw_chunk(const StepArgs& P, const StepFactors
         a = truncated(fma(P.one_b1d, x, P.b1d * (double)a));
         b = truncated(fma(P.one_b2d * x, x, P.b2d * (double)b));
       }
-      pv[k][e] -= fmaf(F.decay, pv[k][e], F.size * (a * frcp(fmaf(__builtin_amdgcn_sqrtf(b), F.root, P.eps))));
+      pv[k][e] -= fmaf(F.decay, pv[k][e], F.size * (a * frcp(fmaf(root_of(b), F.root, P.eps))));
     }
     store_some<kWhole>(pv[k], p, i, n);
     if constexpr (kBits == 32) {
@@ -538,7 +547,8 @@ E2V2_API int e2v2_adamw(const e2v2_adamw_args* a, hipStream_t s) {
   P.ln_b1 = (float)log(a->beta1); P.ln_b2 = (float)log(a->beta2);
   P.b1d = a->beta1; P.b2d = a->beta2;
   P.one_b1d = 1 - a->beta1; P.one_b2d = 1 - a->beta2;
-  P.eps = (float)a->eps;
+  // frcp takes numbers below the smallest normal one for zero (roots are far above it)
+  P.eps = a->eps > 0 ? std::max((float)a->eps, FLT_MIN) : 0.f;
   P.wd = (float)a->weight_decay;
   P.max_norm = a->max_norm;
   const dim3 grid(a->n_chunks), block(kOptThreads);

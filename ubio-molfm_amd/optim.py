@@ -12,6 +12,7 @@ import math
 from array import array
 from contextlib import nullcontext
 from itertools import chain
+from operator import is_, ne
 from typing import Iterable, Optional, Tuple, Union
 
 import numpy as np
@@ -196,6 +197,7 @@ class _Plan:
         groups = opt.param_groups
         every = [p for g in groups for p in g["params"]]
         # the others may stand in the groups as long as they have no gradient (a model's constants)
+        self.every, self.split = every, [len(g["params"]) for g in groups]
         params = [p for p in every if _usable(p)]
         self.outside = [p for p in every if not _usable(p)]
         _refuse(self.outside)
@@ -212,7 +214,7 @@ class _Plan:
         self.ptrs = [p.data_ptr() for p in params]
         self.params = params
         bits = opt.state_bits
-        sizes = [p.numel() for p in params]
+        self.sizes = sizes = [p.numel() for p in params]
         ends = np.cumsum([0] + [-(-n // _ALIGN) * _ALIGN for n in sizes]).tolist()
         self.total = ends[-1]
         place = dict(zip(params, ends))
@@ -434,10 +436,16 @@ class AdamW(torch.optim.Optimizer):
         return m, v
 
     def _valid(self) -> bool:
-        """Whether the plan holds: no parameter moved, no state was taken out."""
+        """Whether the plan holds: the groups have the same parameters, none was moved, cut or turned, no state was
+        taken out."""
         plan = self._plan
-        return (plan is not None and len(self.state) >= len(plan.params)
-                and list(map(torch.Tensor.data_ptr, plan.params)) == plan.ptrs)
+        if plan is None or len(self.state) < len(plan.params):
+            return False
+        groups = [g["params"] for g in self.param_groups]
+        return (list(map(len, groups)) == plan.split and all(map(is_, chain.from_iterable(groups), plan.every))
+                and not any(map(ne, map(torch.Tensor.data_ptr, plan.params), plan.ptrs))
+                and not any(map(ne, map(torch.Tensor.numel, plan.params), plan.sizes))
+                and all(map(torch.Tensor.is_contiguous, plan.params)) and not any(map(_usable, plan.outside)))
 
     def _current(self) -> _Plan:
         if not self._valid():
@@ -469,10 +477,14 @@ class AdamW(torch.optim.Optimizer):
                 types, dense = _dense(some, "AdamW")
                 if types != {l.dtype}:
                     raise ValueError(f"AdamW: gradients of type {types} for parameters in {l.dtype}")
-                updated += [p for p in l.params if p.grad is not None] if len(some) < len(grads) else l.params
+                all_there = len(some) == len(grads)
+                sizes = l.grads.numel if all_there else [n for n, g in zip(l.grads.numel, grads) if g is not None]
+                if any(map(ne, map(torch.Tensor.numel, dense), sizes)):
+                    raise ValueError("AdamW: gradients of other sizes than their parameters")
+                updated += l.params if all_there else [p for p in l.params if p.grad is not None]
                 it = iter(dense)
-                l.grads.set([0 if g is None else next(it).data_ptr() for g in grads] if len(some) < len(grads)
-                            else map(torch.Tensor.data_ptr, dense))
+                l.grads.set(map(torch.Tensor.data_ptr, dense) if all_there
+                            else [0 if g is None else next(it).data_ptr() for g in grads])
                 keep.append(dense)
             else:
                 l.grads.set([0] * len(grads))
