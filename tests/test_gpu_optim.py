@@ -635,6 +635,14 @@ def test_tiny_gradients_without_eps(pkg, cuda):
     assert (v > 0).all() and v.min() < 1e-42
     want = -1e-3 / (1 - 0.9) * m / (v / (1 - 0.999)).sqrt()
     assert (p.detach().double() - want).abs().le((24 + 3) * U * want.abs()).all()
+    # eps on both sides of 2^-38 / (1 - b2)^(1/2): second moments that still count beside it, and that round away
+    for eps in (2e-21, 1.1e-10, 1.2e-10, 1e-8):
+        p.data.zero_()
+        opt = optim.AdamW([p], lr=1e-3, eps=eps, weight_decay=0.0)
+        opt.step()
+        m, v = (opt.state[p][k].double() for k in ("exp_avg", "exp_avg_sq"))
+        want = -1e-3 / (1 - 0.9) * m / ((v / (1 - 0.999)).sqrt() + eps)
+        assert (p.detach().double() - want).abs().le((24 + 3) * U * want.abs() + 1e-42).all()
     q = torch.ones(5, device=cuda).requires_grad_(True)
     q.grad = torch.zeros(5, device=cuda)
     optim.AdamW([q], eps=1e-42, weight_decay=0.0).step()

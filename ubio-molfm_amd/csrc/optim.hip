@@ -278,9 +278,11 @@ __device__ __forceinline__ float truncated(double a) {
   return (float)__builtin_bit_cast(double, __builtin_bit_cast(uint64_t, a) & ~0x1FFFFFFFull);
 }
 
-// The root of a >= 0.  The instruction takes numbers below the smallest normal one for zero, and with eps = 0 the update
-// would be infinite: they are moved up before.  (1 ulp, as the instruction.)
+// The root of a >= 0.  The instruction takes numbers below the smallest normal one for zero; kTiny: they are moved up
+// before (1 ulp, as the instruction).
+template <bool kTiny>
 __device__ __forceinline__ float root_of(float a) {
+  if constexpr (!kTiny) return __builtin_amdgcn_sqrtf(a);
   const bool low = a < 0x1p-100f;
   const float r = __builtin_amdgcn_sqrtf(low ? a * 0x1p64f : a);
   return low ? r * 0x1p-32f : r;
@@ -294,7 +296,7 @@ struct StepFactors {
 
 // One chunk.  kWhole: all of its elements are there; then the loads of both halves are in flight before the first is
 // used.
-template <bool kWhole, typename T, int kBits>
+template <bool kWhole, bool kTiny, typename T, int kBits>
 __device__ __forceinline__ void adamw_chunk(const StepArgs& P, const StepFactors& F, const T* g, T* p, int n,
                                             int64_t off) {
   constexpr int N = 8, K = kOptChunk / (kOptThreads * N);
@@ -345,7 +347,7 @@ __device__ __forceinline__ void adamw_chunk(const StepArgs& P, const StepFactors
         a = truncated(fma(P.one_b1d, x, P.b1d * (double)a));
         b = truncated(fma(P.one_b2d * x, x, P.b2d * (double)b));
       }
-      pv[k][e] -= fmaf(F.decay, pv[k][e], F.size * (a * frcp(fmaf(root_of(b), F.root, P.eps))));
+      pv[k][e] -= fmaf(F.decay, pv[k][e], F.size * (a * frcp(fmaf(root_of<kTiny>(b), F.root, P.eps))));
     }
     store_some<kWhole>(pv[k], p, i, n);
     if constexpr (kBits == 32) {
@@ -370,7 +372,7 @@ __device__ __forceinline__ void adamw_chunk(const StepArgs& P, const StepFactors
   }
 }
 
-template <typename T, int kBits>
+template <typename T, int kBits, bool kTiny>
 __global__ __launch_bounds__(kOptThreads) void k_adamw(StepArgs P) {
   const e2v2_opt_chunk ch = P.chunks[blockIdx.x];
   StepFactors F;
@@ -397,8 +399,8 @@ __global__ __launch_bounds__(kOptThreads) void k_adamw(StepArgs P) {
   F.decay = lr * P.wd;
   F.key = kBits == 8 ? mix32(mix32(P.seed) + (uint32_t)t * kGolden + (uint32_t)((uint64_t)ch.off >> 32) * kRoot2) : 0;
   T* p = static_cast<T*>(ch.p) + ch.at;
-  if (ch.n == kOptChunk) adamw_chunk<true, T, kBits>(P, F, g + ch.at, p, ch.n, ch.off);
-  else adamw_chunk<false, T, kBits>(P, F, g + ch.at, p, ch.n, ch.off);
+  if (ch.n == kOptChunk) adamw_chunk<true, kTiny, T, kBits>(P, F, g + ch.at, p, ch.n, ch.off);
+  else adamw_chunk<false, kTiny, T, kBits>(P, F, g + ch.at, p, ch.n, ch.off);
 }
 
 // The values that codes stand for, eight a thread; exact in each of the three types as long as they are normal there.
@@ -552,14 +554,22 @@ E2V2_API int e2v2_adamw(const e2v2_adamw_args* a, hipStream_t s) {
   P.wd = (float)a->weight_decay;
   P.max_norm = a->max_norm;
   const dim3 grid(a->n_chunks), block(kOptThreads);
-  auto go = [&](auto type) {
+  auto go = [&](auto type, auto tiny) {
     using T = decltype(type);
-    if (a->bits == 32) hipLaunchKernelGGL((k_adamw<T, 32>), grid, block, 0, s, P);
-    else hipLaunchKernelGGL((k_adamw<T, 8>), grid, block, 0, s, P);
+    constexpr bool kTiny = decltype(tiny)::value;
+    if (a->bits == 32) hipLaunchKernelGGL((k_adamw<T, 32, kTiny>), grid, block, 0, s, P);
+    else hipLaunchKernelGGL((k_adamw<T, 8, kTiny>), grid, block, 0, s, P);
   };
-  if (a->type == E2V2_F32) go(float{});
-  else if (a->type == E2V2_BF16) go(__bf16{});
-  else go(_Float16{});
+  auto go_as = [&](auto tiny) {
+    if (a->type == E2V2_F32) go(float{}, tiny);
+    else if (a->type == E2V2_BF16) go(__bf16{}, tiny);
+    else go(_Float16{}, tiny);
+  };
+  // Roots of v below 2^-126 are below 2^-63, and (1 - b2^t)^(-1/2) is largest in the first step: beside a larger eps they
+  // round away.  With a smaller one, zero among them, the update would be too large or infinite.  (24.5 M parameters in
+  // fp32: 125 us without, 128 with these roots or with a branch in the kernel.)
+  if (a->eps < 0x1p-38 / sqrt(1 - a->beta2)) go_as(std::true_type{});
+  else go_as(std::false_type{});
   E2V2_LAUNCHED("k_adamw");
   return 0;
 }

@@ -11,8 +11,8 @@ import ctypes as C
 import math
 from array import array
 from contextlib import nullcontext
-from itertools import chain
-from operator import is_, ne
+from itertools import chain, compress, repeat
+from operator import attrgetter, is_, is_not
 from typing import Iterable, Optional, Tuple, Union
 
 import numpy as np
@@ -25,6 +25,7 @@ _CHUNK = 4096           # E2V2_OPT_CHUNK
 _LIST = 384             # tensors of one step launch
 _ALIGN = 64             # a tensor's moments start at a multiple of this many elements
 _RUN = 32               # elements that share a scale byte
+_NBYTES = attrgetter("nbytes")
 
 
 class _Lists:
@@ -172,7 +173,27 @@ class _Launch:
         self.group, self.dtype, self.params = group, dtype, params
         self.first_tensor, self.chunk0, self.n_chunks = first_tensor, chunk0, n_chunks
         self.grads = _Lists(dtype, [0] * len(params), [p.numel() for p in params])
+        self.nbytes = [p.nbytes for p in params]
         self.args = _lib.AdamWArgs()
+
+
+def _matching(grads, launch, which):
+    """The gradients of the launch's parameters (of those that ``which`` says; True: all), contiguous: of their types
+    and sizes."""
+    sizes = launch.nbytes if which is True else list(compress(launch.nbytes, which))
+    try:
+        # bytes that agree leave the type open only between the two of 16 bits
+        if (all(map(torch.Tensor.is_contiguous, grads)) and list(map(_NBYTES, grads)) == sizes
+                and (launch.dtype == torch.float32 or {g.dtype for g in grads} == {launch.dtype})):
+            return grads
+    except RuntimeError:                       # sparse tensors do not answer
+        pass
+    types, grads = _dense(grads, "AdamW")
+    if types != {launch.dtype}:
+        raise ValueError(f"AdamW: gradients of type {types} for parameters in {launch.dtype}")
+    if list(map(_NBYTES, grads)) != sizes:
+        raise ValueError("AdamW: gradients of other sizes than their parameters")
+    return grads
 
 
 def _chunk_table(ptrs, offs, sizes):
@@ -425,7 +446,7 @@ class AdamW(torch.optim.Optimizer):
         8-bit moments are exact in each as long as they are normal there)."""
         if dtype not in (None, *_TYPES):
             raise ValueError(f"AdamW.moments: {dtype}")
-        plan = self._current()
+        plan = self._plan if self._same_groups() else self._current()
         if self.state_bits == 32:
             return (plan.m, plan.v) if dtype is None else (plan.m.to(dtype), plan.v.to(dtype))
         dtype = dtype or torch.float32
@@ -435,16 +456,19 @@ class AdamW(torch.optim.Optimizer):
                       _lib.i32(_TYPES[dtype]), _lib.i64(plan.total), _lib.stream(plan.device))
         return m, v
 
-    def _valid(self) -> bool:
-        """Whether the plan holds: the groups have the same parameters, none was moved, cut or turned, no state was
-        taken out."""
+    def _same_groups(self) -> bool:
+        """Whether the plan is that of the groups' parameters, in their order, and no state was taken out."""
         plan = self._plan
         if plan is None or len(self.state) < len(plan.params):
             return False
         groups = [g["params"] for g in self.param_groups]
-        return (list(map(len, groups)) == plan.split and all(map(is_, chain.from_iterable(groups), plan.every))
-                and not any(map(ne, map(torch.Tensor.data_ptr, plan.params), plan.ptrs))
-                and not any(map(ne, map(torch.Tensor.numel, plan.params), plan.sizes))
+        return list(map(len, groups)) == plan.split and all(map(is_, chain.from_iterable(groups), plan.every))
+
+    def _valid(self) -> bool:
+        """Whether the plan holds for a step: the same groups, and no parameter was moved, cut or turned."""
+        plan = self._plan
+        return (self._same_groups() and list(map(torch.Tensor.data_ptr, plan.params)) == plan.ptrs
+                and list(map(torch.Tensor.numel, plan.params)) == plan.sizes
                 and all(map(torch.Tensor.is_contiguous, plan.params)) and not any(map(_usable, plan.outside)))
 
     def _current(self) -> _Plan:
@@ -471,19 +495,14 @@ class AdamW(torch.optim.Optimizer):
         keep, updated = [], []
         for l in plan.launches:
             grads = [p.grad for p in l.params]
-            some = [g for g in grads if g is not None]
+            all_there = all(map(is_not, grads, repeat(None)))
+            some = grads if all_there else [g for g in grads if g is not None]
             if some:
                 # a gradient lies on its parameter's device (torch sees to it where it is set)
-                types, dense = _dense(some, "AdamW")
-                if types != {l.dtype}:
-                    raise ValueError(f"AdamW: gradients of type {types} for parameters in {l.dtype}")
-                all_there = len(some) == len(grads)
-                sizes = l.grads.numel if all_there else [n for n, g in zip(l.grads.numel, grads) if g is not None]
-                if any(map(ne, map(torch.Tensor.numel, dense), sizes)):
-                    raise ValueError("AdamW: gradients of other sizes than their parameters")
-                updated += l.params if all_there else [p for p in l.params if p.grad is not None]
+                dense = _matching(some, l, all_there or [g is not None for g in grads])
+                updated += l.params if all_there else [p for p, g in zip(l.params, grads) if g is not None]
                 it = iter(dense)
-                l.grads.set(map(torch.Tensor.data_ptr, dense) if all_there
+                l.grads.set(list(map(torch.Tensor.data_ptr, dense)) if all_there
                             else [0 if g is None else next(it).data_ptr() for g in grads])
                 keep.append(dense)
             else:
