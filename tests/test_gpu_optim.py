@@ -712,3 +712,24 @@ def test_parameters_whose_memory_is_cut_turned_or_brought(pkg, cuda):
     q.data = q.data.t()
     with pytest.raises(ValueError, match="contiguous"):
         opt.step()
+
+
+@pytest.mark.parametrize("max_norm", [None, 1.0])
+def test_gradients_left_behind_on_the_host(pkg, cuda, max_norm):
+    """A parameter brought to the GPU by .data keeps its host gradient, and a gradient can be moved by its own .data:
+    the step refuses both and goes on once they are together."""
+    from ubio_molfm_amd import optim
+    p, q = torch.ones(6).requires_grad_(True), torch.ones(5, device=cuda).requires_grad_(True)
+    p.grad, q.grad = torch.ones(6), torch.ones(5, device=cuda)
+    p.data = p.data.to(cuda)
+    opt = optim.AdamW([q, p], lr=1e-2, max_norm=max_norm)
+    with pytest.raises(RuntimeError, match="gradients on"):
+        opt.step()
+    p.grad = p.grad.to(cuda)
+    opt.step()
+    after = p.detach().clone()
+    assert (after < 1).all() and int(opt.state[p]["step"]) == 1
+    p.grad.data = p.grad.data.cpu()
+    with pytest.raises(RuntimeError, match="gradients on"):
+        opt.step()
+    assert torch.equal(p.detach(), after) and int(opt.state[q]["step"]) == 1

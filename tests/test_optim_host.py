@@ -1,4 +1,6 @@
 """What optim refuses and checks without a GPU, and the entry points' checks of their arguments."""
+from types import SimpleNamespace
+
 import pytest
 import torch
 
@@ -97,3 +99,25 @@ def test_chunk_table():
     assert got == [(ptrs[k], at, offs[k] + at, min(4096, n - at), k) for k, n in enumerate(sizes)
                    for at in range(0, n, 4096)]
     assert [len(x) for x in optim._chunk_table([], [], [])] == [0, 0]
+
+
+class _OnGpu1(torch.Tensor):
+    """A host tensor that says it lies on the second GPU."""
+
+    @classmethod
+    def __torch_function__(cls, func, types, args=(), kwargs=None):
+        return 1 if func is torch.Tensor.get_device else super().__torch_function__(func, types, args, kwargs or {})
+
+
+@pytest.mark.parametrize("device,second", [(0, torch.Tensor), (1, torch.Tensor), (1, _OnGpu1), (0, _OnGpu1)])
+def test_gradients_that_lie_elsewhere(device, second):
+    """.data moves a parameter, or a gradient, without the other: the step sees it before it takes an address."""
+    grads = [torch.ones(4).as_subclass(_OnGpu1 if device else torch.Tensor), torch.ones(6).as_subclass(second)]
+    launch = SimpleNamespace(device=device, dtype=torch.float32, nbytes=[16, 24])
+    if device and second is _OnGpu1:
+        assert optim._matching(grads, launch, True) is grads
+        return
+    with pytest.raises(RuntimeError, match="gradients on"):
+        optim._matching(grads, launch, True)
+    with pytest.raises(RuntimeError, match="gradients on"):
+        optim._matching(grads[1:], launch, [False, True])

@@ -172,14 +172,18 @@ class _Launch:
     def __init__(self, group, dtype, params, first_tensor, chunk0, n_chunks):
         self.group, self.dtype, self.params = group, dtype, params
         self.first_tensor, self.chunk0, self.n_chunks = first_tensor, chunk0, n_chunks
+        self.device = params[0].get_device()
         self.grads = _Lists(dtype, [0] * len(params), [p.numel() for p in params])
         self.nbytes = [p.nbytes for p in params]
         self.args = _lib.AdamWArgs()
 
 
 def _matching(grads, launch, which):
-    """The gradients of the launch's parameters (of those that ``which`` says; True: all), contiguous: of their types
-    and sizes."""
+    """The gradients of the launch's parameters (of those that ``which`` says; True: all), contiguous: on their device, of
+    their types and sizes.  torch checks a gradient where it is set, but .data moves a parameter or a gradient alone."""
+    if set(map(torch.Tensor.get_device, grads)) != {launch.device}:
+        raise RuntimeError(f"AdamW: gradients on {sorted({str(g.device) for g in grads})} for parameters on "
+                           f"cuda:{launch.device}")
     sizes = launch.nbytes if which is True else list(compress(launch.nbytes, which))
     try:
         # bytes that agree leave the type open only between the two of 16 bits
@@ -498,7 +502,6 @@ class AdamW(torch.optim.Optimizer):
             all_there = all(map(is_not, grads, repeat(None)))
             some = grads if all_there else [g for g in grads if g is not None]
             if some:
-                # a gradient lies on its parameter's device (torch sees to it where it is set)
                 dense = _matching(some, l, all_there or [g is not None for g in grads])
                 updated += l.params if all_there else [p for p, g in zip(l.params, grads) if g is not None]
                 it = iter(dense)
