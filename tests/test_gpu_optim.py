@@ -733,3 +733,31 @@ def test_gradients_left_behind_on_the_host(pkg, cuda, max_norm):
     with pytest.raises(RuntimeError, match="gradients on"):
         opt.step()
     assert torch.equal(p.detach(), after) and int(opt.state[q]["step"]) == 1
+
+
+def test_a_captured_rate_after_load_state_dict(pkg, cuda):
+    """A step captured with its learning rate on the device takes the loaded rate, and what is written to it later."""
+    from ubio_molfm_amd import optim
+    ps, qs = (_params(SHAPES, torch.float32, cuda, 54) for _ in range(2))
+    a, b = (optim.AdamW(x, lr=torch.tensor(1e-3, device=cuda)) for x in (ps, qs))
+    a.step(), b.step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        a.step()
+    saved = copy.deepcopy(b.state_dict())
+    for rate in (torch.tensor(4e-3), 2e-3):
+        saved["param_groups"][0]["lr"] = rate
+        a.load_state_dict(saved)
+        b.load_state_dict(saved)
+        for p, q in zip(ps, qs):
+            p.data.copy_(q.data)
+        junk = [torch.full((), 1e3, device=cuda) for _ in range(64)]      # takes memory that was let go
+        for k in range(3):
+            graph.replay()
+            torch.cuda.synchronize()
+            b.step()
+            assert all(torch.equal(p, q) for p, q in zip(ps, qs)), (rate, k)
+            for o in (a, b):
+                o.param_groups[0]["lr"].mul_(0.5)
+        del junk

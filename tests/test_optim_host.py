@@ -121,3 +121,29 @@ def test_gradients_that_lie_elsewhere(device, second):
         optim._matching(grads, launch, True)
     with pytest.raises(RuntimeError, match="gradients on"):
         optim._matching(grads[1:], launch, [False, True])
+
+
+@pytest.mark.parametrize("loaded", [0.25, torch.tensor(0.25), torch.tensor([0.25], dtype=torch.float64)])
+def test_rates_that_are_tensors_stay(loaded, monkeypatch):
+    """load_state_dict writes the loaded learning rate into the tensor that a captured step (and a scheduler) holds."""
+    monkeypatch.setattr(optim, "_Plan", lambda opt: None)
+    lr = torch.tensor(1e-3)
+    opt = optim.AdamW([dict(params=[_p(3)], lr=lr), dict(params=[_p(2)], lr=0.5)])
+    sd = opt.state_dict()
+    for g, value in zip(sd["param_groups"], (loaded, 0.125)):
+        g["lr"] = value
+    opt.load_state_dict(sd)
+    assert opt.param_groups[0]["lr"] is lr and float(lr) == 0.25 and opt.param_groups[1]["lr"] == 0.125
+    opt.load_state_dict(opt.state_dict())
+    assert opt.param_groups[0]["lr"] is lr and float(lr) == 0.25
+
+
+def test_one_rate_for_groups_that_are_loaded_with_two(monkeypatch):
+    monkeypatch.setattr(optim, "_Plan", lambda opt: None)
+    lr = torch.tensor(1e-3)
+    opt = optim.AdamW([dict(params=[_p(3)]), dict(params=[_p(2)])], lr=lr)
+    assert opt.param_groups[1]["lr"] is lr
+    sd = opt.state_dict()
+    sd["param_groups"][0]["lr"], sd["param_groups"][1]["lr"] = 0.25, torch.tensor(0.5)
+    opt.load_state_dict(sd)
+    assert opt.param_groups[0]["lr"] is lr and [float(g["lr"]) for g in opt.param_groups] == [0.25, 0.5]

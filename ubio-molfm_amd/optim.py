@@ -337,7 +337,8 @@ class AdamW(torch.optim.Optimizer):
     without either).
 
     A step after the first can be captured into a graph and replayed: step counts are on the device.  Such a graph goes
-    on after load_state_dict; parameters that move and groups that are added void it.  As with any graph torch does not
+    on after load_state_dict (numbers among a group's values are those of the capture; a learning rate that is a tensor
+    is the loaded one); parameters that move and groups that are added void it.  As with any graph torch does not
     see that a replay changed the parameters: torch.autograd.graph.increment_version(parameters) says so to what is
     kept per weight version (the evaluation path's packed weights and tables).  ``state`` entries are views of flat
     buffers: moments can be written in place, step counts through load_state_dict; an entry that is taken out starts
@@ -406,7 +407,8 @@ class AdamW(torch.optim.Optimizer):
         return self._skipped if self.skip_nonfinite else None
 
     def load_state_dict(self, state_dict):
-        """As torch's, with moments kept in their own types: fp32, or codes and scale bytes."""
+        """As torch's, with moments kept in their own types: fp32, or codes and scale bytes.  Learning rates that are
+        tensors stay and take the loaded values."""
         saved, groups = state_dict["state"], state_dict["param_groups"]
         names = ["step", "exp_avg", "exp_avg_sq"]
         if self.state_bits == 8:
@@ -434,7 +436,16 @@ class AdamW(torch.optim.Optimizer):
         for g in groups:
             self._check_group(g)
         plan = self._plan if self._valid() else None
+        rates = [g["lr"] for g in self.param_groups]
         super().load_state_dict({**state_dict, "state": {}})      # refuses groups of other sizes
+        values = {}
+        for g, lr in zip(self.param_groups, rates):               # captured steps read the rates that are there
+            if isinstance(lr, torch.Tensor):
+                value = float(g["lr"])
+                if values.setdefault(id(lr), value) == value:     # else one tensor for groups of several rates
+                    with torch.no_grad():
+                        lr.fill_(value)
+                    g["lr"] = lr
         if plan is None:
             self.state.update(new)
             self._plan = _Plan(self)
