@@ -345,3 +345,31 @@ def test_run_seq_calls_modules_that_do_more(pkg, cuda):
     hooked.register_forward_hook(lambda m, i, o: o + 1)
     for net in (torch.nn.Sequential(hooked), torch.nn.Sequential(Scaled(24).to(cuda))):
         assert torch.equal(so.run_seq(net, x), net(x))
+
+
+@pytest.mark.parametrize("frozen", [True, False])
+def test_run_seq_under_transforms(pkg, cuda, frozen):
+    """Forward-mode tangents, torch.func's transforms and a trace go through the module, as in nn.Sequential."""
+    from torch.autograd import forward_ad
+    from ubio_molfm_amd import second_order as so
+    torch.manual_seed(5)
+    net = torch.nn.Sequential(torch.nn.Linear(6, 24), torch.nn.LayerNorm(24), torch.nn.Linear(24, 3)).to(cuda)
+    net.requires_grad_(not frozen)
+    x, t = torch.randn(7, 6, device=cuda), torch.randn(7, 6, device=cuda)
+
+    def both(f):
+        got, ref = f(lambda v: so.run_seq(net, v)), f(net)
+        assert len(got) == len(ref) and all(torch.equal(a, r) for a, r in zip(got, ref))
+
+    def dual(f):
+        with forward_ad.dual_level():
+            y = forward_ad.unpack_dual(f(forward_ad.make_dual(x, t)))
+            assert y.tangent is not None
+            return [y.primal.detach().clone(), y.tangent.detach().clone()]
+
+    both(dual)
+    both(lambda f: [torch.func.vmap(f)(torch.stack([x, t]))])
+    both(lambda f: list(torch.func.jvp(f, (x,), (t,))))
+    both(lambda f: [torch.func.grad(lambda v: f(v).square().sum())(x)])
+    traced = torch.jit.trace(lambda v: so.run_seq(net, v), (x,))
+    assert torch.equal(traced(t), net(t))

@@ -1,6 +1,7 @@
 """What norms.layer_norm and its entry points refuse, before any kernel or HIP call.  No GPU needed."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from ubio_molfm_amd import _lib, norms
 
@@ -38,6 +39,20 @@ def test_refusals(x, kw, match, monkeypatch):
     monkeypatch.setattr(_lib, "call", lambda *a: pytest.fail("a kernel was called"))
     with pytest.raises(ValueError, match=match):
         norms.layer_norm(x(), **kw)
+
+
+@pytest.mark.parametrize("which", ["rows", "weight", "bias"])
+def test_forward_mode_tangents_are_refused(which, monkeypatch):
+    """A result without the tangent would be a wrong derivative without a word."""
+    monkeypatch.setattr(_lib, "call", lambda *a: pytest.fail("a kernel was called"))
+    monkeypatch.setattr(norms, "_call", lambda *a: None)
+    t = dict(rows=_gpu(3, 8), weight=_gpu(8), bias=_gpu(8))
+    monkeypatch.setattr(_OnGpu, "get_device", lambda self: 0, raising=False)
+    with forward_ad.dual_level():
+        assert norms.layer_norm(t["rows"], t["weight"], t["bias"]).shape == (3, 8)     # no tangent: as ever
+        t[which] = forward_ad.make_dual(t[which], torch.ones_like(t[which]))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            norms.layer_norm(t["rows"], t["weight"], t["bias"])
 
 
 @pytest.mark.parametrize("shape,stride,ld", [

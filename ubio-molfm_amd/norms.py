@@ -11,6 +11,7 @@ import struct
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -163,6 +164,12 @@ class _LayerNormGradFn(torch.autograd.Function):
         return dgy, dx, dg, None, None, None, None, None
 
 
+def has_tangent(*tensors: Optional[torch.Tensor]) -> bool:
+    """Whether a tensor carries a forward-mode tangent."""
+    return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None
+                                                  for t in tensors)
+
+
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
                eps: float = 1e-5) -> torch.Tensor:
     """(x - mean) / sqrt(var + eps) * weight + bias over the last dimension of x, as
@@ -170,7 +177,8 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
 
     x: fp32, bf16 or fp16 on the GPU, of any shape with a last dimension of 1 to 16384; read where it lies if its rows
     are consecutive and evenly spaced.  weight, bias: [w], fp32 or x's type, or None.  The result has x's type
-    and is contiguous.  Differentiable twice (a third derivative raises)."""
+    and is contiguous.  Differentiable twice in reverse mode (a third derivative, forward-mode tangents and torch.func's
+    transforms raise)."""
     if not isinstance(x, torch.Tensor) or not x.is_cuda:
         raise RuntimeError("layer_norm runs on the GPU only (HIP library, no CPU path): got "
                            f"{x.device if isinstance(x, torch.Tensor) else type(x).__name__}")
@@ -185,6 +193,8 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
                               or not p.is_cuda or p.get_device() != x.get_device()):
             raise ValueError(f"layer_norm: {name} [{w}] in fp32 or {dtype} on {x.device}, got {tuple(p.shape)} "
                              f"{p.dtype} on {p.device}")
+    if has_tangent(x, weight, bias):
+        raise RuntimeError("layer_norm: forward-mode tangents are not supported")
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
                                     or (bias is not None and bias.requires_grad)):
         return _LayerNormFn.apply(x, weight, bias, float(eps))

@@ -38,7 +38,7 @@ import torch.nn.functional as F
 from . import _lib
 from . import so3
 from . import sparse_ops
-from .norms import MAX_WIDTH as _LN_MAX_WIDTH, _will_run, layer_norm
+from .norms import MAX_WIDTH as _LN_MAX_WIDTH, _will_run, has_tangent, layer_norm
 from .ops import ENV_A, ENV_B, ENV_C
 
 _EXPAND = {}
@@ -226,13 +226,20 @@ def ln_silu(ln: nn.LayerNorm, x: torch.Tensor) -> torch.Tensor:
     return y.view(x.shape)
 
 
+_PLAIN = {torch.Tensor, nn.Parameter, type(None)}
+
+
 def _layer_norm_takes(ln: nn.LayerNorm, x: torch.Tensor) -> bool:
     """Whether norms.layer_norm computes ln(x): fp32 rows on the GPU, normalised over their last dimension, by a module
-    that does no more (a subclass or a hook may)."""
+    that does no more (a subclass or a hook may), outside of what only torch's own operators go through: forward mode,
+    torch.func's transforms, tracing and tensor subclasses."""
+    if (torch._C._are_functorch_transforms_active() or torch.jit.is_tracing()
+            or not {type(x), type(ln.weight), type(ln.bias)} <= _PLAIN or has_tangent(x, ln.weight, ln.bias)):
+        return False
     w = x.shape[-1]
     return (type(ln) is nn.LayerNorm and not (ln._forward_hooks or ln._forward_pre_hooks or ln._backward_hooks
                                               or ln._backward_pre_hooks)
-            and x.is_cuda and x.dtype == torch.float32 and tuple(ln.normalized_shape) == (w,) and w <= _LN_MAX_WIDTH
+            and x.is_cuda and x.dtype == torch.float32 and tuple(ln.normalized_shape) == (w,) and 1 <= w <= _LN_MAX_WIDTH
             and all(p is None or (p.is_cuda and p.dtype == torch.float32) for p in (ln.weight, ln.bias)))
 
 
