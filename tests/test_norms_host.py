@@ -111,3 +111,32 @@ def test_entry_point_checks():
     for fn, args in ((lib.e2v2_layer_norm_bwd, (_lib.vp(64), None, _lib.vp(64))),
                      (lib.e2v2_layer_norm_bwd2, (_lib.vp(64), _lib.vp(64)))):
         assert fn(_lib.C.byref(a), *args, _lib.i64(need - 4), None) != 0 and b"workspace" in lib.e2v2_last_error()
+
+
+@pytest.mark.parametrize("affine", [True, False])
+@pytest.mark.parametrize("asked", ["xgb", "x", "g", "b", "xb", "gb"])
+def test_the_composed_second_order(affine, asked):
+    """What a third derivative differentiates, in float64: the second order's values as autograd gives them, and its own
+    gradients against differences."""
+    g = torch.Generator().manual_seed(3)
+    x, gy, q, w, b, qg, qb = (torch.randn(*s, generator=g, dtype=torch.float64)
+                              for s in ((2, 3, 5), (2, 3, 5), (2, 3, 5), (5,), (5,), (5,), (5,)))
+    if not affine and asked != "x":
+        return
+    x, gy, w, b = (t.requires_grad_(True) for t in (x, gy, w, b))
+    W = w if affine else None
+    ups = {"x": q, "g": qg, "b": qb}
+    first = torch.autograd.grad(torch.nn.functional.layer_norm(x, (5,), W, b if affine else None, 0.1),
+                                [x, *([w, b] if affine else [])], gy, create_graph=True)
+    first = dict(zip("xgb", first))
+    ref = torch.autograd.grad([first[k] for k in asked], [gy, x, w], [ups[k] for k in asked], allow_unused=True)
+
+    def second(gy, x, w):
+        return norms._composed2(gy, x, w if affine else None, 0.1, *(ups[k] if k in asked else None for k in "xgb"))
+
+    got = second(gy, x, w)
+    for a, r in zip(got, ref):
+        assert (a is None or not a.abs().max()) if r is None else torch.allclose(a, r, rtol=1e-11, atol=1e-12)
+    if asked != "b":
+        assert torch.autograd.gradcheck(lambda *t: [y for y in second(*t) if y is not None and y.requires_grad],
+                                        (gy, x, w) if affine else (gy, x, w.detach()))

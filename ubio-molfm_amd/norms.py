@@ -114,11 +114,11 @@ def _backward(gy, x, g, b, stats, eps, need_g, need_b):
 class _LayerNormFn(torch.autograd.Function):
 
     @staticmethod
-    def forward(ctx, x, g, b, eps: float):
+    def forward(ctx, x, g, b, eps: float, any_order: bool):
         stats = x.new_empty(2 * (x.numel() // x.shape[-1]), dtype=torch.float32)
         y = _forward(x, g, b, eps, stats)
         ctx.save_for_backward(x, g, b, stats)
-        ctx.eps = eps
+        ctx.eps, ctx.any_order = eps, any_order
         return y
 
     @staticmethod
@@ -134,8 +134,9 @@ class _LayerNormFn(torch.autograd.Function):
             nodes = [next(nodes)[0] for t in (g, b) if t is not None]
             if not any([_will_run(n) for n in nodes]):
                 need_g = need_b = False
-            gx, gg, gb = _LayerNormGradFn.apply(gy, x, g, b, stats, ctx.eps, need_g, need_b)
-        return gx if ctx.needs_input_grad[0] else None, gg, gb, None
+            fn = _LayerNormGradAnyFn if ctx.any_order else _LayerNormGradFn
+            gx, gg, gb = fn.apply(gy, x, g, b, stats, ctx.eps, need_g, need_b)
+        return gx if ctx.needs_input_grad[0] else None, gg, gb, None, None
 
 
 class _LayerNormGradFn(torch.autograd.Function):
@@ -153,15 +154,56 @@ class _LayerNormGradFn(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, qx, qg, qb):
-        gy, x, g, b, stats = ctx.saved_tensors
-        if qx is None and qg is None and qb is None:
-            return (None,) * 8
-        dgy, dx = _empty_rows(x), _empty_rows(x)
-        dg = _empty_rows(g) if ctx.needs_input_grad[2] else None
-        ws, n = _workspace(x) if dg is not None else (None, 0)
-        a, keep = _args(x, g, b, stats, ctx.eps, gy=gy, qx=qx, qg=qg, qb=qb, y=dgy, gx=dx)
-        _call("e2v2_layer_norm_bwd2", x.device, a, _ptr(dg), _ptr(ws), _lib.i64(n))
-        return dgy, dx, dg, None, None, None, None, None
+        return _backward2(ctx, qx, qg, qb)
+
+
+class _LayerNormGradAnyFn(_LayerNormGradFn):
+    """The same, differentiable on: where its own backward is to be differentiated (a third derivative of the norm),
+    that is composed of torch's operators."""
+
+    @staticmethod
+    def backward(ctx, qx, qg, qb):
+        if not torch.is_grad_enabled() or (qx is None and qg is None and qb is None):
+            return _backward2(ctx, qx, qg, qb)
+        gy, x, g, _, _ = ctx.saved_tensors
+        return (*_composed2(gy, x, g, ctx.eps, qx, qg, qb), None, None, None, None, None)
+
+
+def _backward2(ctx, qx, qg, qb):
+    """The gradients of _LayerNormGradFn's inputs through e2v2_layer_norm_bwd2."""
+    gy, x, g, b, stats = ctx.saved_tensors
+    if qx is None and qg is None and qb is None:
+        return (None,) * 8
+    dgy, dx = _empty_rows(x), _empty_rows(x)
+    dg = _empty_rows(g) if ctx.needs_input_grad[2] else None
+    ws, n = _workspace(x) if dg is not None else (None, 0)
+    a, keep = _args(x, g, b, stats, ctx.eps, gy=gy, qx=qx, qg=qg, qb=qb, y=dgy, gx=dx)
+    _call("e2v2_layer_norm_bwd2", x.device, a, _ptr(dg), _ptr(ws), _lib.i64(n))
+    return dgy, dx, dg, None, None, None, None, None
+
+
+def _composed2(gy, x, g, eps, qx, qg, qb):
+    """(dgy, dx, dg) of the second order by the formulas at the head of csrc/norm.hip."""
+    def mean(t):
+        return t.mean(-1, keepdim=True)
+
+    z = x - mean(x)
+    r = torch.rsqrt(mean(z * z) + eps)
+    h, u = z * r, gy if g is None else gy * g
+    dgy, t, extra, dg = 0, 0, 0, None
+    if qx is not None:
+        c, m = mean(u * h), mean(qx * h)
+        a = r * (qx - mean(qx) - h * m)
+        dgy = a if g is None else a * g
+        t = -r * (c * qx + m * u)
+        extra = r * h * mean(qx * r * (u - mean(u) - h * c))
+        dg = None if g is None else (gy * a).sum_to_size(g.shape)
+    if qg is not None:
+        dgy, t = dgy + qg * h, t + qg * gy
+    if qb is not None:
+        dgy = dgy + qb
+    dx = None if qx is None and qg is None else r * (t - mean(t) - h * mean(t * h)) - extra
+    return dgy.expand_as(gy), dx, dg
 
 
 def has_tangent(*tensors: Optional[torch.Tensor]) -> bool:
@@ -179,6 +221,12 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     are consecutive and evenly spaced.  weight, bias: [w], fp32 or x's type, or None.  The result has x's type
     and is contiguous.  Differentiable twice in reverse mode (a third derivative, forward-mode tangents and torch.func's
     transforms raise)."""
+    return _layer_norm(x, weight, bias, eps, any_order=False)
+
+
+def _layer_norm(x, weight, bias, eps: float, any_order: bool) -> torch.Tensor:
+    """layer_norm; any_order: differentiable as often as the nn.LayerNorm in whose place it stands, from the third
+    derivative on by torch's operators."""
     if not isinstance(x, torch.Tensor) or not x.is_cuda:
         raise RuntimeError("layer_norm runs on the GPU only (HIP library, no CPU path): got "
                            f"{x.device if isinstance(x, torch.Tensor) else type(x).__name__}")
@@ -197,5 +245,5 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
         raise RuntimeError("layer_norm: forward-mode tangents are not supported")
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
                                     or (bias is not None and bias.requires_grad)):
-        return _LayerNormFn.apply(x, weight, bias, float(eps))
+        return _LayerNormFn.apply(x, weight, bias, float(eps), any_order)
     return _forward(x, weight, bias, float(eps), None)

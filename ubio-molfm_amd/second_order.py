@@ -38,7 +38,7 @@ import torch.nn.functional as F
 from . import _lib
 from . import so3
 from . import sparse_ops
-from .norms import MAX_WIDTH as _LN_MAX_WIDTH, _will_run, has_tangent, layer_norm
+from .norms import MAX_WIDTH as _LN_MAX_WIDTH, _layer_norm, _will_run, has_tangent
 from .ops import ENV_A, ENV_B, ENV_C
 
 _EXPAND = {}
@@ -255,7 +255,7 @@ def run_seq(mods, h: torch.Tensor) -> torch.Tensor:
             h = ln_silu(mods[i], h)
             i += 2
         elif isinstance(mods[i], nn.LayerNorm) and _layer_norm_takes(mods[i], h):
-            h = layer_norm(h, mods[i].weight, mods[i].bias, mods[i].eps)
+            h = _layer_norm(h, mods[i].weight, mods[i].bias, mods[i].eps, any_order=True)
             i += 1
         elif isinstance(mods[i], nn.Linear) and h.dim() == 2 and h.shape[0] >= _EDGE_ROWS:
             h = edge_linear(mods[i], h)
