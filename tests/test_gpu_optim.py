@@ -761,3 +761,26 @@ def test_a_captured_rate_after_load_state_dict(pkg, cuda):
             for o in (a, b):
                 o.param_groups[0]["lr"].mul_(0.5)
         del junk
+
+
+@pytest.mark.parametrize("kind", ["group", "type", "list"])
+def test_the_norm_of_a_step_behind_empty_tensors(pkg, cuda, kind):
+    """A group, a type or a whole launch of parameters without elements comes first: the norm is this step's all the
+    same, and steps left out are counted."""
+    from ubio_molfm_amd import optim
+    empty = torch.zeros(0, device=cuda, dtype=torch.float16 if kind == "type" else torch.float32, requires_grad=True)
+    empties = [empty] + [torch.zeros(0, device=cuda, requires_grad=True) for _ in range(400 if kind == "list" else 0)]
+    ps = _params([(30,), (5000,)], torch.float32, cuda, 55)
+    for p in empties:
+        p.grad = torch.zeros_like(p)
+    groups = [dict(params=empties), dict(params=ps)] if kind == "group" else [dict(params=empties + ps)]
+    opt = optim.AdamW(groups, max_norm=0.5, skip_nonfinite=True)
+    for scale in (1.0, 3.0):
+        for p in ps:
+            p.grad.mul_(scale)
+        opt.step()
+        norm = math.sqrt(sum(float(p.grad.double().square().sum()) for p in ps))
+        assert abs(float(opt.grad_norm) - norm) <= 2 * U * norm
+    ps[1].grad[7] = float("nan")
+    opt.step()
+    assert int(opt.skipped) == 1 and opt.grad_norm.isnan() and int(opt.state[ps[0]]["step"]) == 2

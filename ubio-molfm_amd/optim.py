@@ -538,7 +538,8 @@ class AdamW(torch.optim.Optimizer):
             a.eps, a.weight_decay = g["eps"], g["weight_decay"]
             a.parts, a.n_parts = plan.parts.data_ptr(), count.value
             a.max_norm = math.inf if self.max_norm is None else self.max_norm
-            a.norm, norm = norm, None
+            a.norm = norm if l.n_chunks else None      # one launch writes it; without chunks there is none
+            norm = None if l.n_chunks else norm
             a.skip_nonfinite = int(self.skip_nonfinite)
             a.skipped = self._skipped.data_ptr()
             _lib.call("e2v2_adamw", C.byref(a), st)
