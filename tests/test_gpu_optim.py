@@ -784,3 +784,26 @@ def test_the_norm_of_a_step_behind_empty_tensors(pkg, cuda, kind):
     ps[1].grad[7] = float("nan")
     opt.step()
     assert int(opt.skipped) == 1 and opt.grad_norm.isnan() and int(opt.state[ps[0]]["step"]) == 2
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_gaps_stay_zero_under_a_nan_factor(pkg, cuda, bits):
+    """One NaN gradient makes the clipping factor NaN, and so all moments; the gaps between tensors are none, and a good
+    checkpoint loaded in place brings everything back."""
+    from ubio_molfm_amd import optim
+    ps = _params(SHAPES, torch.float32, cuda, 56)
+    opt = optim.AdamW(ps, state_bits=bits, max_norm=0.5)
+    opt.step()
+    good = copy.deepcopy(opt.state_dict())
+    want = [x.clone() for x in opt.moments(torch.float32)]
+    inside = torch.zeros(want[0].numel(), dtype=torch.bool, device=cuda)
+    off = 0
+    for p in ps:
+        inside[off:off + p.numel()] = True
+        off += -(-p.numel() // 64) * 64
+    ps[5].grad[3, 4] = float("nan")
+    opt.step()
+    for x in opt.moments(torch.float32):
+        assert x[inside].isnan().all() and not x[~inside].any()
+    opt.load_state_dict(good)
+    assert all(torch.equal(x, y) for x, y in zip(opt.moments(torch.float32), want))

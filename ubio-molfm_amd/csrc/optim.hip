@@ -347,6 +347,7 @@ __device__ __forceinline__ void adamw_chunk(const StepArgs& P, const StepFactors
         a = truncated(fma(P.one_b1d, x, P.b1d * (double)a));
         b = truncated(fma(P.one_b2d * x, x, P.b2d * (double)b));
       }
+      if (!kWhole && i + e >= n) a = b = 0.f;        // the gap behind a tensor stays zero under a NaN factor too
       pv[k][e] -= fmaf(F.decay, pv[k][e], F.size * (a * frcp(fmaf(root_of<kTiny>(b), F.root, P.eps))));
     }
     store_some<kWhole>(pv[k], p, i, n);
