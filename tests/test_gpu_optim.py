@@ -807,3 +807,66 @@ def test_gaps_stay_zero_under_a_nan_factor(pkg, cuda, bits):
         assert x[inside].isnan().all() and not x[~inside].any()
     opt.load_state_dict(good)
     assert all(torch.equal(x, y) for x, y in zip(opt.moments(torch.float32), want))
+
+
+def test_entries_taken_out_behind_others(pkg, cuda):
+    """Entries left over from a group that was popped, and empty ones that reading the state makes, do not hide one that
+    was taken out; a captured step goes on in the same buffers."""
+    from ubio_molfm_amd import optim
+    ps = _params([(100,), (5000,), (70,)], torch.float32, cuda, 57)
+    opt = optim.AdamW([dict(params=ps[:2]), dict(params=ps[2:])], lr=1e-3)
+    opt.step(), opt.step()
+    opt.param_groups.pop()
+    opt.step()
+    steps = lambda: [int(opt.state[p]["step"]) for p in ps[:2]]
+    assert steps() == [3, 3] and ps[2] in opt.state
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    m = opt.state[ps[0]]["exp_avg"]
+    del opt.state[ps[0]]
+    with pytest.raises(RuntimeError, match="captured"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            opt.step()
+    opt.step()
+    assert steps() == [1, 4] and opt.state[ps[0]]["exp_avg"] is m
+    assert torch.equal(m, _first_moments(ps[0].grad, 1))
+    del opt.state[ps[0]]
+    assert opt.state[ps[0]] == {}                                    # reading makes an entry
+    opt.step()
+    assert steps() == [1, 5]
+    graph.replay()
+    torch.cuda.synchronize()
+    assert steps() == [2, 6] and torch.allclose(m, _first_moments(ps[0].grad, 2))
+    del opt.state[ps[1]]
+    assert not opt.moments()[1][128:].any() and opt.moments()[1][:100].any() and int(opt.state[ps[1]]["step"]) == 0
+
+
+def _first_moments(g, steps):
+    """First moments after steps with the same gradient, each rounding as the kernel's."""
+    b1, one_b1 = (torch.tensor(x, dtype=torch.float32) for x in (0.9, 1 - 0.9))
+    m = torch.zeros_like(g)
+    for _ in range(steps):
+        m = (one_b1.double().item() * g.double() + (b1.to(g.device) * m).double()).float()
+    return m
+
+
+def test_entries_put_in_by_hand(pkg, cuda):
+    from ubio_molfm_amd import optim
+    ps = _params([(100,), (5000,)], torch.float32, cuda, 58)
+    opt = optim.AdamW(ps, lr=1e-3)
+    opt.step()
+    saved = {k: t.clone() for k, t in opt.state[ps[1]].items()}
+    params = ps[1].detach().clone()
+    opt.step()
+    after = ps[1].detach().clone()
+    ps[1].data.copy_(params)
+    opt.state[ps[1]] = saved
+    opt.step()
+    assert torch.equal(ps[1], after) and int(opt.state[ps[1]]["step"]) == 2 and int(opt.state[ps[0]]["step"]) == 3
+    for broken in ({"step": 1}, {**saved, "exp_avg": saved["exp_avg"][:5]}):
+        opt.state[ps[1]] = broken
+        with pytest.raises(ValueError, match="exp_avg"):
+            opt.step()
+    assert torch.equal(ps[1], after)

@@ -280,8 +280,9 @@ class _Plan:
         self.state = {p: self._views(p, place[p], first[p]) for p in params}
         if opt._skipped is None or opt._skipped.device != dev:
             opt._skipped = torch.zeros((), dtype=torch.int32, device=dev)
-        self.fill({p: opt.state[p] for p in params if opt.state.get(p)})
+        self.fill({p: opt._entry(p, opt.state[p], f"a parameter {tuple(p.shape)}") for p in params if opt.state.get(p)})
         opt.state.update(self.state)
+        self.entries = list(opt.state.values())
 
     def fill(self, entries):
         """Takes over the states in entries (of the plan's parameters)."""
@@ -342,7 +343,8 @@ class AdamW(torch.optim.Optimizer):
     see that a replay changed the parameters: torch.autograd.graph.increment_version(parameters) says so to what is
     kept per weight version (the evaluation path's packed weights and tables).  ``state`` entries are views of flat
     buffers: moments can be written in place, step counts through load_state_dict; an entry that is taken out starts
-    anew."""
+    anew and one that is put in its place is taken over, both in the buffers that are there, by a step that is not
+    captured."""
 
     _plan: Optional[_Plan] = None
     _OPTIONS = ("state_bits", "max_norm", "skip_nonfinite", "seed")
@@ -406,13 +408,26 @@ class AdamW(torch.optim.Optimizer):
         skip_nonfinite."""
         return self._skipped if self.skip_nonfinite else None
 
+    def _entry(self, p, e, name):
+        """What belongs to the parameter's state of a loaded or hand-made entry."""
+        names = ["step", "exp_avg", "exp_avg_sq"]
+        if self.state_bits == 8:
+            names += ["exp_avg_scale", "exp_avg_sq_scale"]
+        for k in names:
+            if k not in e:
+                raise ValueError(f"AdamW: the state of {name} has no {k} (moments of {self.state_bits} bits)")
+        for k in names[1:]:
+            size = (-(-p.numel() // _RUN),) if k.endswith("scale") else tuple(p.shape)
+            right = e[k].is_floating_point() if self.state_bits == 32 else e[k].dtype == torch.uint8
+            if tuple(e[k].shape) != size or not right:
+                raise ValueError(f"AdamW: {k} of {name} is {tuple(e[k].shape)} {e[k].dtype}, not {size} "
+                                 f"{'in a floating type' if self.state_bits == 32 else torch.uint8}")
+        return {k: e[k] for k in names}
+
     def load_state_dict(self, state_dict):
         """As torch's, with moments kept in their own types: fp32, or codes and scale bytes.  Learning rates that are
         tensors stay and take the loaded values."""
         saved, groups = state_dict["state"], state_dict["param_groups"]
-        names = ["step", "exp_avg", "exp_avg_sq"]
-        if self.state_bits == 8:
-            names += ["exp_avg_scale", "exp_avg_sq_scale"]
         new = {}
         for i, p in zip(chain.from_iterable(g["params"] for g in groups),
                         chain.from_iterable(g["params"] for g in self.param_groups)):
@@ -422,17 +437,7 @@ class AdamW(torch.optim.Optimizer):
             if not _usable(p):
                 raise ValueError(f"AdamW: state for parameter {i}, which is not contiguous in fp32, bf16 or fp16 on "
                                  "the GPU")
-            for k in names:
-                if k not in e:
-                    raise ValueError(f"AdamW: the state of parameter {i} has no {k} (moments of {self.state_bits} "
-                                     "bits)")
-            for k in names[1:]:
-                size = (-(-p.numel() // _RUN),) if k.endswith("scale") else tuple(p.shape)
-                right = e[k].is_floating_point() if self.state_bits == 32 else e[k].dtype == torch.uint8
-                if tuple(e[k].shape) != size or not right:
-                    raise ValueError(f"AdamW: {k} of parameter {i} is {tuple(e[k].shape)} {e[k].dtype}, not {size} "
-                                     f"{'in a floating type' if self.state_bits == 32 else torch.uint8}")
-            new[p] = {k: e[k] for k in names}
+            new[p] = self._entry(p, e, f"parameter {i}")
         for g in groups:
             self._check_group(g)
         plan = self._plan if self._valid() else None
@@ -453,6 +458,7 @@ class AdamW(torch.optim.Optimizer):
             plan.fill(new)                                        # new may be the plan's own state
             plan.clear([p for p in plan.params if p not in new])
             self.state.update(plan.state)
+            plan.entries = list(self.state.values())
             self._plan = plan
 
     def moments(self, dtype: Optional[torch.dtype] = None) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -461,7 +467,7 @@ class AdamW(torch.optim.Optimizer):
         8-bit moments are exact in each as long as they are normal there)."""
         if dtype not in (None, *_TYPES):
             raise ValueError(f"AdamW.moments: {dtype}")
-        plan = self._plan if self._same_groups() else self._current()
+        plan = self._with_entries(self._plan) if self._same_groups() else self._current()
         if self.state_bits == 32:
             return (plan.m, plan.v) if dtype is None else (plan.m.to(dtype), plan.v.to(dtype))
         dtype = dtype or torch.float32
@@ -472,9 +478,9 @@ class AdamW(torch.optim.Optimizer):
         return m, v
 
     def _same_groups(self) -> bool:
-        """Whether the plan is that of the groups' parameters, in their order, and no state was taken out."""
+        """Whether the plan is that of the groups' parameters, in their order."""
         plan = self._plan
-        if plan is None or len(self.state) < len(plan.params):
+        if plan is None:
             return False
         groups = [g["params"] for g in self.param_groups]
         return list(map(len, groups)) == plan.split and all(map(is_, chain.from_iterable(groups), plan.every))
@@ -486,10 +492,28 @@ class AdamW(torch.optim.Optimizer):
                 and list(map(torch.Tensor.numel, plan.params)) == plan.sizes
                 and all(map(torch.Tensor.is_contiguous, plan.params)) and not any(map(_usable, plan.outside)))
 
+    def _with_entries(self, plan: _Plan) -> _Plan:
+        """The plan, with the states of entries that were taken out or put in their place by hand: zeros, or what they
+        hold, written into the buffers that are there, so that captured steps go on."""
+        state = self.state
+        if len(state) == len(plan.entries) and all(map(is_, state.values(), plan.entries)):
+            return plan
+        changed = {p: state.get(p) for p in plan.params if state.get(p) is not plan.state[p]}
+        if changed:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("AdamW: the first step after a change of the states cannot be captured: take it "
+                                   "before the capture")
+            new = {p: self._entry(p, e, f"a parameter {tuple(p.shape)}") for p, e in changed.items() if e}
+            plan.fill(new)
+            plan.clear([p for p in changed if p not in new])
+            state.update({p: plan.state[p] for p in changed})
+        plan.entries = list(state.values())
+        return plan
+
     def _current(self) -> _Plan:
         if not self._valid():
             self._plan = _Plan(self)
-        return self._plan
+        return self._with_entries(self._plan)
 
     @torch.no_grad()
     def step(self, closure=None):
