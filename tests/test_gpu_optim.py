@@ -870,3 +870,24 @@ def test_entries_put_in_by_hand(pkg, cuda):
         with pytest.raises(ValueError, match="exp_avg"):
             opt.step()
     assert torch.equal(ps[1], after)
+
+
+def test_tensors_put_into_entries(pkg, cuda, tmp_path):
+    """A moment and a step count put into an entry are the next step's; a saved state is made of plain dicts."""
+    from ubio_molfm_amd import optim
+    (p,), (q,) = (_params([(9001,)], torch.float32, cuda, 59) for _ in range(2))
+    a, b = optim.AdamW([p], lr=1e-3), optim.AdamW([q], lr=1e-3)
+    for _ in range(3):
+        a.step()
+    b.step()
+    for k in ("exp_avg", "exp_avg_sq", "step"):
+        b.state[q][k] = a.state[p][k].clone()
+    q.data.copy_(p.data)
+    a.step(), b.step()
+    assert torch.equal(p, q) and int(b.state[q]["step"]) == 4 and torch.equal(a.moments()[1], b.moments()[1])
+    torch.save(a.state_dict(), tmp_path / "a.pt")
+    sd = torch.load(tmp_path / "a.pt", weights_only=True)
+    assert type(a.state_dict()["state"][0]) is dict
+    b.load_state_dict(sd)
+    a.step(), b.step()
+    assert torch.equal(p, q)

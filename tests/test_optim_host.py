@@ -1,4 +1,6 @@
 """What optim refuses and checks without a GPU, and the entry points' checks of their arguments."""
+import copy
+import pickle
 from types import SimpleNamespace
 
 import pytest
@@ -147,3 +149,28 @@ def test_one_rate_for_groups_that_are_loaded_with_two(monkeypatch):
     sd["param_groups"][0]["lr"], sd["param_groups"][1]["lr"] = 0.25, torch.tensor(0.5)
     opt.load_state_dict(sd)
     assert opt.param_groups[0]["lr"] is lr and [float(g["lr"]) for g in opt.param_groups] == [0.25, 0.5]
+
+
+def test_what_is_put_into_an_entry():
+    """Tensors put in the place of an entry's own are copied into the buffers that the step reads."""
+    m, v, steps = torch.zeros(6), torch.zeros(6, dtype=torch.uint8), torch.zeros(3, dtype=torch.int32)
+    e = optim._Entry({"step": steps[0], "exp_avg": m.view(2, 3), "exp_avg_sq": v.view(2, 3)}, steps)
+    own = dict(e)
+    for k in list(e):
+        e[k] = e[k]                                           # as a loop that moves a state to a device does
+    e["exp_avg"] = torch.arange(6.0, dtype=torch.float64).view(2, 3)
+    e.update(step=torch.tensor(7.0), exp_avg_sq=torch.full((2, 3), 9, dtype=torch.uint8))
+    e |= {"exp_avg": e["exp_avg"] + 1}
+    assert m.tolist() == [1, 2, 3, 4, 5, 6] and steps.tolist() == [7] * 3 and v.tolist() == [9] * 6
+    assert all(e[k] is own[k] for k in own)
+    for k, t in (("exp_avg", torch.zeros(6)), ("exp_avg", torch.zeros(2, 3, dtype=torch.int32)),
+                 ("exp_avg_sq", torch.zeros(2, 3))):
+        with pytest.raises(ValueError, match=k):
+            e[k] = t
+    with pytest.raises(KeyError, match="max_exp_avg_sq"):
+        e["max_exp_avg_sq"] = m
+    for change in (lambda: e.pop("step"), lambda: e.clear(), lambda: e.__delitem__("step")):
+        with pytest.raises(TypeError, match="stay"):
+            change()
+    for plain in (copy.deepcopy(e), copy.copy(e), e.copy(), pickle.loads(pickle.dumps(e))):
+        assert type(plain) is dict and plain.keys() == own.keys() and torch.equal(plain["exp_avg"], e["exp_avg"])

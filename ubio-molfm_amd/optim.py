@@ -215,6 +215,47 @@ def _chunk_table(ptrs, offs, sizes):
     return t, first.tolist()
 
 
+class _Entry(dict):
+    """A parameter's state: views of the plan's buffers, and its step count in every chunk.  A tensor that is put in a
+    view's place is copied into it; copies and pickles are plain dicts."""
+
+    def __init__(self, views, steps):
+        super().__init__(views)
+        self.steps = steps
+
+    def __setitem__(self, k, t):
+        if k not in self:
+            raise KeyError(f"AdamW: the state has no {k}")
+        own = self[k]
+        if t is own:
+            return
+        t = torch.as_tensor(t).detach()
+        if k == "step":
+            t = t.clone().view(())
+            own.copy_(t)
+            self.steps.copy_(t)
+            return
+        if t.shape != own.shape or not (t.is_floating_point() if own.is_floating_point() else t.dtype == own.dtype):
+            raise ValueError(f"AdamW: {k} of {tuple(t.shape)} {t.dtype}, not {tuple(own.shape)} {own.dtype}")
+        own.copy_(t)
+
+    def update(self, *args, **kw):
+        for k, t in dict(*args, **kw).items():
+            self[k] = t
+
+    def __ior__(self, other):
+        self.update(other)
+        return self
+
+    def _stay(self, *args):
+        raise TypeError("AdamW: the tensors of a state stay; take the parameter's whole entry out")
+
+    __delitem__ = pop = popitem = clear = _stay
+
+    def __reduce__(self):
+        return dict, (dict(self),)
+
+
 class _Plan:
     """What stays from step to step: moments and step counts of all parameters, the chunks' table, the launches."""
 
@@ -302,7 +343,7 @@ class _Plan:
     def clear(self, params):
         """Zero states for some of the plan's parameters."""
         for p in params:
-            self.steps[self.first[p]:self.first[p] - (-p.numel() // _CHUNK)].zero_()
+            self.state[p].steps.zero_()
             for t in self.state[p].values():
                 t.zero_()
 
@@ -314,7 +355,7 @@ class _Plan:
             st[k] = t[o:o + n].view(p.shape)
             if s is not None:
                 st[k + "_scale"] = s[o // _RUN:o // _RUN + -(-n // _RUN)]
-        return st
+        return _Entry(st, self.steps[chunk:chunk - (-n // _CHUNK)])
 
 
 class AdamW(torch.optim.Optimizer):
@@ -342,9 +383,9 @@ class AdamW(torch.optim.Optimizer):
     is the loaded one); parameters that move and groups that are added void it.  As with any graph torch does not
     see that a replay changed the parameters: torch.autograd.graph.increment_version(parameters) says so to what is
     kept per weight version (the evaluation path's packed weights and tables).  ``state`` entries are views of flat
-    buffers: moments can be written in place, step counts through load_state_dict; an entry that is taken out starts
-    anew and one that is put in its place is taken over, both in the buffers that are there, by a step that is not
-    captured."""
+    buffers: moments can be written in place, and what is put in an entry's place or in that of one of its tensors (step
+    counts only so) is copied into the buffers that are there; an entry that is taken out starts anew.  Entries are looked
+    over by steps that are not captured."""
 
     _plan: Optional[_Plan] = None
     _OPTIONS = ("state_bits", "max_norm", "skip_nonfinite", "seed")
@@ -423,6 +464,12 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError(f"AdamW: {k} of {name} is {tuple(e[k].shape)} {e[k].dtype}, not {size} "
                                  f"{'in a floating type' if self.state_bits == 32 else torch.uint8}")
         return {k: e[k] for k in names}
+
+    def state_dict(self):
+        """As torch's; the entries refer to the state itself."""
+        sd = super().state_dict()
+        sd["state"] = {k: dict(e) if type(e) is _Entry else e for k, e in sd["state"].items()}
+        return sd
 
     def load_state_dict(self, state_dict):
         """As torch's, with moments kept in their own types: fp32, or codes and scale bytes.  Learning rates that are
