@@ -408,3 +408,16 @@ def test_run_seq_to_third_order(pkg, cuda, affine):
     assert len(got) == len(ref)
     for a, r in zip(got, ref):
         assert float((a.double() - r).norm() / r.norm()) < 64 * 60 * U
+
+
+def test_run_seq_with_hooks_for_all_modules(pkg, cuda):
+    from ubio_molfm_amd import second_order as so
+    net = torch.nn.Sequential(torch.nn.Linear(8, 24), torch.nn.LayerNorm(24)).to(cuda)
+    x = torch.randn(7, 8, device=cuda)
+    seen = []
+    handle = torch.nn.modules.module.register_module_forward_hook(
+        lambda m, i, o: (seen.append(type(m)), 2 * o)[1] if isinstance(m, torch.nn.LayerNorm) else None)
+    try:
+        assert torch.equal(so.run_seq(net, x), net(x)) and seen == [torch.nn.LayerNorm] * 2
+    finally:
+        handle.remove()

@@ -83,3 +83,38 @@ def test_value_aggregation_of_other_types_and_sizes(monkeypatch, dtype, rows, ch
                        for k in range(3)])
     # up to 30 terms of three factors, each product and sum rounded once in the type
     assert _rel(got.double(), ref) < 40 * torch.finfo(dtype).eps
+
+
+def test_modules_that_do_more_are_told():
+    """second_order._bare: hooks of a module's own and those for all modules, subclasses, a forward of its own."""
+    class Scaled(torch.nn.LayerNorm):
+        pass
+
+    def ln():
+        return torch.nn.LayerNorm(8)
+
+    def hooked(name, *args):
+        m = ln()
+        getattr(m, name)(*args)
+        return m
+
+    def nothing(*_):
+        pass
+
+    assert so._bare(ln(), torch.nn.LayerNorm) and not so._bare(ln(), torch.nn.SiLU)
+    own = ln()
+    own.forward = lambda x: x
+    parametrized = torch.nn.utils.parametrize.register_parametrization(ln(), "weight", torch.nn.Identity())
+    for m in (Scaled(8), own, parametrized, hooked("register_forward_hook", nothing),
+              hooked("register_forward_pre_hook", nothing), hooked("register_full_backward_hook", nothing),
+              hooked("register_full_backward_pre_hook", nothing)):
+        assert not so._bare(m, torch.nn.LayerNorm)
+    for register in (torch.nn.modules.module.register_module_forward_hook,
+                     torch.nn.modules.module.register_module_forward_pre_hook,
+                     torch.nn.modules.module.register_module_full_backward_hook):
+        handle = register(nothing)
+        try:
+            assert not so._bare(ln(), torch.nn.LayerNorm)
+        finally:
+            handle.remove()
+    assert so._bare(ln(), torch.nn.LayerNorm)

@@ -229,17 +229,23 @@ def ln_silu(ln: nn.LayerNorm, x: torch.Tensor) -> torch.Tensor:
 _PLAIN = {torch.Tensor, nn.Parameter, type(None)}
 
 
+def _bare(module: nn.Module, kind: type) -> bool:
+    """Whether calling the module is kind's forward pass and no more: a subclass, a hook of its own or one for all
+    modules, or a forward set on the module may do more."""
+    return (type(module) is kind and "forward" not in module.__dict__ and not nn.modules.module._has_any_global_hook()
+            and not (module._forward_hooks or module._forward_pre_hooks or module._backward_hooks
+                     or module._backward_pre_hooks))
+
+
 def _layer_norm_takes(ln: nn.LayerNorm, x: torch.Tensor) -> bool:
-    """Whether norms.layer_norm computes ln(x): fp32 rows on the GPU, normalised over their last dimension, by a module
-    that does no more (a subclass or a hook may), outside of what only torch's own operators go through: forward mode,
-    torch.func's transforms, tracing and tensor subclasses."""
-    if (torch._C._are_functorch_transforms_active() or torch.jit.is_tracing()
-            or not {type(x), type(ln.weight), type(ln.bias)} <= _PLAIN or has_tangent(x, ln.weight, ln.bias)):
+    """Whether norms.layer_norm computes ln(x): fp32 rows on the GPU, normalised over their last dimension, outside of
+    what only torch's own operators go through (forward mode, torch.func's transforms, tracing, tensor subclasses)."""
+    if (not _bare(ln, nn.LayerNorm) or not {type(x), type(ln.weight), type(ln.bias)} <= _PLAIN
+            or torch._C._are_functorch_transforms_active() or torch.jit.is_tracing()
+            or has_tangent(x, ln.weight, ln.bias)):
         return False
     w = x.shape[-1]
-    return (type(ln) is nn.LayerNorm and not (ln._forward_hooks or ln._forward_pre_hooks or ln._backward_hooks
-                                              or ln._backward_pre_hooks)
-            and x.is_cuda and x.dtype == torch.float32 and tuple(ln.normalized_shape) == (w,) and 1 <= w <= _LN_MAX_WIDTH
+    return (x.is_cuda and x.dtype == torch.float32 and tuple(ln.normalized_shape) == (w,) and 1 <= w <= _LN_MAX_WIDTH
             and all(p is None or (p.is_cuda and p.dtype == torch.float32) for p in (ln.weight, ln.bias)))
 
 
