@@ -421,3 +421,26 @@ def test_run_seq_with_hooks_for_all_modules(pkg, cuda):
         assert torch.equal(so.run_seq(net, x), net(x)) and seen == [torch.nn.LayerNorm] * 2
     finally:
         handle.remove()
+
+
+@pytest.mark.parametrize("which", ["norm hook", "silu hook", "norm subclass", "linear hook", "none"])
+def test_run_seq_with_hooks_behind_fused_pairs(pkg, cuda, which):
+    """Widths and rows that the fused LayerNorm + SiLU and the Linear over edges take: hooks and subclasses still run."""
+    from ubio_molfm_amd import second_order as so
+
+    class Scaled(torch.nn.LayerNorm):
+        def forward(self, x):
+            return 3 * super().forward(x)
+
+    torch.manual_seed(4)
+    net = torch.nn.Sequential(torch.nn.Linear(8, 128), (Scaled if which == "norm subclass" else torch.nn.LayerNorm)(128),
+                              torch.nn.SiLU()).to(cuda)
+    seen = []
+    k = {"linear hook": 0, "norm hook": 1, "silu hook": 2}.get(which)
+    if k is not None:
+        net[k].register_forward_hook(lambda m, i, o: (seen.append(k), o + 1)[1])
+    x = torch.randn(so._EDGE_ROWS, 8, device=cuda)
+    with torch.no_grad():
+        got, ref = so.run_seq(net, x), net.double()(x.double())
+    # a Linear of 8 products, a norm of 128 elements and a SiLU: below 200 u of values below 30
+    assert (got.double() - ref).abs().max() < 200 * U * 30 and len(seen) == (0 if k is None else 2)

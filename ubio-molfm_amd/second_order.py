@@ -252,18 +252,19 @@ def _layer_norm_takes(ln: nn.LayerNorm, x: torch.Tensor) -> bool:
 def run_seq(mods, h: torch.Tensor) -> torch.Tensor:
     """nn.Sequential over mods with each nn.LayerNorm + nn.SiLU pair as ln_silu (where
     ln_silu_fusable), every other nn.LayerNorm on GPU rows as norms.layer_norm and
-    each nn.Linear on at least _EDGE_ROWS rows as edge_linear."""
+    each nn.Linear on at least _EDGE_ROWS rows as edge_linear; modules that do more
+    than their kind's forward pass (_bare) run as they are."""
     mods = list(mods) if isinstance(mods, (nn.Sequential, list, tuple)) else [mods]
     i = 0
     while i < len(mods):
-        if (isinstance(mods[i], nn.LayerNorm) and i + 1 < len(mods) and isinstance(mods[i + 1], nn.SiLU)
+        if (i + 1 < len(mods) and _bare(mods[i], nn.LayerNorm) and _bare(mods[i + 1], nn.SiLU)
                 and ln_silu_fusable(mods[i], h)):
             h = ln_silu(mods[i], h)
             i += 2
         elif isinstance(mods[i], nn.LayerNorm) and _layer_norm_takes(mods[i], h):
             h = _layer_norm(h, mods[i].weight, mods[i].bias, mods[i].eps, any_order=True)
             i += 1
-        elif isinstance(mods[i], nn.Linear) and h.dim() == 2 and h.shape[0] >= _EDGE_ROWS:
+        elif _bare(mods[i], nn.Linear) and h.dim() == 2 and h.shape[0] >= _EDGE_ROWS:
             h = edge_linear(mods[i], h)
             i += 1
         else:
