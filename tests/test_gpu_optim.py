@@ -891,3 +891,32 @@ def test_tensors_put_into_entries(pkg, cuda, tmp_path):
     b.load_state_dict(sd)
     a.step(), b.step()
     assert torch.equal(p, q)
+
+
+@pytest.mark.parametrize("dtype", [torch.float64, torch.bfloat16, torch.int64])
+def test_a_rate_on_the_gpu_in_another_type(pkg, cuda, dtype):
+    """It is taken to fp32 there: a step reads nothing back, and a captured one follows the tensor."""
+    from ubio_molfm_amd import optim
+    (p,), (q,) = (_params([(5000,)], torch.float32, cuda, 60) for _ in range(2))
+    lr = torch.tensor(1 if dtype == torch.int64 else 0.0625 if dtype == torch.bfloat16 else 1e-3, dtype=dtype, device=cuda)
+    a, b = optim.AdamW([p], lr=lr), optim.AdamW([q], lr=lr.item())
+    a.step(), b.step()
+    torch.cuda.synchronize()
+    mode = torch.cuda.get_sync_debug_mode()
+    torch.cuda.set_sync_debug_mode("error")
+    try:
+        a.step()
+    finally:
+        torch.cuda.set_sync_debug_mode(mode)
+    b.step()
+    assert torch.equal(p, q)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        a.step()
+    for rate in (2.0, 4.0, 1.0):
+        lr.fill_(rate)
+        b.param_groups[0]["lr"] = rate
+        graph.replay()
+        torch.cuda.synchronize()
+        b.step()
+        assert torch.equal(p, q)

@@ -365,8 +365,8 @@ class AdamW(torch.optim.Optimizer):
         p = p (1 - lr weight_decay) - lr / (1 - b1^t) m / (sqrt(v / (1 - b2^t)) + eps)
 
     params: contiguous fp32, bf16 or fp16 parameters on one GPU (others only without a gradient), or groups of them
-    with their own lr, betas, eps and weight_decay (lr may be a tensor of one fp32 element on that GPU, read by the
-    step itself).  Parameters without a gradient are left out of a step, as in torch.  Arithmetic and 32-bit moments
+    with their own lr, betas, eps and weight_decay (lr may be a tensor of one element on that GPU, read by the step
+    itself).  Parameters without a gradient are left out of a step, as in torch.  Arithmetic and 32-bit moments
     are fp32 whatever the parameters' type, which are rounded to nearest once a step.
 
     state_bits=8 keeps both moments in 8 bits (runs of 32 elements share a power-of-two scale; 3 mantissa bits, rounded
@@ -601,7 +601,9 @@ class AdamW(torch.optim.Optimizer):
             a, g = l.args, self.param_groups[l.group]
             a.grads = l.grads.address()
             lr = g["lr"]
-            if isinstance(lr, torch.Tensor) and lr.device == plan.device and lr.dtype == torch.float32:
+            if isinstance(lr, torch.Tensor) and lr.is_cuda:
+                lr = lr.to(plan.device, torch.float32)     # itself, or on the GPU: nothing is read back
+                keep.append(lr)
                 a.lr_dev, a.lr = lr.data_ptr(), 0.0
             else:
                 a.lr_dev, a.lr = None, float(lr)
