@@ -920,3 +920,27 @@ def test_a_rate_on_the_gpu_in_another_type(pkg, cuda, dtype):
         torch.cuda.synchronize()
         b.step()
         assert torch.equal(p, q)
+
+
+def test_step_counts_are_loaded_together(pkg, cuda, monkeypatch):
+    """Step counts of a checkpoint in host memory (tensors, numbers, torch's floating ones) go to the GPU in one copy,
+    into every chunk of their tensors."""
+    from ubio_molfm_amd import optim
+    ps = _params([(k % 5 * 3000 + k % 2,) for k in range(200)], torch.float32, cuda, 61)
+    opt = optim.AdamW(ps)
+    opt.step()
+    sd = copy.deepcopy(opt.state_dict())
+    for k, e in sd["state"].items():
+        e["step"] = (torch.tensor(float(k)), k, torch.tensor([k], dtype=torch.int64))[k % 3]
+    copies = []
+    real = torch.Tensor.to
+    monkeypatch.setattr(torch.Tensor, "to", lambda t, *a, **k: (copies.append(t.is_cuda), real(t, *a, **k))[1])
+    opt.load_state_dict(sd)
+    monkeypatch.undo()
+    assert copies.count(False) <= 3, len(copies)
+    for k, p in enumerate(ps):
+        st = opt.state[p]
+        assert int(st["step"]) == k and (st.steps == k).all() and st.steps.numel() == -(-p.numel() // 4096)
+    sd["state"][3]["step"] = torch.tensor(50, device=cuda)               # some of them on the GPU
+    opt.load_state_dict(sd)
+    assert int(opt.state[ps[3]]["step"]) == 50 and int(opt.state[ps[4]]["step"]) == 4

@@ -330,10 +330,17 @@ class _Plan:
         if not entries:
             return
         dev = self.device
-        steps = torch.stack([torch.as_tensor(e["step"]).to(dev, torch.int32).view(()) for e in entries.values()])
-        where = [torch.arange(self.first[p], self.first[p] - (-p.numel() // _CHUNK)) for p in entries]
-        counts = torch.tensor([len(w) for w in where], device=dev)
-        self.steps[torch.cat(where).to(dev)] = steps.repeat_interleave(counts)
+        steps = [torch.as_tensor(e["step"]) for e in entries.values()]
+        if any(t.is_cuda for t in steps):
+            steps = torch.stack([t.to(dev, torch.int32).view(()) for t in steps])
+        else:
+            steps = torch.tensor([int(t) for t in steps], dtype=torch.int32).to(dev)      # one copy for all
+        counts = np.array([-(-p.numel() // _CHUNK) for p in entries])
+        ends = np.cumsum(counts)
+        where = np.arange(ends[-1]) + np.repeat(np.array([self.first[p] for p in entries]) - (ends - counts), counts)
+        which = np.repeat(np.arange(len(entries)), counts)
+        where, which = torch.from_numpy(np.stack([where, which])).to(dev)
+        self.steps[where] = steps[which]
         for p, step in zip(entries, steps):
             if not p.numel():
                 self.state[p]["step"].copy_(step)
