@@ -944,3 +944,29 @@ def test_step_counts_are_loaded_together(pkg, cuda, monkeypatch):
     sd["state"][3]["step"] = torch.tensor(50, device=cuda)               # some of them on the GPU
     opt.load_state_dict(sd)
     assert int(opt.state[ps[3]]["step"]) == 50 and int(opt.state[ps[4]]["step"]) == 4
+
+
+def test_clipping_of_gradients_that_share_memory(pkg, cuda):
+    """Their elements would be scaled by two workgroups at once, or twice: refused, and left as they were."""
+    from ubio_molfm_amd import optim
+    flat = torch.ones(10000, device=cuda)
+
+    def params(*grads):
+        out = []
+        for g in grads:
+            p = torch.zeros(g.shape, dtype=g.dtype, device=cuda, requires_grad=True)
+            p.grad = g
+            out.append(p)
+        return out
+
+    turned = params(flat.view(100, 100).t())[0]
+    row = params(flat[:50].expand(30, 50))[0]
+    for ps, match in ((params(flat[:6000], flat[5000:]), "share"), (params(flat, flat[3:4]), "share"),
+                      (params(flat[:100], flat[40:100].view(torch.float16)), "share"), ([turned, turned], "twice"),
+                      ([row], "share"), (params(flat[:50], flat[60:90].expand(3, 30)), "share")):
+        with pytest.raises(ValueError, match=match):
+            optim.clip_grad_norm_(ps, 0.1)
+        assert (flat == 1).all()
+    one = params(torch.ones(1, 30, 50, device=cuda).as_strided((1, 30, 50), (0, 1, 30)))
+    optim.clip_grad_norm_(params(flat[:100], flat[100:100], flat[100:]) + one, 1.0)
+    assert torch.allclose(flat, torch.full_like(flat, 1 / math.sqrt(11500))) and (one[0].grad < 0.01).all()

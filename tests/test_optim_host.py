@@ -174,3 +174,18 @@ def test_what_is_put_into_an_entry():
             change()
     for plain in (copy.deepcopy(e), copy.copy(e), e.copy(), pickle.loads(pickle.dumps(e))):
         assert type(plain) is dict and plain.keys() == own.keys() and torch.equal(plain["exp_avg"], e["exp_avg"])
+
+
+def test_memory_that_tensors_share():
+    buf = torch.zeros(100)
+
+    def overlap(*ts):
+        return optim._overlap(optim._by_type(ts, {t.dtype for t in ts}))
+
+    assert torch.zeros(0).data_ptr() == buf[50:50].data_ptr() == 0      # those without elements lie nowhere
+    assert not overlap(buf[60:], buf[:50], buf[50:60], buf[50:50], torch.zeros(0), buf.new_zeros(5))
+    assert not overlap(buf) and not overlap(torch.zeros(0), torch.zeros(0))
+    for ts in ((buf, buf), (buf[:51], buf[50:]), (buf, buf[7:8]), (buf[50:], torch.zeros(9), buf[:99]),
+               (buf, buf[40:].view(torch.bfloat16)[3:5])):
+        assert overlap(*ts) and overlap(*ts[::-1])
+    assert not overlap(buf[:50], buf[50:].view(torch.float16))

@@ -32,7 +32,7 @@ class _Lists:
     """Dense tensors of one type as the library takes them: their addresses (0: left out) and sizes."""
 
     def __init__(self, dtype, ptrs, numels):
-        self.type = _lib.i32(_TYPES[dtype])
+        self.type, self.itemsize = _lib.i32(_TYPES[dtype]), dtype.itemsize
         self.numel = array("q", numels)
         self.n = _lib.i32(len(self.numel))
         self.set(ptrs)
@@ -100,6 +100,15 @@ def _norm_parts(lists, dev, st):
     return parts, count
 
 
+def _overlap(lists) -> bool:
+    """Whether tensors of the lists share memory."""
+    at = np.concatenate([np.frombuffer(l.ptrs, np.uint64) for l in lists])
+    size = np.concatenate([np.frombuffer(l.numel, np.int64) * l.itemsize for l in lists]).astype(np.uint64)
+    order = np.argsort(at)
+    at, end = at[order], (at + size)[order]
+    return bool((end[:-1] > at[1:]).any())
+
+
 def _on(dev):
     """A context with dev as the current device."""
     return nullcontext() if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
@@ -123,7 +132,8 @@ def grad_norm(tensors: Iterable[torch.Tensor]) -> torch.Tensor:
 
 def clip_grad_norm_(parameters, max_norm: float) -> torch.Tensor:
     """Scales the parameters' gradients in place by min(1, max_norm / (norm + 1e-6)), norm their global 2-norm, which
-    is returned (an fp32 tensor of one element), as torch.nn.utils.clip_grad_norm_.  A norm that is not finite scales
+    is returned (an fp32 tensor of one element), as torch.nn.utils.clip_grad_norm_.  Gradients that share memory are
+    refused.  A norm that is not finite scales
     by what the quotient gives (0, or NaN); nothing is read back to the host."""
     max_norm = float(max_norm)
     if not max_norm >= 0:
@@ -134,9 +144,13 @@ def clip_grad_norm_(parameters, max_norm: float) -> torch.Tensor:
         return torch.zeros((), device="cuda" if torch.cuda.is_available() else None)
     dev, types, dense = _check(grads, "clip_grad_norm_")
     lists = _by_type(dense, types)
-    ptrs = [p for l in lists for p in l.ptrs if p]
-    if len(set(ptrs)) < len(ptrs):
-        raise ValueError("clip_grad_norm_: the same gradient twice")
+    if _overlap(lists):
+        raise ValueError("clip_grad_norm_: the same gradient twice, or gradients that share memory")
+    if dense is not grads:
+        if len(set(map(id, grads))) < len(grads):
+            raise ValueError("clip_grad_norm_: the same gradient twice")
+        if any(step == 0 and n > 1 for g in grads for step, n in zip(g.stride(), g.shape)):
+            raise ValueError("clip_grad_norm_: a gradient whose elements share memory")
     out = torch.zeros((), dtype=torch.float32, device=dev)
     with _on(dev):
         st = _lib.stream(dev)
