@@ -970,3 +970,22 @@ def test_clipping_of_gradients_that_share_memory(pkg, cuda):
     one = params(torch.ones(1, 30, 50, device=cuda).as_strided((1, 30, 50), (0, 1, 30)))
     optim.clip_grad_norm_(params(flat[:100], flat[100:100], flat[100:]) + one, 1.0)
     assert torch.allclose(flat, torch.full_like(flat, 1 / math.sqrt(11500))) and (one[0].grad < 0.01).all()
+
+
+def test_clipping_gradients_with_a_history(pkg, cuda):
+    """Gradients of a backward pass with create_graph: scaled as without, outside of their history."""
+    from ubio_molfm_amd import optim
+    x = torch.randn(40, 30, device=cuda)
+    ps = [torch.nn.Parameter(torch.randn(30, 40, device=cuda)) for _ in range(2)]
+    ((ps[0] @ x).square().sum() + (ps[1].t() @ x.t()).pow(3).sum()).backward(create_graph=True)
+    ps[1].grad = ps[1].grad.t().contiguous().t()
+    want = [p.grad.detach().double().clone() for p in ps]
+    norm = math.sqrt(sum(float(g.square().sum()) for g in want))
+    own = [ps[0].grad, ps[1].grad._base]                                 # the second is a view
+    fns = [g.grad_fn for g in own]
+    assert all(fns) and not ps[1].grad.is_contiguous()
+    assert abs(float(optim.clip_grad_norm_(ps, 0.5)) - norm) <= 2 * U * norm
+    assert all(g.grad_fn is fn for g, fn in zip(own, fns))
+    for p, g in zip(ps, want):
+        c = 0.5 / (norm + 1e-6)
+        assert (p.grad.double() - c * g).abs().le(4 * U * (c * g).abs()).all()

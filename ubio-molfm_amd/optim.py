@@ -130,6 +130,7 @@ def grad_norm(tensors: Iterable[torch.Tensor]) -> torch.Tensor:
     return out
 
 
+@torch.no_grad()
 def clip_grad_norm_(parameters, max_norm: float) -> torch.Tensor:
     """Scales the parameters' gradients in place by min(1, max_norm / (norm + 1e-6)), norm their global 2-norm, which
     is returned (an fp32 tensor of one element), as torch.nn.utils.clip_grad_norm_.  Gradients that share memory are
