@@ -989,3 +989,19 @@ def test_clipping_gradients_with_a_history(pkg, cuda):
     for p, g in zip(ps, want):
         c = 0.5 / (norm + 1e-6)
         assert (p.grad.double() - c * g).abs().le(4 * U * (c * g).abs()).all()
+
+
+@pytest.mark.parametrize("before,after", [(torch.float32, torch.bfloat16), (torch.float16, torch.bfloat16)])
+def test_parameters_that_take_another_type_in_place(pkg, cuda, before, after):
+    """.data of another type at the same address with as many elements: updated as what it is now."""
+    from ubio_molfm_amd import optim
+    p, q = (torch.ones(5000, dtype=t, device=cuda, requires_grad=True) for t in (before, after))
+    p.grad, q.grad = torch.ones_like(p), torch.ones_like(q)
+    opt, ref = optim.AdamW([p], lr=1e-2), optim.AdamW([q], lr=1e-2)
+    opt.step()
+    p.grad = None
+    p.data = p.data.view(after)[:5000].fill_(1.0)
+    p.grad = torch.ones(5000, dtype=after, device=cuda)
+    opt.state[p] = {"step": 0, "exp_avg": torch.zeros(5000), "exp_avg_sq": torch.zeros(5000)}
+    opt.step(), ref.step()
+    assert torch.equal(p, q) and (p < 1).all()

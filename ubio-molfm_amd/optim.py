@@ -292,10 +292,11 @@ class _Plan:
             raise RuntimeError("AdamW: the first step, and the one after a change of parameters or groups, cannot be "
                                "captured: take it before the capture")
         self.device = dev = params[0].device if params else torch.device("cuda", torch.cuda.current_device())
-        self.ptrs = [p.data_ptr() for p in params]
+        self.ptrs, self.nbytes = [p.data_ptr() for p in params], [p.nbytes for p in params]
+        self.types = None if all(p.dtype == torch.float32 for p in params) else [p.dtype for p in params]
         self.params = params
         bits = opt.state_bits
-        self.sizes = sizes = [p.numel() for p in params]
+        sizes = [p.numel() for p in params]
         ends = np.cumsum([0] + [-(-n // _ALIGN) * _ALIGN for n in sizes]).tolist()
         self.total = ends[-1]
         place = dict(zip(params, ends))
@@ -555,10 +556,12 @@ class AdamW(torch.optim.Optimizer):
         return list(map(len, groups)) == plan.split and all(map(is_, chain.from_iterable(groups), plan.every))
 
     def _valid(self) -> bool:
-        """Whether the plan holds for a step: the same groups, and no parameter was moved, cut or turned."""
+        """Whether the plan holds for a step: the same groups, and no parameter was moved, cut, turned or given another
+        type (bytes tell fp32 from those of 16 bits)."""
         plan = self._plan
         return (self._same_groups() and list(map(torch.Tensor.data_ptr, plan.params)) == plan.ptrs
-                and list(map(torch.Tensor.numel, plan.params)) == plan.sizes
+                and list(map(_NBYTES, plan.params)) == plan.nbytes
+                and (plan.types is None or [p.dtype for p in plan.params] == plan.types)
                 and all(map(torch.Tensor.is_contiguous, plan.params)) and not any(map(_usable, plan.outside)))
 
     def _with_entries(self, plan: _Plan) -> _Plan:
