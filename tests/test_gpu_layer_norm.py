@@ -444,3 +444,47 @@ def test_run_seq_with_hooks_behind_fused_pairs(pkg, cuda, which):
         got, ref = so.run_seq(net, x), net.double()(x.double())
     # a Linear of 8 products, a norm of 128 elements and a SiLU: below 200 u of values below 30
     assert (got.double() - ref).abs().max() < 200 * U * 30 and len(seen) == (0 if k is None else 2)
+
+
+@pytest.mark.parametrize("w", [3, 24, 100, 129, 500, 1000, 1500, 5001, 8193, 16383])
+def test_rows_of_one_value(pkg, cuda, w):
+    """They give the bias, whatever the value: a mean off by its sum's rounding (at most 48 u: 32 additions in a lane, 16
+    across) is found again with the same relative error, and 48^2 u^2 |x| r |g| is left, r = eps^(-1/2).  Rows between
+    them that are not constant, or not in the same way, come out as alone."""
+    from ubio_molfm_amd import norms
+    values = torch.tensor([0.1, 1000.1, -37.77, 30000.3, 1e-6, 7.0, -0.3], device=cuda)
+    x, gy, wt, b = _inputs(40, w, torch.float32, torch.float32, w, cuda)
+    plain = norms.layer_norm(x, wt, b, EPS)
+    mixed = x.clone()
+    mixed[3:38:5] = values[:, None]
+    X = mixed.requires_grad_(True)
+    y = norms.layer_norm(X, wt, b, EPS)
+    rest = torch.ones(40, dtype=torch.bool, device=cuda)
+    rest[3:38:5] = False
+    assert torch.equal(y[rest], plain[rest])
+    r = EPS ** -0.5
+    left = 48 ** 2 * U * U * values.abs().double()[:, None] * r
+    assert (y[~rest].double() - b.double()).abs().le(left * wt.abs() + U * b.abs()).all()
+    gx, = torch.autograd.grad(y, X, gy)
+    u = gy[~rest].double() * wt.double()
+    ref = r * (u - u.mean(-1, keepdim=True))
+    size = u.abs() + u.abs().mean(-1, keepdim=True)
+    # the mean is stored in fp32, off by u |x|: xh <u xh> beside it
+    xh = left + U * values.abs().double()[:, None] * r
+    assert (gx[~rest].double() - ref).abs().le(64 * U * r * size + r * xh * xh * size + U * ref.abs()).all()
+
+
+def test_rows_far_narrower_than_their_mean(pkg, cuda):
+    """A spread of 2^-12 to 2^-6 of the mean on both sides of where the mean is corrected: where it is, y is off by what
+    the rounding of x - mean leaves (4 u of the mean, 64 u of the rest), elsewhere by the mean's 48 u."""
+    from ubio_molfm_amd import norms
+    g = torch.Generator().manual_seed(6)
+    for w in (24, 129, 1000, 5001):
+        for e in range(6, 13):
+            x = (100 + 100 * 2.0 ** -e * torch.randn(50, w, generator=g)).to(cuda)
+            y = norms.layer_norm(x, eps=1e-12).double()
+            X = x.double()
+            z = X - X.mean(-1, keepdim=True)
+            ref = z / ((z * z).mean(-1, keepdim=True) + 1e-12).sqrt()
+            bound = (4 if e > 8 else 48) * U * 2.0 ** e * 1.5 + 64 * U * (ref.abs() + 1)
+            assert (y - ref).abs().le(bound).all(), (w, e, float((y - ref).abs().max()))

@@ -282,22 +282,38 @@ __global__ __launch_bounds__(kL > 64 ? kL : 256) void k_layer_norm_fwd(LnArgs P)
   int turn = 0;
   for (int64_t row = (int64_t)blockIdx.x * kR + rg; row < P.n; row += (int64_t)gridDim.x * kR) {
     const T* xr = static_cast<const T*>(P.x) + row * P.ldx;
-    float x[E], s[1] = {0.f}, q[1] = {0.f};
+    float x[E], s[1] = {0.f}, q[1];
     RowLoad<T, V, kL, NV> rx;
     rx.load(xr, l, w);
     rx.get(l, w, x);
 #pragma unroll
     for (int e = 0; e < E; ++e) s[0] += x[e];
     group_sum<kL, 1>(s, red, turn);
-    const float mean = s[0] / (float)w;       // a true quotient: exact for a row of one short value
-    each_vec<V, kL, NV>(l, w, [&](int k, int c, auto whole) {
+    float mean = s[0] / (float)w;             // a true quotient: exact for a row of one short value
+    auto centre = [&](float by) {
+      q[0] = 0.f;
+      each_vec<V, kL, NV>(l, w, [&](int k, int c, auto whole) {
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        x[k * V + e] = whole || c + e < w ? x[k * V + e] - mean : 0.f;
-        q[0] = fmaf(x[k * V + e], x[k * V + e], q[0]);
-      }
-    });
-    group_sum<kL, 1>(q, red, turn);
+        for (int e = 0; e < V; ++e) {
+          x[k * V + e] = whole || c + e < w ? x[k * V + e] - by : 0.f;
+          q[0] = fmaf(x[k * V + e], x[k * V + e], q[0]);
+        }
+      });
+      group_sum<kL, 1>(q, red, turn);
+    };
+    centre(mean);
+    // Rows far narrower than their mean: what the sum's rounding left in it is taken off too.  It counts beside their
+    // spread and beside eps: a row of 129 times 1000.1 came out 0.02 from the bias.  (The same for every row costs 7%
+    // at 32,768 x 2048 bf16.)  All lanes of a row, and so all wavefronts of a wide one, take one branch.
+    if (q[0] * inv < 0x1p-16f * mean * mean) {
+      s[0] = 0.f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) s[0] += x[e];
+      group_sum<kL, 1>(s, red, turn);
+      const float left = s[0] * inv;
+      centre(left);
+      mean += left;
+    }
     const float rstd = 1.0f / sqrtf(q[0] * inv + P.eps);
     T* yr = static_cast<T*>(P.y) + row * w;
     each_vec<V, kL, NV>(l, w, [&](int k, int c, auto whole) {
