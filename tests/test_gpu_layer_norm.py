@@ -488,3 +488,57 @@ def test_rows_far_narrower_than_their_mean(pkg, cuda):
             ref = z / ((z * z).mean(-1, keepdim=True) + 1e-12).sqrt()
             bound = (4 if e > 8 else 48) * U * 2.0 ** e * 1.5 + 64 * U * (ref.abs() + 1)
             assert (y - ref).abs().le(bound).all(), (w, e, float((y - ref).abs().max()))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("w", [5, 31, 128, 129, 700, 2049])
+def test_rows_off_16_byte_boundaries(pkg, cuda, dtype, w):
+    """Every start and stride of rows, and of upstream gradients, runs the code of contiguous ones: bitwise its results
+    to second order."""
+    from ubio_molfm_amd import norms
+    x, gy, wt, b = _inputs(37, w, dtype, torch.float32, 3 * w, cuda)
+    q = gy.roll(1, 0)
+
+    def run(x, gy, q):
+        X, G, W = (t.detach().requires_grad_(True) for t in (x, gy, wt))
+        y = norms.layer_norm(X, W, b, EPS)
+        gx, gg = torch.autograd.grad(y, (X, W), G, create_graph=True)
+        return [y, gx, gg, *torch.autograd.grad(gx, (X, G, W), q)]
+
+    def placed(t, shift, extra):
+        buf = torch.full((t.shape[0], w + extra), float("nan"), dtype=dtype, device=cuda).view(-1)
+        out = torch.cat([buf, buf[:16]])[shift:shift + buf.numel()].view(t.shape[0], -1)[:, :w]
+        return out.copy_(t)
+
+    ref = run(x, gy, q)
+    for shift in range(1, 8):
+        got = run(placed(x, shift, 3), placed(gy, 8 - shift, 5), placed(q, shift, 8))
+        assert all(torch.equal(a, r) for a, r in zip(got, ref)), shift
+
+
+@pytest.mark.parametrize("w,dtype", [(w, torch.float32) for w in (2, 3, 7, 15, 31, 37, 61, 85, 125, 189, 253, 300, 500,
+                                                                  700, 1001, 1500, 3001, 4001, 6001, 12001)]
+                         + [(w, torch.bfloat16) for w in (3, 5, 13, 27, 61, 93, 125, 189, 253, 381, 509, 765, 1021,
+                                                          1501, 2049, 5001, 8001, 12001)]
+                         + [(w, torch.float16) for w in (61, 765, 5001)])
+def test_second_order_of_every_shape(pkg, cuda, w, dtype):
+    """Each number of lanes and vectors that a row can lie in, the last vector in part; as test_second_order, with its
+    bound."""
+    from ubio_molfm_amd import norms
+    n = 23
+    x, gy, wt, b = _inputs(n, w, dtype, dtype, 11 * w, cuda)
+    g = torch.Generator().manual_seed(w)
+    R = [torch.randn(*s, generator=g).to(dtype).to(cuda) for s in ((n, w), (w,), (w,))]
+
+    def run(f, cast):
+        X, G, W, B = (cast(t).detach().requires_grad_(True) for t in (x, gy, wt, b))
+        first = torch.autograd.grad(f(X, W, B), (X, W, B), G, create_graph=True)
+        return [*first, *torch.autograd.grad(first, (X, W, G), [cast(r) for r in R])]
+
+    got = run(lambda X, W, B: norms.layer_norm(X, W, B, EPS), lambda t: t)
+    ref = run(_ref, lambda t: t.double())
+    for name, a, r in zip(["gx", "dg", "db", "d2x", "d2g", "d2gy"], got, ref):
+        if w == 2 and name in ("gx", "d2x"):
+            continue                # two elements: x - <x> is +-d, gx all but cancels; the others see the same sums
+        rel = float(((a.double() - r).norm() / r.norm()).detach())
+        assert rel < 2e-5 + (0 if dtype == torch.float32 else 2 * UT[dtype]), (name, rel)
