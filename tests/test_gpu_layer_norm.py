@@ -542,3 +542,34 @@ def test_second_order_of_every_shape(pkg, cuda, w, dtype):
             continue                # two elements: x - <x> is +-d, gx all but cancels; the others see the same sums
         rel = float(((a.double() - r).norm() / r.norm()).detach())
         assert rel < 2e-5 + (0 if dtype == torch.float32 else 2 * UT[dtype]), (name, rel)
+
+
+def test_run_seq_with_batched_gradients(pkg, cuda):
+    """Jacobians in one call (is_grads_batched), of the sequence and of its gradient, and upstream gradients with
+    forward-mode tangents: as through the modules."""
+    import copy
+    from torch.autograd import forward_ad
+    from ubio_molfm_amd import norms, second_order as so
+    torch.manual_seed(6)
+    net = torch.nn.Sequential(torch.nn.Linear(6, 24), torch.nn.LayerNorm(24), torch.nn.Linear(24, 3)).to(cuda)
+    ref = copy.deepcopy(net).double()
+    x, t = torch.randn(5, 6, device=cuda), torch.randn(5, 3, device=cuda)
+
+    def jacobians(f, x):
+        first = torch.autograd.functional.jacobian(f, x, vectorize=True)
+        x = x.clone().requires_grad_(True)
+        g, = torch.autograd.grad((f(x) ** 2).sum(), x, create_graph=True)
+        second, = torch.autograd.grad(g, x, torch.eye(x.numel(), device=cuda, dtype=x.dtype).view(-1, *x.shape),
+                                      is_grads_batched=True)
+        x = x.detach().requires_grad_(True)
+        y = f(x)
+        with forward_ad.dual_level():
+            up = forward_ad.make_dual(torch.ones_like(y), t.to(y.dtype))
+            return first, second, forward_ad.unpack_dual(torch.autograd.grad(y, x, up)[0]).tangent
+
+    for a, r in zip(jacobians(lambda v: so.run_seq(net, v), x), jacobians(ref, x.double())):
+        assert float((a.double() - r).norm() / r.norm()) < 1e-4       # as test_run_seq_uses_it
+    X = x.clone().requires_grad_(True)
+    y = norms.layer_norm(X)
+    with pytest.raises(RuntimeError, match="batched"):
+        torch.autograd.grad(y, X, torch.ones(2, 5, 6, device=cuda), is_grads_batched=True)

@@ -140,3 +140,66 @@ def test_the_composed_second_order(affine, asked):
     if asked != "b":
         assert torch.autograd.gradcheck(lambda *t: [y for y in second(*t) if y is not None and y.requires_grad],
                                         (gy, x, w) if affine else (gy, x, w.detach()))
+
+
+class _Emulated:
+    """The kernels' three calls by elementary operators on host tensors."""
+
+    def __init__(self, monkeypatch, any_order):
+        monkeypatch.setattr(norms, "_forward", lambda x, g, b, eps, stats: self.norm(x, g, b, eps))
+        monkeypatch.setattr(norms, "_backward",
+                            lambda gy, x, g, b, stats, eps, need_g, need_b: norms._composed(gy, x, g, b, eps))
+        monkeypatch.setattr(norms, "_backward2", lambda ctx, *q: (
+            *norms._composed2(*ctx.saved_tensors[:3], ctx.eps, *q), *[None] * 5))
+        self.any_order = any_order
+
+    @staticmethod
+    def norm(x, g, b, eps):
+        z = x - x.mean(-1, keepdim=True)
+        return z / ((z * z).mean(-1, keepdim=True) + eps).sqrt() * g + b
+
+    def __call__(self, x, g, b):
+        return norms._LayerNormFn.apply(x, g, b, 0.1, self.any_order)
+
+
+def _operands():
+    g = torch.Generator().manual_seed(4)
+    x, w, b = (torch.randn(*s, generator=g, dtype=torch.float64).requires_grad_(True) for s in ((3, 5), (5,), (5,)))
+    return x, w, b, torch.randn(4, 3, 5, generator=g, dtype=torch.float64)
+
+
+def test_batched_gradients(monkeypatch):
+    """is_grads_batched over a module's LayerNorm (jacobians), first and second order; the public one refuses."""
+    x, w, b, G = _operands()
+    f, ref = _Emulated(monkeypatch, True), lambda x, w, b: _Emulated.norm(x, w, b, 0.1)
+    for fn_pair in (((lambda h: h(x, w, b)), G),
+                    ((lambda h: torch.autograd.grad(h(x, w, b), x, G[0], create_graph=True)[0]), G)):
+        make, up = fn_pair
+        got, want = (torch.autograd.grad(make(h), (x, w), up, is_grads_batched=True) for h in (f, ref))
+        assert all(torch.allclose(a, r, rtol=1e-11, atol=1e-12) for a, r in zip(got, want))
+    y = _Emulated(monkeypatch, False)(x, w, b)
+    with pytest.raises(RuntimeError, match="batched"):
+        torch.autograd.grad(y, x, G, is_grads_batched=True, retain_graph=True)
+    gx, = torch.autograd.grad(y, x, G[0], create_graph=True)
+    with pytest.raises(RuntimeError, match="batched"):
+        torch.autograd.grad(gx, x, G, is_grads_batched=True)
+
+
+def test_upstream_gradients_with_tangents(monkeypatch):
+    x, w, b, G = _operands()
+    f, ref = _Emulated(monkeypatch, True), lambda x, w, b: _Emulated.norm(x, w, b, 0.1)
+    own = _Emulated(monkeypatch, False)
+
+    def tangents(h, order):
+        y = h(x, w, b)
+        if order == 2:
+            y, = torch.autograd.grad(y, x, G[2], create_graph=True)
+        with forward_ad.dual_level():
+            out = torch.autograd.grad(y, (x, w), forward_ad.make_dual(G[0], G[1]))
+            return [forward_ad.unpack_dual(t).tangent for t in out]
+
+    for order in (1, 2):
+        for a, r in zip(tangents(f, order), tangents(ref, order)):
+            assert torch.allclose(a, r, rtol=1e-11, atol=1e-12)
+        with pytest.raises(RuntimeError, match="tangents"):
+            tangents(own, order)

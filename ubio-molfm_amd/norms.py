@@ -125,7 +125,9 @@ class _LayerNormFn(torch.autograd.Function):
     def backward(ctx, gy):
         x, g, b, stats = ctx.saved_tensors
         need_g, need_b = ctx.needs_input_grad[1:3]
-        if not torch.is_grad_enabled():
+        if _only_torch_takes(ctx.any_order, gy):
+            gx, gg, gb = _composed(gy, x, g, b, ctx.eps)
+        elif not torch.is_grad_enabled():
             gx, gg, gb = _backward(gy, x, g, b, stats, ctx.eps, need_g, need_b)
         else:
             # the forces' first differentiation asks for neither weight nor bias; their sums come together.
@@ -154,6 +156,7 @@ class _LayerNormGradFn(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, qx, qg, qb):
+        _only_torch_takes(False, ctx.saved_tensors[0], qx, qg, qb)
         return _backward2(ctx, qx, qg, qb)
 
 
@@ -163,9 +166,10 @@ class _LayerNormGradAnyFn(_LayerNormGradFn):
 
     @staticmethod
     def backward(ctx, qx, qg, qb):
-        if not torch.is_grad_enabled() or (qx is None and qg is None and qb is None):
-            return _backward2(ctx, qx, qg, qb)
         gy, x, g, _, _ = ctx.saved_tensors
+        if qx is None and qg is None and qb is None or not (torch.is_grad_enabled()
+                                                            or _only_torch_takes(True, gy, qx, qg, qb)):
+            return _backward2(ctx, qx, qg, qb)
         return (*_composed2(gy, x, g, ctx.eps, qx, qg, qb), None, None, None, None, None)
 
 
@@ -180,6 +184,18 @@ def _backward2(ctx, qx, qg, qb):
     a, keep = _args(x, g, b, stats, ctx.eps, gy=gy, qx=qx, qg=qg, qb=qb, y=dgy, gx=dx)
     _call("e2v2_layer_norm_bwd2", x.device, a, _ptr(dg), _ptr(ws), _lib.i64(n))
     return dgy, dx, dg, None, None, None, None, None
+
+
+def _composed(gy, x, g, b, eps):
+    """(gx, dg, db) by the formulas at the head of csrc/norm.hip."""
+    def mean(t):
+        return t.mean(-1, keepdim=True)
+
+    z = x - mean(x)
+    r = torch.rsqrt(mean(z * z) + eps)
+    h, u, w = z * r, gy if g is None else gy * g, x.shape[-1]
+    return (r * (u - mean(u) - h * mean(u * h)), None if g is None else (gy * h).reshape(-1, w).sum(0),
+            None if b is None else gy.reshape(-1, w).sum(0))
 
 
 def _composed2(gy, x, g, eps, qx, qg, qb):
@@ -197,7 +213,7 @@ def _composed2(gy, x, g, eps, qx, qg, qb):
         dgy = a if g is None else a * g
         t = -r * (c * qx + m * u)
         extra = r * h * mean(qx * r * (u - mean(u) - h * c))
-        dg = None if g is None else (gy * a).sum_to_size(g.shape)
+        dg = None if g is None else (gy * a).reshape(-1, x.shape[-1]).sum(0)
     if qg is not None:
         dgy, t = dgy + qg * h, t + qg * gy
     if qb is not None:
@@ -212,6 +228,16 @@ def has_tangent(*tensors: Optional[torch.Tensor]) -> bool:
                                                   for t in tensors)
 
 
+def _only_torch_takes(composed: bool, *tensors: Optional[torch.Tensor]) -> bool:
+    """Whether an upstream gradient is one that no kernel reads (batched by is_grads_batched or torch.func, or with a
+    tangent); an error unless the pass can be composed of torch's operators."""
+    if has_tangent(*tensors) or not all(t is None or torch._C._has_storage(t) for t in tensors):
+        if not composed:
+            raise RuntimeError("layer_norm: batched gradients and gradients with forward-mode tangents are not supported")
+        return True
+    return False
+
+
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
                eps: float = 1e-5) -> torch.Tensor:
     """(x - mean) / sqrt(var + eps) * weight + bias over the last dimension of x, as
@@ -219,8 +245,8 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
 
     x: fp32, bf16 or fp16 on the GPU, of any shape with a last dimension of 1 to 16384; read where it lies if its rows
     are consecutive and evenly spaced.  weight, bias: [w], fp32 or x's type, or None.  The result has x's type
-    and is contiguous.  Differentiable twice in reverse mode (a third derivative, forward-mode tangents and torch.func's
-    transforms raise)."""
+    and is contiguous.  Differentiable twice in reverse mode (a third derivative, forward-mode tangents, batched gradients
+    and torch.func's transforms raise)."""
     return _layer_norm(x, weight, bias, eps, any_order=False)
 
 
