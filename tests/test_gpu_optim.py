@@ -1005,3 +1005,25 @@ def test_parameters_that_take_another_type_in_place(pkg, cuda, before, after):
     opt.state[p] = {"step": 0, "exp_avg": torch.zeros(5000), "exp_avg_sq": torch.zeros(5000)}
     opt.step(), ref.step()
     assert torch.equal(p, q) and (p < 1).all()
+
+
+@pytest.mark.parametrize("how", ["load", "state"])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_states_that_change_places(pkg, cuda, bits, how):
+    """An optimizer's own states loaded back in another order, or exchanged in place: none is read after it is written."""
+    from ubio_molfm_amd import optim
+    ps = _params([(5000,), (5000,), (5000,)], torch.float32, cuda, 62)
+    opt = optim.AdamW(ps, state_bits=bits)
+    opt.step()
+    opt.state[ps[1]]["step"] = 5
+    before = [{k: t.clone() for k, t in opt.state[p].items()} for p in ps]
+    if how == "load":
+        sd = opt.state_dict()
+        sd["state"] = {0: sd["state"][1], 1: sd["state"][2], 2: sd["state"][0]}
+        opt.load_state_dict(sd)
+    else:
+        opt.state[ps[0]], opt.state[ps[1]], opt.state[ps[2]] = (opt.state[ps[k]] for k in (1, 2, 0))
+        opt.moments()
+    for p, k in zip(ps, (1, 2, 0)):
+        assert all(torch.equal(t, before[k][name]) for name, t in opt.state[p].items())
+    assert [int(opt.state[p]["step"]) for p in ps] == [5, 1, 1]

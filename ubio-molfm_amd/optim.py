@@ -361,6 +361,10 @@ class _Plan:
             if not p.numel():
                 self.state[p]["step"].copy_(step)
         pairs = [(t, e[k]) for p, e in entries.items() for k, t in self.state[p].items() if k != "step"]
+        # another parameter's views of these buffers may be written before they are read
+        buffers = {t.untyped_storage().data_ptr() for t in (self.m, self.v, self.ms, self.vs) if t is not None}
+        pairs = [(d, o.clone() if o.untyped_storage().data_ptr() in buffers and o.data_ptr() != d.data_ptr() else o)
+                 for d, o in pairs]
         torch._foreach_copy_([d for d, _ in pairs], [o for _, o in pairs])
 
     def clear(self, params):
