@@ -189,3 +189,29 @@ def test_memory_that_tensors_share():
                (buf, buf[40:].view(torch.bfloat16)[3:5])):
         assert overlap(*ts) and overlap(*ts[::-1])
     assert not overlap(buf[:50], buf[50:].view(torch.float16))
+
+
+def test_hooks_of_loading(monkeypatch):
+    """They see the whole state and may change it; what belongs to no parameter is kept."""
+    plans = []
+    monkeypatch.setattr(optim, "_Plan", lambda opt: plans.append(dict(opt.state)))
+    monkeypatch.setattr(optim, "_usable", lambda p: True)
+    p = _p(3)
+    opt = optim.AdamW([p], lr=0.5)
+    entry = {"step": 4, "exp_avg": torch.ones(3), "exp_avg_sq": torch.ones(3)}
+    given = {"state": {0: entry, "run": [1, 2]}, "param_groups": opt.state_dict()["param_groups"]}
+    seen = []
+
+    def double(o, sd):
+        seen.append(list(sd["state"]))
+        return {**sd, "state": {**sd["state"], 0: {**entry, "exp_avg": 2 * entry["exp_avg"]}}}
+
+    opt.register_load_state_dict_pre_hook(double)
+    opt.register_load_state_dict_post_hook(lambda o: seen.append(len(plans)))
+    for _ in range(2):
+        opt.load_state_dict(given)
+    assert seen == [[0, "run"], 1, [0, "run"], 2] and list(given["state"]) == [0, "run"]
+    assert plans[0][p]["exp_avg"].tolist() == [2, 2, 2] and plans[0]["run"] == [1, 2]
+    with pytest.raises(ValueError, match="parameter groups"):
+        opt.load_state_dict({"state": {}, "param_groups": given["param_groups"] * 2})
+    assert len(opt._optimizer_load_state_dict_pre_hooks) == len(opt._optimizer_load_state_dict_post_hooks) == 1

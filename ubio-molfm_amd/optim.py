@@ -10,6 +10,7 @@ from __future__ import annotations
 import ctypes as C
 import math
 from array import array
+from collections import OrderedDict
 from contextlib import nullcontext
 from itertools import chain, compress, repeat
 from operator import attrgetter, is_, is_not
@@ -501,11 +502,22 @@ class AdamW(torch.optim.Optimizer):
     def load_state_dict(self, state_dict):
         """As torch's, with moments kept in their own types: fp32, or codes and scale bytes.  Learning rates that are
         tensors stay and take the loaded values."""
-        saved, groups = state_dict["state"], state_dict["param_groups"]
-        new = {}
+        pre, post = self._optimizer_load_state_dict_pre_hooks, self._optimizer_load_state_dict_post_hooks
+        state_dict = state_dict.copy()
+        for hook in pre.values():                                 # they see the whole state, which torch's part does not
+            changed = hook(self, state_dict)
+            state_dict = state_dict if changed is None else changed
+        self._load(state_dict)
+        for hook in post.values():
+            hook(self)
+
+    def _load(self, state_dict):
+        """load_state_dict without hooks; torch's part gets the groups and what belongs to no parameter."""
+        groups = state_dict["param_groups"]
+        saved, new = dict(state_dict["state"]), {}
         for i, p in zip(chain.from_iterable(g["params"] for g in groups),
                         chain.from_iterable(g["params"] for g in self.param_groups)):
-            e = saved.get(i)
+            e = saved.pop(i, None)
             if not e:
                 continue
             if not _usable(p):
@@ -516,7 +528,12 @@ class AdamW(torch.optim.Optimizer):
             self._check_group(g)
         plan = self._plan if self._valid() else None
         rates = [g["lr"] for g in self.param_groups]
-        super().load_state_dict({**state_dict, "state": {}})      # refuses groups of other sizes
+        hooks = self._optimizer_load_state_dict_pre_hooks, self._optimizer_load_state_dict_post_hooks
+        self._optimizer_load_state_dict_pre_hooks = self._optimizer_load_state_dict_post_hooks = OrderedDict()
+        try:                                                      # refuses groups of other sizes
+            super().load_state_dict({**state_dict, "state": saved})
+        finally:
+            self._optimizer_load_state_dict_pre_hooks, self._optimizer_load_state_dict_post_hooks = hooks
         values = {}
         for g, lr in zip(self.param_groups, rates):               # captured steps read the rates that are there
             if isinstance(lr, torch.Tensor):
