@@ -900,10 +900,6 @@ def _linear(x, lin: nn.Linear, padded_rows: bool = False):
     return torch.nn.functional.linear(x, lin.weight.detach(), None if lin.bias is None else lin.bias.detach())
 
 
-def _layer_norm(x, ln: nn.LayerNorm):
-    return torch.nn.functional.layer_norm(x, ln.normalized_shape, ln.weight.detach(), ln.bias.detach(), ln.eps)
-
-
 class GaussianSmearing(nn.Module):
     """module_utils.py:1853-1869 (evaluated inside the HIP edge kernels)."""
 
