@@ -12,8 +12,8 @@ import math
 from array import array
 from collections import OrderedDict
 from contextlib import nullcontext
-from itertools import chain, compress, repeat
-from operator import attrgetter, is_, is_not
+from itertools import chain, compress
+from operator import attrgetter, is_
 from typing import Iterable, Optional, Tuple, Union
 
 import numpy as np
@@ -103,9 +103,10 @@ def _norm_parts(lists, dev, st):
 
 def _overlap(lists) -> bool:
     """Whether tensors of the lists share memory."""
-    at = np.concatenate([np.frombuffer(l.ptrs, np.uint64) for l in lists])
-    size = np.concatenate([np.frombuffer(l.numel, np.int64) * l.itemsize for l in lists]).astype(np.uint64)
-    order = np.argsort(at)
+    at, size = ([f(l) for l in lists] for f in (lambda l: np.frombuffer(l.ptrs, np.int64),
+                                                lambda l: np.frombuffer(l.numel, np.int64) * l.itemsize))
+    at, size = (x[0] if len(x) == 1 else np.concatenate(x) for x in (at, size))
+    order = at.argsort()
     at, end = at[order], (at + size)[order]
     return bool((end[:-1] > at[1:]).any())
 
@@ -131,7 +132,6 @@ def grad_norm(tensors: Iterable[torch.Tensor]) -> torch.Tensor:
     return out
 
 
-@torch.no_grad()
 def clip_grad_norm_(parameters, max_norm: float) -> torch.Tensor:
     """Scales the parameters' gradients in place by min(1, max_norm / (norm + 1e-6)), norm their global 2-norm, which
     is returned (an fp32 tensor of one element), as torch.nn.utils.clip_grad_norm_.  Gradients that share memory are
@@ -160,9 +160,10 @@ def clip_grad_norm_(parameters, max_norm: float) -> torch.Tensor:
         for l in lists:
             l.scale(parts, count, max_norm, out, st)
     if dense is not grads:
-        for g, d in zip(grads, dense):
-            if d is not g:
-                g.copy_(d)
+        with torch.no_grad():
+            for g, d in zip(grads, dense):
+                if d is not g:
+                    g.copy_(d)
     torch.autograd.graph.increment_version(grads)
     return out
 
@@ -194,6 +195,10 @@ class _Launch:
         self.args = _lib.AdamWArgs()
 
 
+class _OtherTypes(Exception):
+    """The parameters were given another type in place."""
+
+
 def _matching(grads, launch, which):
     """The gradients of the launch's parameters (of those that ``which`` says; True: all), contiguous: on their device, of
     their types and sizes.  torch checks a gradient where it is set, but .data moves a parameter or a gradient alone."""
@@ -210,6 +215,8 @@ def _matching(grads, launch, which):
         pass
     types, grads = _dense(grads, "AdamW")
     if types != {launch.dtype}:
+        if any(p.dtype != launch.dtype for p in launch.params):
+            raise _OtherTypes
         raise ValueError(f"AdamW: gradients of type {types} for parameters in {launch.dtype}")
     if list(map(_NBYTES, grads)) != sizes:
         raise ValueError("AdamW: gradients of other sizes than their parameters")
@@ -275,6 +282,7 @@ class _Entry(dict):
 class _Plan:
     """What stays from step to step: moments and step counts of all parameters, the chunks' table, the launches."""
 
+    @torch.no_grad()
     def __init__(self, opt: "AdamW"):
         groups = opt.param_groups
         every = [p for g in groups for p in g["params"]]
@@ -294,7 +302,6 @@ class _Plan:
                                "captured: take it before the capture")
         self.device = dev = params[0].device if params else torch.device("cuda", torch.cuda.current_device())
         self.ptrs, self.nbytes = [p.data_ptr() for p in params], [p.nbytes for p in params]
-        self.types = None if all(p.dtype == torch.float32 for p in params) else [p.dtype for p in params]
         self.params = params
         bits = opt.state_bits
         sizes = [p.numel() for p in params]
@@ -342,6 +349,7 @@ class _Plan:
         opt.state.update(self.state)
         self.entries = list(opt.state.values())
 
+    @torch.no_grad()
     def fill(self, entries):
         """Takes over the states in entries (of the plan's parameters)."""
         if not entries:
@@ -577,12 +585,11 @@ class AdamW(torch.optim.Optimizer):
         return list(map(len, groups)) == plan.split and all(map(is_, chain.from_iterable(groups), plan.every))
 
     def _valid(self) -> bool:
-        """Whether the plan holds for a step: the same groups, and no parameter was moved, cut, turned or given another
-        type (bytes tell fp32 from those of 16 bits)."""
+        """Whether the plan holds for a step: the same groups, and no parameter was moved, cut, turned or given a type of
+        another size (of one of that size, the gradients' types tell)."""
         plan = self._plan
         return (self._same_groups() and list(map(torch.Tensor.data_ptr, plan.params)) == plan.ptrs
                 and list(map(_NBYTES, plan.params)) == plan.nbytes
-                and (plan.types is None or [p.dtype for p in plan.params] == plan.types)
                 and all(map(torch.Tensor.is_contiguous, plan.params)) and not any(map(_usable, plan.outside)))
 
     def _with_entries(self, plan: _Plan) -> _Plan:
@@ -608,15 +615,19 @@ class AdamW(torch.optim.Optimizer):
             self._plan = _Plan(self)
         return self._with_entries(self._plan)
 
-    @torch.no_grad()
     def step(self, closure=None):
         loss = None
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
         plan = self._current()
-        with _on(plan.device):
-            self._launch(plan)
+        try:
+            with _on(plan.device):
+                self._launch(plan)
+        except _OtherTypes:
+            self._plan = plan = _Plan(self)
+            with _on(plan.device):
+                self._launch(plan)
         return loss
 
     def _launch(self, plan: _Plan):
@@ -627,17 +638,18 @@ class AdamW(torch.optim.Optimizer):
         keep, updated = [], []
         for l in plan.launches:
             grads = [p.grad for p in l.params]
-            all_there = all(map(is_not, grads, repeat(None)))
-            some = grads if all_there else [g for g in grads if g is not None]
-            if some:
-                dense = _matching(some, l, all_there or [g is not None for g in grads])
-                updated += l.params if all_there else [p for p, g in zip(l.params, grads) if g is not None]
+            try:
+                dense = _matching(grads, l, True)
+                updated += l.params
+                l.grads.set(list(map(torch.Tensor.data_ptr, dense)))
+            except TypeError:                  # some parameters have none
+                there = [g is not None for g in grads]
+                dense = list(compress(grads, there))
+                dense = _matching(dense, l, there) if dense else []
+                updated += compress(l.params, there)
                 it = iter(dense)
-                l.grads.set(list(map(torch.Tensor.data_ptr, dense)) if all_there
-                            else [0 if g is None else next(it).data_ptr() for g in grads])
-                keep.append(dense)
-            else:
-                l.grads.set([0] * len(grads))
+                l.grads.set([next(it).data_ptr() if t else 0 for t in there])
+            keep.append(dense)
             if normed:
                 l.grads.norm(plan.parts, count, st)
         if normed and not count.value:
