@@ -9,14 +9,14 @@
 //                  dx = r (X - <X> - xh <X xh>) - r <qx gx> xh,  d(g) = sum_rows gy A
 // (<qx gx> is r (<qx u> - <qx> <u> - c m); d(b) is zero.)  Rows are rounded to their type once, at the store;
 // statistics, row sums and the parameters' sums are fp32, the variance taken about the mean in a second pass over the
-// registers.
+// registers (and the mean itself once more where a row is far narrower than it).
 //
 // One pass over memory: a row stays in the registers of kL lanes (2 to 64 of a wavefront, or a workgroup of 256 or
 // 1024), read as 16-byte vectors on whatever element boundary the row starts (the hardware takes them unaligned); a
 // row's last vector may start early, its end is stored in pieces.  A workgroup strides over the rows and keeps its
 // columns' parameter sums in registers; each leaves one partial row, added in order by a second launch, so results
-// repeat bitwise.  Bound: HBM (127,113 x 128 fp32: forward 25 us, 5.2 TB/s; backward with the parameters 42, 4.7;
-// second order 67, 4.8; 32,768 x 2048 bf16: 52, 88 and 140 us).
+// repeat bitwise.  Bound: HBM (127,113 x 128 fp32: forward 24 us, 5.4 TB/s; backward 31 and its parameters' sums 4,
+// 5.6; second order 53 and 4, 5.7; 32,768 x 2048 bf16: 47 us, 88 + 4 and 130 + 5, 5.7, 4.4 and 5.0 TB/s).
 #include <algorithm>
 #include <type_traits>
 

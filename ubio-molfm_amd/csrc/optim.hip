@@ -6,8 +6,8 @@
 // Arithmetic is fp32 (the norm's sum fp64: it neither loses small tensors beside large ones nor overflows; 8-bit
 // moments fp64 up to their code); bf16 and fp16 parameters are rounded to nearest once.  Every element is read and
 // written once by one thread, the sums run in a fixed order: no atomics, results repeat bitwise.  Bound: HBM (241 M
-// bf16 parameters with 32-bit moments 1.02 ms, 5.2 TB/s; 241 M fp32 parameters with 8-bit moments 0.74 ms, 5.2 TB/s;
-// 24.5 M fp32 in 240 tensors 133 us, a norm before it 20 us cold).
+// bf16 parameters with 32-bit moments 1.02 ms, 5.2 TB/s; 241 M fp32 parameters with 8-bit moments 0.76 ms, 5.1 TB/s;
+// 24.5 M fp32 in 240 tensors 135 us, behind a norm, which leaves gradients in the caches, 124; the norm 18 to 32).
 //
 // The tensors are cut into chunks, one workgroup each.  What does not change from step to step (addresses and places
 // of the parameters) is a table in device memory; the gradients' addresses, which may, come with the launch.  The step

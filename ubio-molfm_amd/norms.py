@@ -3,8 +3,9 @@ libe2v2.so: any width up to 16384, fp32, bf16 or fp16 rows, weight and bias in t
 with the gradients of rows, weight and bias and the derivative of that backward pass (force training differentiates
 the forces once more).  Statistics, row sums and the parameters' sums are fp32; each result is rounded once.
 
-The equivariant RMS norm is in ``modules`` / ``second_order``, the fused LayerNorm + SiLU of the radial profiles in
-``second_order.ln_silu``.  There is no CPU path."""
+The equivariant RMS norm is in ``modules`` / ``second_order``, the fused LayerNorm + SiLU of the radial profiles, and so
+every LayerNorm of the models built here, in ``second_order.ln_silu``; ``second_order.run_seq`` calls this one for the
+others of a user's net.  There is no CPU path."""
 from __future__ import annotations
 
 import struct

@@ -134,8 +134,8 @@ def grad_norm(tensors: Iterable[torch.Tensor]) -> torch.Tensor:
 
 def clip_grad_norm_(parameters, max_norm: float) -> torch.Tensor:
     """Scales the parameters' gradients in place by min(1, max_norm / (norm + 1e-6)), norm their global 2-norm, which
-    is returned (an fp32 tensor of one element), as torch.nn.utils.clip_grad_norm_.  Gradients that share memory are
-    refused.  A norm that is not finite scales
+    is returned (an fp32 tensor of one element), as torch.nn.utils.clip_grad_norm_.  Contiguous gradients that share
+    memory, and the same one twice, are refused.  A norm that is not finite scales
     by what the quotient gives (0, or NaN); nothing is read back to the host."""
     max_norm = float(max_norm)
     if not max_norm >= 0:
