@@ -135,8 +135,8 @@ def grad_norm(tensors: Iterable[torch.Tensor]) -> torch.Tensor:
 def clip_grad_norm_(parameters, max_norm: float) -> torch.Tensor:
     """Scales the parameters' gradients in place by min(1, max_norm / (norm + 1e-6)), norm their global 2-norm, which
     is returned (an fp32 tensor of one element), as torch.nn.utils.clip_grad_norm_.  Contiguous gradients that share
-    memory, and the same one twice, are refused.  A norm that is not finite scales
-    by what the quotient gives (0, or NaN); nothing is read back to the host."""
+    memory, and the same one twice, are refused.  A norm that is not finite scales by what the quotient gives (0, or
+    NaN); nothing is read back to the host."""
     max_norm = float(max_norm)
     if not max_norm >= 0:
         raise ValueError(f"clip_grad_norm_: max_norm {max_norm}")
@@ -509,7 +509,8 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """As torch's, with moments kept in their own types: fp32, or codes and scale bytes.  Learning rates that are
-        tensors stay and take the loaded values."""
+        tensors stay and take the loaded values (one tensor for several groups where these agree; the others get the
+        loaded ones, which a step captured before does not read)."""
         pre, post = self._optimizer_load_state_dict_pre_hooks, self._optimizer_load_state_dict_post_hooks
         state_dict = state_dict.copy()
         for hook in pre.values():                                 # they see the whole state, which torch's part does not
