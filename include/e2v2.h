@@ -626,6 +626,92 @@ int e2v2_layer_norm_bwd(const e2v2_layer_norm_args* args, void* gg, void* gb, fl
 int e2v2_layer_norm_bwd2(const e2v2_layer_norm_args* args, void* gg, float* workspace, int64_t workspace_bytes,
                          hipStream_t s);
 
+/* ---- root-mean-square norm of rows with the residual's addition, its output also in 8 bits, and its backward pass ----
+ * No counterpart in the reference (its RMS norm is the equivariant one, e2v2_rmsnorm_*); the kind of norm that stands
+ * before a product in a generic network.  Rows as in e2v2_layer_norm_*; the weight may be NULL (1).
+ *   fwd:  h = x + res rounded to the rows' type (res NULL: h is x and is not written), y = h rstd w, rstd [n] unless
+ *         NULL.  h is contiguous.  With scales, y holds e4m3 codes, rows ldy bytes apart (a multiple of 16), and
+ *         scales [n][ceil(width / 128)] a byte s for each 128 columns that stands for 2^(s - 127); rstd is not written.
+ *         Else y is contiguous and ldy is not read.
+ *   bwd:  x holds the forward's h; gx from h, gy, rstd and gh (the gradient of h itself, or NULL), and unless gw is NULL
+ *         the weight's gradient; the workspace holds one partial row of its sums per workgroup. */
+typedef struct {
+  const void* x; const void* res; const void* w;
+  void* h; void* y;
+  uint8_t* scales;
+  float* rstd;
+  const void* gy; const void* gh; void* gx;
+  int64_t n, ldx, ldres, ldgy, ldgh, ldy;
+  int32_t width, type, w_type;
+  float eps;
+} e2v2_rms_rows_args;
+int e2v2_rms_rows_fwd(const e2v2_rms_rows_args* args, hipStream_t s);
+int64_t e2v2_rms_rows_workspace(int64_t n, int width);
+int e2v2_rms_rows_bwd(const e2v2_rms_rows_args* args, void* gw, float* workspace, int64_t workspace_bytes, hipStream_t s);
+
+/* ---- 8-bit floats with block scales ----
+ * No counterpart in the reference.  e4m3 codes; each block has a scale byte s that stands for 2^(s - 127), the smallest
+ * power of two (2^-126 at least) with which its largest finite value is at most 448.  What is not finite becomes NaN.
+ *   quantize8  x [n][width] in fp32, bf16 or fp16, rows ldx elements apart.
+ *     ROWS   codes [n][ldc], scales [n][ceil(width / 128)]: blocks of 1 x 128.
+ *     TILES  blocks of 128 x 128: codes with scales [ceil(n / 128)][ceil(width / 128)] and the same codes transposed,
+ *            codes_t [width][ldt] with scales_t [ceil(width / 128)][ceil(n / 128)]; either pair may be NULL.  `batch`
+ *            matrices x_batch elements apart; their outputs follow one another.
+ *     BOTH   ROWS, and the transpose of x quantised by rows: codes_t [width][ldt], scales_t [width][ceil(n / 128)]; either
+ *            pair may be NULL.
+ *     Rows of codes lie a multiple of 16 bytes apart.
+ *   values8    what codes stand for, contiguous, in the type; tiles: scales of 128 x 128 blocks of weights of
+ *              rows_each rows. */
+#define E2V2_QUANT_ROWS 0
+#define E2V2_QUANT_TILES 1
+#define E2V2_QUANT_BOTH 2
+typedef struct {
+  const void* x;
+  uint8_t* codes; uint8_t* scales; uint8_t* codes_t; uint8_t* scales_t;
+  int64_t n, width, ldx, ldc, ldt, x_batch;
+  int32_t batch, type, mode;
+} e2v2_quantize8_args;
+int e2v2_quantize8(const e2v2_quantize8_args* args, hipStream_t s);
+int e2v2_values8(const uint8_t* codes, int64_t ldc, const uint8_t* scales, int tiles, int64_t n, int64_t width,
+                 int64_t rows_each, void* out, int type, hipStream_t s);
+
+/* ---- products of 8-bit operands with block scales ----
+ * No counterpart in the reference.  y [m][n] = a b^T: a [m][k] and b [n][k] e4m3 codes, rows lda and ldb bytes apart, sa
+ * [m][ceil(k / 128)], sb [n][ceil(k / 128)] or (b_tiles) [ceil(n / 128)][ceil(k / 128)]; any m, n, k and alignment.
+ * fp32 accumulation; y in fp32, bf16 or fp16, rows ldy elements apart.  With offsets (device, [groups + 1], increasing):
+ * rows offsets[e] .. offsets[e + 1] of a meet b + e b_group bytes, the experts' scales follow one another; rows of no
+ * expert become zeros (fill) or stay as they are.  The workspace (dense only) holds the sums of parts of k. */
+typedef struct {
+  const void* a; const void* b;
+  const uint8_t* sa; const uint8_t* sb;
+  void* y;
+  const int32_t* offsets;
+  int64_t m, n, k, lda, ldb, ldy, b_group;
+  int32_t groups, b_tiles, out_type, fill;
+} e2v2_product8_args;
+int64_t e2v2_product8_workspace(int64_t m, int64_t n, int64_t k);
+int e2v2_product8(const e2v2_product8_args* args, float* workspace, int64_t workspace_bytes, hipStream_t s);
+
+/* ---- products grouped by expert, ragged sizes on the device ----
+ * No counterpart in the reference.  Rows offsets[e] .. offsets[e + 1] (device, [experts + 1], increasing, clamped to the
+ * rows) belong to expert e with the weight w + e w_group, [n][k]; strides in elements; one type for all, fp32 accumulation.
+ *   FORWARD  y [rows][n] from x [rows][k];   ROWS  y [rows][k] from gy [rows][n]: the gradient of x;
+ *   WEIGHTS  y [experts][n][k] from gy and x: the gradient of w (ldy: from row to row of it).
+ * Rows of no expert become zeros (fill) or stay as they are.  The workspace (WEIGHTS) holds the sums of parts of the
+ * rows. */
+#define E2V2_EXPERT_FORWARD 0
+#define E2V2_EXPERT_ROWS 1
+#define E2V2_EXPERT_WEIGHTS 2
+typedef struct {
+  const void* x; const void* w; const void* gy;
+  void* y;
+  const int32_t* offsets;
+  int64_t rows, n, k, ldx, ldw, ldgy, ldy, w_group;
+  int32_t experts, type, fill;
+} e2v2_expert_args;
+int64_t e2v2_expert_product_workspace(int64_t rows, int64_t n, int64_t k, int experts);
+int e2v2_expert_product(const e2v2_expert_args* args, int pass, float* workspace, int64_t workspace_bytes, hipStream_t s);
+
 /* ---- the parameter update of training, over many tensors at once ----
  * No counterpart in the reference's own code: its trainer calls torch's clipping and optimizer
  * (src/molfm/pipeline/trainer.py:114-662).  Tensors are contiguous fp32, bf16 or fp16; `grads` and `numel` are host

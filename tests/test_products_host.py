@@ -1,0 +1,176 @@
+"""What the RMS norm, the 8-bit operators and the products grouped by expert refuse, before any kernel or HIP call.  No GPU
+needed."""
+import ctypes
+import struct
+
+import pytest
+import torch
+
+from ubio_molfm_amd import _lib, experts, fp8, norms
+
+F8, U8, BF16 = torch.float8_e4m3fn, torch.uint8, torch.bfloat16
+
+
+class _OnGpu(torch.Tensor):
+    """A host tensor that says it lies on the GPU: the checks behind the device's."""
+    is_cuda = True
+
+
+def _gpu(*shape, dtype=torch.float32):
+    return torch.zeros(shape).to(dtype).as_subclass(_OnGpu)
+
+
+def _i32(*v):
+    return torch.tensor(v, dtype=torch.int32).as_subclass(_OnGpu)
+
+
+@pytest.fixture(autouse=True)
+def no_kernels(monkeypatch):
+    monkeypatch.setattr(_lib, "call", lambda *a: pytest.fail("a kernel was called"))
+
+
+def test_host_tensors_are_refused():
+    x = torch.rand(3, 16)
+    for call in (lambda: norms.rms_norm(x), lambda: norms.rms_norm_fp8(x), lambda: norms.rms_norm([1.0]),
+                 lambda: fp8.quantize(x), lambda: fp8.linear(x, x), lambda: fp8.linear(x, 3.0),
+                 lambda: fp8.dequantize(x.to(F8), torch.zeros(3, 1, dtype=U8)),
+                 lambda: fp8.gemm(x.to(F8), torch.zeros(3, 1, dtype=U8), x.to(F8), torch.zeros(3, 1, dtype=U8)),
+                 lambda: experts.expert_linear(x, x[None], torch.tensor([0, 3])),
+                 lambda: experts.expert_gemm_fp8(x.to(F8), torch.zeros(3, 1, dtype=U8), x[None].to(F8),
+                                                 torch.zeros(1, 1, 1, dtype=U8), torch.tensor([0, 3]))):
+        with pytest.raises(RuntimeError, match="GPU only"):
+            call()
+
+
+@pytest.mark.parametrize("fn", [norms.rms_norm, norms.rms_norm_fp8])
+@pytest.mark.parametrize("x,kw,match", [
+    (lambda: _gpu(3, 8, dtype=torch.float64), {}, "fp32, bf16 or fp16"),
+    (lambda: _gpu(), {}, "fp32, bf16 or fp16"),
+    (lambda: _gpu(3, 0), {}, "width 0"),
+    (lambda: _gpu(1, norms.MAX_WIDTH + 1), {}, "width 16385"),
+    (lambda: _gpu(3, 8), dict(weight=torch.ones(8)), "weight"),
+    (lambda: _gpu(3, 8), dict(weight=_gpu(7)), "weight"),
+    (lambda: _gpu(3, 8), dict(weight=_gpu(8, dtype=BF16)), "weight"),
+    (lambda: _gpu(3, 8), dict(residual=_gpu(8)), "residual"),
+    (lambda: _gpu(3, 8), dict(residual=_gpu(3, 8, dtype=BF16)), "residual"),
+    (lambda: _gpu(3, 8), dict(residual=torch.zeros(3, 8)), "residual"),
+])
+def test_norm_refusals(fn, x, kw, match):
+    with pytest.raises(ValueError, match=match):
+        fn(x(), **kw)
+
+
+def test_8_bit_refusals():
+    a, sa, w, sw = _gpu(3, 200, dtype=F8), _gpu(3, 2, dtype=U8), _gpu(130, 200, dtype=F8), _gpu(2, 2, dtype=U8)
+    for call, match in (
+            (lambda: fp8.quantize(_gpu(3, 8, dtype=torch.float64)), "fp32, bf16 or fp16"),
+            (lambda: fp8.quantize(_gpu(3, 0)), "at least one value"),
+            (lambda: fp8.quantize(_gpu(3), tiles=True), "weights"),
+            (lambda: fp8.gemm(a, sa, w[:, :199], sw), "w \\[n, k\\]"),
+            (lambda: fp8.gemm(a, sa, w, sw, dtype=torch.float64), "out in"),
+            (lambda: fp8.gemm(a, sa[:, :1], w, sw), "a in e4m3"),
+            (lambda: fp8.gemm(a, sa.float(), w, sw), "a in e4m3"),
+            (lambda: fp8.gemm(a.float(), sa, w, sw), "a in e4m3"),
+            (lambda: fp8.gemm(a, sa, w, sw[:1]), "w in e4m3"),
+            (lambda: fp8.dequantize(a, sa[:2]), "codes in e4m3"),
+            (lambda: fp8.dequantize(a, sa, torch.float64), "values in"),
+            (lambda: fp8.linear(_gpu(3, 8), _gpu(4, 9)), "weight \\[n, k\\]"),
+            (lambda: fp8.linear(_gpu(3, 8), _gpu(4, 8, dtype=torch.int32)), "fp32, bf16 or fp16"),
+            (lambda: fp8.linear(_gpu(3, 8), _gpu(0, 8)), "weight \\[n, k\\]")):
+        with pytest.raises(ValueError, match=match):
+            call()
+
+
+def test_expert_refusals():
+    x, w, offs = _gpu(5, 16), _gpu(2, 8, 16), _i32(0, 2, 5)
+    for call, match in (
+            (lambda: experts.expert_linear(x[0], w, offs), "x \\[rows, k\\]"),
+            (lambda: experts.expert_linear(x, w[0], offs), "x \\[rows, k\\]"),
+            (lambda: experts.expert_linear(x, w[..., :8], offs), "x \\[rows, k\\]"),
+            (lambda: experts.expert_linear(x, w.bfloat16(), offs), "x \\[rows, k\\]"),
+            (lambda: experts.expert_linear(x, w[:0], offs[:1]), "x \\[rows, k\\]"),
+            (lambda: experts.expert_linear(x, w, offs[:2]), "offsets \\[3\\]"),
+            (lambda: experts.expert_linear(x, w, offs.float()), "offsets \\[3\\]"),
+            (lambda: experts.expert_linear(x, w, [0, 2, 5]), "offsets \\[3\\]"),
+            (lambda: experts.expert_linear(x, w, offs, out=_gpu(5, 9)), "out"),
+            (lambda: experts.expert_linear(x, w, offs, out=_gpu(8, 5).t()), "out"),
+            (lambda: experts.expert_linear(x, w, offs, out=_gpu(5, 8, dtype=BF16)), "out"),
+            (lambda: experts.expert_gemm_fp8(x.to(F8), _gpu(5, 1, dtype=U8), w.to(F8), _gpu(2, 1, 2, dtype=U8), offs),
+             "weight in e4m3"),
+            (lambda: experts.expert_gemm_fp8(x.to(F8), _gpu(5, 2, dtype=U8), w.to(F8), _gpu(2, 1, 1, dtype=U8), offs),
+             "x in e4m3")):
+        with pytest.raises(ValueError, match=match):
+            call()
+    with pytest.raises(RuntimeError, match="no gradients"):
+        experts.expert_linear(x, torch.nn.Parameter(w.as_subclass(torch.Tensor)).as_subclass(_OnGpu), offs, out=_gpu(5, 8))
+
+
+def test_packed_arguments_are_the_structures():
+    for c, s in ((_lib.RmsRowsArgs, norms._RMS_ARGS), (_lib.Quantize8Args, fp8._QUANT_ARGS),
+                 (_lib.Product8Args, fp8._PRODUCT_ARGS), (_lib.ExpertArgs, experts._ARGS)):
+        assert ctypes.sizeof(c) == s.size
+        fields = [f for f, t in c._fields_]
+        values = list(range(1, len(fields) + 1))
+        a = c.from_buffer_copy(s.pack(*values))
+        assert [int(getattr(a, f) or 0) for f in fields] == values
+
+
+def test_entry_points_check_on_the_host():
+    lib = _lib.load()
+
+    def refused(rc, what):
+        assert rc != 0 and what in lib.e2v2_last_error(), lib.e2v2_last_error()
+
+    a = _lib.RmsRowsArgs()
+    a.x = a.y = 16
+    a.n, a.ldx, a.width = 4, 8, 0
+    refused(lib.e2v2_rms_rows_fwd(ctypes.byref(a), None), b"width 0")
+    a.width, a.type = 8, 7
+    refused(lib.e2v2_rms_rows_fwd(ctypes.byref(a), None), b"types")
+    a.type, a.scales, a.ldy = 0, 16, 8
+    refused(lib.e2v2_rms_rows_fwd(ctypes.byref(a), None), b"multiple of 16")
+    a.scales, a.x = None, 18
+    refused(lib.e2v2_rms_rows_fwd(ctypes.byref(a), None), b"misaligned")
+    a.x, a.gy, a.gx, a.rstd = 16, 16, 16, 16
+    refused(lib.e2v2_rms_rows_bwd(ctypes.byref(a), ctypes.c_void_p(16), None, ctypes.c_int64(0), None), b"workspace")
+    assert lib.e2v2_rms_rows_workspace(5, 8) == 160 and lib.e2v2_rms_rows_workspace(0, 8) == 0
+
+    q = _lib.Quantize8Args()
+    q.x = q.codes = q.scales = 16
+    q.n, q.width, q.ldx, q.ldc, q.batch = 4, 20, 20, 20, 1
+    refused(lib.e2v2_quantize8(ctypes.byref(q), None), b"multiple of 16")
+    q.ldc, q.mode = 32, 9
+    refused(lib.e2v2_quantize8(ctypes.byref(q), None), b"mode 9")
+    q.mode, q.codes_t, q.scales_t, q.ldt = 2, 16, 16, 3
+    refused(lib.e2v2_quantize8(ctypes.byref(q), None), b"transposed")
+    refused(lib.e2v2_values8(ctypes.c_void_p(16), ctypes.c_int64(8), ctypes.c_void_p(16), 1, ctypes.c_int64(9),
+                             ctypes.c_int64(8), ctypes.c_int64(4), ctypes.c_void_p(16), 0, None), b"weights of 4")
+
+    p = _lib.Product8Args()
+    p.a = p.b = p.sa = p.sb = p.y = 16
+    p.m, p.n, p.k, p.lda, p.ldb, p.ldy = 4, 8, 64, 63, 64, 8
+    refused(lib.e2v2_product8(ctypes.byref(p), None, ctypes.c_int64(0), None), b"apart")
+    p.lda = (1 << 22) + 16
+    refused(lib.e2v2_product8(ctypes.byref(p), None, ctypes.c_int64(0), None), b"apart")
+    p.lda, p.out_type = 64, 3
+    refused(lib.e2v2_product8(ctypes.byref(p), None, ctypes.c_int64(0), None), b"output type")
+    p.out_type, p.offsets = 0, 16
+    refused(lib.e2v2_product8(ctypes.byref(p), None, ctypes.c_int64(0), None), b"0 experts")
+    p.offsets, p.lda, p.ldb, p.m, p.n, p.k = None, 1 << 16, 1 << 16, 100, 128, 1 << 16
+    p.ldy = 128
+    need = lib.e2v2_product8_workspace(100, 128, 1 << 16)
+    assert need > 0
+    refused(lib.e2v2_product8(ctypes.byref(p), ctypes.c_void_p(16), ctypes.c_int64(need - 1), None), b"workspace")
+
+    e = _lib.ExpertArgs()
+    e.x = e.w = e.gy = e.y = e.offsets = 16
+    e.rows, e.n, e.k, e.ldx, e.ldw, e.ldgy, e.ldy = 4, 8, 16, 16, 16, 8, 8
+    refused(lib.e2v2_expert_product(ctypes.byref(e), 0, None, ctypes.c_int64(0), None), b"0 experts")
+    e.experts, e.type = 2, 5
+    refused(lib.e2v2_expert_product(ctypes.byref(e), 0, None, ctypes.c_int64(0), None), b"type 5")
+    e.type = 0
+    refused(lib.e2v2_expert_product(ctypes.byref(e), 3, None, ctypes.c_int64(0), None), b"pass 3")
+    e.ldx = 15
+    refused(lib.e2v2_expert_product(ctypes.byref(e), 0, None, ctypes.c_int64(0), None), b"row strides")
+    e.ldx, e.x = 16, 18
+    refused(lib.e2v2_expert_product(ctypes.byref(e), 0, None, ctypes.c_int64(0), None), b"misaligned")

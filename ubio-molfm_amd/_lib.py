@@ -22,6 +22,8 @@ EXPORTS = [
     "e2v2_edge_to_pos", "e2v2_rmsnorm_fwd", "e2v2_add_rmsnorm_fwd", "e2v2_rmsnorm_bwd", "e2v2_rmsnorm_bwd_param", "e2v2_rmsnorm_bwd2", "e2v2_gate_fwd",
     "e2v2_gate_bwd", "e2v2_gate_bwd2", "e2v2_ln_silu_fwd", "e2v2_ln_silu_bwd", "e2v2_ln_silu_bwd_param", "e2v2_ln_silu_bwd2",
     "e2v2_layer_norm_fwd", "e2v2_layer_norm_workspace", "e2v2_layer_norm_bwd", "e2v2_layer_norm_bwd2",
+    "e2v2_rms_rows_fwd", "e2v2_rms_rows_workspace", "e2v2_rms_rows_bwd", "e2v2_quantize8", "e2v2_values8",
+    "e2v2_product8", "e2v2_product8_workspace", "e2v2_expert_product", "e2v2_expert_product_workspace",
     "e2v2_grad_norm_parts", "e2v2_grad_norm", "e2v2_grad_norm_value", "e2v2_grad_scale", "e2v2_adamw", "e2v2_moments",
     "e2v2_pairdot_fwd", "e2v2_pairdot_bwd", "e2v2_qk_proj_fwd", "e2v2_qk_proj_bwd",
     "e2v2_qk_proj_fwd_bf16", "e2v2_qk_proj_bwd_bf16",
@@ -112,6 +114,30 @@ class LayerNormArgs(C.Structure):
                 ("g_type", i32), ("b_type", i32), ("eps", f32)]
 
 
+class RmsRowsArgs(C.Structure):
+    _fields_ = [("x", vp), ("res", vp), ("w", vp), ("h", vp), ("y", vp), ("scales", vp), ("rstd", vp), ("gy", vp),
+                ("gh", vp), ("gx", vp), ("n", i64), ("ldx", i64), ("ldres", i64), ("ldgy", i64), ("ldgh", i64),
+                ("ldy", i64), ("width", i32), ("type", i32), ("w_type", i32), ("eps", f32)]
+
+
+class Quantize8Args(C.Structure):
+    _fields_ = [("x", vp), ("codes", vp), ("scales", vp), ("codes_t", vp), ("scales_t", vp), ("n", i64), ("width", i64),
+                ("ldx", i64), ("ldc", i64), ("ldt", i64), ("x_batch", i64), ("batch", i32), ("type", i32),
+                ("mode", i32)]
+
+
+class Product8Args(C.Structure):
+    _fields_ = [("a", vp), ("b", vp), ("sa", vp), ("sb", vp), ("y", vp), ("offsets", vp), ("m", i64), ("n", i64),
+                ("k", i64), ("lda", i64), ("ldb", i64), ("ldy", i64), ("b_group", i64), ("groups", i32),
+                ("b_tiles", i32), ("out_type", i32), ("fill", i32)]
+
+
+class ExpertArgs(C.Structure):
+    _fields_ = [("x", vp), ("w", vp), ("gy", vp), ("y", vp), ("offsets", vp), ("rows", i64), ("n", i64), ("k", i64),
+                ("ldx", i64), ("ldw", i64), ("ldgy", i64), ("ldy", i64), ("w_group", i64), ("experts", i32),
+                ("type", i32), ("fill", i32)]
+
+
 class OptChunk(C.Structure):
     _fields_ = [("p", vp), ("at", i64), ("off", i64), ("n", i32), ("tensor", i32)]
 
@@ -174,6 +200,12 @@ def load():
     lib.e2v2_qkdot_gate_bwd_workspace.argtypes = [C.c_int64]
     lib.e2v2_layer_norm_workspace.restype = C.c_int64
     lib.e2v2_layer_norm_workspace.argtypes = [C.c_int64, C.c_int32]
+    lib.e2v2_rms_rows_workspace.restype = C.c_int64
+    lib.e2v2_rms_rows_workspace.argtypes = [C.c_int64, C.c_int32]
+    lib.e2v2_product8_workspace.restype = C.c_int64
+    lib.e2v2_product8_workspace.argtypes = [C.c_int64, C.c_int64, C.c_int64]
+    lib.e2v2_expert_product_workspace.restype = C.c_int64
+    lib.e2v2_expert_product_workspace.argtypes = [C.c_int64, C.c_int64, C.c_int64, C.c_int32]
     lib.e2v2_gemm_packed_bytes.restype = C.c_int64
     lib.e2v2_gemm_packed_bytes.argtypes = [C.c_int32, C.c_int32, C.c_int32, C.c_int32]
     _lib = lib

@@ -1,0 +1,109 @@
+// Products grouped by expert in fp32, bf16 and fp16 (mm.h): rows offsets[e] .. offsets[e + 1] belong to expert e, and
+//   forward          y[t] = W[e] x[t]              W [experts][n][k], read as it lies
+//   rows' gradient   gx[t] = W[e]^T gy[t]          W read along its columns
+//   weights' grad.   gW[e] = sum_t gy[t] x[t]^T    both operands read along their columns, over ragged rows
+// Rows of no expert give zeros.
+#include <algorithm>
+
+#include "mm.h"
+
+namespace e2v2 {
+namespace {
+
+constexpr int64_t kMaxPitch = 1 << 22;       // bytes between rows: a tile's offsets stay below 2^30
+
+// The parts that the rows of each expert are cut into for the weights' gradient: enough workgroups for the 256 CUs where
+// experts and tiles are few.
+int splits_of(int64_t rows, int64_t n, int64_t k, int groups) {
+  const int64_t tiles = groups * ((n + 127) / 128) * ((k + 127) / 128);
+  if (tiles >= 192) return 1;
+  return (int)std::max<int64_t>(1, std::min<int64_t>({512 / tiles, rows / groups / 256, 16}));
+}
+
+template <int kT, bool kAO, bool kBO, int kGroup, bool kStaged>
+void run(const MmArgs& P, hipStream_t s) {
+  if constexpr (!kStaged && kT != kF32) {
+    const int64_t m = kGroup == kRed ? P.m : P.m / P.groups;
+    const int64_t tiles = (kGroup == kRed ? (int64_t)P.groups * ((P.m + 255) / 256) : P.m / 256 + P.groups) *
+                          ((P.n + 255) / 256);
+    if (tiles >= 200 && m >= 192) return launch_mm<kT, kAO, kBO, 256, 256, 2, 4, kGroup, false>(P, s);
+  }
+  launch_mm<kT, kAO, kBO, 128, 128, 2, 2, kGroup, kStaged>(P, s);
+}
+
+template <int kT>
+void run_pass(const MmArgs& P, int pass, bool staged, hipStream_t s) {
+  if (pass == E2V2_EXPERT_FORWARD)
+    staged ? run<kT, false, false, kRows, true>(P, s) : run<kT, false, false, kRows, false>(P, s);
+  else if (pass == E2V2_EXPERT_ROWS)
+    staged ? run<kT, false, true, kRows, true>(P, s) : run<kT, false, true, kRows, false>(P, s);
+  else
+    staged ? run<kT, true, true, kRed, true>(P, s) : run<kT, true, true, kRed, false>(P, s);
+}
+
+}  // namespace
+}  // namespace e2v2
+
+using namespace e2v2;
+
+E2V2_API int64_t e2v2_expert_product_workspace(int64_t rows, int64_t n, int64_t k, int experts) {
+  if (rows <= 0 || n <= 0 || k <= 0 || experts <= 0) return 0;
+  const int splits = splits_of(rows, n, k, experts);
+  return splits > 1 ? splits * experts * n * k * 4 : 0;
+}
+
+E2V2_API int e2v2_expert_product(const e2v2_expert_args* a, int pass, float* ws, int64_t ws_bytes, hipStream_t s) {
+  E2V2_REQUIRE(a, "expert_product: null arguments");
+  E2V2_REQUIRE(pass >= E2V2_EXPERT_FORWARD && pass <= E2V2_EXPERT_WEIGHTS, "expert_product: pass %d", pass);
+  E2V2_REQUIRE(a->rows >= 0 && a->n >= 0 && a->k >= 0 && a->rows <= INT32_MAX / 2 && a->n <= INT32_MAX / 2 &&
+                   a->k <= INT32_MAX / 2 && a->experts > 0, "expert_product: %lld rows, %d experts of %lld x %lld",
+               (long long)a->rows, a->experts, (long long)a->n, (long long)a->k);
+  E2V2_REQUIRE(a->type >= E2V2_F32 && a->type <= E2V2_F16, "expert_product: type %d", a->type);
+  const int size = a->type == E2V2_F32 ? 4 : 2;
+  // rows [T][..] of each pass, its product's extents and its operands
+  const bool fwd = pass == E2V2_EXPERT_FORWARD, wgrad = pass == E2V2_EXPERT_WEIGHTS;
+  MmArgs P{};
+  P.m = (int)(wgrad ? a->n : a->rows);
+  P.n = (int)(fwd ? a->n : a->k);
+  P.k = (int)(fwd ? a->k : wgrad ? a->rows : a->n);
+  if (P.m == 0 || P.n == 0) return 0;
+  const void* pa = fwd ? a->x : a->gy;
+  const void* pb = wgrad ? a->x : a->w;
+  const int64_t lda = fwd ? a->ldx : a->ldgy, ldb = wgrad ? a->ldx : a->ldw;
+  E2V2_REQUIRE(a->y && a->offsets && (a->rows == 0 || P.k == 0 || (pa && pb)), "expert_product: null operand");
+  const int64_t wide = (fwd || wgrad ? a->k : 0), wide_gy = fwd ? 0 : a->n;
+  E2V2_REQUIRE(a->ldx >= wide && a->ldgy >= wide_gy && (wgrad || a->ldw >= a->k) && a->ldy >= P.n &&
+                   lda * size <= kMaxPitch && ldb * size <= kMaxPitch, "expert_product: row strides %lld, %lld, %lld, %lld",
+               (long long)a->ldx, (long long)a->ldw, (long long)a->ldgy, (long long)a->ldy);
+  E2V2_REQUIRE(((uintptr_t)pa | (uintptr_t)pb | (uintptr_t)a->y) % size == 0 && (uintptr_t)a->offsets % 4 == 0 &&
+                   (uintptr_t)ws % 16 == 0, "expert_product: misaligned operand");
+  P.a = static_cast<const uint8_t*>(pa);
+  P.b = static_cast<const uint8_t*>(pb);
+  P.y = a->y;
+  P.part = ws;
+  P.offsets = a->offsets;
+  P.lda = lda * size;
+  P.ldb = ldb * size;
+  P.b_group = a->w_group * size;
+  P.ldy = a->ldy;
+  P.groups = a->experts;
+  P.out_type = a->type;
+  P.fill = a->fill;
+  P.splits = wgrad ? splits_of(a->rows, a->n, a->k, a->experts) : 1;
+  E2V2_REQUIRE(P.splits == 1 || (ws && ws_bytes >= e2v2_expert_product_workspace(a->rows, a->n, a->k, a->experts)),
+               "expert_product: workspace of %lld bytes", (long long)ws_bytes);
+  const int64_t tiles = wgrad ? (int64_t)a->experts * ((P.m + 127) / 128) * ((P.n + 127) / 128)
+                              : (a->rows / 128 + a->experts + 2) * ((P.n + 127) / 128);
+  E2V2_REQUIRE(tiles < INT32_MAX / 2, "expert_product: %lld tiles", (long long)tiles);
+  const bool staged = ((uintptr_t)pa | (uintptr_t)pb | (uintptr_t)P.lda | (uintptr_t)P.ldb |
+                       (uintptr_t)(wgrad ? 0 : P.b_group)) % 16 != 0;
+  if (a->type == E2V2_F32) run_pass<kF32>(P, pass, staged, s);
+  else if (a->type == E2V2_BF16) run_pass<kBf16>(P, pass, staged, s);
+  else run_pass<kF16>(P, pass, staged, s);
+  E2V2_LAUNCHED("k_mm");
+  if (P.splits > 1) {
+    launch_mm_sum(P, (int64_t)P.groups * P.m, s);
+    E2V2_LAUNCHED("k_mm_sum");
+  }
+  return 0;
+}

@@ -1,0 +1,96 @@
+// Products of 8-bit rows and 8-bit weights with block scales, dense or with a weight for each expert (mm.h).  The scales
+// are powers of two that the matrix instruction applies itself: v_mfma_scale_f32_16x16x128_f8f6f4 takes a scale byte for
+// each row of its operands, and its 128 values of k are one block.
+#include <algorithm>
+
+#include "mm.h"
+
+namespace e2v2 {
+namespace {
+
+constexpr int64_t kMaxPitch = 1 << 22;       // bytes between rows: a tile's offsets stay below 2^30
+
+// Tiles of 256 x 256 where they fill the 256 CUs, else 128 x 128.
+bool big_tiles(int64_t m, int64_t n, int groups) {
+  return (m / 256 + (groups > 1 ? groups : 1)) * ((n + 255) / 256) >= 200 && m / groups >= 192;
+}
+
+int splits_of(int64_t m, int64_t n, int64_t k) {
+  const bool big = big_tiles(m, n, 1);
+  const int64_t t = big ? 256 : 128, tiles = ((m + t - 1) / t) * ((n + t - 1) / t), steps = (k + 127) / 128;
+  if (tiles >= 192 || steps < 16) return 1;
+  return (int)std::max<int64_t>(1, std::min<int64_t>({512 / tiles, steps / 8, 16}));
+}
+
+template <int kGroup, bool kStaged>
+void run8(const MmArgs& P, bool big, hipStream_t s) {
+  if constexpr (!kStaged) {
+    if (big) return launch_mm<kE4m3, false, false, 256, 256, 2, 4, kGroup, false>(P, s);
+  }
+  launch_mm<kE4m3, false, false, 128, 128, 2, 2, kGroup, kStaged>(P, s);
+}
+
+}  // namespace
+}  // namespace e2v2
+
+using namespace e2v2;
+
+E2V2_API int64_t e2v2_product8_workspace(int64_t m, int64_t n, int64_t k) {
+  if (m <= 0 || n <= 0 || k <= 0) return 0;
+  const int splits = splits_of(m, n, k);
+  return splits > 1 ? splits * m * n * 4 : 0;
+}
+
+E2V2_API int e2v2_product8(const e2v2_product8_args* a, float* ws, int64_t ws_bytes, hipStream_t s) {
+  E2V2_REQUIRE(a, "product8: null arguments");
+  E2V2_REQUIRE(a->m >= 0 && a->n >= 0 && a->k >= 0 && a->m <= INT32_MAX / 2 && a->n <= INT32_MAX / 2 &&
+                   a->k <= INT32_MAX / 2, "product8: %lld x %lld x %lld", (long long)a->m, (long long)a->n, (long long)a->k);
+  E2V2_REQUIRE(a->out_type >= E2V2_F32 && a->out_type <= E2V2_F16, "product8: output type %d", a->out_type);
+  E2V2_REQUIRE(!a->offsets || a->groups > 0, "product8: %d experts", a->groups);
+  if (a->m == 0 || a->n == 0) return 0;
+  E2V2_REQUIRE(a->a && a->b && a->sa && a->sb && a->y, "product8: null operand");
+  E2V2_REQUIRE(a->lda >= a->k && a->ldb >= a->k && a->lda <= kMaxPitch && a->ldb <= kMaxPitch && a->ldy >= a->n,
+               "product8: rows %lld, %lld and %lld apart", (long long)a->lda, (long long)a->ldb, (long long)a->ldy);
+  E2V2_REQUIRE((uintptr_t)a->y % (a->out_type == E2V2_F32 ? 4 : 2) == 0 && (uintptr_t)a->offsets % 4 == 0 &&
+                   (uintptr_t)ws % 16 == 0, "product8: misaligned operand");
+  const int64_t nb = (a->k + 127) / 128, sb_each = (a->b_tiles ? (a->n + 127) / 128 : a->n) * nb;
+  const bool grouped = a->offsets != nullptr;
+  MmArgs P{};
+  P.a = static_cast<const uint8_t*>(a->a);
+  P.b = static_cast<const uint8_t*>(a->b);
+  P.sa = a->sa;
+  P.sb = a->sb;
+  P.y = a->y;
+  P.part = ws;
+  P.offsets = a->offsets;
+  P.lda = a->lda;
+  P.ldb = a->ldb;
+  P.b_group = a->b_group;
+  P.sb_group = sb_each;
+  P.ldy = a->ldy;
+  P.sa_bytes = a->m * nb;
+  P.sb_bytes = sb_each;
+  P.m = (int)a->m;
+  P.n = (int)a->n;
+  P.k = (int)a->k;
+  P.groups = grouped ? a->groups : 1;
+  P.sb_rows = a->b_tiles ? 128 : 1;
+  P.out_type = a->out_type;
+  P.fill = a->fill;
+  P.splits = grouped ? 1 : splits_of(a->m, a->n, a->k);
+  E2V2_REQUIRE(P.splits == 1 || (ws && ws_bytes >= e2v2_product8_workspace(a->m, a->n, a->k)),
+               "product8: workspace of %lld bytes", (long long)ws_bytes);
+  const bool staged = ((uintptr_t)a->a | (uintptr_t)a->b | (uintptr_t)a->lda | (uintptr_t)a->ldb |
+                       (uintptr_t)(grouped ? a->b_group : 0)) % 16 != 0;
+  const bool big = big_tiles(a->m, a->n, P.groups);
+  const int64_t tiles = (a->m / 128 + P.groups + 2) * ((a->n + 127) / 128);
+  E2V2_REQUIRE(tiles < INT32_MAX / 2, "product8: %lld tiles", (long long)tiles);
+  if (grouped) staged ? run8<kRows, true>(P, big, s) : run8<kRows, false>(P, big, s);
+  else staged ? run8<kDense, true>(P, big, s) : run8<kDense, false>(P, big, s);
+  E2V2_LAUNCHED("k_mm");
+  if (P.splits > 1) {
+    launch_mm_sum(P, P.m, s);
+    E2V2_LAUNCHED("k_mm_sum");
+  }
+  return 0;
+}

@@ -1,0 +1,152 @@
+"""Products grouped by expert: rows sorted by expert, each expert's rows times its own weight, in one launch whose sizes only
+the GPU knows (no counterpart in the reference).  ``gemm.gemm_grouped`` joins up to four products of sizes that the host
+knows; here the experts' row counts are read from a tensor of offsets by the kernel, so that a router's or a sorted
+batch's result (one weight for each element, say) needs no wait and a captured graph takes other counts on replay.
+
+There is no CPU path."""
+from __future__ import annotations
+
+import struct
+from typing import Optional
+
+import torch
+
+from . import _lib
+from .fp8 import MAX_PITCH, _blocks, _check_codes, _on_gpu, _product, _row_operand
+from .norms import _TYPES, _address, _call, _first_order, has_tangent
+
+_FORWARD, _ROWS, _WEIGHTS = 0, 1, 2         # E2V2_EXPERT_*
+# e2v2_expert_args as bytes
+_ARGS = struct.Struct("5Q8q3i4x")
+
+
+def _matrix(t: torch.Tensor, rows: Optional[int] = None):
+    """(t as the kernel reads it, its row stride): consecutive elements in a row."""
+    w = t.shape[-1]
+    if t.stride(-1) != 1 and w > 1 or t.stride(-2) < w and t.shape[-2] > 1 or t.stride(-2) * t.element_size() > MAX_PITCH:
+        t = t.contiguous()
+    return t, t.stride(-2) if t.shape[-2] > 1 else w
+
+
+def _experts_of(name, offsets, experts, dev):
+    if (not isinstance(offsets, torch.Tensor) or offsets.dim() != 1 or offsets.shape[0] != experts + 1
+            or offsets.dtype not in (torch.int32, torch.int64) or offsets.device != dev):
+        got = (f"{tuple(offsets.shape)} {offsets.dtype} on {offsets.device}" if isinstance(offsets, torch.Tensor)
+               else type(offsets).__name__)
+        raise ValueError(f"{name}: offsets [{experts + 1}] int32 or int64 on {dev}, got {got}")
+    return offsets.to(torch.int32).contiguous()
+
+
+def _launch(which, x, w_shape, w, gy, y, offsets, fill):
+    experts, n, k = w_shape
+    ldx = ldw = ldgy = group = 0
+    if x is not None:
+        x, ldx = _matrix(x)
+    if gy is not None:
+        gy, ldgy = _matrix(gy)
+    if w is not None:
+        w, ldw = _matrix(w)
+        group = w.stride(0)
+    rows = (gy if x is None else x).shape[0]
+    need = _lib.load().e2v2_expert_product_workspace(rows, n, k, experts) if which == _WEIGHTS else 0
+    ws = torch.empty(need // 4, dtype=torch.float32, device=y.device) if need else None
+    a = _ARGS.pack(_address(x), _address(w), _address(gy), y.data_ptr(), offsets.data_ptr(), rows, n, k, max(ldx, k),
+                   max(ldw, k), max(ldgy, n), y.stride(-2) if y.shape[-2] > 1 else y.shape[-1], group, experts,
+                   _TYPES[y.dtype], fill)
+    _call("e2v2_expert_product", y.device, a, _lib.i32(which), _lib.vp(_address(ws)), _lib.i64(need))
+    return y
+
+
+class _ExpertLinearFn(torch.autograd.Function):
+
+    @staticmethod
+    def forward(ctx, x, w, offsets):
+        y = torch.empty((x.shape[0], w.shape[1]), dtype=x.dtype, device=x.device)
+        need_x, need_w = ctx.needs_input_grad[:2]
+        ctx.save_for_backward(x if need_w else None, w if need_x else None, offsets)
+        ctx.x_shape, ctx.w_shape = x.shape, w.shape
+        return _launch(_FORWARD, x, w.shape, w, None, y, offsets, True) if y.numel() else y
+
+    @staticmethod
+    def backward(ctx, gy):
+        _first_order("expert_linear", gy)
+        x, w, offsets = ctx.saved_tensors
+        need_x, need_w = ctx.needs_input_grad[:2]
+        gx = gw = None
+        if need_x:
+            gx = torch.empty(ctx.x_shape, dtype=gy.dtype, device=gy.device)
+            if gx.numel():
+                _launch(_ROWS, None, ctx.w_shape, w, gy, gx, offsets, True)
+        if need_w:
+            gw = torch.empty(ctx.w_shape, dtype=gy.dtype, device=gy.device)
+            if ctx.x_shape[0] == 0:
+                gw.zero_()
+            else:
+                _launch(_WEIGHTS, x, ctx.w_shape, None, gy, gw, offsets, True)
+        return gx, gw, None
+
+
+def expert_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor,
+                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """y[t] = weight[e] x[t] for the rows t = offsets[e] .. offsets[e + 1] - 1 of each expert e.
+
+    x [rows, k] and weight [experts, n, k] in one of fp32, bf16 and fp16; offsets [experts + 1], int32 or int64 on the GPU,
+    not decreasing, an expert without rows where two are equal (what lies outside 0 .. rows is clamped, never read).  Rows of
+    no expert give zeros and take no part in gradients.  Sums are fp32 (fp32 operands are split exactly into bf16 pieces, as
+    in ``gemm``: a product with an infinite operand is NaN there).  Differentiable once in reverse mode, in x and weight.
+
+    out [rows, n]: written instead of a new tensor, rows of no expert left as they were; for calls without gradients."""
+    dev = _on_gpu("expert_linear", x, weight)
+    if (x.dim() != 2 or weight.dim() != 3 or weight.shape[2] != x.shape[1] or weight.numel() == 0
+            or x.dtype not in _TYPES or weight.dtype != x.dtype):
+        raise ValueError("expert_linear: x [rows, k] and weight [experts, n, k] in one of fp32, bf16 and fp16, got "
+                         f"{tuple(x.shape)} {x.dtype} and {tuple(weight.shape)} {weight.dtype}")
+    offsets = _experts_of("expert_linear", offsets, weight.shape[0], dev)
+    if has_tangent(x, weight):
+        raise RuntimeError("expert_linear: forward-mode tangents are not supported")
+    grads = torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad)
+    if out is None:
+        if grads:
+            return _ExpertLinearFn.apply(x, weight, offsets)
+        y, fill = torch.empty((x.shape[0], weight.shape[1]), dtype=x.dtype, device=dev), True
+    else:
+        _check_out("expert_linear", out, (x.shape[0], weight.shape[1]), x.dtype, dev, grads)
+        y, fill = out, False
+    return _launch(_FORWARD, x, weight.shape, weight, None, y, offsets, fill) if y.numel() else y
+
+
+def _check_out(name, out, shape, dtype, dev, grads):
+    if grads or (torch.is_grad_enabled() and out.requires_grad):
+        raise RuntimeError(f"{name}: out= has no gradients: call it under torch.no_grad()")
+    if (out.shape != shape or out.dtype != dtype or out.device != dev or (shape[1] > 1 and out.stride(1) != 1)
+            or (shape[0] > 1 and out.stride(0) < shape[1])):
+        raise ValueError(f"{name}: out {shape} {dtype} on {dev} with consecutive elements in a row, got "
+                         f"{tuple(out.shape)} {out.dtype} on {out.device} with strides {out.stride()}")
+
+
+def expert_gemm_fp8(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
+                    offsets: torch.Tensor, dtype: torch.dtype = torch.bfloat16,
+                    out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The product of :func:`expert_linear` in 8 bits (the format of ``fp8``): x [rows, k] with x_scale
+    [rows, ceil(k / 128)], weight [experts, n, k] with weight_scale [experts, ceil(n / 128), ceil(k / 128)].  The result is
+    fp32, bf16 or fp16 (out's type where it is given).  No gradients: ``fp8.linear`` trains a single weight in 8 bits."""
+    dev = _on_gpu("expert_gemm_fp8", x, x_scale, weight, weight_scale)
+    dtype = dtype if out is None else out.dtype
+    if x.dim() != 2 or weight.dim() != 3 or weight.shape[2] != x.shape[1] or weight.numel() == 0 or dtype not in _TYPES:
+        raise ValueError("expert_gemm_fp8: x [rows, k] and weight [experts, n, k], out in fp32, bf16 or fp16, got "
+                         f"{tuple(x.shape)}, {tuple(weight.shape)} and {dtype}")
+    (rows, k), (experts, n, _) = x.shape, weight.shape
+    _check_codes("expert_gemm_fp8", "x", x, x_scale, [torch.Size((rows, _blocks(k)))])
+    _check_codes("expert_gemm_fp8", "weight", weight, weight_scale, [torch.Size((experts, _blocks(n), _blocks(k)))])
+    offsets = _experts_of("expert_gemm_fp8", offsets, experts, dev)
+    if out is None:
+        y, fill = torch.empty((rows, n), dtype=dtype, device=dev), True
+    else:
+        _check_out("expert_gemm_fp8", out, (rows, n), dtype, dev, False)
+        y, fill = out, False
+    if y.numel() == 0:
+        return y
+    xr, ldx = _row_operand("expert_gemm_fp8", x)
+    w, ldw = _matrix(weight)
+    return _product(xr, ldx, x_scale.contiguous(), w, ldw, weight_scale.contiguous(), True, y, rows, n, k, offsets,
+                    experts, w.stride(0), fill)

@@ -1,7 +1,12 @@
-"""Layer norm of rows (the reference's nn.LayerNorm, module_utils.py:2151-2178, 2230-2233) as HIP kernels of
-libe2v2.so: any width up to 16384, fp32, bf16 or fp16 rows, weight and bias in the rows' type or fp32 or absent,
+"""Norms of rows as HIP kernels of libe2v2.so.
+
+Layer norm (the reference's nn.LayerNorm, module_utils.py:2151-2178, 2230-2233): any width up to 16384, fp32, bf16 or fp16 rows, weight and bias in the rows' type or fp32 or absent,
 with the gradients of rows, weight and bias and the derivative of that backward pass (force training differentiates
 the forces once more).  Statistics, row sums and the parameters' sums are fp32; each result is rounded once.
+
+RMS norm (no counterpart in the reference, whose RMS norm is the equivariant one): the same rows, the residual's addition
+before it in the same pass, its first gradients; or its output in 8 bits with block scales (``fp8``), for the product
+behind it.
 
 The equivariant RMS norm is in ``modules`` / ``second_order``, the fused LayerNorm + SiLU of the radial profiles, and so
 every LayerNorm of the models built here, in ``second_order.ln_silu``; ``second_order.run_seq`` calls this one for the
@@ -274,3 +279,137 @@ def _layer_norm(x, weight, bias, eps: float, any_order: bool) -> torch.Tensor:
                                     or (bias is not None and bias.requires_grad)):
         return _LayerNormFn.apply(x, weight, bias, float(eps), any_order)
     return _forward(x, weight, bias, float(eps), None)
+
+
+# ---------------------------------------------------------------------------------------------
+# RMS norm
+
+# e2v2_rms_rows_args as bytes
+_RMS_ARGS = struct.Struct("10Q6q3if")
+_BLOCK = 128                                # columns that share a scale in 8 bits
+
+
+def _address(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+def _rms_forward(x, g, eps, res, rstd):
+    """(y, h) with rstd written unless None; h is x without a residual."""
+    (xr, ldx), w = _rows(x), x.shape[-1]
+    rr, ldr = (None, 0) if res is None else _rows(res)
+    y = _empty_rows(x)
+    h = x if res is None else _empty_rows(x)
+    a = _RMS_ARGS.pack(xr.data_ptr(), _address(rr), _address(g), 0 if res is None else h.data_ptr(), y.data_ptr(), 0,
+                       _address(rstd), 0, 0, 0, x.numel() // w, ldx, ldr, 0, 0, 0, w, _TYPES[x.dtype],
+                       0 if g is None else _TYPES[g.dtype], eps)
+    _call("e2v2_rms_rows_fwd", x.device, a)
+    return y, h
+
+
+class _RmsNormFn(torch.autograd.Function):
+    """(y, h) of x and a residual, or y of x alone."""
+
+    @staticmethod
+    def forward(ctx, x, g, eps: float, res):
+        rstd = x.new_empty(x.numel() // x.shape[-1], dtype=torch.float32)
+        y, h = _rms_forward(x, g, eps, res, rstd)
+        ctx.save_for_backward(h, g, rstd)
+        ctx.set_materialize_grads(False)
+        return y if res is None else (y, h)
+
+    @staticmethod
+    def backward(ctx, gy, gh=None):
+        h, g, rstd = ctx.saved_tensors
+        _first_order("rms_norm", gy, gh)
+        need_x, need_g, _, need_res = ctx.needs_input_grad
+        if gy is None:                          # y was not used
+            return gh if need_x else None, None, None, gh if need_res else None
+        w = h.shape[-1]
+        (hr, ldh), (gyr, ldy) = _rows(h), _rows(gy)
+        ghr, ldgh = (None, 0) if gh is None else _rows(gh)
+        gx = _empty_rows(h)
+        gg = ws = None
+        n = 0
+        if need_g:
+            gg = _empty_rows(g)
+            n = min(h.numel() // w, _MAX_PARTS) * w
+            ws = h.new_empty(n, dtype=torch.float32)
+        a = _RMS_ARGS.pack(hr.data_ptr(), 0, _address(g), 0, 0, 0, rstd.data_ptr(), gyr.data_ptr(), _address(ghr),
+                           gx.data_ptr(), h.numel() // w, ldh, 0, ldy, ldgh, 0, w, _TYPES[h.dtype],
+                           0 if g is None else _TYPES[g.dtype], 0.0)
+        _call("e2v2_rms_rows_bwd", h.device, a, _ptr(gg), _ptr(ws), _lib.i64(4 * n))
+        return gx if need_x else None, gg, None, gx if need_res else None
+
+
+def _first_order(name: str, *tensors: Optional[torch.Tensor]) -> None:
+    """A backward pass that is to be differentiated itself is refused, and so are upstream gradients that no kernel reads
+    (batched, or with a tangent)."""
+    if torch.is_grad_enabled():
+        raise NotImplementedError(f"{name} is differentiable once: create_graph=True is not supported")
+    if has_tangent(*tensors) or not all(t is None or torch._C._has_storage(t) for t in tensors):
+        raise RuntimeError(f"{name}: batched gradients and gradients with forward-mode tangents are not supported")
+
+
+def _rms_check(name, x, weight, residual):
+    if not isinstance(x, torch.Tensor) or not x.is_cuda:
+        raise RuntimeError(f"{name} runs on the GPU only (HIP library, no CPU path): got "
+                           f"{x.device if isinstance(x, torch.Tensor) else type(x).__name__}")
+    dtype = x.dtype
+    if dtype not in _TYPES or x.dim() == 0:
+        raise ValueError(f"{name}: rows in fp32, bf16 or fp16, got {tuple(x.shape)} {dtype}")
+    w = x.shape[-1]
+    if not 1 <= w <= MAX_WIDTH:
+        raise ValueError(f"{name}: width {w} (1 to {MAX_WIDTH})")
+    if weight is not None and (weight.dim() != 1 or weight.shape[0] != w or not weight.is_cuda
+                               or (weight.dtype != dtype and weight.dtype != torch.float32)
+                               or weight.get_device() != x.get_device()):
+        raise ValueError(f"{name}: weight [{w}] in fp32 or {dtype} on {x.device}, got {tuple(weight.shape)} "
+                         f"{weight.dtype} on {weight.device}")
+    if residual is not None and (residual.shape != x.shape or residual.dtype != dtype or not residual.is_cuda
+                                 or residual.get_device() != x.get_device()):
+        raise ValueError(f"{name}: residual {tuple(x.shape)} {dtype} on {x.device}, got {tuple(residual.shape)} "
+                         f"{residual.dtype} on {residual.device}")
+    if has_tangent(x, weight, residual):
+        raise RuntimeError(f"{name}: forward-mode tangents are not supported")
+    return weight if weight is None or weight.is_contiguous() else weight.contiguous()
+
+
+def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: float = 1e-5,
+             residual: Optional[torch.Tensor] = None):
+    """h / sqrt(mean(h^2) + eps) * weight over the last dimension, with h = x, or with a residual h = x + residual rounded to
+    x's type; returns the norm, with a residual (norm, h).
+
+    x: fp32, bf16 or fp16 on the GPU, of any shape with a last dimension of 1 to 16384, the residual like it; both are read
+    where they lie if their rows are consecutive and evenly spaced.  weight: [w], fp32 or x's type, or None.  Results
+    have x's type and are contiguous.  Differentiable once in reverse mode (create_graph=True raises)."""
+    weight = _rms_check("rms_norm", x, weight, residual)
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
+                                    or (residual is not None and residual.requires_grad)):
+        return _RmsNormFn.apply(x, weight, float(eps), residual)
+    y, h = _rms_forward(x, weight, float(eps), residual, None)
+    return y if residual is None else (y, h)
+
+
+def rms_norm_fp8(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: float = 1e-5,
+                 residual: Optional[torch.Tensor] = None):
+    """rms_norm with its output in 8 bits for ``fp8.gemm`` or ``experts.expert_gemm_fp8``: (codes, scales), with a residual
+    (codes, scales, h).  The codes are those of the norm before it is rounded to x's type.  No gradients: call it under
+    torch.no_grad(), or with tensors that need none."""
+    weight = _rms_check("rms_norm_fp8", x, weight, residual)
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
+                                    or (residual is not None and residual.requires_grad)):
+        raise RuntimeError("rms_norm_fp8 has no gradients: call it under torch.no_grad()")
+    w = x.shape[-1]
+    n, pitch, blocks = x.numel() // w, (w + 15) // 16 * 16, (w + _BLOCK - 1) // _BLOCK
+    (xr, ldx), (rr, ldr) = _rows(x), (None, 0) if residual is None else _rows(residual)
+    lead = x.shape[:-1]
+    codes = torch.empty((*lead, pitch), dtype=torch.float8_e4m3fn, device=x.device)
+    scales = torch.empty((*lead, blocks), dtype=torch.uint8, device=x.device)
+    h = x if residual is None else _empty_rows(x)
+    a = _RMS_ARGS.pack(xr.data_ptr(), _address(rr), _address(weight), 0 if residual is None else h.data_ptr(),
+                       codes.data_ptr(), scales.data_ptr(), 0, 0, 0, 0, n, ldx, ldr, 0, 0, pitch, w, _TYPES[x.dtype],
+                       0 if weight is None else _TYPES[weight.dtype], float(eps))
+    _call("e2v2_rms_rows_fwd", x.device, a)
+    if pitch != w:
+        codes = codes[..., :w]
+    return (codes, scales) if residual is None else (codes, scales, h)
