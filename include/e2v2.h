@@ -677,16 +677,17 @@ int e2v2_values8(const uint8_t* codes, int64_t ldc, const uint8_t* scales, int t
 
 /* ---- products of 8-bit operands with block scales ----
  * No counterpart in the reference.  y [m][n] = a b^T: a [m][k] and b [n][k] e4m3 codes, rows lda and ldb bytes apart, sa
- * [m][ceil(k / 128)], sb [n][ceil(k / 128)] or (b_tiles) [ceil(n / 128)][ceil(k / 128)]; any m, n, k and alignment.
+ * [m][ceil(k / 128)], sb [n][ceil(k / 128)] or (b_tiles) [ceil(n / 128)][ceil(k / 128)], their rows s*_ld and blocks s*_k
+ * bytes apart; any m, n, k and alignment.
  * fp32 accumulation; y in fp32, bf16 or fp16, rows ldy elements apart.  With offsets (device, [groups + 1], increasing):
- * rows offsets[e] .. offsets[e + 1] of a meet b + e b_group bytes, the experts' scales follow one another; rows of no
- * expert become zeros (fill) or stay as they are.  The workspace (dense only) holds the sums of parts of k. */
+ * rows offsets[e] .. offsets[e + 1] of a meet b + e b_group bytes with sb + e sb_group; rows of no expert
+ * become zeros (fill) or stay as they are.  The workspace (dense only) holds the sums of parts of k. */
 typedef struct {
   const void* a; const void* b;
   const uint8_t* sa; const uint8_t* sb;
   void* y;
   const int32_t* offsets;
-  int64_t m, n, k, lda, ldb, ldy, b_group;
+  int64_t m, n, k, lda, ldb, ldy, b_group, sa_ld, sa_k, sb_ld, sb_k, sb_group;
   int32_t groups, b_tiles, out_type, fill;
 } e2v2_product8_args;
 int64_t e2v2_product8_workspace(int64_t m, int64_t n, int64_t k);

@@ -128,8 +128,8 @@ class Quantize8Args(C.Structure):
 
 class Product8Args(C.Structure):
     _fields_ = [("a", vp), ("b", vp), ("sa", vp), ("sb", vp), ("y", vp), ("offsets", vp), ("m", i64), ("n", i64),
-                ("k", i64), ("lda", i64), ("ldb", i64), ("ldy", i64), ("b_group", i64), ("groups", i32),
-                ("b_tiles", i32), ("out_type", i32), ("fill", i32)]
+                ("k", i64), ("lda", i64), ("ldb", i64), ("ldy", i64), ("b_group", i64), ("sa_ld", i64),
+                ("sa_k", i64), ("sb_ld", i64), ("sb_k", i64), ("sb_group", i64), ("groups", i32), ("b_tiles", i32), ("out_type", i32), ("fill", i32)]
 
 
 class ExpertArgs(C.Structure):

@@ -22,11 +22,19 @@ int splits_of(int64_t rows, int64_t n, int64_t k, int groups) {
 
 template <int kT, bool kAO, bool kBO, int kGroup, bool kStaged>
 void run(const MmArgs& P, hipStream_t s) {
-  if constexpr (!kStaged && kT != kF32) {
+  if constexpr (!kStaged) {
+    if constexpr (!kAO && !kBO) {
+      if (thin_rows(P.m, P.n, (int64_t)P.k * elem_size(kT), P.groups)) return launch_thin<kT, 1, kGroup>(P, s);
+    }
+    // tiles of 256 where they fill the 256 CUs, of 64 where not even those of 128 do
     const int64_t m = kGroup == kRed ? P.m : P.m / P.groups;
-    const int64_t tiles = (kGroup == kRed ? (int64_t)P.groups * ((P.m + 255) / 256) : P.m / 256 + P.groups) *
-                          ((P.n + 255) / 256);
-    if (tiles >= 200 && m >= 192) return launch_mm<kT, kAO, kBO, 256, 256, 2, 4, kGroup, false>(P, s);
+    auto tiles = [&](int64_t t) {
+      return (kGroup == kRed ? P.groups * ((P.m + t - 1) / t) : P.m / t + std::min(P.groups, P.m)) * ((P.n + t - 1) / t);
+    };
+    if constexpr (kT != kF32) {
+      if (tiles(256) >= 200 && m >= 192) return launch_mm<kT, kAO, kBO, 256, 256, 2, 4, kGroup, false>(P, s);
+    }
+    if (tiles(128) * P.splits < 256) return launch_mm<kT, kAO, kBO, 64, 64, 2, 1, kGroup, false>(P, s);
   }
   launch_mm<kT, kAO, kBO, 128, 128, 2, 2, kGroup, kStaged>(P, s);
 }
@@ -92,8 +100,8 @@ E2V2_API int e2v2_expert_product(const e2v2_expert_args* a, int pass, float* ws,
   P.splits = wgrad ? splits_of(a->rows, a->n, a->k, a->experts) : 1;
   E2V2_REQUIRE(P.splits == 1 || (ws && ws_bytes >= e2v2_expert_product_workspace(a->rows, a->n, a->k, a->experts)),
                "expert_product: workspace of %lld bytes", (long long)ws_bytes);
-  const int64_t tiles = wgrad ? (int64_t)a->experts * ((P.m + 127) / 128) * ((P.n + 127) / 128)
-                              : (a->rows / 128 + a->experts + 2) * ((P.n + 127) / 128);
+  const int64_t tiles = wgrad ? (int64_t)a->experts * ((P.m + 63) / 64) * ((P.n + 63) / 64)
+                              : (a->rows / 16 + a->experts) * ((P.n + 15) / 16);
   E2V2_REQUIRE(tiles < INT32_MAX / 2, "expert_product: %lld tiles", (long long)tiles);
   const bool staged = ((uintptr_t)pa | (uintptr_t)pb | (uintptr_t)P.lda | (uintptr_t)P.ldb |
                        (uintptr_t)(wgrad ? 0 : P.b_group)) % 16 != 0;

@@ -10,22 +10,29 @@ namespace {
 
 constexpr int64_t kMaxPitch = 1 << 22;       // bytes between rows: a tile's offsets stay below 2^30
 
-// Tiles of 256 x 256 where they fill the 256 CUs, else 128 x 128.
-bool big_tiles(int64_t m, int64_t n, int groups) {
-  return (m / 256 + (groups > 1 ? groups : 1)) * ((n + 255) / 256) >= 200 && m / groups >= 192;
+// The side of the tiles: 256 where they fill the 256 CUs, 64 where not even those of 128 do.
+int tile_side(int64_t m, int64_t n, int groups) {
+  auto tiles = [&](int64_t t) { return (m / t + (groups < m ? groups : m)) * ((n + t - 1) / t); };
+  if (tiles(256) >= 200 && m / groups >= 192) return 256;
+  return tiles(128) >= 256 ? 128 : 64;
 }
 
+// Parts of k, where the tiles are few and k is long.
 int splits_of(int64_t m, int64_t n, int64_t k) {
-  const bool big = big_tiles(m, n, 1);
-  const int64_t t = big ? 256 : 128, tiles = ((m + t - 1) / t) * ((n + t - 1) / t), steps = (k + 127) / 128;
+  if (thin_rows(m, n, k, 1)) return 1;
+  const int64_t t = tile_side(m, n, 1) == 256 ? 256 : 128, tiles = ((m + t - 1) / t) * ((n + t - 1) / t);
+  const int64_t steps = (k + 127) / 128;
   if (tiles >= 192 || steps < 16) return 1;
   return (int)std::max<int64_t>(1, std::min<int64_t>({512 / tiles, steps / 8, 16}));
 }
 
 template <int kGroup, bool kStaged>
-void run8(const MmArgs& P, bool big, hipStream_t s) {
+void run8(const MmArgs& P, hipStream_t s) {
+  const int side = tile_side(P.m, P.n, P.groups);
   if constexpr (!kStaged) {
-    if (big) return launch_mm<kE4m3, false, false, 256, 256, 2, 4, kGroup, false>(P, s);
+    if (P.splits == 1 && thin_rows(P.m, P.n, P.k, P.groups)) return launch_thin<kE4m3, 1, kGroup>(P, s);
+    if (side == 256) return launch_mm<kE4m3, false, false, 256, 256, 2, 4, kGroup, false>(P, s);
+    if (side == 64 && P.splits == 1) return launch_mm<kE4m3, false, false, 64, 64, 2, 1, kGroup, false>(P, s);
   }
   launch_mm<kE4m3, false, false, 128, 128, 2, 2, kGroup, kStaged>(P, s);
 }
@@ -53,7 +60,13 @@ E2V2_API int e2v2_product8(const e2v2_product8_args* a, float* ws, int64_t ws_by
                "product8: rows %lld, %lld and %lld apart", (long long)a->lda, (long long)a->ldb, (long long)a->ldy);
   E2V2_REQUIRE((uintptr_t)a->y % (a->out_type == E2V2_F32 ? 4 : 2) == 0 && (uintptr_t)a->offsets % 4 == 0 &&
                    (uintptr_t)ws % 16 == 0, "product8: misaligned operand");
-  const int64_t nb = (a->k + 127) / 128, sb_each = (a->b_tiles ? (a->n + 127) / 128 : a->n) * nb;
+  const int64_t nb = (a->k + 127) / 128, sb_each = a->b_tiles ? (a->n + 127) / 128 : a->n;
+  auto fits = [](int64_t rows, int64_t ld, int64_t blocks, int64_t step) {
+    return ld >= 0 && step >= 0 && (rows - 1) * ld + (blocks - 1) * step < INT32_MAX / 2;
+  };
+  E2V2_REQUIRE(fits(std::min<int64_t>(a->m, 256), a->sa_ld, nb, a->sa_k) && fits(std::min<int64_t>(sb_each, 256), a->sb_ld, nb, a->sb_k),
+               "product8: scales %lld and %lld apart, %lld and %lld", (long long)a->sa_ld, (long long)a->sa_k,
+               (long long)a->sb_ld, (long long)a->sb_k);
   const bool grouped = a->offsets != nullptr;
   MmArgs P{};
   P.a = static_cast<const uint8_t*>(a->a);
@@ -66,10 +79,12 @@ E2V2_API int e2v2_product8(const e2v2_product8_args* a, float* ws, int64_t ws_by
   P.lda = a->lda;
   P.ldb = a->ldb;
   P.b_group = a->b_group;
-  P.sb_group = sb_each;
+  P.sb_group = a->sb_group;
   P.ldy = a->ldy;
-  P.sa_bytes = a->m * nb;
-  P.sb_bytes = sb_each;
+  P.sa_ld = a->sa_ld;
+  P.sa_k = a->sa_k;
+  P.sb_ld = a->sb_ld;
+  P.sb_k = a->sb_k;
   P.m = (int)a->m;
   P.n = (int)a->n;
   P.k = (int)a->k;
@@ -77,16 +92,15 @@ E2V2_API int e2v2_product8(const e2v2_product8_args* a, float* ws, int64_t ws_by
   P.sb_rows = a->b_tiles ? 128 : 1;
   P.out_type = a->out_type;
   P.fill = a->fill;
+  const bool staged = ((uintptr_t)a->a | (uintptr_t)a->b | (uintptr_t)a->lda | (uintptr_t)a->ldb |
+                       (uintptr_t)(grouped ? a->b_group : 0)) % 16 != 0;
   P.splits = grouped ? 1 : splits_of(a->m, a->n, a->k);
   E2V2_REQUIRE(P.splits == 1 || (ws && ws_bytes >= e2v2_product8_workspace(a->m, a->n, a->k)),
                "product8: workspace of %lld bytes", (long long)ws_bytes);
-  const bool staged = ((uintptr_t)a->a | (uintptr_t)a->b | (uintptr_t)a->lda | (uintptr_t)a->ldb |
-                       (uintptr_t)(grouped ? a->b_group : 0)) % 16 != 0;
-  const bool big = big_tiles(a->m, a->n, P.groups);
-  const int64_t tiles = (a->m / 128 + P.groups + 2) * ((a->n + 127) / 128);
+  const int64_t tiles = (a->m / 16 + P.groups) * ((a->n + 15) / 16);
   E2V2_REQUIRE(tiles < INT32_MAX / 2, "product8: %lld tiles", (long long)tiles);
-  if (grouped) staged ? run8<kRows, true>(P, big, s) : run8<kRows, false>(P, big, s);
-  else staged ? run8<kDense, true>(P, big, s) : run8<kDense, false>(P, big, s);
+  if (grouped) staged ? run8<kRows, true>(P, s) : run8<kRows, false>(P, s);
+  else staged ? run8<kDense, true>(P, s) : run8<kDense, false>(P, s);
   E2V2_LAUNCHED("k_mm");
   if (P.splits > 1) {
     launch_mm_sum(P, P.m, s);

@@ -148,5 +148,5 @@ def expert_gemm_fp8(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor
         return y
     xr, ldx = _row_operand("expert_gemm_fp8", x)
     w, ldw = _matrix(weight)
-    return _product(xr, ldx, x_scale.contiguous(), w, ldw, weight_scale.contiguous(), True, y, rows, n, k, offsets,
+    return _product(xr, ldx, x_scale, w, ldw, weight_scale, True, y, rows, n, k, offsets,
                     experts, w.stride(0), fill)

@@ -25,7 +25,7 @@ _ROWS, _TILES, _BOTH = 0, 1, 2              # E2V2_QUANT_*
 
 # e2v2_quantize8_args and e2v2_product8_args as bytes
 _QUANT_ARGS = struct.Struct("5Q6q3i4x")
-_PRODUCT_ARGS = struct.Struct("6Q7q4i")
+_PRODUCT_ARGS = struct.Struct("6Q12q4i")
 
 
 def _blocks(n: int) -> int:
@@ -136,8 +136,8 @@ def _product(a, lda, sa, b, ldb, sb, b_tiles, y, m, n, k, offsets=None, groups=0
     need = 0 if offsets is not None else _lib.load().e2v2_product8_workspace(m, n, k)
     ws = torch.empty(need // 4, dtype=torch.float32, device=y.device) if need else None
     args = _PRODUCT_ARGS.pack(a.data_ptr(), b.data_ptr(), sa.data_ptr(), sb.data_ptr(), y.data_ptr(), _address(offsets),
-                              m, n, k, lda, ldb, y.stride(-2) if y.dim() > 1 and y.shape[-2] > 1 else n, b_group,
-                              groups, b_tiles, _TYPES[y.dtype], fill)
+                              m, n, k, lda, ldb, y.stride(0) if m > 1 else n, b_group,
+                              *sa.stride(), *sb.stride()[-2:], sb.stride(0) if groups else 0, groups, b_tiles, _TYPES[y.dtype], fill)
     _call("e2v2_product8", y.device, args, _lib.vp(_address(ws)), _lib.i64(need))
     return y
 
@@ -167,7 +167,7 @@ def gemm(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch
     if y.numel() == 0:
         return y
     (ar, lda), (wr, ldw) = _row_operand("gemm", a), _row_operand("gemm", w)
-    return _product(ar, lda, a_scale.contiguous(), wr, ldw, w_scale.contiguous(), w_scale.shape == shapes[1],
+    return _product(ar, lda, a_scale.reshape(-1, a_scale.shape[-1]), wr, ldw, w_scale, w_scale.shape == shapes[1],
                     y.view(-1, n), y.numel() // n, n, k).view(y.shape)
 
 
