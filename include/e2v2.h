@@ -631,7 +631,7 @@ int e2v2_layer_norm_bwd2(const e2v2_layer_norm_args* args, void* gg, float* work
  * before a product in a generic network.  Rows as in e2v2_layer_norm_*; the weight may be NULL (1).
  *   fwd:  h = x + res rounded to the rows' type (res NULL: h is x and is not written), y = h rstd w, rstd [n] unless
  *         NULL.  h is contiguous.  With scales, y holds e4m3 codes, rows ldy bytes apart (a multiple of 16), and
- *         scales [n][ceil(width / 128)] a byte s for each 128 columns that stands for 2^(s - 127); rstd is not written.
+ *         scales [ceil(width / 128)][n] a byte s for each 128 columns that stands for 2^(s - 127); rstd is not written.
  *         Else y is contiguous and ldy is not read.
  *   bwd:  x holds the forward's h; gx from h, gy, rstd and gh (the gradient of h itself, or NULL), and unless gw is NULL
  *         the weight's gradient; the workspace holds one partial row of its sums per workgroup. */
@@ -653,15 +653,15 @@ int e2v2_rms_rows_bwd(const e2v2_rms_rows_args* args, void* gw, float* workspace
  * No counterpart in the reference.  e4m3 codes; each block has a scale byte s that stands for 2^(s - 127), the smallest
  * power of two (2^-126 at least) with which its largest finite value is at most 448.  What is not finite becomes NaN.
  *   quantize8  x [n][width] in fp32, bf16 or fp16, rows ldx elements apart.
- *     ROWS   codes [n][ldc], scales [n][ceil(width / 128)]: blocks of 1 x 128.
+ *     ROWS   codes [n][ldc], scales [ceil(width / 128)][n]: blocks of 1 x 128.
  *     TILES  blocks of 128 x 128: codes with scales [ceil(n / 128)][ceil(width / 128)] and the same codes transposed,
  *            codes_t [width][ldt] with scales_t [ceil(width / 128)][ceil(n / 128)]; either pair may be NULL.  `batch`
  *            matrices x_batch elements apart; their outputs follow one another.
- *     BOTH   ROWS, and the transpose of x quantised by rows: codes_t [width][ldt], scales_t [width][ceil(n / 128)]; either
+ *     BOTH   ROWS, and the transpose of x quantised by rows: codes_t [width][ldt], scales_t [ceil(n / 128)][width]; either
  *            pair may be NULL.
  *     Rows of codes lie a multiple of 16 bytes apart.
- *   values8    what codes stand for, contiguous, in the type; tiles: scales of 128 x 128 blocks of weights of
- *              rows_each rows. */
+ *   values8    what codes stand for, contiguous, in the type; a row's scales lie s_ld, a block's s_k bytes apart; tiles:
+ *              scales of 128 x 128 blocks of weights of rows_each rows. */
 #define E2V2_QUANT_ROWS 0
 #define E2V2_QUANT_TILES 1
 #define E2V2_QUANT_BOTH 2
@@ -672,8 +672,8 @@ typedef struct {
   int32_t batch, type, mode;
 } e2v2_quantize8_args;
 int e2v2_quantize8(const e2v2_quantize8_args* args, hipStream_t s);
-int e2v2_values8(const uint8_t* codes, int64_t ldc, const uint8_t* scales, int tiles, int64_t n, int64_t width,
-                 int64_t rows_each, void* out, int type, hipStream_t s);
+int e2v2_values8(const uint8_t* codes, int64_t ldc, const uint8_t* scales, int64_t s_ld, int64_t s_k, int tiles, int64_t n,
+                 int64_t width, int64_t rows_each, void* out, int type, hipStream_t s);
 
 /* ---- products of 8-bit operands with block scales ----
  * No counterpart in the reference.  y [m][n] = a b^T: a [m][k] and b [n][k] e4m3 codes, rows lda and ldb bytes apart, sa

@@ -143,8 +143,9 @@ def test_entry_points_check_on_the_host():
     refused(lib.e2v2_quantize8(ctypes.byref(q), None), b"mode 9")
     q.mode, q.codes_t, q.scales_t, q.ldt = 2, 16, 16, 3
     refused(lib.e2v2_quantize8(ctypes.byref(q), None), b"transposed")
-    refused(lib.e2v2_values8(ctypes.c_void_p(16), ctypes.c_int64(8), ctypes.c_void_p(16), 1, ctypes.c_int64(9),
-                             ctypes.c_int64(8), ctypes.c_int64(4), ctypes.c_void_p(16), 0, None), b"weights of 4")
+    refused(lib.e2v2_values8(ctypes.c_void_p(16), ctypes.c_int64(8), ctypes.c_void_p(16), ctypes.c_int64(1),
+                             ctypes.c_int64(1), 1, ctypes.c_int64(9), ctypes.c_int64(8), ctypes.c_int64(4),
+                             ctypes.c_void_p(16), 0, None), b"weights of 4")
 
     p = _lib.Product8Args()
     p.a = p.b = p.sa = p.sb = p.y = 16

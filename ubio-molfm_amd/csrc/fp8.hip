@@ -33,18 +33,8 @@ __device__ __forceinline__ void load8(const T* row, int c, int w, float (&v)[8])
   }
 }
 
-__device__ __forceinline__ uint32_t top8(const float (&v)[8]) {
-  uint32_t m = 0;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) m = max(m, finite_bits(v[e]));
-  return m;
-}
-
 __device__ __forceinline__ uint2 codes8(const float (&v)[8], float up) {
-  float t[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) t[e] = scaled8(v[e], up);
-  return make_uint2(codes4(t[0], t[1], t[2], t[3]), codes4(t[4], t[5], t[6], t[7]));
+  return make_uint2(codes4(v[0] * up, v[1] * up, v[2] * up, v[3] * up), codes4(v[4] * up, v[5] * up, v[6] * up, v[7] * up));
 }
 
 // 16 lanes a block of 128 columns.  Rows of codes lie a multiple of 16 bytes apart; their padding gets zeros.
@@ -57,9 +47,14 @@ __global__ __launch_bounds__(256) void k_quant_rows(QuantArgs P) {
     const int c = (int)b * kBlock8 + l * 8;
     float v[8];
     load8(static_cast<const T*>(P.x) + (int64_t)row * P.ldx, c, P.w, v);
-    const int s = scale_byte(lanes_max<16>(top8(v)));
+    const int s = scale_byte(top_bits([&](auto bits) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) m = max(m, bits(v[e]));
+      return lanes_max<16>(m);
+    }));
     if (c < P.ldc) *reinterpret_cast<uint2*>(P.codes + (int64_t)row * P.ldc + c) = codes8(v, scale_up(s));
-    if (l == 0) P.scales[(int64_t)row * nb + b] = (uint8_t)s;
+    if (l == 0) P.scales[(int64_t)b * P.n + row] = (uint8_t)s;
   }
 }
 
@@ -67,34 +62,28 @@ __global__ __launch_bounds__(256) void k_quant_rows(QuantArgs P) {
 // tile, codes and codes_t (either may be NULL) the same values; else codes with a scale for each row of the tile and
 // codes_t with one for each column.  The transpose goes through LDS: column j's 128 codes are one row there, its 8-byte
 // pieces moved round by j / 8, so that the 16 lanes that write pieces of 16 columns do not meet in one bank.
-template <typename T, bool kTile>
-__global__ __launch_bounds__(256) void k_quant_tiles(QuantArgs P) {
-  __shared__ uint32_t most[4][kBlock8];
-  __shared__ __attribute__((aligned(16))) uint8_t turned[kBlock8][kBlock8];
+// bits: of the values' magnitudes; all: the largest in the tile, or kInfBits where some are not finite.
+template <bool kTile, typename Bits>
+__device__ __forceinline__ void quant_tile(const QuantArgs& P, const float (&v)[8][8], uint32_t (*most)[kBlock8],
+                                           uint8_t (*turned)[kBlock8], Bits bits, uint32_t all) {
   const int l = threadIdx.x & 15, r = threadIdx.x >> 4, wv = threadIdx.x >> 6;
   const int r0 = blockIdx.y * kBlock8 + r * 8, c0 = blockIdx.x * kBlock8, c = c0 + l * 8;
   const int64_t z = blockIdx.z;
-  const T* x = static_cast<const T*>(P.x) + z * P.x_batch;
-  float v[8][8];
-#pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    if (r0 + k < P.n) {
-      load8(x + (int64_t)(r0 + k) * P.ldx, c, P.w, v[k]);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[k][e] = 0.f;
-    }
-  }
   float up[8];                                     // of the thread's rows, then of its columns
   const int nb = (P.w + kBlock8 - 1) / kBlock8, nbt = (P.n + kBlock8 - 1) / kBlock8;
   if constexpr (kTile) {
-    uint32_t m = 0;
+    if (all >= kInfBits) {
+      uint32_t m = 0;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) m = max(m, top8(v[k]));
-    m = lanes_max<64>(m);
-    if ((threadIdx.x & 63) == 0) most[wv][0] = m;
-    __syncthreads();
-    const int s = scale_byte(max(max(most[0][0], most[1][0]), max(most[2][0], most[3][0])));
+      for (int k = 0; k < 8; ++k)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) m = max(m, bits(v[k][e]));
+      m = lanes_max<64>(m);
+      if ((threadIdx.x & 63) == 0) most[wv][0] = m;
+      __syncthreads();
+      all = max(max(most[0][0], most[1][0]), max(most[2][0], most[3][0]));
+    }
+    const int s = scale_byte(all);
     if (threadIdx.x == 0) {
       if (P.scales) P.scales[z * P.s_batch + (int64_t)blockIdx.y * nb + blockIdx.x] = (uint8_t)s;
       if (P.scales_t) P.scales_t[z * P.st_batch + (int64_t)blockIdx.x * nbt + blockIdx.y] = (uint8_t)s;
@@ -104,9 +93,12 @@ __global__ __launch_bounds__(256) void k_quant_tiles(QuantArgs P) {
   } else {
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const int s = scale_byte(lanes_max<16>(top8(v[k])));
+      uint32_t m = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) m = max(m, bits(v[k][e]));
+      const int s = scale_byte(lanes_max<16>(m));
       up[k] = scale_up(s);
-      if (P.scales && l == 0 && r0 + k < P.n) P.scales[(int64_t)(r0 + k) * nb + blockIdx.x] = (uint8_t)s;
+      if (P.scales && l == 0 && r0 + k < P.n) P.scales[(int64_t)blockIdx.x * P.n + r0 + k] = (uint8_t)s;
     }
   }
   if (P.codes) {
@@ -121,7 +113,7 @@ __global__ __launch_bounds__(256) void k_quant_tiles(QuantArgs P) {
     for (int e = 0; e < 8; ++e) {
       uint32_t m = 0;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) m = max(m, finite_bits(v[k][e]));
+      for (int k = 0; k < 8; ++k) m = max(m, bits(v[k][e]));
       auto a = __builtin_amdgcn_permlane16_swap(m, m, false, false);
       m = max((uint32_t)a[0], (uint32_t)a[1]);
       a = __builtin_amdgcn_permlane32_swap(m, m, false, false);
@@ -134,7 +126,7 @@ __global__ __launch_bounds__(256) void k_quant_tiles(QuantArgs P) {
       const int j = l * 8 + e;
       const int s = scale_byte(max(max(most[0][j], most[1][j]), max(most[2][j], most[3][j])));
       up[e] = scale_up(s);
-      if (r == 0 && c + e < P.w) P.scales_t[(int64_t)(c + e) * nbt + blockIdx.y] = (uint8_t)s;
+      if (r == 0 && c + e < P.w) P.scales_t[(int64_t)blockIdx.y * P.w + c + e] = (uint8_t)s;
     }
   }
 #pragma unroll
@@ -154,9 +146,41 @@ __global__ __launch_bounds__(256) void k_quant_tiles(QuantArgs P) {
   }
 }
 
+template <typename T, bool kTile>
+__global__ __launch_bounds__(256) void k_quant_tiles(QuantArgs P) {
+  __shared__ uint32_t most[4][kBlock8];
+  __shared__ __attribute__((aligned(16))) uint8_t turned[kBlock8][kBlock8];
+  const int l = threadIdx.x & 15, r = threadIdx.x >> 4, wv = threadIdx.x >> 6;
+  const int r0 = blockIdx.y * kBlock8 + r * 8, c0 = blockIdx.x * kBlock8, c = c0 + l * 8;
+  const T* x = static_cast<const T*>(P.x) + blockIdx.z * P.x_batch;
+  float v[8][8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    if (r0 + k < P.n) {
+      load8(x + (int64_t)(r0 + k) * P.ldx, c, P.w, v[k]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[k][e] = 0.f;
+    }
+  }
+  // whether a value of the tile is not finite, and the function of those left that is taken
+  uint32_t all = 0;
+#pragma unroll
+  for (int k = 0; k < 8; ++k)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) all = max(all, abs_bits(v[k][e]));
+  all = lanes_max<64>(all);
+  if ((threadIdx.x & 63) == 0) most[wv][0] = all;
+  __syncthreads();
+  all = max(max(most[0][0], most[1][0]), max(most[2][0], most[3][0]));
+  __syncthreads();
+  if (all < kInfBits) quant_tile<kTile>(P, v, most, turned, [](float x) { return abs_bits(x); }, all);
+  else quant_tile<kTile>(P, v, most, turned, [](float x) { return finite_bits(x); }, kInfBits);
+}
+
 struct ValueArgs {
   const uint8_t* codes; const uint8_t* scales; void* out;
-  int64_t ldc;
+  int64_t ldc, s_ld, s_k;
   int n, w, block_rows, rows_each;     // rows_each: rows of one of several weights
   bool aligned;
 };
@@ -175,7 +199,7 @@ __global__ __launch_bounds__(256) void k_values8(ValueArgs P) {
       const unsigned each = (unsigned)P.rows_each, of = row / each;
       srow = of * ((each + kBlock8 - 1) / kBlock8) + (row - of * each) / kBlock8;
     }
-    const float s = scale_value(P.scales[(int64_t)srow * nb + b]);
+    const float s = scale_value(P.scales[(int64_t)srow * P.s_ld + (int64_t)b * P.s_k]);
     const uint8_t* q = P.codes + (int64_t)row * P.ldc + c;
     uint2 u = make_uint2(0, 0);
     if (P.aligned && c + 8 <= P.w) {
@@ -249,10 +273,10 @@ E2V2_API int e2v2_quantize8(const e2v2_quantize8_args* a, hipStream_t s) {
   return 0;
 }
 
-E2V2_API int e2v2_values8(const uint8_t* codes, int64_t ldc, const uint8_t* scales, int tiles, int64_t n, int64_t width,
-                          int64_t rows_each, void* out, int type, hipStream_t s) {
+E2V2_API int e2v2_values8(const uint8_t* codes, int64_t ldc, const uint8_t* scales, int64_t s_ld, int64_t s_k, int tiles,
+                          int64_t n, int64_t width, int64_t rows_each, void* out, int type, hipStream_t s) {
   E2V2_REQUIRE(type_ok(type), "values8: type %d", type);
-  E2V2_REQUIRE(n >= 0 && width >= 0 && width <= INT32_MAX && n <= INT32_MAX && ldc >= 0,
+  E2V2_REQUIRE(n >= 0 && width >= 0 && width <= INT32_MAX && n <= INT32_MAX && ldc >= 0 && s_ld >= 0 && s_k >= 0,
                "values8: %lld x %lld", (long long)n, (long long)width);
   if (n == 0 || width == 0) return 0;
   const int64_t nb = (width + kBlock8 - 1) / kBlock8;
@@ -260,7 +284,7 @@ E2V2_API int e2v2_values8(const uint8_t* codes, int64_t ldc, const uint8_t* scal
   E2V2_REQUIRE(!tiles || (rows_each > 0 && n % rows_each == 0), "values8: %lld rows of weights of %lld", (long long)n,
                (long long)rows_each);
   E2V2_REQUIRE(n * nb < INT32_MAX, "values8: %lld blocks", (long long)(n * nb));
-  const ValueArgs P{codes, scales, out, ldc, (int)n, (int)width, tiles ? kBlock8 : 1, (int)(tiles ? rows_each : n),
+  const ValueArgs P{codes, scales, out, ldc, s_ld, s_k, (int)n, (int)width, tiles ? kBlock8 : 1, (int)(tiles ? rows_each : n),
                     ldc % 8 == 0 && (uintptr_t)codes % 8 == 0};
   const dim3 grid(row_blocks(n * nb));
   if (type == E2V2_F32) hipLaunchKernelGGL(k_values8<float>, grid, dim3(256), 0, s, P);

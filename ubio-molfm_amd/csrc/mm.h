@@ -344,43 +344,47 @@ struct Frag {
 template <>
 struct Frag<kF32> {
   bf16x8 p[3];
+  // Pieces rounded by integer arithmetic (halves away from zero: the difference is exact either way), the last one exact;
+  // the conversion instruction runs at a quarter of the rate.
   __device__ __forceinline__ void take(const intx4 (&u)[2]) {
+    uint32_t w[3][4];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float x = __builtin_bit_cast(float, (int)u[e >> 2][e & 3]);
-      const __bf16 x0 = (__bf16)x;
-      const float r1 = x - (float)x0;
-      const __bf16 x1 = (__bf16)r1;
-      p[0][e] = x0;
-      p[1][e] = x1;
-      p[2][e] = (__bf16)(r1 - (float)x1);
+    for (int e = 0; e < 8; e += 2) {
+      uint32_t x[3][2];
+#pragma unroll
+      for (int d = 0; d < 2; ++d) {
+        const uint32_t v = (uint32_t)(int)u[(e + d) >> 2][(e + d) & 3];
+        x[0][d] = (v + 0x8000u) & 0xffff0000u;
+        const float r1 = __builtin_bit_cast(float, v) - __builtin_bit_cast(float, x[0][d]);
+        x[1][d] = (__builtin_bit_cast(uint32_t, r1) + 0x8000u) & 0xffff0000u;
+        x[2][d] = __builtin_bit_cast(uint32_t, r1 - __builtin_bit_cast(float, x[1][d]));
+      }
+#pragma unroll
+      for (int k = 0; k < 3; ++k) w[k][e >> 1] = __builtin_amdgcn_perm(x[k][1], x[k][0], 0x07060302u);   // the upper halves
     }
+#pragma unroll
+    for (int k = 0; k < 3; ++k) p[k] = __builtin_bit_cast(bf16x8, intx4{(int)w[k][0], (int)w[k][1], (int)w[k][2], (int)w[k][3]});
   }
 };
 
+// The matrix instructions of a product of fragments, one after another on the same accumulator: part q of kParts.
+template <int kT>
+constexpr int kParts = kT == kE4m3 ? 1 : kT == kF32 ? 6 : 2;
 // sb, sa: four scale bytes each, of which kSB and kSA are the fragments'.
-template <int kT, int kSB, int kSA>
+template <int kT, int kSB, int kSA, int q>
 __device__ __forceinline__ floatx4 multiply(const Frag<kT>& b, const Frag<kT>& a, floatx4 c, int sb, int sa) {
   if constexpr (kT == kE4m3) {
     const intx8 x = __builtin_shufflevector(b.v[0], b.v[1], 0, 1, 2, 3, 4, 5, 6, 7);
     const intx8 y = __builtin_shufflevector(a.v[0], a.v[1], 0, 1, 2, 3, 4, 5, 6, 7);
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, c, 0, 0, kSB, sb, kSA, sa);
   } else if constexpr (kT == kF32) {
-    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b.p[2], a.p[0], c, 0, 0, 0);
-    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b.p[1], a.p[1], c, 0, 0, 0);
-    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b.p[0], a.p[2], c, 0, 0, 0);
-    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b.p[1], a.p[0], c, 0, 0, 0);
-    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b.p[0], a.p[1], c, 0, 0, 0);
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(b.p[0], a.p[0], c, 0, 0, 0);
+    constexpr int pb[6] = {2, 1, 0, 1, 0, 0}, pa[6] = {0, 1, 2, 0, 1, 0};      // the smallest first
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(b.p[pb[q]], a.p[pa[q]], c, 0, 0, 0);
   } else if constexpr (kT == kBf16) {
-    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, b.v[0]), __builtin_bit_cast(bf16x8, a.v[0]), c,
-                                                0, 0, 0);
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, b.v[1]), __builtin_bit_cast(bf16x8, a.v[1]),
-                                                   c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, b.v[q]), __builtin_bit_cast(bf16x8, a.v[q]), c,
+                                                   0, 0, 0);
   } else {
-    c = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, b.v[0]), __builtin_bit_cast(f16x8, a.v[0]), c,
-                                               0, 0, 0);
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, b.v[1]), __builtin_bit_cast(f16x8, a.v[1]), c,
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, b.v[q]), __builtin_bit_cast(f16x8, a.v[q]), c,
                                                   0, 0, 0);
   }
 }
@@ -712,7 +716,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_mm(MmArgs) {
   // stores of 16 bytes at least besides, which need not have ended in the first step and at the next one's beginning
   constexpr int kWhole = kStaged ? 0 : kSend1 + kSend2, kMid = kStaged ? 0 : kHalves ? kWhole : kSend1;
   constexpr int kStores = kStaged ? 0 : FM * FN / 2;
-  constexpr int kPer1 = (kSend1 + FN - 1) / FN, kPer2 = (kSend2 + FN - 1) / FN;      // loads behind each of b's fragments
+  constexpr int kPer1 = (kSend1 + 1) / 2, kPer2 = (kSend2 + 1) / 2;      // loads behind each two of b's fragments
   int c = 0;                                       // steps done, of all tiles
   bool stored = false;
   while (true) {
@@ -721,15 +725,26 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_mm(MmArgs) {
     for (int f = 0; f < FM; ++f)
 #pragma unroll
       for (int h = 0; h < FN; ++h) acc[f][h] = floatx4{0.f, 0.f, 0.f, 0.f};
+    // A half of a with two fragments of b: the chains of each accumulator's instructions side by side.
+    auto products = [&](auto half, auto n) {
+      each<kParts<kT>>([&](auto q) {
+        each<2>([&](auto h) {
+          each<FH>([&](auto f) {
+            constexpr int b = 2 * n + h, at = half * FH + f;
+            acc[at][b] = multiply<kT, b, f, q>(fb[b], fa[half][f], acc[at][b], sb, sa[half]);
+          });
+        });
+      });
+    };
     for (int t = 0; t < now.steps; ++t, ++c) {
       prepare();
       if (stored && t < 2) meet(std::integral_constant<int, kWhole + kStores>{});
       else meet(std::integral_constant<int, kWhole>{});
       read_a(c, 1);
-      each<FN>([&](auto h) {
-        each<FH>([&](auto f) { acc[f][h] = multiply<kT, h, f>(fb[h], fa[0][f], acc[f][h], sb, sa[0]); });
+      each<2>([&](auto n) {
+        products(std::integral_constant<int, 0>{}, n);
         __builtin_amdgcn_sched_barrier(0);
-        each<kPer1>([&](auto p) { send1(std::integral_constant<int, h * kPer1 + p>{}); });
+        each<kPer1>([&](auto p) { send1(std::integral_constant<int, n * kPer1 + p>{}); });
       });
       // the products stay in front of the barrier: the compiler moved them behind the branch there
 #pragma unroll
@@ -743,13 +758,12 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_mm(MmArgs) {
       clear(in ? t + 1 : 0, in ? now.tail : then.tail, in ? now.length : then.length, c + 1);
       read_a(c + 1, 0);                            // behind the last step: what lies there is not used
       const int next_sb = read_sb(c + 1);
-      each<FN>([&](auto h) {
-        each<FH>([&](auto f) {
-          acc[FH + f][h] = multiply<kT, h, f>(fb[h], fa[1][f], acc[FH + f][h], sb, sa[1]);
-        });
-        __builtin_amdgcn_sched_barrier(0);         // the fragment's registers are free here, and taken at once
-        read_b(c + 1, h);
-        each<kPer2>([&](auto p) { send2(std::integral_constant<int, h * kPer2 + p>{}); });
+      each<2>([&](auto n) {
+        products(std::integral_constant<int, 1>{}, n);
+        __builtin_amdgcn_sched_barrier(0);         // the fragments' registers are free here, and taken at once
+        read_b(c + 1, 2 * n);
+        read_b(c + 1, 2 * n + 1);
+        each<kPer2>([&](auto p) { send2(std::integral_constant<int, n * kPer2 + p>{}); });
       });
       sb = next_sb;
       ++ft, ++fc;
@@ -869,7 +883,7 @@ __global__ __launch_bounds__(64 * kThinWaves, 4) void k_thin(MmArgs) {
           if (tail) clear(ua[u][f]);
           Frag<kT> fa;
           fa.take(ua[u][f]);
-          acc[f] = multiply<kT, 0, 0>(fb, fa, acc[f], sb[u], k8 ? sa[u][f] : 0);
+          each<kParts<kT>>([&](auto q) { acc[f] = multiply<kT, 0, 0, q>(fb, fa, acc[f], sb[u], k8 ? sa[u][f] : 0); });
         }
       }
     }

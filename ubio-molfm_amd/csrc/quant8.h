@@ -11,10 +11,22 @@ namespace e2v2 {
 
 constexpr int kBlock8 = 128;                 // values that share a scale
 
-// The bits of |v| where it is finite, else 0: compared as integers they order as the values do.
+// The bits of |v|: compared as integers they order as the values do, what is not finite from kInfBits on.
+constexpr uint32_t kInfBits = 0x7f800000u;
+__device__ __forceinline__ uint32_t abs_bits(float v) { return __builtin_bit_cast(uint32_t, v) & 0x7fffffffu; }
+// The same where v is finite, else 0.
 __device__ __forceinline__ uint32_t finite_bits(float v) {
-  const uint32_t u = __builtin_bit_cast(uint32_t, v) & 0x7fffffffu;
-  return u < 0x7f800000u ? u : 0u;
+  const uint32_t u = abs_bits(v);
+  return u < kInfBits ? u : 0u;
+}
+// f(bits), f being the largest of these bits over some of the wavefront's values, in every lane that shares it: over all
+// values first, and where that finds one that is not finite once more without those (a test of each cost as much as the
+// rest of quantising it).
+template <typename F>
+__device__ __forceinline__ uint32_t top_bits(F&& f) {
+  const uint32_t m = f([](float v) { return abs_bits(v); });
+  if (!__any(m >= kInfBits)) return m;
+  return f([](float v) { return finite_bits(v); });
 }
 // The scale byte of a block whose largest finite value has these bits: 1 to 247.
 __device__ __forceinline__ int scale_byte(uint32_t top) { return max((int)((top + 0x1fffffu) >> 23) - 8, 1); }
@@ -24,10 +36,8 @@ __device__ __forceinline__ float scale_up(int s) { return __builtin_bit_cast(flo
 __device__ __forceinline__ float scale_value(int s) {
   return __builtin_bit_cast(float, s == 0 ? 0x00400000 : s == 255 ? 0x7fc00000 : s << 23);
 }
-// v scaled for conversion; NaN where v is not finite.
-__device__ __forceinline__ float scaled8(float v, float up) { return finite_bits(v) || v == 0.f ? v * up : __builtin_nanf(""); }
 
-// Four codes in a dword.
+// Four codes in a dword; the conversion makes NaN of what is not finite.
 __device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
   int r = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true);

@@ -49,34 +49,39 @@ __device__ __forceinline__ void block_max(uint32_t (&m)[NV]) {
   }
 }
 
-// A row's codes and scale bytes: whole vectors, into the row's padding too (rows of codes lie a multiple of 16 bytes
-// apart, the padding holds zeros).
+// A row's codes and scale bytes (row `at` of a table of n rows, the rows' bytes of a block side by side): whole vectors,
+// into the row's padding too (rows of codes lie a multiple of 16 bytes apart, the padding holds zeros).
 template <int V, int kL, int NV>
 __device__ __forceinline__ void store_codes(const float (&y)[NV * V], int l, int w, uint8_t* row, int64_t ld,
-                                            uint8_t* scales) {
+                                            uint8_t* scales, int64_t at, int64_t n) {
   uint32_t m[NV];
+  auto largest = [&](auto bits) {
+    uint32_t all = 0;
 #pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    m[k] = 0;
+    for (int k = 0; k < NV; ++k) {
+      m[k] = 0;
 #pragma unroll
-    for (int e = 0; e < V; ++e) m[k] = max(m[k], finite_bits(y[k * V + e]));
-  }
+      for (int e = 0; e < V; ++e) m[k] = max(m[k], bits(y[k * V + e]));
+      all = max(all, m[k]);
+    }
+    return all;
+  };
+  top_bits(largest);
   block_max<V, kL, NV>(m);
   each_vec<V, kL, NV>(l, [&](int k, int c) {
     const int s = scale_byte(m[k]);
     const float up = scale_up(s);
     if constexpr (V == 1) {
-      if (c < w) row[c] = (uint8_t)codes4(scaled8(y[k], up), 0.f, 0.f, 0.f);
+      if (c < w) row[c] = (uint8_t)codes4(y[k] * up, 0.f, 0.f, 0.f);
     } else if (c < ld) {
       uint32_t q[V / 4];
 #pragma unroll
       for (int e = 0; e < V; e += 4)
-        q[e / 4] = codes4(scaled8(y[k * V + e], up), scaled8(y[k * V + e + 1], up), scaled8(y[k * V + e + 2], up),
-                          scaled8(y[k * V + e + 3], up));
+        q[e / 4] = codes4(y[k * V + e] * up, y[k * V + e + 1] * up, y[k * V + e + 2] * up, y[k * V + e + 3] * up);
       if constexpr (V == 4) *reinterpret_cast<uint32_t*>(row + c) = q[0];
       else *reinterpret_cast<uint2*>(row + c) = make_uint2(q[0], q[1]);
     }
-    if (c % kBlock8 == 0 && c < w) scales[c / kBlock8] = (uint8_t)s;
+    if (c % kBlock8 == 0 && c < w) scales[c / kBlock8 * n + at] = (uint8_t)s;
   });
 }
 
@@ -109,8 +114,7 @@ __global__ __launch_bounds__(kL > 64 ? kL : 256) void k_rms_fwd(RmsArgs P) {
 #pragma unroll
     for (int e = 0; e < E; ++e) h[e] = h[e] * r * g[e];
     if constexpr (kOut8) {
-      store_codes<V, kL, NV>(h, l, w, static_cast<uint8_t*>(P.y) + row * P.ldy, P.ldy,
-                             P.scales + row * ((w + kBlock8 - 1) / kBlock8));
+      store_codes<V, kL, NV>(h, l, w, static_cast<uint8_t*>(P.y) + row * P.ldy, P.ldy, P.scales, row, P.n);
     } else {
       T* yr = static_cast<T*>(P.y) + row * w;
       each_vec<V, kL, NV>(l, w, [&](int k, int c, auto whole) { store_row<T, V>(h + k * V, yr, c, w, whole); });

@@ -67,7 +67,7 @@ def _quantize(x, ldx, mode, codes=None, scales=None, codes_t=None, scales_t=None
 def quantize(x: torch.Tensor, tiles: bool = False):
     """(codes, scales) of x in fp32, bf16 or fp16.
 
-    tiles=False: x [..., w], codes of x's shape, scales [..., ceil(w / 128)].  tiles=True: weights [n, k] or
+    tiles=False: x [..., w], codes of x's shape, scales [..., ceil(w / 128)] (a view: a block's lie side by side).  tiles=True: weights [n, k] or
     [experts, n, k], scales [(experts,) ceil(n / 128), ceil(k / 128)].  Rows of codes lie a multiple of 16 bytes apart, so
     codes are a view where the width is not one.  No gradients."""
     _on_gpu("quantize", x)
@@ -80,8 +80,8 @@ def quantize(x: torch.Tensor, tiles: bool = False):
         xr, ldx = _rows(x)
         lead = x.shape[:-1]
         codes = torch.empty((*lead, _pitch(w)), dtype=CODES, device=x.device)
-        scales = torch.empty((*lead, _blocks(w)), dtype=torch.uint8, device=x.device)
-        _quantize(xr, ldx, _ROWS, codes, scales, n=x.numel() // w)
+        scales, held = _block_major(lead, x.numel() // w, _blocks(w), x.device)
+        _quantize(xr, ldx, _ROWS, codes, held, n=x.numel() // w)
     else:
         if x.dim() not in (2, 3):
             raise ValueError(f"quantize: weights [n, k] or [experts, n, k], got {tuple(x.shape)}")
@@ -124,11 +124,37 @@ def dequantize(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = t
         return out
     w = codes.shape[-1]
     tiles = scales.shape != shapes[0]
-    (cr, ldc), sr = _rows(codes), scales.contiguous()
-    _call("e2v2_values8", dev, _lib.vp(cr.data_ptr()), _lib.i64(ldc), _lib.vp(sr.data_ptr()),
-          _lib.i32(tiles), _lib.i64(codes.numel() // w), _lib.i64(w), _lib.i64(codes.shape[-2] if tiles else 0),
+    cr, ldc = _rows(codes)
+    sr, s_ld = _scale_rows(scales)
+    _call("e2v2_values8", dev, _lib.vp(cr.data_ptr()), _lib.i64(ldc), _lib.vp(sr.data_ptr()), _lib.i64(s_ld),
+          _lib.i64(sr.stride(-1)), _lib.i32(tiles), _lib.i64(codes.numel() // w), _lib.i64(w), _lib.i64(codes.shape[-2] if tiles else 0),
           _lib.vp(out.data_ptr()), _lib.i32(_TYPES[dtype]))
     return out
+
+
+def _scale_rows(scales):
+    """(scales as the kernels read them, bytes from row to row): rows one stride apart; a copy where they do not lie so."""
+    if scales.dim() < 2:
+        return scales, 0
+    ld = scales.stride(-2) if scales.shape[-2] > 1 else 0
+    if scales.dim() > 2:
+        span = None
+        for size, stride in zip(reversed(scales.shape[:-1]), reversed(scales.stride()[:-1])):
+            if size > 1:
+                if span is None:
+                    ld = stride
+                elif stride != span:
+                    scales = scales.contiguous()
+                    return scales, scales.shape[-1]
+                span = size * stride
+    return scales, ld
+
+
+def _block_major(lead, rows: int, blocks: int, dev):
+    """Scales [*lead, blocks] of rows that lie side by side block by block (so a tile's are read together), and the tensor
+    that the kernels write."""
+    held = torch.empty((blocks, rows), dtype=torch.uint8, device=dev)
+    return held.t().view(*lead, blocks) if len(lead) != 1 else held.t(), held
 
 
 def _product(a, lda, sa, b, ldb, sb, b_tiles, y, m, n, k, offsets=None, groups=0, b_group=0, fill=False):
@@ -163,12 +189,13 @@ def gemm(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch
     _check_codes("gemm", "a", a, a_scale, _scale_shapes(a)[:1])
     _check_codes("gemm", "w", w, w_scale, shapes)
     n, k = w.shape
+    m = a.numel() // k
     y = torch.empty((*a.shape[:-1], n), dtype=dtype, device=dev)
-    if y.numel() == 0:
+    if m == 0:
         return y
     (ar, lda), (wr, ldw) = _row_operand("gemm", a), _row_operand("gemm", w)
-    return _product(ar, lda, a_scale.reshape(-1, a_scale.shape[-1]), wr, ldw, w_scale, w_scale.shape == shapes[1],
-                    y.view(-1, n), y.numel() // n, n, k).view(y.shape)
+    return _product(ar, lda, a_scale.reshape(m, a_scale.shape[-1]), wr, ldw, w_scale, w_scale.shape == shapes[1],
+                    y.view(m, n), m, n, k).view(y.shape)
 
 
 class _LinearFn(torch.autograd.Function):
@@ -194,11 +221,11 @@ class _LinearFn(torch.autograd.Function):
             ctx.save_for_backward(wt, wst, None, None)
             return y
         xq, _ = _matrix_codes(m, k, dev)
-        xs = torch.empty((m, kb), dtype=torch.uint8, device=dev)
+        xs = torch.empty((kb, m), dtype=torch.uint8, device=dev)
         if need_w:
-            xt, xst = _matrix_codes(k, m, dev)[0], torch.empty((k, _blocks(m)), dtype=torch.uint8, device=dev)
+            xt, xst = _matrix_codes(k, m, dev)[0], torch.empty((_blocks(m), k), dtype=torch.uint8, device=dev)
         _quantize(xr, ldx, _BOTH if need_w else _ROWS, xq, xs, xt, xst, n=m)
-        _product(xq, xq.shape[1], xs, wq, wq.shape[1], ws, True, y.view(m, n), m, n, k)
+        _product(xq, xq.shape[1], xs.t(), wq, wq.shape[1], ws, True, y.view(m, n), m, n, k)
         ctx.save_for_backward(wt, wst, xt, xst)
         return y
 
@@ -215,16 +242,16 @@ class _LinearFn(torch.autograd.Function):
         gr, ldg = _rows(gy)
         gq = gs = gt = gst = None
         if need_x:
-            gq, gs = _matrix_codes(m, n, dev)[0], torch.empty((m, _blocks(n)), dtype=torch.uint8, device=dev)
+            gq, gs = _matrix_codes(m, n, dev)[0], torch.empty((_blocks(n), m), dtype=torch.uint8, device=dev)
         if need_w:
-            gt, gst = _matrix_codes(n, m, dev)[0], torch.empty((n, _blocks(m)), dtype=torch.uint8, device=dev)
+            gt, gst = _matrix_codes(n, m, dev)[0], torch.empty((_blocks(m), n), dtype=torch.uint8, device=dev)
         _quantize(gr, ldg, _BOTH if need_w else _ROWS, gq, gs, gt, gst, n=m)
         if need_x:
-            _product(gq, gq.shape[1], gs, wt, wt.shape[1], wst, True, gx.view(m, k), m, k, n)
+            _product(gq, gq.shape[1], gs.t(), wt, wt.shape[1], wst, True, gx.view(m, k), m, k, n)
         gw = None
         if need_w:
             gw = torch.empty((n, k), dtype=w_type, device=dev)
-            _product(gt, gt.shape[1], gst, xt, xt.shape[1], xst, False, gw, n, k, m)
+            _product(gt, gt.shape[1], gst.t(), xt, xt.shape[1], xst.t(), False, gw, n, k, m)
         return gx, gw
 
 

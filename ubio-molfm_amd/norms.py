@@ -404,12 +404,13 @@ def rms_norm_fp8(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: fl
     (xr, ldx), (rr, ldr) = _rows(x), (None, 0) if residual is None else _rows(residual)
     lead = x.shape[:-1]
     codes = torch.empty((*lead, pitch), dtype=torch.float8_e4m3fn, device=x.device)
-    scales = torch.empty((*lead, blocks), dtype=torch.uint8, device=x.device)
+    held = torch.empty((blocks, n), dtype=torch.uint8, device=x.device)      # a block's scales side by side
     h = x if residual is None else _empty_rows(x)
     a = _RMS_ARGS.pack(xr.data_ptr(), _address(rr), _address(weight), 0 if residual is None else h.data_ptr(),
-                       codes.data_ptr(), scales.data_ptr(), 0, 0, 0, 0, n, ldx, ldr, 0, 0, pitch, w, _TYPES[x.dtype],
+                       codes.data_ptr(), held.data_ptr(), 0, 0, 0, 0, n, ldx, ldr, 0, 0, pitch, w, _TYPES[x.dtype],
                        0 if weight is None else _TYPES[weight.dtype], float(eps))
     _call("e2v2_rms_rows_fwd", x.device, a)
     if pitch != w:
         codes = codes[..., :w]
+    scales = held.t() if len(lead) == 1 else held.t().view(*lead, blocks)
     return (codes, scales) if residual is None else (codes, scales, h)
