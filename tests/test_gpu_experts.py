@@ -131,6 +131,8 @@ def test_layouts(dtype, cuda):
         near(experts.expert_linear(x, wide(w, left), offs), want)
     assert torch.equal(experts.expert_linear(x.t().contiguous().t(), w, offs), want)
     assert torch.equal(experts.expert_linear(x, w.transpose(1, 2).contiguous().transpose(1, 2), offs), want)
+    row = x[:1].expand(x.shape[0], -1)
+    assert torch.equal(experts.expert_linear(row, w, offs), experts.expert_linear(row.contiguous(), w, offs))
     one = w[:1].expand(3, -1, -1)
     assert torch.equal(experts.expert_linear(x, one, offs), experts.expert_linear(x, one.contiguous(), offs))
     xg, wg = wide(x, 1).requires_grad_(True), wide(w, 3).requires_grad_(True)
@@ -163,7 +165,8 @@ def test_offsets_outside_the_rows_are_clamped(cuda):
         assert torch.equal(got, want)
 
 
-@pytest.mark.parametrize("sizes,spare,n,k", CASES + [([600, 0, 500, 701], 9, 2560, 512)])
+@pytest.mark.parametrize("sizes,spare,n,k", CASES + [([600, 0, 500, 701], 9, 2560, 512),
+                                                     ([1500, 0, 1300, 900, 1296], 40, 2560, 1000)])
 def test_8_bits(sizes, spare, n, k, cuda):
     x, w, gy, offs = _inputs(sizes, spare, n, k, F32, 8, cuda)
     (xq, sx), (wq, sw) = fp8.quantize(x), fp8.quantize(w, tiles=True)

@@ -179,6 +179,20 @@ def test_products_on_any_boundary(m, n, k, cuda):
     assert torch.equal(fp8.gemm(aq.view(1, m, k) if aq.is_contiguous() else aq[None], sa[None], wq, sw, dtype=F32)[0], want)
 
 
+def test_rows_that_share_bytes(cuda):
+    """A row repeated by expand() and overlapping windows are read where they are, not past their end."""
+    aq, sa, wq, sw = _product(cuda, 1, 40, 256, 3)
+    one = fp8.gemm(aq, sa, wq, sw, dtype=F32)
+    assert torch.equal(fp8.gemm(aq.expand(130, 256), sa.expand(130, 2), wq, sw, dtype=F32), one.expand(130, 40))
+    wide = _bits(_product(cuda, 1, 8, 1024, 4)[0]).view(-1)
+    windows = wide.as_strided((7, 256), (128, 1)).view(torch.float8_e4m3fn)
+    s7 = torch.full((7, 2), 127, dtype=torch.uint8, device=cuda)
+    assert torch.equal(fp8.gemm(windows, s7, wq, sw, dtype=F32), fp8.gemm(windows.contiguous(), s7, wq, sw, dtype=F32))
+    x = torch.randn(1, 64, device=cuda)
+    w = torch.randn(24, 64, device=cuda)
+    assert torch.equal(fp8.linear(x.expand(9, 64), w), fp8.linear(x, w).expand(9, 24))
+
+
 def test_products_keep_nan_to_their_row(cuda):
     aq, sa, wq, sw = _product(cuda, 40, 50, 300, 9)
     want = fp8.gemm(aq, sa, wq, sw, dtype=F32)

@@ -258,7 +258,7 @@ def set_timer(t):
 
 
 def _call_raw(name, *args):
-    lib = load()
+    lib = _lib or load()
     rc = getattr(lib, name)(*args)
     if rc != 0:
         msg = lib.e2v2_last_error().decode(errors="replace")

@@ -6,13 +6,14 @@ batch's result (one weight for each element, say) needs no wait and a captured g
 There is no CPU path."""
 from __future__ import annotations
 
+import functools
 import struct
 from typing import Optional
 
 import torch
 
 from . import _lib
-from .fp8 import MAX_PITCH, _blocks, _check_codes, _on_gpu, _product, _row_operand
+from .fp8 import MAX_PITCH, _has_tiles, _on_gpu, _product, _row_operand
 from .norms import _TYPES, _address, _call, _first_order, has_tangent
 
 _FORWARD, _ROWS, _WEIGHTS = 0, 1, 2         # E2V2_EXPERT_*
@@ -34,7 +35,14 @@ def _experts_of(name, offsets, experts, dev):
         got = (f"{tuple(offsets.shape)} {offsets.dtype} on {offsets.device}" if isinstance(offsets, torch.Tensor)
                else type(offsets).__name__)
         raise ValueError(f"{name}: offsets [{experts + 1}] int32 or int64 on {dev}, got {got}")
-    return offsets.to(torch.int32).contiguous()
+    if offsets.dtype is not torch.int32:
+        offsets = offsets.to(torch.int32)
+    return offsets if offsets.is_contiguous() else offsets.contiguous()
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(rows: int, n: int, k: int, experts: int) -> int:
+    return _lib.load().e2v2_expert_product_workspace(rows, n, k, experts)
 
 
 def _launch(which, x, w_shape, w, gy, y, offsets, fill):
@@ -48,7 +56,7 @@ def _launch(which, x, w_shape, w, gy, y, offsets, fill):
         w, ldw = _matrix(w)
         group = w.stride(0)
     rows = (gy if x is None else x).shape[0]
-    need = _lib.load().e2v2_expert_product_workspace(rows, n, k, experts) if which == _WEIGHTS else 0
+    need = _workspace_bytes(rows, n, k, experts) if which == _WEIGHTS else 0
     ws = torch.empty(need // 4, dtype=torch.float32, device=y.device) if need else None
     a = _ARGS.pack(_address(x), _address(w), _address(gy), y.data_ptr(), offsets.data_ptr(), rows, n, k, max(ldx, k),
                    max(ldw, k), max(ldgy, n), y.stride(-2) if y.shape[-2] > 1 else y.shape[-1], group, experts,
@@ -136,8 +144,8 @@ def expert_gemm_fp8(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor
         raise ValueError("expert_gemm_fp8: x [rows, k] and weight [experts, n, k], out in fp32, bf16 or fp16, got "
                          f"{tuple(x.shape)}, {tuple(weight.shape)} and {dtype}")
     (rows, k), (experts, n, _) = x.shape, weight.shape
-    _check_codes("expert_gemm_fp8", "x", x, x_scale, [torch.Size((rows, _blocks(k)))])
-    _check_codes("expert_gemm_fp8", "weight", weight, weight_scale, [torch.Size((experts, _blocks(n), _blocks(k)))])
+    _has_tiles("expert_gemm_fp8", "x", x, x_scale, tiles=False)
+    _has_tiles("expert_gemm_fp8", "weight", weight, weight_scale, rows=False)
     offsets = _experts_of("expert_gemm_fp8", offsets, experts, dev)
     if out is None:
         y, fill = torch.empty((rows, n), dtype=dtype, device=dev), True

@@ -10,6 +10,7 @@ scales themselves; they add the products of eight values on a grid of 2^-13 of t
 There is no CPU path."""
 from __future__ import annotations
 
+import functools
 import struct
 from typing import Optional
 
@@ -38,16 +39,16 @@ def _pitch(n: int) -> int:
 
 def _on_gpu(name: str, *tensors) -> torch.device:
     """The one GPU that all tensors are on."""
-    dev = None
+    index = None
     for t in tensors:
         if not isinstance(t, torch.Tensor) or not t.is_cuda:
             raise RuntimeError(f"{name} runs on the GPU only (HIP library, no CPU path): got "
                                f"{t.device if isinstance(t, torch.Tensor) else type(t).__name__}")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise ValueError(f"{name}: operands on {dev} and {t.device}")
-    return dev
+        if index is None:
+            index = t.get_device()
+        elif t.get_device() != index:
+            raise ValueError(f"{name}: operands on {tensors[0].device} and {t.device}")
+    return tensors[0].device
 
 
 def _matrix_codes(rows: int, width: int, dev):
@@ -95,20 +96,19 @@ def quantize(x: torch.Tensor, tiles: bool = False):
     return (codes if codes.shape[-1] == w else codes[..., :w]), scales
 
 
-def _check_codes(name, what, codes, scales, blocks):
-    """blocks: the shapes that the scales may have."""
-    if codes.dtype != CODES or scales.dtype != torch.uint8 or scales.shape not in blocks:
-        raise ValueError(f"{name}: {what} in e4m3 with uint8 scales {' or '.join(str(tuple(b)) for b in blocks)}, got "
-                         f"{tuple(codes.shape)} {codes.dtype} and {tuple(scales.shape)} {scales.dtype}")
-
-
-def _scale_shapes(codes):
-    """Scales by rows, and by tiles."""
-    lead, k = codes.shape[:-1], _blocks(codes.shape[-1])
-    shapes = [torch.Size((*lead, k))]
-    if codes.dim() >= 2:
-        shapes.append(torch.Size((*lead[:-1], _blocks(lead[-1]), k)))
-    return shapes
+def _has_tiles(name, what, codes, scales, rows=True, tiles=True) -> bool:
+    """Whether scales are those of tiles, not of rows; an error where they are of neither that may be."""
+    shape, got = tuple(codes.shape), tuple(scales.shape)
+    k = _blocks(shape[-1])
+    by_row, by_tile = (*shape[:-1], k), (*shape[:-2], _blocks(shape[-2]), k) if len(shape) > 1 else None
+    if codes.dtype is CODES and scales.dtype is torch.uint8:
+        if rows and got == by_row:
+            return False
+        if tiles and got == by_tile:
+            return True
+    raise ValueError(f"{name}: {what} in e4m3 with uint8 scales "
+                     f"{' or '.join(str(b) for b, may in ((by_row, rows), (by_tile, tiles)) if may and b)}, got "
+                     f"{shape} {codes.dtype} and {got} {scales.dtype}")
 
 
 def dequantize(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = torch.float32) -> torch.Tensor:
@@ -117,13 +117,11 @@ def dequantize(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = t
     dev = _on_gpu("dequantize", codes, scales)
     if dtype not in _TYPES or codes.dim() == 0:
         raise ValueError(f"dequantize: codes {tuple(codes.shape)}, values in fp32, bf16 or fp16, got {dtype}")
-    shapes = _scale_shapes(codes)
-    _check_codes("dequantize", "codes", codes, scales, shapes)
+    tiles = _has_tiles("dequantize", "codes", codes, scales)
     out = torch.empty(codes.shape, dtype=dtype, device=dev)
     if out.numel() == 0:
         return out
     w = codes.shape[-1]
-    tiles = scales.shape != shapes[0]
     cr, ldc = _rows(codes)
     sr, s_ld = _scale_rows(scales)
     _call("e2v2_values8", dev, _lib.vp(cr.data_ptr()), _lib.i64(ldc), _lib.vp(sr.data_ptr()), _lib.i64(s_ld),
@@ -157,9 +155,14 @@ def _block_major(lead, rows: int, blocks: int, dev):
     return held.t().view(*lead, blocks) if len(lead) != 1 else held.t(), held
 
 
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(m: int, n: int, k: int) -> int:
+    return _lib.load().e2v2_product8_workspace(m, n, k)
+
+
 def _product(a, lda, sa, b, ldb, sb, b_tiles, y, m, n, k, offsets=None, groups=0, b_group=0, fill=False):
     """y = a b^T by e2v2_product8; all operands are as the kernel reads them."""
-    need = 0 if offsets is not None else _lib.load().e2v2_product8_workspace(m, n, k)
+    need = 0 if offsets is not None else _workspace_bytes(m, n, k)
     ws = torch.empty(need // 4, dtype=torch.float32, device=y.device) if need else None
     args = _PRODUCT_ARGS.pack(a.data_ptr(), b.data_ptr(), sa.data_ptr(), sb.data_ptr(), y.data_ptr(), _address(offsets),
                               m, n, k, lda, ldb, y.stride(0) if m > 1 else n, b_group,
@@ -170,9 +173,12 @@ def _product(a, lda, sa, b, ldb, sb, b_tiles, y, m, n, k, offsets=None, groups=0
 
 def _row_operand(name, codes):
     rows, ld = _rows(codes)
+    w = codes.shape[-1]
+    if ld < w and codes.numel() > w:            # rows that share bytes
+        rows, ld = rows.contiguous(), w
     if ld > MAX_PITCH:
         raise ValueError(f"{name}: rows {ld} bytes apart (at most {MAX_PITCH})")
-    return rows, max(ld, codes.shape[-1])
+    return rows, max(ld, w)
 
 
 def gemm(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
@@ -185,48 +191,51 @@ def gemm(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch
     if a.dim() == 0 or w.dim() != 2 or w.shape[1] != a.shape[-1] or w.shape[1] == 0 or dtype not in _TYPES:
         raise ValueError(f"gemm: a [..., k] and w [n, k], out in fp32, bf16 or fp16; got {tuple(a.shape)}, "
                          f"{tuple(w.shape)} and {dtype}")
-    shapes = _scale_shapes(w)
-    _check_codes("gemm", "a", a, a_scale, _scale_shapes(a)[:1])
-    _check_codes("gemm", "w", w, w_scale, shapes)
+    _has_tiles("gemm", "a", a, a_scale, tiles=False)
+    tiles = _has_tiles("gemm", "w", w, w_scale)
     n, k = w.shape
     m = a.numel() // k
-    y = torch.empty((*a.shape[:-1], n), dtype=dtype, device=dev)
+    y = torch.empty((m, n), dtype=dtype, device=dev)
+    if m:
+        (ar, lda), (wr, ldw) = _row_operand("gemm", a), _row_operand("gemm", w)
+        _product(ar, lda, a_scale if a.dim() == 2 else a_scale.reshape(m, a_scale.shape[-1]), wr, ldw, w_scale, tiles,
+                 y, m, n, k)
+    return y if a.dim() == 2 else y.view(*a.shape[:-1], n)
+
+
+def _linear_forward(x, w, need_x: bool, need_w: bool):
+    """(y, and what the gradients of x and w read: the transposed codes and scales of w, and those of x)."""
+    n, k = w.shape
+    xr, ldx = _rows(x)
+    m, dev = x.numel() // k, x.device
+    if w.stride(1) != 1 and k > 1:
+        w = w.contiguous()
+    kb, nb = _blocks(k), _blocks(n)
+    y = torch.empty((*x.shape[:-1], n), dtype=x.dtype, device=dev)
+    wt = wst = xt = xst = None
     if m == 0:
-        return y
-    (ar, lda), (wr, ldw) = _row_operand("gemm", a), _row_operand("gemm", w)
-    return _product(ar, lda, a_scale.reshape(m, a_scale.shape[-1]), wr, ldw, w_scale, w_scale.shape == shapes[1],
-                    y.view(m, n), m, n, k).view(y.shape)
+        return y, wt, wst, xt, xst
+    wq, _ = _matrix_codes(n, k, dev)
+    ws = torch.empty((nb, kb), dtype=torch.uint8, device=dev)
+    if need_x:
+        wt, wst = _matrix_codes(k, n, dev)[0], torch.empty((kb, nb), dtype=torch.uint8, device=dev)
+    _quantize(w, w.stride(0), _TILES, wq, ws, wt, wst, n=n)
+    xq, _ = _matrix_codes(m, k, dev)
+    xs = torch.empty((kb, m), dtype=torch.uint8, device=dev)
+    if need_w:
+        xt, xst = _matrix_codes(k, m, dev)[0], torch.empty((_blocks(m), k), dtype=torch.uint8, device=dev)
+    _quantize(xr, ldx, _BOTH if need_w else _ROWS, xq, xs, xt, xst, n=m)
+    _product(xq, xq.shape[1], xs.t(), wq, wq.shape[1], ws, True, y.view(m, n), m, n, k)
+    return y, wt, wst, xt, xst
 
 
 class _LinearFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, w):
-        n, k = w.shape
-        xr, ldx = _rows(x)
-        m, dev = x.numel() // k, x.device
-        if w.stride(1) != 1 and k > 1:
-            w = w.contiguous()
-        need_x, need_w = ctx.needs_input_grad
-        kb, nb = _blocks(k), _blocks(n)
-        y = torch.empty((*x.shape[:-1], n), dtype=x.dtype, device=dev)
-        ctx.sizes, ctx.x_shape, ctx.types = (m, n, k), x.shape, (x.dtype, w.dtype)
-        wq, _ = _matrix_codes(n, k, dev)
-        ws = torch.empty((nb, kb), dtype=torch.uint8, device=dev)
-        wt = wst = xt = xst = None
-        if need_x:
-            wt, wst = _matrix_codes(k, n, dev)[0], torch.empty((kb, nb), dtype=torch.uint8, device=dev)
-        _quantize(w, w.stride(0), _TILES, wq, ws, wt, wst, n=n)
-        if m == 0:
-            ctx.save_for_backward(wt, wst, None, None)
-            return y
-        xq, _ = _matrix_codes(m, k, dev)
-        xs = torch.empty((kb, m), dtype=torch.uint8, device=dev)
-        if need_w:
-            xt, xst = _matrix_codes(k, m, dev)[0], torch.empty((_blocks(m), k), dtype=torch.uint8, device=dev)
-        _quantize(xr, ldx, _BOTH if need_w else _ROWS, xq, xs, xt, xst, n=m)
-        _product(xq, xq.shape[1], xs.t(), wq, wq.shape[1], ws, True, y.view(m, n), m, n, k)
-        ctx.save_for_backward(wt, wst, xt, xst)
+        y, *held = _linear_forward(x, w, *ctx.needs_input_grad)
+        ctx.sizes, ctx.x_shape, ctx.types = (x.numel() // w.shape[1], *w.shape), x.shape, (x.dtype, w.dtype)
+        ctx.save_for_backward(*held)
         return y
 
     @staticmethod
@@ -272,4 +281,6 @@ def linear(x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
         raise RuntimeError("linear: forward-mode tangents are not supported")
     if max(_pitch(weight.shape[0]), _pitch(weight.shape[1]), _pitch(x.numel() // weight.shape[1])) > MAX_PITCH:
         raise ValueError(f"linear: sizes up to {MAX_PITCH}, got {tuple(x.shape)} and {tuple(weight.shape)} on {dev}")
-    return _LinearFn.apply(x, weight)
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
+        return _LinearFn.apply(x, weight)
+    return _linear_forward(x, weight, False, False)[0]

@@ -94,8 +94,9 @@ def _workspace(x):
 
 
 def _call(name, dev, *args):
-    if torch.cuda.current_device() == dev.index:
-        return _lib.call(name, *args, _lib.stream(dev))
+    index = dev.index                           # a tensor lies there, so that the device is up: the short ways to ask
+    if torch._C._cuda_getDevice() == index:
+        return _lib.call(name, *args, _lib.vp(torch._C._cuda_getCurrentRawStream(index)))
     with torch.cuda.device(dev):
         _lib.call(name, *args, _lib.stream(dev))
 
