@@ -16,7 +16,7 @@ constexpr int64_t kMaxPitch = 1 << 22;       // bytes between rows: a tile's off
 // experts and tiles are few.
 int splits_of(int64_t rows, int64_t n, int64_t k, int groups) {
   const int64_t tiles = groups * ((n + 127) / 128) * ((k + 127) / 128);
-  if (tiles >= 192) return 1;
+  if (tiles >= (rows / groups >= 4096 ? 257 : 192)) return 1;
   return (int)std::max<int64_t>(1, std::min<int64_t>({512 / tiles, rows / groups / 256, 16}));
 }
 
@@ -26,13 +26,17 @@ void run(const MmArgs& P, hipStream_t s) {
     if constexpr (!kAO && !kBO) {
       if (thin_rows(P.m, P.n, (int64_t)P.k * elem_size(kT), P.groups)) return launch_thin<kT, 1, kGroup>(P, s);
     }
-    // tiles of 256 where they fill the 256 CUs, of 64 where not even those of 128 do
-    const int64_t m = kGroup == kRed ? P.m : P.m / P.groups;
+    // Tiles of 256 where they fill the 256 CUs and an expert has rows for several of them (32 experts of 512 rows, 1408 x
+    // 2048 bf16, forward and both gradients: 134, 133 and 137 us, with tiles of 128 131, 120 and 129; 16 of 2048 rows, 2048 x
+    // 2048: 280, 289 and 254, and 306, 301 and 295); of 64 where not even those of 128 fill them (8 experts of 62 rows,
+    // 512 x 1024 bf16: 11 us, 14).
+    const int64_t rows = kGroup == kRed ? P.k : P.m, each = rows / P.groups;
     auto tiles = [&](int64_t t) {
       return (kGroup == kRed ? P.groups * ((P.m + t - 1) / t) : P.m / t + std::min(P.groups, P.m)) * ((P.n + t - 1) / t);
     };
     if constexpr (kT != kF32) {
-      if (tiles(256) >= 200 && m >= 192) return launch_mm<kT, kAO, kBO, 256, 256, 2, 4, kGroup, false>(P, s);
+      if (tiles(256) >= 200 && each >= (P.groups > 1 ? 1024 : 192))
+        return launch_mm<kT, kAO, kBO, 256, 256, 2, 4, kGroup, false>(P, s);
     }
     if (tiles(128) * P.splits < 256) return launch_mm<kT, kAO, kBO, 64, 64, 2, 1, kGroup, false>(P, s);
   }

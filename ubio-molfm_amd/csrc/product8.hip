@@ -10,17 +10,20 @@ namespace {
 
 constexpr int64_t kMaxPitch = 1 << 22;       // bytes between rows: a tile's offsets stay below 2^30
 
-// The side of the tiles: 256 where they fill the 256 CUs, 64 where not even those of 128 do.
-int tile_side(int64_t m, int64_t n, int groups) {
+// The side of the tiles: 256 where they fill the 256 CUs (8192 x 8192 x 2048: 129 us, with tiles of 128 150) and, with
+// experts, where those have rows for several and k is not short (64 experts of 512 rows, 2048 x 1408: 160 and 144; 16 of
+// 2048 rows 134 and 121; 64 of 512 rows, 2048 x 4096: 350 and 358); 64 where not even those of 128 fill them (500 x 1000 x
+// 1000: 7.9, and 9.8 with tiles of 128).
+int tile_side(int64_t m, int64_t n, int64_t k, int groups) {
   auto tiles = [&](int64_t t) { return (m / t + (groups < m ? groups : m)) * ((n + t - 1) / t); };
-  if (tiles(256) >= 200 && m / groups >= 192) return 256;
+  if (tiles(256) >= 200 && (groups > 1 ? k >= 2048 && m / groups >= 1024 : m >= 192)) return 256;
   return tiles(128) >= 256 ? 128 : 64;
 }
 
 // Parts of k, where the tiles are few and k is long.
 int splits_of(int64_t m, int64_t n, int64_t k) {
   if (thin_rows(m, n, k, 1)) return 1;
-  const int64_t t = tile_side(m, n, 1) == 256 ? 256 : 128, tiles = ((m + t - 1) / t) * ((n + t - 1) / t);
+  const int64_t t = tile_side(m, n, k, 1) == 256 ? 256 : 128, tiles = ((m + t - 1) / t) * ((n + t - 1) / t);
   const int64_t steps = (k + 127) / 128;
   if (tiles >= 192 || steps < 16) return 1;
   return (int)std::max<int64_t>(1, std::min<int64_t>({512 / tiles, steps / 8, 16}));
@@ -28,7 +31,7 @@ int splits_of(int64_t m, int64_t n, int64_t k) {
 
 template <int kGroup, bool kStaged>
 void run8(const MmArgs& P, hipStream_t s) {
-  const int side = tile_side(P.m, P.n, P.groups);
+  const int side = tile_side(P.m, P.n, P.k, P.groups);
   if constexpr (!kStaged) {
     if (P.splits == 1 && thin_rows(P.m, P.n, P.k, P.groups)) return launch_thin<kE4m3, 1, kGroup>(P, s);
     if (side == 256) return launch_mm<kE4m3, false, false, 256, 256, 2, 4, kGroup, false>(P, s);
