@@ -105,6 +105,21 @@ def test_expert_refusals():
         experts.expert_linear(x, torch.nn.Parameter(w.as_subclass(torch.Tensor)).as_subclass(_OnGpu), offs, out=_gpu(5, 8))
 
 
+def test_out_may_not_share_elements_with_an_operand():
+    table = _gpu(12, 40)
+    w, offs = _gpu(2, 16, 16), _i32(0, 2, 5)
+    x = table[2:7, :16]
+    for out in (x, table[2:7, 8:24], table[4:9, :16], table[3:8, 15:31], table.reshape(-1)[30:110].view(5, 16),
+                w.reshape(-1)[100:180].view(5, 16), w[1, :5]):
+        with pytest.raises(ValueError, match="shares elements"):
+            experts.expert_linear(x, w, offs, out=out)
+    for out in (table[2:7, 16:32], table[2:7, 24:], table[:5, 16:32], table[4:9, 17:33], table[7:12, :16], _gpu(5, 16)):
+        assert not experts._overlap(out, x) and not experts._overlap(out, w)
+    one = table[3:4]
+    assert experts._overlap(one[:, :16], one[:, 15:31]) and not experts._overlap(one[:, :16], one[:, 16:32])
+    assert not experts._overlap(one[:0], one)
+
+
 def test_packed_arguments_are_the_structures():
     for c, s in ((_lib.RmsRowsArgs, norms._RMS_ARGS), (_lib.Quantize8Args, fp8._QUANT_ARGS),
                  (_lib.Product8Args, fp8._PRODUCT_ARGS), (_lib.ExpertArgs, experts._ARGS)):

@@ -3,6 +3,9 @@
 //   rows' gradient   gx[t] = W[e]^T gy[t]          W read along its columns
 //   weights' grad.   gW[e] = sum_t gy[t] x[t]^T    both operands read along their columns, over ragged rows
 // Rows of no expert give zeros.
+//
+// 16,384 rows over 32 experts of 1408 x 2048 bf16: 136, 129 and 208 us (95 GFLOP each; the weights' gradient writes 184 MB);
+// 10,000 rows over 6 of 256 x 256 fp32: 25, 25 and 40.
 #include <algorithm>
 
 #include "mm.h"
@@ -10,10 +13,8 @@
 namespace e2v2 {
 namespace {
 
-constexpr int64_t kMaxPitch = 1 << 22;       // bytes between rows: a tile's offsets stay below 2^30
-
 // The parts that the rows of each expert are cut into for the weights' gradient: enough workgroups for the 256 CUs where
-// experts and tiles are few.
+// experts and tiles are few (one expert of 16,384 rows, 1536 x 2048 bf16: 131 us, uncut 162).
 int splits_of(int64_t rows, int64_t n, int64_t k, int groups) {
   const int64_t tiles = groups * ((n + 127) / 128) * ((k + 127) / 128);
   if (tiles >= (rows / groups >= 4096 ? 257 : 192)) return 1;
@@ -24,7 +25,7 @@ template <int kT, bool kAO, bool kBO, int kGroup, bool kStaged>
 void run(const MmArgs& P, hipStream_t s) {
   if constexpr (!kStaged) {
     if constexpr (!kAO && !kBO) {
-      if (thin_rows(P.m, P.n, (int64_t)P.k * elem_size(kT), P.groups)) return launch_thin<kT, 1, kGroup>(P, s);
+      if (thin_rows(P.m, P.n, (int64_t)P.k * elem_size(kT), P.groups)) return launch_thin<kT, kGroup>(P, s);
     }
     // Tiles of 256 where they fill the 256 CUs and an expert has rows for several of them (32 experts of 512 rows, 1408 x
     // 2048 bf16, forward and both gradients: 134, 133 and 137 us, with tiles of 128 131, 120 and 129; 16 of 2048 rows, 2048 x

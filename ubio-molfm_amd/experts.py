@@ -99,11 +99,13 @@ def expert_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor,
     """y[t] = weight[e] x[t] for the rows t = offsets[e] .. offsets[e + 1] - 1 of each expert e.
 
     x [rows, k] and weight [experts, n, k] in one of fp32, bf16 and fp16; offsets [experts + 1], int32 or int64 on the GPU,
-    not decreasing, an expert without rows where two are equal (what lies outside 0 .. rows is clamped, never read).  Rows of
-    no expert give zeros and take no part in gradients.  Sums are fp32 (fp32 operands are split exactly into bf16 pieces, as
-    in ``gemm``: a product with an infinite operand is NaN there).  Differentiable once in reverse mode, in x and weight.
+    not decreasing, an expert without rows where two are equal (what lies outside 0 .. rows is clamped; int64 ones are read
+    as int32).  Rows of no expert give zeros and take no part in gradients.  Sums are fp32 (fp32 operands are split exactly
+    into bf16 pieces, as in ``gemm``: a product with an operand that bf16 rounds to infinity, from 3.3961e38 on, is NaN
+    there).  Differentiable once in reverse mode, in x and weight.
 
-    out [rows, n]: written instead of a new tensor, rows of no expert left as they were; for calls without gradients."""
+    out [rows, n]: written instead of a new tensor, rows of no expert left as they were; for calls without gradients.  It may
+    not share elements with the operands."""
     dev = _on_gpu("expert_linear", x, weight)
     if (x.dim() != 2 or weight.dim() != 3 or weight.shape[2] != x.shape[1] or weight.numel() == 0
             or x.dtype not in _TYPES or weight.dtype != x.dtype):
@@ -118,18 +120,38 @@ def expert_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor,
             return _ExpertLinearFn.apply(x, weight, offsets)
         y, fill = torch.empty((x.shape[0], weight.shape[1]), dtype=x.dtype, device=dev), True
     else:
-        _check_out("expert_linear", out, (x.shape[0], weight.shape[1]), x.dtype, dev, grads)
+        _check_out("expert_linear", out, (x.shape[0], weight.shape[1]), x.dtype, dev, grads, x, weight)
         y, fill = out, False
     return _launch(_FORWARD, x, weight.shape, weight, None, y, offsets, fill) if y.numel() else y
 
 
-def _check_out(name, out, shape, dtype, dev, grads):
+def _check_out(name, out, shape, dtype, dev, grads, *operands):
     if grads or (torch.is_grad_enabled() and out.requires_grad):
         raise RuntimeError(f"{name}: out= has no gradients: call it under torch.no_grad()")
     if (out.shape != shape or out.dtype != dtype or out.device != dev or (shape[1] > 1 and out.stride(1) != 1)
             or (shape[0] > 1 and out.stride(0) < shape[1])):
         raise ValueError(f"{name}: out {shape} {dtype} on {dev} with consecutive elements in a row, got "
                          f"{tuple(out.shape)} {out.dtype} on {out.device} with strides {out.stride()}")
+    if any(_overlap(out, t) for t in operands):
+        raise ValueError(f"{name}: out shares elements with an operand")
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether matrices with consecutive elements in a row may share elements: their bytes overlap, and they are not
+    columns side by side of one table."""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    (a0, a1), (b0, b1) = ((t.data_ptr(), t.data_ptr() + t.element_size()
+                           * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))) for t in (a, b))
+    if a1 <= b0 or b1 <= a0:
+        return False
+    pitch = a.stride(0) * a.element_size()
+    if (a.dim() != 2 or b.dim() != 2 or a.stride(1) != 1 or b.stride(1) != 1 or pitch == 0
+            or b.stride(0) * b.element_size() != pitch):
+        return True
+    (lo, wide), (hi, _) = sorted(((a0, a.shape[1] * a.element_size()), (b0, b.shape[1] * b.element_size())))
+    between = (hi - lo) % pitch                      # from the lower one's column to the other's, in the table's rows
+    return between < wide or between + (b if hi == b0 else a).shape[1] * a.element_size() > pitch
 
 
 def expert_gemm_fp8(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
@@ -150,7 +172,7 @@ def expert_gemm_fp8(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor
     if out is None:
         y, fill = torch.empty((rows, n), dtype=dtype, device=dev), True
     else:
-        _check_out("expert_gemm_fp8", out, (rows, n), dtype, dev, False)
+        _check_out("expert_gemm_fp8", out, (rows, n), dtype, dev, False, x, weight)
         y, fill = out, False
     if y.numel() == 0:
         return y

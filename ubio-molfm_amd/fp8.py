@@ -68,9 +68,9 @@ def _quantize(x, ldx, mode, codes=None, scales=None, codes_t=None, scales_t=None
 def quantize(x: torch.Tensor, tiles: bool = False):
     """(codes, scales) of x in fp32, bf16 or fp16.
 
-    tiles=False: x [..., w], codes of x's shape, scales [..., ceil(w / 128)] (a view: a block's lie side by side).  tiles=True: weights [n, k] or
-    [experts, n, k], scales [(experts,) ceil(n / 128), ceil(k / 128)].  Rows of codes lie a multiple of 16 bytes apart, so
-    codes are a view where the width is not one.  No gradients."""
+    tiles=False: x [..., w], codes of x's shape, scales [..., ceil(w / 128)] (a view: a block's lie side by side).
+    tiles=True: weights [n, k] or [experts, n, k], scales [(experts,) ceil(n / 128), ceil(k / 128)].  Rows of codes lie a
+    multiple of 16 bytes apart, so codes are a view where the width is not one.  No gradients."""
     _on_gpu("quantize", x)
     if x.dtype not in _TYPES or x.dim() == 0 or x.shape[-1] == 0:
         raise ValueError(f"quantize: fp32, bf16 or fp16 rows of at least one value, got {tuple(x.shape)} {x.dtype}")
@@ -125,8 +125,8 @@ def dequantize(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = t
     cr, ldc = _rows(codes)
     sr, s_ld = _scale_rows(scales)
     _call("e2v2_values8", dev, _lib.vp(cr.data_ptr()), _lib.i64(ldc), _lib.vp(sr.data_ptr()), _lib.i64(s_ld),
-          _lib.i64(sr.stride(-1)), _lib.i32(tiles), _lib.i64(codes.numel() // w), _lib.i64(w), _lib.i64(codes.shape[-2] if tiles else 0),
-          _lib.vp(out.data_ptr()), _lib.i32(_TYPES[dtype]))
+          _lib.i64(sr.stride(-1)), _lib.i32(tiles), _lib.i64(codes.numel() // w), _lib.i64(w),
+          _lib.i64(codes.shape[-2] if tiles else 0), _lib.vp(out.data_ptr()), _lib.i32(_TYPES[dtype]))
     return out
 
 
@@ -166,7 +166,8 @@ def _product(a, lda, sa, b, ldb, sb, b_tiles, y, m, n, k, offsets=None, groups=0
     ws = torch.empty(need // 4, dtype=torch.float32, device=y.device) if need else None
     args = _PRODUCT_ARGS.pack(a.data_ptr(), b.data_ptr(), sa.data_ptr(), sb.data_ptr(), y.data_ptr(), _address(offsets),
                               m, n, k, lda, ldb, y.stride(0) if m > 1 else n, b_group,
-                              *sa.stride(), *sb.stride()[-2:], sb.stride(0) if groups else 0, groups, b_tiles, _TYPES[y.dtype], fill)
+                              *sa.stride(), *sb.stride()[-2:], sb.stride(0) if groups else 0, groups, b_tiles,
+                              _TYPES[y.dtype], fill)
     _call("e2v2_product8", y.device, args, _lib.vp(_address(ws)), _lib.i64(need))
     return y
 

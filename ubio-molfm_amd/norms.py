@@ -1,8 +1,9 @@
 """Norms of rows as HIP kernels of libe2v2.so.
 
-Layer norm (the reference's nn.LayerNorm, module_utils.py:2151-2178, 2230-2233): any width up to 16384, fp32, bf16 or fp16 rows, weight and bias in the rows' type or fp32 or absent,
-with the gradients of rows, weight and bias and the derivative of that backward pass (force training differentiates
-the forces once more).  Statistics, row sums and the parameters' sums are fp32; each result is rounded once.
+Layer norm (the reference's nn.LayerNorm, module_utils.py:2151-2178, 2230-2233): any width up to 16384, fp32, bf16 or
+fp16 rows, weight and bias in the rows' type or fp32 or absent, with the gradients of rows, weight and bias and the
+derivative of that backward pass (force training differentiates the forces once more).  Statistics, row sums and the
+parameters' sums are fp32; each result is rounded once.
 
 RMS norm (no counterpart in the reference, whose RMS norm is the equivariant one): the same rows, the residual's addition
 before it in the same pass, its first gradients; or its output in 8 bits with block scales (``fp8``), for the product
