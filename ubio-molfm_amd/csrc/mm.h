@@ -560,8 +560,8 @@ __device__ __forceinline__ void fill_rows(Args& P) {
 // step, the rest in the second), between the products, and are waited for more than a step later.  Products stand on both
 // sides of the two barriers of a step.
 //
-// Bound: the matrix units' issue and the loads into LDS.  8192 x 8192 x 4096: e4m3 242 us (2.27 PFLOP/s, matrix units 49%
-// busy), bf16 422 forward, 417 rows' gradient, 438 weights' (1.26 to 1.32 PFLOP/s, 54 to 58%).  8192^3 bf16: a step's loads in
+// Bound: the matrix units' issue and the loads into LDS.  8192 x 8192 x 4096: e4m3 239 us (2.30 PFLOP/s, matrix units 49%
+// busy), bf16 417 forward, 411 rows' gradient, 424 weights' (1.30 to 1.34 PFLOP/s, 55 to 58%).  8192^3 bf16: a step's loads in
 // one clump behind one barrier 977 us, sent between the products with descriptors kept 856, and sent into each half of a tile
 // as soon as it is free 794.  A change of tiles costs 8 us, 6.7 of which its stores take at 5 TB/s.
 template <int kT, bool kAO, bool kBO, int BM, int BN, int WM, int WN, int kGroup, bool kStaged>
