@@ -165,6 +165,33 @@ def test_offsets_outside_the_rows_are_clamped(cuda):
         assert torch.equal(got, want)
 
 
+def test_offsets_past_32_bits(cuda):
+    """Weights of 6.4 GB, and 70,001 rows of 4.6 GB: what lies past 2^31 elements and bytes is read and written in its place."""
+    w = torch.zeros(3, 32768, 32768, dtype=BF16, device=cuda)
+    w[2, 32767, ::3] = 1.5
+    w[2, 3] = 0.25
+    x = torch.ones(300, 32768, dtype=BF16, device=cuda)
+    y = experts.expert_linear(x, w, torch.tensor([0, 1, 1, 300], dtype=torch.int32, device=cuda))
+    want = torch.zeros(300, 32768, dtype=BF16, device=cuda)
+    want[1:, 32767], want[1:, 3] = 16384.0, 8192.0   # 10,923 terms of 1.5 (16384.5, rounded) and 32,768 of 0.25
+    assert torch.equal(y, want)
+    del w, x, y, want
+    rows, k, n = 70_001, 32768, 16
+    x = torch.zeros(rows, k, dtype=BF16, device=cuda)
+    x[-1, -1] = 2.0
+    w = torch.zeros(2, n, k, dtype=BF16, device=cuda)
+    w[1, :, -1] = 3.0
+    offs = torch.tensor([0, 60_000, rows], dtype=torch.int32, device=cuda)
+    xg, wg = x.requires_grad_(True), w.requires_grad_(True)
+    gy = torch.zeros(rows, n, dtype=BF16, device=cuda)
+    gy[-1] = 0.5
+    y = experts.expert_linear(xg, wg, offs)
+    gx, gw = torch.autograd.grad(y, (xg, wg), gy)
+    assert (y[-1] == 6).all() and (y[:-1] == 0).all()
+    assert gx[-1, -1] == 1.5 * n and gx.count_nonzero() == 1
+    assert (gw[1, :, -1] == 1).all() and gw.count_nonzero() == n
+
+
 @pytest.mark.parametrize("sizes,spare,n,k", CASES + [([600, 0, 500, 701], 9, 2560, 512),
                                                      ([1500, 0, 1300, 900, 1296], 40, 2560, 1000)])
 def test_8_bits(sizes, spare, n, k, cuda):

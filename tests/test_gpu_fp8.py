@@ -14,6 +14,7 @@ from ubio_molfm_amd import fp8
 pytestmark = pytest.mark.gpu
 
 UT = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+F8 = torch.float8_e4m3fn
 F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
 
 
@@ -314,6 +315,29 @@ def test_offsets_past_32_bits(cuda):
     want[::100_003] = k
     want[-1] = 2 * k
     assert torch.equal(y, want[:, None].expand(m, n))
+
+
+def test_quantised_past_32_bits(cuda):
+    """140,000 x 16384 bf16 (4.6 GB): blocks past 2^31 elements, along rows, in tiles and along columns."""
+    n, w = 140_000, 16384
+    x = torch.zeros(n, w, dtype=BF16, device=cuda)
+    x[-1, -2:] = torch.tensor([3.0, -448.0], dtype=BF16)
+    codes, scales = fp8.quantize(x)
+    assert fp8.dequantize(codes[-1:], scales[-1:])[0, -2:].tolist() == [3.0, -448.0]
+    assert codes[:-1].view(torch.uint8).count_nonzero() == 0 and scales[-1, -1] == 127 and (scales[:-1] == 1).all()
+    back = fp8.dequantize(codes, scales, BF16)
+    assert torch.equal(back, x)
+    del codes, scales, back
+    codes, scales = fp8.quantize(x, tiles=True)
+    assert scales[-1, -1] == 127 and (scales.view(-1)[:-1] == 1).all()
+    assert torch.equal(fp8.dequantize(codes, scales, BF16), x)
+    del codes, scales
+    turned = torch.empty((w, n), dtype=F8, device=cuda)
+    by_column = torch.empty((-(-n // 128), w), dtype=torch.uint8, device=cuda)
+    codes, by_row = torch.empty((n, w), dtype=F8, device=cuda), torch.empty((w // 128, n), dtype=torch.uint8, device=cuda)
+    fp8._quantize(x, w, fp8._BOTH, codes, by_row, turned, by_column, n=n)
+    assert torch.equal(fp8.dequantize(codes, by_row.t(), BF16), x)
+    assert torch.equal(fp8.dequantize(turned, by_column.t(), BF16), x.t())
 
 
 def test_refused_derivatives(cuda):

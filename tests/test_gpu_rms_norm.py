@@ -119,6 +119,33 @@ def test_which_gradients(cuda):
     assert torch.equal(xg.grad, rg.grad) and xg.grad.data_ptr() != rg.grad.data_ptr()
 
 
+def test_a_tensor_is_its_own_residual(cuda):
+    x, _, wt, gy, gh = _inputs(40, 300, F32, F32, 4, cuda)
+    xg = x.clone().requires_grad_(True)
+    y, h = norms.rms_norm(xg, wt, EPS, residual=xg)
+    gx, = torch.autograd.grad((y, h), xg, (gy, gh))
+    _check(x, x, wt, gy, gh, y, h, gx / 2, None)     # halving is exact
+
+
+def test_offsets_past_32_bits(cuda):
+    """140,000 rows of 16384 bf16 (4.6 GB): the last ones have the values and gradients that they have alone."""
+    n, w = 140_000, 16384
+    x, res, wt, gy, gh = _inputs(3, w, BF16, BF16, 5, cuda)
+    big, up = torch.zeros(n, w, dtype=BF16, device=cuda), torch.zeros(n, w, dtype=BF16, device=cuda)
+    big[-3:], up[-3:] = x, gy
+    few = x.clone().requires_grad_(True)
+    want = norms.rms_norm(few, wt, EPS)
+    gx_want, = torch.autograd.grad(want, few, gy)
+    big.requires_grad_(True)
+    y = norms.rms_norm(big, wt, EPS)
+    gx, = torch.autograd.grad(y, big, up)
+    assert torch.equal(y[-3:], want) and torch.equal(gx[-3:], gx_want)
+    assert y[:-3].count_nonzero() == 0 and gx[:-3].count_nonzero() == 0
+    with torch.no_grad():
+        for a, b in zip(norms.rms_norm_fp8(big, wt, EPS), norms.rms_norm_fp8(few, wt, EPS)):
+            assert torch.equal(a[-3:].view(torch.uint8), b.view(torch.uint8))
+
+
 def test_against_differences(cuda):
     """The gradient in a direction against central differences of the definition in float64: their error is of the order of
     step^2 = 1e-8 of third derivatives of the order of 1."""

@@ -21,6 +21,6 @@ model.py       E2FormerBackbone / MolfmAtomic / energy head / forces
 calculator.py  E2FormerCalculator-style batched energy+forces entry point
 md.py          device-resident velocity-Verlet (NVE) loop
 optim.py       AdamW over many tensors at once (moments in 32 or 8 bits), gradient clipping
-systems.py     seeded synthetic workloads (BASELINE configs 1-5)
+systems.py     seeded synthetic workloads
 """
 __version__ = "0.1.0"
