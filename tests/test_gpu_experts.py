@@ -165,6 +165,21 @@ def test_offsets_outside_the_rows_are_clamped(cuda):
         assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("rows", [100, 3000])
+def test_offsets_that_decrease_stay_inside(rows, cuda):
+    """Rows that two experts claim hold the one's or the other's products; all others are right."""
+    a, b, c = rows // 5, rows // 2, rows
+    x, w, gy, _ = _inputs([a, b - a, c - b], 0, 256, 320, BF16, 8, cuda)
+    table = torch.full((rows + 64, 256), 7.0, dtype=BF16, device=cuda)
+    offs = torch.tensor([0, b, a, c], dtype=torch.int32, device=cuda)
+    y = experts.expert_linear(x, w, offs, out=table[32:-32])
+    first = experts.expert_linear(x, w, torch.tensor([0, b, b, b], dtype=torch.int32, device=cuda))
+    third = experts.expert_linear(x, w, torch.tensor([0, 0, a, c], dtype=torch.int32, device=cuda))
+    assert torch.equal(y[:a], first[:a]) and torch.equal(y[b:], third[b:])
+    assert ((y[a:b] == first[a:b]) | (y[a:b] == third[a:b])).all()
+    assert (table[:32] == 7).all() and (table[-32:] == 7).all()
+
+
 def test_offsets_past_32_bits(cuda):
     """Weights of 6.4 GB, and 70,001 rows of 4.6 GB: what lies past 2^31 elements and bytes is read and written in its place."""
     w = torch.zeros(3, 32768, 32768, dtype=BF16, device=cuda)
