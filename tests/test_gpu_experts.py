@@ -314,3 +314,22 @@ def test_feed_forward_of_experts(cuda):
     assert torch.equal(h8, h)
     # four operands rounded to 3 bits, 2^-4 / sqrt(3) rms each at most, on the branch alone
     assert float((out8.double() - outd).norm()) < 4 * 2.0 ** -4 / 3 ** 0.5 * float((outd - hd).norm())
+
+
+def test_out_counts_as_changed(cuda):
+    """A graph that saved out's old elements, also those of a view, raises instead of taking the new ones."""
+    x, w, gy, offs = _inputs([9, 0, 140], 8, 48, 64, BF16, 12, cuda)
+    codes, scales = fp8.quantize(x)
+    wq, ws = fp8.quantize(w, tiles=True)
+    buf = torch.zeros(x.shape[0], 60, dtype=BF16, device=cuda)
+    gain = torch.ones_like(buf, requires_grad=True)
+    for call in (lambda out: experts.expert_linear(x, w, offs, out=out),
+                 lambda out: experts.expert_gemm_fp8(codes, scales, wq, ws, offs, out=out)):
+        z = buf * gain
+        call(buf[:, 3:51])
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            z.sum().backward()
+        torch.autograd.grad((buf * gain).sum(), gain)
+    with torch.inference_mode():
+        out = torch.empty(x.shape[0], 48, dtype=BF16, device=cuda)
+        assert torch.equal(experts.expert_linear(x, w, offs, out=out)[:149], experts.expert_linear(x, w, offs)[:149])

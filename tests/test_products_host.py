@@ -190,3 +190,22 @@ def test_entry_points_check_on_the_host():
     refused(lib.e2v2_expert_product(ctypes.byref(e), 0, None, ctypes.c_int64(0), None), b"row strides")
     e.ldx, e.x = 16, 18
     refused(lib.e2v2_expert_product(ctypes.byref(e), 0, None, ctypes.c_int64(0), None), b"misaligned")
+
+
+def test_out_counts_as_changed(monkeypatch):
+    """out= is written past torch: autograd is told, so that a graph that saved the old elements raises."""
+    x, w, offs = _gpu(5, 16), _gpu(2, 8, 16), _i32(0, 2, 5)
+    buf = torch.zeros(5, 8)
+    gain = torch.ones(5, 8, requires_grad=True)
+    monkeypatch.setattr(experts, "_launch", lambda *a: a[5])
+    monkeypatch.setattr(experts, "_product", lambda *a: a[7])
+    xq, wq = x.to(F8), w.to(F8)
+    for call in (lambda out: experts.expert_linear(x, w, offs, out=out),
+                 lambda out: experts.expert_gemm_fp8(xq, _gpu(5, 1, dtype=U8), wq, _gpu(2, 1, 1, dtype=U8), offs, out=out)):
+        z = buf * gain
+        assert call(buf.as_subclass(_OnGpu)) is not None
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            z.sum().backward()
+    with torch.inference_mode():
+        out = _gpu(5, 8)
+        experts.expert_linear(x, w, offs, out=out)

@@ -11,6 +11,7 @@ import struct
 from typing import Optional
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _lib
 from .fp8 import MAX_PITCH, _has_tiles, _on_gpu, _product, _row_operand
@@ -105,7 +106,7 @@ def expert_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor,
     there).  Differentiable once in reverse mode, in x and weight.
 
     out [rows, n]: written instead of a new tensor, rows of no expert left as they were; for calls without gradients.  It may
-    not share elements with the operands."""
+    not share elements with the operands.  It counts as changed in place: a graph that saved its old elements raises."""
     dev = _on_gpu("expert_linear", x, weight)
     if (x.dim() != 2 or weight.dim() != 3 or weight.shape[2] != x.shape[1] or weight.numel() == 0
             or x.dtype not in _TYPES or weight.dtype != x.dtype):
@@ -122,7 +123,11 @@ def expert_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor,
     else:
         _check_out("expert_linear", out, (x.shape[0], weight.shape[1]), x.dtype, dev, grads, x, weight)
         y, fill = out, False
-    return _launch(_FORWARD, x, weight.shape, weight, None, y, offsets, fill) if y.numel() else y
+    if y.numel():
+        _launch(_FORWARD, x, weight.shape, weight, None, y, offsets, fill)
+        if out is not None:
+            increment_version(out)
+    return y
 
 
 def _check_out(name, out, shape, dtype, dev, grads, *operands):
@@ -178,5 +183,7 @@ def expert_gemm_fp8(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor
         return y
     xr, ldx = _row_operand("expert_gemm_fp8", x)
     w, ldw = _matrix(weight)
-    return _product(xr, ldx, x_scale, w, ldw, weight_scale, True, y, rows, n, k, offsets,
-                    experts, w.stride(0), fill)
+    _product(xr, ldx, x_scale, w, ldw, weight_scale, True, y, rows, n, k, offsets, experts, w.stride(0), fill)
+    if out is not None:
+        increment_version(out)
+    return y
