@@ -209,3 +209,29 @@ def test_out_counts_as_changed(monkeypatch):
     with torch.inference_mode():
         out = _gpu(5, 8)
         experts.expert_linear(x, w, offs, out=out)
+
+
+def test_out_may_not_share_elements_with_offsets_or_scales():
+    """Other workgroups still read those while rows are stored."""
+    x, w, offs = _gpu(5, 16), _gpu(2, 8, 16), _i32(0, 2, 5)
+    store = torch.zeros(4096, dtype=U8)
+
+    def at(first, dtype, *shape):
+        n = torch.Size(shape).numel() * torch.empty(0, dtype=dtype).element_size()
+        return store[first:first + n].view(dtype).view(shape).as_subclass(_OnGpu)
+
+    out = at(1024, torch.float32, 5, 8)                  # bytes 1024 to 1184
+    xq, sx, wq, sw = x.to(F8), _gpu(5, 1, dtype=U8), w.to(F8), _gpu(2, 1, 1, dtype=U8)
+    for first in (1016, 1024, 1100, 1180):
+        held = at(first, torch.int32, 3)
+        held.copy_(offs)
+        with pytest.raises(ValueError, match="shares elements"):
+            experts.expert_linear(x, w, held, out=out)
+        with pytest.raises(ValueError, match="shares elements"):
+            experts.expert_gemm_fp8(xq, sx, wq, sw, held, out=out)
+    for first in (1020, 1024, 1183):
+        with pytest.raises(ValueError, match="shares elements"):
+            experts.expert_gemm_fp8(xq, at(first, U8, 5, 1), wq, sw, offs, out=out)
+        with pytest.raises(ValueError, match="shares elements"):
+            experts.expert_gemm_fp8(xq, sx, wq, at(first + (first == 1020) * 3, U8, 2, 1, 1), offs, out=out)
+    assert not experts._overlap(out, at(1012, torch.int32, 3)) and not experts._overlap(out, at(1184, U8, 5, 1))

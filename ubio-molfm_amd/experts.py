@@ -121,7 +121,7 @@ def expert_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor,
             return _ExpertLinearFn.apply(x, weight, offsets)
         y, fill = torch.empty((x.shape[0], weight.shape[1]), dtype=x.dtype, device=dev), True
     else:
-        _check_out("expert_linear", out, (x.shape[0], weight.shape[1]), x.dtype, dev, grads, x, weight)
+        _check_out("expert_linear", out, (x.shape[0], weight.shape[1]), x.dtype, dev, grads, x, weight, offsets)
         y, fill = out, False
     if y.numel():
         _launch(_FORWARD, x, weight.shape, weight, None, y, offsets, fill)
@@ -142,8 +142,8 @@ def _check_out(name, out, shape, dtype, dev, grads, *operands):
 
 
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether matrices with consecutive elements in a row may share elements: their bytes overlap, and they are not
-    columns side by side of one table."""
+    """Whether tensors may share elements: their bytes overlap, and they are not matrices with consecutive elements in a
+    row that are columns side by side of one table."""
     if a.numel() == 0 or b.numel() == 0:
         return False
     (a0, a1), (b0, b1) = ((t.data_ptr(), t.data_ptr() + t.element_size()
@@ -177,7 +177,7 @@ def expert_gemm_fp8(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor
     if out is None:
         y, fill = torch.empty((rows, n), dtype=dtype, device=dev), True
     else:
-        _check_out("expert_gemm_fp8", out, (rows, n), dtype, dev, False, x, weight)
+        _check_out("expert_gemm_fp8", out, (rows, n), dtype, dev, False, x, x_scale, weight, weight_scale, offsets)
         y, fill = out, False
     if y.numel() == 0:
         return y
