@@ -235,3 +235,20 @@ def test_out_may_not_share_elements_with_offsets_or_scales():
         with pytest.raises(ValueError, match="shares elements"):
             experts.expert_gemm_fp8(xq, sx, wq, at(first + (first == 1020) * 3, U8, 2, 1, 1), offs, out=out)
     assert not experts._overlap(out, at(1012, torch.int32, 3)) and not experts._overlap(out, at(1184, U8, 5, 1))
+
+
+def test_traces(monkeypatch):
+    """A trace gets Functions, which it replays; what is none is refused."""
+    x, w, offs = _gpu(5, 16), _gpu(2, 8, 16), _i32(0, 2, 5)
+    xq, sx, wq, sw = x.to(F8), _gpu(5, 1, dtype=U8), w.to(F8), _gpu(2, 1, 1, dtype=U8)
+    monkeypatch.setattr(torch.jit, "is_tracing", lambda: True)
+    for fn in (norms._LayerNormFn, norms._RmsNormFn, fp8._LinearFn, experts._ExpertLinearFn):
+        monkeypatch.setattr(fn, "apply", lambda *a, fn=fn: fn)
+    assert norms.layer_norm(x) is norms._LayerNormFn and norms.rms_norm(x) is norms._RmsNormFn
+    assert norms.rms_norm(x, residual=x) is norms._RmsNormFn and fp8.linear(x, w[0]) is fp8._LinearFn
+    assert experts.expert_linear(x, w, offs) is experts._ExpertLinearFn
+    for call in (lambda: norms.rms_norm_fp8(x), lambda: fp8.quantize(x), lambda: fp8.dequantize(xq, sx),
+                 lambda: fp8.gemm(xq, sx, wq[0], sw[0]), lambda: experts.expert_linear(x, w, offs, out=_gpu(5, 8)),
+                 lambda: experts.expert_gemm_fp8(xq, sx, wq, sw, offs)):
+        with pytest.raises(RuntimeError, match="torch.jit.trace"):
+            call()

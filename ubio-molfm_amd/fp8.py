@@ -17,7 +17,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .norms import _TYPES, _address, _call, _first_order, _rows, has_tangent
+from .norms import _TYPES, _address, _call, _first_order, _no_trace, _rows, has_tangent
 
 BLOCK = 128
 CODES = torch.float8_e4m3fn
@@ -76,6 +76,7 @@ def quantize(x: torch.Tensor, tiles: bool = False):
         raise ValueError(f"quantize: fp32, bf16 or fp16 rows of at least one value, got {tuple(x.shape)} {x.dtype}")
     if (torch.is_grad_enabled() and x.requires_grad) or has_tangent(x):
         raise RuntimeError("quantize has no gradients: call it under torch.no_grad()")
+    _no_trace("quantize")
     w = x.shape[-1]
     if not tiles:
         xr, ldx = _rows(x)
@@ -118,6 +119,7 @@ def dequantize(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = t
     if dtype not in _TYPES or codes.dim() == 0:
         raise ValueError(f"dequantize: codes {tuple(codes.shape)}, values in fp32, bf16 or fp16, got {dtype}")
     tiles = _has_tiles("dequantize", "codes", codes, scales)
+    _no_trace("dequantize")
     out = torch.empty(codes.shape, dtype=dtype, device=dev)
     if out.numel() == 0:
         return out
@@ -194,6 +196,7 @@ def gemm(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch
                          f"{tuple(w.shape)} and {dtype}")
     _has_tiles("gemm", "a", a, a_scale, tiles=False)
     tiles = _has_tiles("gemm", "w", w, w_scale)
+    _no_trace("gemm")
     n, k = w.shape
     m = a.numel() // k
     y = torch.empty((m, n), dtype=dtype, device=dev)
@@ -282,6 +285,6 @@ def linear(x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
         raise RuntimeError("linear: forward-mode tangents are not supported")
     if max(_pitch(weight.shape[0]), _pitch(weight.shape[1]), _pitch(x.numel() // weight.shape[1])) > MAX_PITCH:
         raise ValueError(f"linear: sizes up to {MAX_PITCH}, got {tuple(x.shape)} and {tuple(weight.shape)} on {dev}")
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
+    if torch.jit.is_tracing() or torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
         return _LinearFn.apply(x, weight)
     return _linear_forward(x, weight, False, False)[0]

@@ -277,8 +277,8 @@ def _layer_norm(x, weight, bias, eps: float, any_order: bool) -> torch.Tensor:
                              f"{p.dtype} on {p.device}")
     if has_tangent(x, weight, bias):
         raise RuntimeError("layer_norm: forward-mode tangents are not supported")
-    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
-                                    or (bias is not None and bias.requires_grad)):
+    if torch.jit.is_tracing() or torch.is_grad_enabled() and (
+            x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)):
         return _LayerNormFn.apply(x, weight, bias, float(eps), any_order)
     return _forward(x, weight, bias, float(eps), None)
 
@@ -352,6 +352,13 @@ def _first_order(name: str, *tensors: Optional[torch.Tensor]) -> None:
         raise RuntimeError(f"{name}: batched gradients and gradients with forward-mode tangents are not supported")
 
 
+def _no_trace(name: str) -> None:
+    """torch.jit.trace records a Function as one call, but of a kernel that is launched here only the empty tensor that it
+    writes: what is no Function is refused there."""
+    if torch.jit.is_tracing():
+        raise RuntimeError(f"{name}: torch.jit.trace does not record it")
+
+
 def _rms_check(name, x, weight, residual):
     if not isinstance(x, torch.Tensor) or not x.is_cuda:
         raise RuntimeError(f"{name} runs on the GPU only (HIP library, no CPU path): got "
@@ -385,8 +392,9 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: float 
     where they lie if their rows are consecutive and evenly spaced.  weight: [w], fp32 or x's type, or None.  Results
     have x's type and are contiguous.  Differentiable once in reverse mode (create_graph=True raises)."""
     weight = _rms_check("rms_norm", x, weight, residual)
-    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
-                                    or (residual is not None and residual.requires_grad)):
+    if torch.jit.is_tracing() or torch.is_grad_enabled() and (
+            x.requires_grad or (weight is not None and weight.requires_grad)
+            or (residual is not None and residual.requires_grad)):
         return _RmsNormFn.apply(x, weight, float(eps), residual)
     y, h = _rms_forward(x, weight, float(eps), residual, None)
     return y if residual is None else (y, h)
@@ -398,6 +406,7 @@ def rms_norm_fp8(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: fl
     (codes, scales, h).  The codes are those of the norm before it is rounded to x's type.  No gradients: call it under
     torch.no_grad(), or with tensors that need none."""
     weight = _rms_check("rms_norm_fp8", x, weight, residual)
+    _no_trace("rms_norm_fp8")
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
                                     or (residual is not None and residual.requires_grad)):
         raise RuntimeError("rms_norm_fp8 has no gradients: call it under torch.no_grad()")
