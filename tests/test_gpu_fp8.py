@@ -347,3 +347,13 @@ def test_refused_derivatives(cuda):
         torch.autograd.grad(fp8.linear(x, w).sum(), x, create_graph=True)
     with pytest.raises(RuntimeError, match="no gradients"):
         fp8.quantize(x)
+
+
+def test_codes_with_a_history_are_refused(cuda):
+    x = torch.randn(4, 32, device=cuda, requires_grad=True)
+    codes, s = x.to(F8), torch.full((4, 1), 127, dtype=torch.uint8, device=cuda)
+    for call in (lambda: fp8.dequantize(codes, s), lambda: fp8.gemm(codes, s, codes.detach(), s)):
+        with pytest.raises(RuntimeError, match="no gradients"):
+            call()
+        with torch.no_grad():
+            call()

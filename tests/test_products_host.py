@@ -252,3 +252,24 @@ def test_traces(monkeypatch):
                  lambda: experts.expert_gemm_fp8(xq, sx, wq, sw, offs)):
         with pytest.raises(RuntimeError, match="torch.jit.trace"):
             call()
+
+
+def test_codes_with_a_history_are_refused():
+    """Codes cast from values that need gradients need them too: their products have none."""
+    x = torch.rand(5, 16, requires_grad=True)
+    (xq, sx), (wq, sw), offs = (x.to(F8).as_subclass(_OnGpu), _gpu(5, 1, dtype=U8)), (_gpu(8, 16, dtype=F8),
+                                                                                    _gpu(1, 1, dtype=U8)), _i32(0, 2, 5)
+    wx = torch.rand(2, 8, 16, requires_grad=True).to(F8).as_subclass(_OnGpu)
+    calls = [lambda: fp8.dequantize(xq, sx), lambda: fp8.gemm(xq, sx, wq, sw), lambda: fp8.gemm(wq, _gpu(8, 1, dtype=U8), xq, sx),
+             lambda: experts.expert_gemm_fp8(xq, sx, wq[None], sw[None], offs[:2]),
+             lambda: experts.expert_gemm_fp8(_gpu(5, 16, dtype=F8), sx, wx, _gpu(2, 1, 1, dtype=U8), offs)]
+    for call in calls:
+        with pytest.raises(RuntimeError, match="no gradients"):
+            call()
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x.detach(), torch.ones(5, 16)).to(F8)
+        xq = dual.as_subclass(_OnGpu)
+        assert norms.has_tangent(xq)
+        for call in calls[:2]:
+            with pytest.raises(RuntimeError, match="no gradients"):
+                call()

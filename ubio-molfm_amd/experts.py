@@ -15,7 +15,7 @@ from torch.autograd.graph import increment_version
 
 from . import _lib
 from .fp8 import MAX_PITCH, _has_tiles, _on_gpu, _product, _row_operand
-from .norms import _TYPES, _address, _call, _first_order, _no_trace, has_tangent
+from .norms import _TYPES, _address, _call, _first_order, _forward_only, _no_trace, has_tangent
 
 _FORWARD, _ROWS, _WEIGHTS = 0, 1, 2         # E2V2_EXPERT_*
 # e2v2_expert_args as bytes
@@ -175,7 +175,7 @@ def expert_gemm_fp8(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor
     _has_tiles("expert_gemm_fp8", "x", x, x_scale, tiles=False)
     _has_tiles("expert_gemm_fp8", "weight", weight, weight_scale, rows=False)
     offsets = _experts_of("expert_gemm_fp8", offsets, experts, dev)
-    _no_trace("expert_gemm_fp8")
+    _forward_only("expert_gemm_fp8", x, weight)
     if out is None:
         y, fill = torch.empty((rows, n), dtype=dtype, device=dev), True
     else:

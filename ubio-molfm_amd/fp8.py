@@ -17,7 +17,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .norms import _TYPES, _address, _call, _first_order, _no_trace, _rows, has_tangent
+from .norms import _TYPES, _address, _call, _first_order, _forward_only, _rows, has_tangent
 
 BLOCK = 128
 CODES = torch.float8_e4m3fn
@@ -74,9 +74,7 @@ def quantize(x: torch.Tensor, tiles: bool = False):
     _on_gpu("quantize", x)
     if x.dtype not in _TYPES or x.dim() == 0 or x.shape[-1] == 0:
         raise ValueError(f"quantize: fp32, bf16 or fp16 rows of at least one value, got {tuple(x.shape)} {x.dtype}")
-    if (torch.is_grad_enabled() and x.requires_grad) or has_tangent(x):
-        raise RuntimeError("quantize has no gradients: call it under torch.no_grad()")
-    _no_trace("quantize")
+    _forward_only("quantize", x)
     w = x.shape[-1]
     if not tiles:
         xr, ldx = _rows(x)
@@ -114,12 +112,12 @@ def _has_tiles(name, what, codes, scales, rows=True, tiles=True) -> bool:
 
 def dequantize(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """The values that codes and scales stand for, contiguous, in fp32, bf16 or fp16 (exact in the first two, but for values
-    outside the type's range).  Whether scales are those of rows or of tiles shows in their shape."""
+    outside the type's range).  Whether scales are those of rows or of tiles shows in their shape.  No gradients."""
     dev = _on_gpu("dequantize", codes, scales)
     if dtype not in _TYPES or codes.dim() == 0:
         raise ValueError(f"dequantize: codes {tuple(codes.shape)}, values in fp32, bf16 or fp16, got {dtype}")
     tiles = _has_tiles("dequantize", "codes", codes, scales)
-    _no_trace("dequantize")
+    _forward_only("dequantize", codes)
     out = torch.empty(codes.shape, dtype=dtype, device=dev)
     if out.numel() == 0:
         return out
@@ -189,14 +187,14 @@ def gemm(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch
     """a w^T of 8-bit rows a [..., k] and an 8-bit weight w [n, k]: [..., n] in fp32, bf16 or fp16.
 
     a_scale [..., ceil(k / 128)]; w_scale [ceil(n / 128), ceil(k / 128)] (tiles) or [n, ceil(k / 128)] (rows).  Any sizes
-    and alignment; rows that start on multiples of 16 bytes (those of :func:`quantize` do) take the faster loads."""
+    and alignment; rows that start on multiples of 16 bytes (those of :func:`quantize` do) take the faster loads.  No gradients."""
     dev = _on_gpu("gemm", a, a_scale, w, w_scale)
     if a.dim() == 0 or w.dim() != 2 or w.shape[1] != a.shape[-1] or w.shape[1] == 0 or dtype not in _TYPES:
         raise ValueError(f"gemm: a [..., k] and w [n, k], out in fp32, bf16 or fp16; got {tuple(a.shape)}, "
                          f"{tuple(w.shape)} and {dtype}")
     _has_tiles("gemm", "a", a, a_scale, tiles=False)
     tiles = _has_tiles("gemm", "w", w, w_scale)
-    _no_trace("gemm")
+    _forward_only("gemm", a, w)
     n, k = w.shape
     m = a.numel() // k
     y = torch.empty((m, n), dtype=dtype, device=dev)

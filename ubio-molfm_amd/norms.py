@@ -359,6 +359,17 @@ def _no_trace(name: str) -> None:
         raise RuntimeError(f"{name}: torch.jit.trace does not record it")
 
 
+def _forward_only(name: str, *tensors: Optional[torch.Tensor]) -> None:
+    """For calls without gradients: one that would need them (of codes too: those cast from values that need them do) is
+    refused instead of losing them, and so is a trace."""
+    for t in tensors:
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError(f"{name} has no gradients: call it under torch.no_grad()")
+    if has_tangent(*tensors):
+        raise RuntimeError(f"{name} has no gradients: a forward-mode tangent would be lost")
+    _no_trace(name)
+
+
 def _rms_check(name, x, weight, residual):
     if not isinstance(x, torch.Tensor) or not x.is_cuda:
         raise RuntimeError(f"{name} runs on the GPU only (HIP library, no CPU path): got "
@@ -406,10 +417,7 @@ def rms_norm_fp8(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: fl
     (codes, scales, h).  The codes are those of the norm before it is rounded to x's type.  No gradients: call it under
     torch.no_grad(), or with tensors that need none."""
     weight = _rms_check("rms_norm_fp8", x, weight, residual)
-    _no_trace("rms_norm_fp8")
-    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
-                                    or (residual is not None and residual.requires_grad)):
-        raise RuntimeError("rms_norm_fp8 has no gradients: call it under torch.no_grad()")
+    _forward_only("rms_norm_fp8", x, weight, residual)
     w = x.shape[-1]
     n, pitch, blocks = x.numel() // w, (w + 15) // 16 * 16, (w + _BLOCK - 1) // _BLOCK
     (xr, ldx), (rr, ldr) = _rows(x), (None, 0) if residual is None else _rows(residual)
