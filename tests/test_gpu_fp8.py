@@ -357,3 +357,24 @@ def test_codes_with_a_history_are_refused(cuda):
             call()
         with torch.no_grad():
             call()
+
+
+def test_linear_with_many_rows(cuda):
+    """More rows than a row of codes may have bytes: x's gradient and calls without gradients have no such rows."""
+    m, n, k = (1 << 22) + 37, 24, 140
+    x = _rand(1000, k, seed=1, spread=0.7).to(BF16).to(cuda).repeat(-(-m // 1000), 1)[:m].requires_grad_(True)
+    w = (_rand(n, k, seed=2, spread=0.5) / k ** 0.5).to(BF16).to(cuda)
+    gy = _rand(1000, n, seed=3, spread=0.7).to(BF16).to(cuda).repeat(-(-m // 1000), 1)[:m]
+    y = fp8.linear(x, w)
+    gx, = torch.autograd.grad(y, x, gy)
+    short = x.detach()[:1000].requires_grad_(True)
+    y0 = fp8.linear(short, w)
+    g0, = torch.autograd.grad(y0, short, gy[:1000])
+    last = m // 1000 * 1000
+    for got, want in ((y, y0), (gx, g0)):
+        assert torch.equal(got[:1000], want) and torch.equal(got[last:], want[:m - last])
+        assert (got[:last].view(-1, 1000, got.shape[1]) == want).all()
+    with torch.no_grad():
+        assert torch.equal(fp8.linear(x, w.requires_grad_(True)), y)
+    with pytest.raises(ValueError, match="linear: sizes up to"):
+        fp8.linear(x, w)

@@ -273,3 +273,21 @@ def test_codes_with_a_history_are_refused():
         for call in calls[:2]:
             with pytest.raises(RuntimeError, match="no gradients"):
                 call()
+
+
+def test_linear_takes_many_rows_where_the_weight_needs_no_gradient(monkeypatch):
+    """Only the weight's gradient reads codes whose rows are as long as x has rows."""
+    monkeypatch.setattr(fp8, "_linear_forward", lambda *a: ("forward",))
+    monkeypatch.setattr(fp8._LinearFn, "apply", lambda *a: "function")
+    many = fp8.MAX_PITCH + 16
+    x, w = _gpu(1, 16).expand(many, 16), _gpu(8, 16)
+    trained = torch.nn.Parameter(torch.zeros(8, 16)).as_subclass(_OnGpu)
+    assert fp8.linear(x, w) == "forward" and fp8.linear(x.detach().requires_grad_(True), w) == "function"
+    with torch.no_grad():
+        assert fp8.linear(x, trained) == "forward"
+    assert fp8.linear(x[16:], trained) == "function"
+    with pytest.raises(ValueError, match="linear: sizes up to"):
+        fp8.linear(x, trained)
+    for shape in ((many, 16), (16, many)):
+        with pytest.raises(ValueError, match="linear: sizes up to"):
+            fp8.linear(_gpu(1, 1).expand(1, shape[1]), _gpu(1, 1).expand(*shape))

@@ -273,7 +273,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
     the weight's.  Rows of x and of the upstream gradient are quantised in blocks of 128 along the reduction of the product
     that they enter (so each has codes along rows and along columns), the weight in tiles of 128 x 128.  The
     gradients are those of the product of the values that the codes stand for; rounding to codes passes them through
-    unchanged.  The backward pass keeps the codes, one byte a value, not x.  Differentiable once in reverse mode."""
+    unchanged.  The backward pass keeps the codes, one byte a value, not x.  Differentiable once in reverse mode.  n, k and,
+    for the weight's gradient, the rows: 4,194,304 at most."""
     dev = _on_gpu("linear", x, weight)
     if (x.dtype not in _TYPES or weight.dtype not in _TYPES or x.dim() == 0 or weight.dim() != 2
             or weight.shape[1] != x.shape[-1] or weight.numel() == 0):
@@ -281,8 +282,11 @@ def linear(x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
                          f"{tuple(weight.shape)} {weight.dtype}")
     if has_tangent(x, weight):
         raise RuntimeError("linear: forward-mode tangents are not supported")
-    if max(_pitch(weight.shape[0]), _pitch(weight.shape[1]), _pitch(x.numel() // weight.shape[1])) > MAX_PITCH:
+    grads = torch.is_grad_enabled()
+    # rows of codes: of k and n values, and for the weight's gradient those of the transposes, as long as x has rows
+    longest = max(weight.shape[0], weight.shape[1], x.numel() // weight.shape[1] if grads and weight.requires_grad else 0)
+    if _pitch(longest) > MAX_PITCH:
         raise ValueError(f"linear: sizes up to {MAX_PITCH}, got {tuple(x.shape)} and {tuple(weight.shape)} on {dev}")
-    if torch.jit.is_tracing() or torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
+    if torch.jit.is_tracing() or grads and (x.requires_grad or weight.requires_grad):
         return _LinearFn.apply(x, weight)
     return _linear_forward(x, weight, False, False)[0]
