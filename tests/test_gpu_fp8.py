@@ -378,3 +378,14 @@ def test_linear_with_many_rows(cuda):
         assert torch.equal(fp8.linear(x, w.requires_grad_(True)), y)
     with pytest.raises(ValueError, match="linear: sizes up to"):
         fp8.linear(x, w)
+
+
+def test_rows_far_apart(cuda):
+    aq, sa, wq, sw = _product(cuda, 3, 40, 200, 11)
+
+    def far(q):
+        t = torch.empty_strided(tuple(q.shape), (fp8.MAX_PITCH + 16, 1), dtype=torch.uint8, device=cuda)
+        return t.copy_(_bits(q)).view(F8)
+
+    for y in (fp8.gemm(far(aq), sa, wq, sw, dtype=F32), fp8.gemm(aq, sa, far(wq), sw, dtype=F32)):
+        _check_product(y, fp8.dequantize(aq, sa), fp8.dequantize(wq, sw), 200)

@@ -291,3 +291,16 @@ def test_linear_takes_many_rows_where_the_weight_needs_no_gradient(monkeypatch):
     for shape in ((many, 16), (16, many)):
         with pytest.raises(ValueError, match="linear: sizes up to"):
             fp8.linear(_gpu(1, 1).expand(1, shape[1]), _gpu(1, 1).expand(*shape))
+
+
+def test_rows_far_apart_are_copied():
+    """Rows of codes further apart than the kernels take."""
+    wide = torch.arange(3, dtype=U8)[:, None].expand(3, 96).contiguous()
+    far = torch.empty_strided((3, 96), (fp8.MAX_PITCH + 16, 1), dtype=U8).copy_(wide).view(F8)
+    rows, ld = fp8._row_operand("gemm", far)
+    assert ld == 96 and rows.is_contiguous() and torch.equal(rows.view(U8), wide)
+    near = torch.empty_strided((3, 96), (fp8.MAX_PITCH, 1), dtype=U8).view(F8)
+    assert fp8._row_operand("gemm", near)[0] is near
+    one = torch.zeros(1, 1, dtype=U8).view(F8).expand(2, fp8.MAX_PITCH + 16)
+    with pytest.raises(ValueError, match="rows of 4194320"):
+        fp8._row_operand("gemm", one)

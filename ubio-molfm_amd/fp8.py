@@ -173,12 +173,12 @@ def _product(a, lda, sa, b, ldb, sb, b_tiles, y, m, n, k, offsets=None, groups=0
 
 
 def _row_operand(name, codes):
-    rows, ld = _rows(codes)
     w = codes.shape[-1]
-    if ld < w and codes.numel() > w:            # rows that share bytes
+    if w > MAX_PITCH:
+        raise ValueError(f"{name}: rows of {w} bytes (at most {MAX_PITCH})")
+    rows, ld = _rows(codes)
+    if (ld < w and codes.numel() > w) or ld > MAX_PITCH:        # rows that share bytes or lie too far apart
         rows, ld = rows.contiguous(), w
-    if ld > MAX_PITCH:
-        raise ValueError(f"{name}: rows {ld} bytes apart (at most {MAX_PITCH})")
     return rows, max(ld, w)
 
 
@@ -187,7 +187,8 @@ def gemm(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch
     """a w^T of 8-bit rows a [..., k] and an 8-bit weight w [n, k]: [..., n] in fp32, bf16 or fp16.
 
     a_scale [..., ceil(k / 128)]; w_scale [ceil(n / 128), ceil(k / 128)] (tiles) or [n, ceil(k / 128)] (rows).  Any sizes
-    and alignment; rows that start on multiples of 16 bytes (those of :func:`quantize` do) take the faster loads.  No gradients."""
+    (k up to 4,194,304) and alignment; rows that start on multiples of 16 bytes (those of :func:`quantize` do) take the
+    faster loads.  No gradients."""
     dev = _on_gpu("gemm", a, a_scale, w, w_scale)
     if a.dim() == 0 or w.dim() != 2 or w.shape[1] != a.shape[-1] or w.shape[1] == 0 or dtype not in _TYPES:
         raise ValueError(f"gemm: a [..., k] and w [n, k], out in fp32, bf16 or fp16; got {tuple(a.shape)}, "
