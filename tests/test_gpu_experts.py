@@ -333,3 +333,29 @@ def test_out_counts_as_changed(cuda):
     with torch.inference_mode():
         out = torch.empty(x.shape[0], 48, dtype=BF16, device=cuda)
         assert torch.equal(experts.expert_linear(x, w, offs, out=out)[:149], experts.expert_linear(x, w, offs)[:149])
+
+
+@pytest.mark.parametrize("sizes,n,k", [([9, 0, 40], 48, 64), ([300, 513, 0, 31], 200, 264), ([40, 90], 33, 65), ([3, 2], 16, 40)])
+def test_largest_fp32_operands(sizes, n, k, cuda):
+    """Operands that bf16 rounds to infinity, up to fp32's largest, have finite pieces as all others have.  First pieces are
+    cut, so that second ones are below 2^-7 and third ones at most 2^-16 of an operand: the products left out stay
+    within the 4 2^-24 |a b| of the tolerance (2 2^-7 2^-16; where both come that near, |a b| is 2^-6 larger than its power
+    of two, more than the 2^-32 of the product of third pieces)."""
+    x, w, gy, offs = _inputs(sizes, 0, n, k, F32, 13, cuda)
+    top = torch.finfo(F32).max
+    gy *= 1e-3
+    x[::4, 3], x[1::4, 3] = 3.3962e38, -top
+    w[:, :, 3] *= 0.1
+    w[:, 1, 2], w[:, 2, 2] = top, -3.4e38
+    x[:, 2] *= 1e-3
+    gy[2, 5], gy[3, 5] = top, -3.3962e38
+    x[2:4] *= 1e-3
+    xg, wg = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    y = experts.expert_linear(xg, wg, offs)
+    gx, gw = torch.autograd.grad(y, (xg, wg), gy)
+    assert y.isfinite().all() and gx.isfinite().all() and gw.isfinite().all()
+    _check(x, w, gy, offs, y, gx, gw)
+    # what is not finite stays in its row
+    x[1, 0], x[0, 0] = float("inf"), float("nan")
+    bad = experts.expert_linear(x, w, offs)
+    assert not bad[:2].isfinite().any() and torch.equal(bad[2:], y[2:])

@@ -102,8 +102,8 @@ def expert_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor,
     x [rows, k] and weight [experts, n, k] in one of fp32, bf16 and fp16; offsets [experts + 1], int32 or int64 on the GPU,
     not decreasing, an expert without rows where two are equal (what lies outside 0 .. rows is clamped; int64 ones are read
     as int32).  Rows of no expert give zeros and take no part in gradients.  Sums are fp32 (fp32 operands are split exactly
-    into bf16 pieces, as in ``gemm``: a product with an operand that bf16 rounds to infinity, from 3.3961e38 on, is NaN
-    there).  Differentiable once in reverse mode, in x and weight.
+    into bf16 pieces, as in ``gemm``: a product with an infinite one is NaN there).  Differentiable once in reverse mode, in x
+    and weight.
 
     out [rows, n]: written instead of a new tensor, rows of no expert left as they were; for calls without gradients.  It may
     not share elements with the operands.  It counts as changed in place: a graph that saved its old elements raises."""
