@@ -359,3 +359,52 @@ def test_largest_fp32_operands(sizes, n, k, cuda):
     x[1, 0], x[0, 0] = float("inf"), float("nan")
     bad = experts.expert_linear(x, w, offs)
     assert not bad[:2].isfinite().any() and torch.equal(bad[2:], y[2:])
+
+
+@pytest.mark.parametrize("sizes,spare,n,k", [([1], 0, 1, 1), ([5, 130, 0, 17], 3, 64, 131), ([3, 0, 2, 1], 2, 40, 515),
+                                             ([20] * 70 + [0] * 3 + [200], 11, 96, 33), ([700, 0, 513], 5, 130, 257),
+                                             ([3000, 0, 2500, 1300], 40, 1500, 145)])
+def test_8_bits_on_any_boundary(sizes, spare, n, k, cuda):
+    """Codes packed without padding, starting on every byte of a dword, with NaN codes around and in rows of no expert."""
+    x, w, gy, offs = _inputs(sizes, spare, n, k, F32, 14, cuda)
+    (xq, sx), (wq, sw) = fp8.quantize(x), fp8.quantize(w, tiles=True)
+    xv, wv = fp8.dequantize(xq, sx), fp8.dequantize(wq, sw)
+    o = offs.tolist()
+    for skew in range(4):
+        def moved(q):
+            flat = torch.full((q.numel() + 40,), 0x7F, dtype=torch.uint8, device=cuda)
+            view = flat[skew:skew + q.numel()].view(q.shape)
+            view.copy_(q.contiguous().view(torch.uint8))
+            return view
+        xs, ws = moved(xq), moved(wq)
+        xs[o[-1]:] = 0x7F
+        y = experts.expert_gemm_fp8(xs.view(torch.float8_e4m3fn), sx, ws.view(torch.float8_e4m3fn), sw, offs, dtype=F32)
+        for e in range(len(sizes)):
+            a, b = xv[o[e]:o[e + 1]].double(), wv[e].double()
+            grid = 7 * 2.0 ** -13 * (_largest_of_8(a) @ _largest_of_8(b).T)
+            _close(y[o[e]:o[e + 1]], a @ b.T, a.abs() @ b.abs().T, k, BF16, grid)
+        assert (y[o[-1]:] == 0).all()
+
+
+# the weights' gradient in parts of the rows; more tiles than workgroups in every pass
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("sizes,spare,n,k", [([5000, 0, 3001], 7, 131, 203), ([9000], 3, 65, 257), ([4000, 0, 3500, 2900], 9, 1027, 1301)])
+def test_odd_widths_with_many_rows(sizes, spare, n, k, dtype, cuda):
+    x, w, gy, offs = _inputs(sizes, spare, n, k, dtype, 15, cuda)
+    x[-spare:], gy[-spare:] = float("nan"), float("inf")
+    cut = experts._workspace_bytes(x.shape[0], n, k, len(sizes)) > 0
+    tiles = [sum(-(-s // 128) for s in sizes) * -(-n // 128), len(sizes) * -(-n // 128) * -(-k // 128)]
+    assert cut or min(tiles) > 256 and tiles[0] > 512
+    x.requires_grad_(True), w.requires_grad_(True)
+    y = experts.expert_linear(x, w, offs)
+    gx, gw = torch.autograd.grad(y, (x, w), gy)
+    _check(x, w, gy, offs, y, gx, gw)
+
+
+def test_more_experts_tiles_than_workgroups_on_odd_widths(cuda):
+    """The weights' gradient with several tiles of different experts in turn for a workgroup."""
+    x, w, gy, offs = _inputs([37, 0, 300, 5, 64, 129, 1, 200] * 8, 3, 387, 519, BF16, 16, cuda)
+    x.requires_grad_(True), w.requires_grad_(True)
+    y = experts.expert_linear(x, w, offs)
+    gx, gw = torch.autograd.grad(y, (x, w), gy)
+    _check(x, w, gy, offs, y, gx, gw)

@@ -389,3 +389,21 @@ def test_rows_far_apart(cuda):
 
     for y in (fp8.gemm(far(aq), sa, wq, sw, dtype=F32), fp8.gemm(aq, sa, far(wq), sw, dtype=F32)):
         _check_product(y, fp8.dequantize(aq, sa), fp8.dequantize(wq, sw), 200)
+
+
+@pytest.mark.parametrize("m,n,k", [(65, 64, 8191), (200, 300, 4100), (33, 130, 6001), (100, 700, 2049), (3000, 5000, 145)])
+def test_long_and_many_tiles_on_any_boundary(m, n, k, cuda):
+    """Codes packed without padding, where k is cut into parts and where a workgroup takes several tiles."""
+    aq, sa, wq, sw = _product(cuda, m, n, k, 17)
+    assert k % 16 and (m <= 64 or k < 4096 or fp8._workspace_bytes(m, n, k) > 0) and (m < 3000 or -(-m // 128) * -(-n // 128) > 512)
+    av, wv = fp8.dequantize(aq, sa), fp8.dequantize(wq, sw)
+    for skew in (0, 1, 2, 3):
+        def moved(q):
+            r, c = q.shape
+            flat = torch.full((r * c + 40,), 0x7F, dtype=torch.uint8, device=cuda)
+            view = flat[skew:skew + r * c].view(r, c)
+            view.copy_(_bits(q))
+            return view.view(F8)
+        y = fp8.gemm(moved(aq), sa, moved(wq), sw, dtype=F32)
+        _check_product(y, av, wv, k)
+        assert torch.equal(y, fp8.gemm(moved(aq), sa, moved(wq), sw, dtype=F32))
