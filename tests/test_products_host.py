@@ -304,3 +304,15 @@ def test_rows_far_apart_are_copied():
     one = torch.zeros(1, 1, dtype=U8).view(F8).expand(2, fp8.MAX_PITCH + 16)
     with pytest.raises(ValueError, match="rows of 4194320"):
         fp8._row_operand("gemm", one)
+
+
+def test_row_strides_whose_bytes_pass_64_bits_are_refused():
+    lib = _lib.load()
+    for field, which in (("ldx", 0), ("ldw", 0), ("ldgy", 1), ("ldw", 1), ("ldgy", 2), ("ldx", 2)):
+        for far in (1 << 62, (1 << 61) + 16, (1 << 20) + 1):
+            e = _lib.ExpertArgs()
+            e.x = e.w = e.gy = e.y = e.offsets = 16
+            e.rows, e.n, e.k, e.ldx, e.ldw, e.ldgy, e.ldy, e.experts = 4, 16, 16, 16, 16, 16, 16, 2
+            setattr(e, field, far)
+            assert lib.e2v2_expert_product(ctypes.byref(e), which, None, ctypes.c_int64(0), None) != 0
+            assert b"row strides" in lib.e2v2_last_error(), (field, which, far, lib.e2v2_last_error())

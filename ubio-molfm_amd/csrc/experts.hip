@@ -86,7 +86,7 @@ E2V2_API int e2v2_expert_product(const e2v2_expert_args* a, int pass, float* ws,
   E2V2_REQUIRE(a->y && a->offsets && (a->rows == 0 || P.k == 0 || (pa && pb)), "expert_product: null operand");
   const int64_t wide = (fwd || wgrad ? a->k : 0), wide_gy = fwd ? 0 : a->n;
   E2V2_REQUIRE(a->ldx >= wide && a->ldgy >= wide_gy && (wgrad || a->ldw >= a->k) && a->ldy >= P.n &&
-                   lda * size <= kMaxPitch && ldb * size <= kMaxPitch, "expert_product: row strides %lld, %lld, %lld, %lld",
+                   lda <= kMaxPitch / size && ldb <= kMaxPitch / size, "expert_product: row strides %lld, %lld, %lld, %lld",
                (long long)a->ldx, (long long)a->ldw, (long long)a->ldgy, (long long)a->ldy);
   E2V2_REQUIRE(((uintptr_t)pa | (uintptr_t)pb | (uintptr_t)a->y) % size == 0 && (uintptr_t)a->offsets % 4 == 0 &&
                    (uintptr_t)ws % 16 == 0, "expert_product: misaligned operand");
