@@ -4,8 +4,8 @@
 //   weights' grad.   gW[e] = sum_t gy[t] x[t]^T    both operands read along their columns, over ragged rows
 // Rows of no expert give zeros.
 //
-// 16,384 rows over 32 experts of 1408 x 2048 bf16: 114, 118 and 127 us (95 GFLOP each; the weights' gradient writes 184 MB),
-// unevenly 139 for the last; 10,000 rows over 6 of 256 x 256 fp32: 21, 21 and 26.
+// 16,384 rows over 32 experts of 1408 x 2048 bf16, operands in turn: 118, 121 and 139 us (95 GFLOP each; the weights' gradient
+// writes 184 MB), unevenly 124, 123 and 145; where rows start off 16 bytes (1408 x 2047) 260, 253 and 345.  10,000 rows over 6 of 256 x 256 fp32: 21, 21 and 26.
 #include <algorithm>
 
 #include "mm.h"

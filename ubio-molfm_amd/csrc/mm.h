@@ -614,7 +614,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_mm(MmArgs) {
         ls.start(P.sa + (int64_t)T.row0 * P.sa_ld + b0 * P.sa_k, P.sa_ld, P.sa_k, min(T.rows, BM), blocks, 1);
       } else {
         const uint8_t* ps = P.sb + (kGroup == kRows ? (int64_t)T.e * P.sb_group : 0);
-        // BN is a multiple of the rows that share a scale
+        // a tile of 64 lies inside one block of the 128 rows that share a scale, larger ones hold whole blocks
         ls.start(ps + (int64_t)(P.sb_rows > 1 ? T.n0 / 128 : T.n0) * P.sb_ld + b0 * P.sb_k, P.sb_ld, P.sb_k,
                  min(P.n - T.n0, BN), blocks, P.sb_rows > 1 ? 128 : 1);
       }
@@ -741,7 +741,8 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_mm(MmArgs) {
   sb = read_sb(0);
 
   // loads that may be on their way at the barriers: those of half a step and of a whole one; behind a whole tile FM FN / 2
-  // stores of 16 bytes at least besides, which need not have ended in the first step and at the next one's beginning
+  // stores of 16 bytes at least besides, which need not have ended in the first step and at the next one's beginning (in
+  // the kernels of 256 with experts most have: they reload spilled registers between the stores, which waits for all before)
   constexpr int kWhole = kStaged ? 0 : kSend1 + kSend2, kMid = kStaged ? 0 : kHalves ? kWhole : kSend1;
   constexpr int kStores = kStaged ? 0 : FM * FN / 2;
   constexpr int kPer1 = (kSend1 + 1) / 2, kPer2 = (kSend2 + 1) / 2;      // loads behind each two of b's fragments

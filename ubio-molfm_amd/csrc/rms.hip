@@ -51,7 +51,8 @@ __device__ __forceinline__ void block_max(uint32_t (&m)[NV]) {
 }
 
 // A row's codes and scale bytes (row `at` of a table of n rows, the rows' bytes of a block side by side): whole vectors,
-// into the row's padding too (rows of codes lie a multiple of 16 bytes apart, the padding holds zeros).
+// into the row's padding too (rows of codes lie a multiple of 16 bytes apart).  What the padding holds is left open: codes
+// of zero times the row's factor as far as vectors reach, and in rows of up to 8 columns old bytes; readers mask it.
 template <int V, int kL, int NV>
 __device__ __forceinline__ void store_codes(const float (&y)[NV * V], int l, int w, uint8_t* row, int64_t ld,
                                             uint8_t* scales, int64_t at, int64_t n) {

@@ -401,7 +401,8 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: float 
 
     x: fp32, bf16 or fp16 on the GPU, of any shape with a last dimension of 1 to 16384, the residual like it; both are read
     where they lie if their rows are consecutive and evenly spaced.  weight: [w], fp32 or x's type, or None.  Results
-    have x's type and are contiguous.  Differentiable once in reverse mode (create_graph=True raises)."""
+    have x's type and are contiguous.  The squares' sum is fp32: a row in which it passes 3.4e38 gives zeros.
+    Differentiable once in reverse mode (create_graph=True raises)."""
     weight = _rms_check("rms_norm", x, weight, residual)
     if torch.jit.is_tracing() or torch.is_grad_enabled() and (
             x.requires_grad or (weight is not None and weight.requires_grad)
